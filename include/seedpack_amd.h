@@ -551,6 +551,45 @@ int spa_r2_copy_rows(void* w, int rowlen, const int64_t* pairs, int npairs, void
  * Replaces build_lut (bf16v2.py:139-145). */
 int spa_rans_build_lut_pb(const uint32_t* cum, int ntab, int pb, uint8_t* lut, void* stream);
 
+/* ---- products with packed weights (no reference counterpart) ----
+ * Weights W are row-major matrices of n rows of k: ggml type 1 (F16) or 30 (BF16), 16-byte aligned, or any of the
+ * 20 block types, at any byte. Inputs and outputs are BF16 or F16 (SPA_SRC_BF16 / SPA_SRC_F16), m rows at a stride
+ * given in elements; columns between a row's end and the stride are neither read nor written. Sums are float32 and
+ * each output is rounded once; where inputs and weights differ in type, weights are taken to 11 bits or better of
+ * their value (rows of any exponent) and inputs exactly. Outputs must not overlap inputs. `work` is device scratch
+ * of at least the call's *_work_bytes, 256-byte aligned, free again when the call's work on the stream is done;
+ * the sizes are those of the widest case, whatever the strides. Nothing is allocated, and calls may be captured. */
+
+/* y[m][n] = sum_k x[m][k] W[n][k] + scale[a] sum_r (sum_k x[m][k] A[a][r][k]) B[a][n][r], a = which[m]: a shared
+ * projection with the low-rank adapters of a batch's requests. a: [pool][rank][k], b: [pool][n][rank] of the inputs'
+ * type, scale: [pool] float32, which: [m]; a row whose number lies outside 0..pool-1 has no adapter. pool = 0: none
+ * (a, b, scale and which are not read). Ranks 1 to 256; adapters of a lower rank than the pool's hold zeros. */
+int spa_project(int type, const void* w, int64_t n, int64_t k, int x_kind, const void* x, int64_t m, int64_t x_stride,
+                void* y, int64_t y_stride, const void* a, const void* b, const float* scale, int64_t pool, int64_t rank,
+                const int32_t* which, void* work, uint64_t work_bytes, void* stream);
+uint64_t spa_project_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m, int64_t pool, int64_t rank);
+
+/* h = act(x gate^T) * (x up^T), the gated half of a feed-forward block; act 0: silu, 1: gelu (tanh form). */
+int spa_gated(int type, const void* gate, const void* up, int64_t n, int64_t k, int x_kind, const void* x, int64_t m,
+              int64_t x_stride, int act, void* h, int64_t h_stride, void* work, uint64_t work_bytes, void* stream);
+uint64_t spa_gated_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m);
+
+/* The gradients of spa_gated from dh: of the inputs (dx, or NULL) and of both matrices (dgate and dup, [n][k], or
+ * NULL; weights of the inputs' own type only). Both projections are computed again: nothing but x is kept from the
+ * forward pass. The inner gradients are rounded to the inputs' type (frozen weights of another type: to 11 bits). */
+int spa_gated_backward(int type, const void* gate, const void* up, int64_t n, int64_t k, int x_kind, const void* x, int64_t m,
+                       int64_t x_stride, int act, const void* dh, int64_t dh_stride, void* dx, int64_t dx_stride,
+                       void* dgate, void* dup, void* work, uint64_t work_bytes, void* stream);
+uint64_t spa_gated_backward_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m, int input_grad, int weight_grads);
+
+/* sums[e][c] += x[r][c]^2 over the rows r of expert e, counts[e] += their number: an importance matrix's "in_sum2"
+ * and "counts" as they are gathered. x: BF16, F16 or F32. which: [rows][each] expert numbers (a row counts once for
+ * each; numbers outside 0..experts-1 are passed over), or NULL with experts = 0: one sum over all rows. The order of
+ * the sums depends on the sizes only. */
+int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_t cols, int64_t x_stride, const int32_t* which,
+                    int64_t each, int64_t experts, float* sums, int64_t* counts, void* work, uint64_t work_bytes, void* stream);
+uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts);
+
 #ifdef __cplusplus
 }
 #endif

@@ -165,6 +165,19 @@ SIGNATURES = {
     "spa_r2_dec_table_bytes": (c_uint64, []),
     "spa_r2_copy_rows": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p]),
     "spa_rans_build_lut_pb": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "spa_project": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                            c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_uint64, c_void_p]),
+    "spa_project_work_bytes": (c_uint64, [c_int, c_int64, c_int64, c_int, c_int64, c_int64, c_int64]),
+    "spa_gated": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_int,
+                          c_void_p, c_int64, c_void_p, c_uint64, c_void_p]),
+    "spa_gated_work_bytes": (c_uint64, [c_int, c_int64, c_int64, c_int, c_int64]),
+    "spa_gated_backward": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_int,
+                                   c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_uint64,
+                                   c_void_p]),
+    "spa_gated_backward_work_bytes": (c_uint64, [c_int, c_int64, c_int64, c_int, c_int64, c_int, c_int]),
+    "spa_add_squares": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                c_void_p, c_void_p, c_uint64, c_void_p]),
+    "spa_add_squares_work_bytes": (c_uint64, [c_int64, c_int64, c_int64]),
 }
 
 

@@ -1,0 +1,274 @@
+// The products for few input rows (up to FEW_ROWS): every weight is read once and used for all of them, so
+// the weights' bytes are the floor. A workgroup of 8 waves computes 16 weight rows (16 of each matrix in the
+// gated form) for all input rows; the waves share k and join their sums in LDS, in the order of the waves.
+#include "../../include/seedpack_amd.h"
+#include "dq.h"
+#include "launch.h"
+#include "linear.h"
+
+namespace spa {
+namespace lin {
+namespace {
+
+constexpr int WAVES = 8, KC = 1024, KW = KC / WAVES;          // k of a chunk, and each wave's part of it
+
+struct FewArgs {
+    Few f;
+    int64_t rowbytes;
+};
+
+__device__ __forceinline__ f4 mul_bf(bf8 a, bf8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// the input rows' fragments of one step of 32 k: row lane & 15 of tile j, k0 + 8 (lane / 16) ..
+template <int MT>
+__device__ __forceinline__ void load_x(const Few& f, int k0, u4 (&x)[MT]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int m = 16 * j + (lane & 15);
+        x[j] = m < f.m ? *reinterpret_cast<const u4*>(f.x + (int64_t)m * f.ldx + k0 + 8 * (lane >> 4)) : u4{0, 0, 0, 0};
+    }
+}
+
+template <int KIND>
+__device__ __forceinline__ void halves(u4 raw, bf8& hi, bf8& lo) {                  // F16 values as two BF16 parts, exact
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = wide(raw[i] & 0xffffu, SRC_F16);
+        v[2 * i + 1] = wide(raw[i] >> 16, SRC_F16);
+    }
+    split8(v, hi, lo);
+}
+
+// acc += x w for weights given as 8 floats a lane (weight row lane & 15, the k of load_x)
+template <int KIND, int MT>
+__device__ __forceinline__ void step(const u4 (&x)[MT], const float (&v)[8], f4 (&acc)[MT]) {
+    bf8 wh, wl;
+    split8(v, wh, wl);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        if (KIND == SRC_BF16) {
+            const bf8 xb = __builtin_bit_cast(bf8, x[j]);
+            acc[j] = mul_bf(xb, wl, acc[j]);
+            acc[j] = mul_bf(xb, wh, acc[j]);
+        } else {
+            bf8 xh, xl;
+            halves<KIND>(x[j], xh, xl);
+            acc[j] = mul_bf(xh, wl, acc[j]);
+            acc[j] = mul_bf(xl, wh, acc[j]);
+            acc[j] = mul_bf(xh, wh, acc[j]);
+        }
+    }
+}
+
+// joins the waves' sums and writes the outputs: red holds [wave][matrix][tile][16 m][16 n]
+template <int MT, bool TWO>
+__device__ __forceinline__ void finish(const Few& f, int n0, float* red, f4 (&acc)[1 + TWO][MT]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s <= TWO; ++s)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                red[((wave * (1 + TWO) + s) * MT + j) * 256 + (4 * (lane >> 4) + c) * 16 + (lane & 15)] = acc[s][j][c];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += WAVES * 64) {
+        const int m = i >> 4, n = n0 + (i & 15);
+        if (m >= f.m || n >= f.n) continue;
+        float v = 0.f, u = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            v += red[w * (1 + TWO) * MT * 256 + i];
+            if (TWO) u += red[(w * 2 + 1) * MT * 256 + i];
+        }
+        if (TWO) {
+            v = act_value(v, f.act) * u;
+        } else if (f.ex.low) {
+            const Expand& ex = f.ex;
+            const int a = ex.which[m];
+            if (a >= 0 && a < ex.pool) {
+                const float* z = ex.low + (int64_t)m * ex.rp;
+                const uint16_t* b = ex.b + ((int64_t)a * f.n + n) * ex.rank;
+                float t = 0.f;
+                int r = 0;
+                if (ex.wide_b) {
+                    for (; r < ex.rank; r += 8) {
+                        const u4 h = *reinterpret_cast<const u4*>(b + r);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            t = fmaf(z[r + 2 * c], wide(h[c] & 0xffffu, ex.kind), t);
+                            t = fmaf(z[r + 2 * c + 1], wide(h[c] >> 16, ex.kind), t);
+                        }
+                    }
+                } else {
+                    for (; r < ex.rank; ++r) t = fmaf(z[r], wide(b[r], ex.kind), t);
+                }
+                v += t;
+            }
+        }
+        f.y[(int64_t)m * f.ldy + n] = narrow(v, f.kind);
+    }
+}
+
+// Block types: a chunk of 1024 k of the 16 rows is copied to LDS as it lies (whole 16-byte words around each
+// row's bytes), and each lane decodes 8 weights of its row in a step.
+template <int T, int QK, int BS, int KIND, int MT, bool TWO>
+__global__ __launch_bounds__(WAVES * 64) void k_few(const FewArgs a, DQ t) {
+    const Few& f = a.f;
+    constexpr int RB = KC / QK * BS, PITCH = (RB + 15 + 15) / 16 * 16 + 16, ROWS = 16 * (1 + TWO);
+    constexpr int RED = WAVES * (1 + TWO) * MT * 256 * 4;
+    constexpr int SIZE = ROWS * PITCH + 16 > RED ? ROWS * PITCH + 16 : RED;
+    __shared__ __align__(16) uint8_t mem[SIZE];
+    __shared__ int8_t kv[16];
+    if (T == 20 || T == 23) {
+        if (threadIdx.x < 16) kv[threadIdx.x] = KV_IQ4NL[threadIdx.x];
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16;
+    const int row = lane & 15, kl = 8 * (lane >> 4);
+    f4 acc[1 + TWO][MT];
+#pragma unroll
+    for (int s = 0; s <= TWO; ++s)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[s][j] = f4{0, 0, 0, 0};
+
+    for (int c0 = 0; c0 < f.k; c0 += KC) {
+        const int kn = tmin(KC, f.k - c0), bytes = kn / QK * BS;
+        const int64_t at = (int64_t)(c0 / QK) * BS;
+        constexpr int WORDS = PITCH / 16 - 1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < ROWS * WORDS; i += WAVES * 64) {
+            const int r = i / WORDS, u = i - r * WORDS, n = tmin(n0 + (r & 15), f.n - 1);
+            const uint8_t* w = TWO && r >= 16 ? f.w1 : f.w0;
+            const uint8_t* src = w + n * a.rowbytes + at;
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + 16 * u;
+            if (p >= src + bytes) continue;
+            u4* d = reinterpret_cast<u4*>(mem + r * PITCH + 16 * u);
+            if (p >= w && p + 16 <= w + f.wbytes) {
+                *d = *reinterpret_cast<const u4*>(p);
+            } else {                                              // the matrix's first or last word: its own bytes only
+                uint8_t* b = reinterpret_cast<uint8_t*>(d);
+                for (int k = 0; k < 16; ++k)
+                    if (p + k >= w && p + k < w + f.wbytes) b[k] = p[k];
+            }
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int s = 0; s < KW / 32; ++s) {
+            const int k = wave * KW + 32 * s;
+            if (k >= kn) break;
+            u4 x[MT];
+            load_x<MT>(f, c0 + k, x);
+            const int e = k + kl, blk = e / QK;
+#pragma unroll
+            for (int h = 0; h <= TWO; ++h) {
+                const uint8_t* src = (h ? f.w1 : f.w0) + (int64_t)tmin(n0 + row, f.n - 1) * a.rowbytes + at;
+                const Blk b{mem, (row + 16 * h) * PITCH + (int)(reinterpret_cast<uintptr_t>(src) & 15) + blk * BS};
+                float v[8], q[4];
+                dq4<T>(b, e - blk * QK, t, kv, q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = q[i];
+                dq4<T>(b, e - blk * QK + 4, t, kv, q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 + i] = q[i];
+                step<KIND, MT>(x, v, acc[h]);
+            }
+        }
+    }
+    finish<MT, TWO>(f, n0, reinterpret_cast<float*>(mem), acc);
+}
+
+// 16-bit weights (rows of a multiple of 32 k, 16-byte aligned): fragments straight from memory
+template <int WKIND, int KIND, int MT, bool TWO>
+__global__ __launch_bounds__(WAVES * 64) void k_few16(const FewArgs a) {
+    const Few& f = a.f;
+    __shared__ float red[WAVES * (1 + TWO) * MT * 256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16;
+    const int64_t wrow = (int64_t)tmin(n0 + (lane & 15), f.n - 1) * a.rowbytes + 16 * (lane >> 4);
+    f4 acc[1 + TWO][MT];
+#pragma unroll
+    for (int s = 0; s <= TWO; ++s)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[s][j] = f4{0, 0, 0, 0};
+    for (int k = wave * 32; k < f.k; k += WAVES * 32) {
+        u4 x[MT];
+        load_x<MT>(f, k, x);
+#pragma unroll
+        for (int h = 0; h <= TWO; ++h) {
+            const u4 w = *reinterpret_cast<const u4*>((h ? f.w1 : f.w0) + wrow + 2 * k);
+            if (WKIND == KIND) {
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    if (KIND == SRC_BF16)
+                        acc[h][j] = mul_bf(__builtin_bit_cast(bf8, x[j]), __builtin_bit_cast(bf8, w), acc[h][j]);
+                    else
+                        acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, x[j]), __builtin_bit_cast(hf8, w), acc[h][j], 0, 0, 0);
+                }
+            } else {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = wide(w[i] & 0xffffu, WKIND);
+                    v[2 * i + 1] = wide(w[i] >> 16, WKIND);
+                }
+                step<KIND, MT>(x, v, acc[h]);
+            }
+        }
+    }
+    finish<MT, TWO>(f, n0, red, acc);
+}
+
+template <int T, int QK, int BS, int KIND, bool TWO>
+int launch(const FewArgs& a, DQ t, hipStream_t st) {
+    const dim3 grid((unsigned)((a.f.n + 15) / 16)), block(WAVES * 64);
+    if constexpr (T == 1 || T == 30) {
+        constexpr int WK = T == 1 ? SRC_F16 : SRC_BF16;
+        if (a.f.m <= 16) hipLaunchKernelGGL((k_few16<WK, KIND, 1, TWO>), grid, block, 0, st, a);
+        else if (a.f.m <= 32) hipLaunchKernelGGL((k_few16<WK, KIND, 2, TWO>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_few16<WK, KIND, 4, TWO>), grid, block, 0, st, a);
+    } else {
+        if (a.f.m <= 16) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 1, TWO>), grid, block, 0, st, a, t);
+        else if (a.f.m <= 32) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 2, TWO>), grid, block, 0, st, a, t);
+        else hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 4, TWO>), grid, block, 0, st, a, t);
+    }
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+template <int T, int QK, int BS>
+int pick(const FewArgs& a, DQ t, hipStream_t st) {
+    if (a.f.w1) return a.f.kind == SRC_BF16 ? launch<T, QK, BS, SRC_BF16, true>(a, t, st) : launch<T, QK, BS, SRC_F16, true>(a, t, st);
+    return a.f.kind == SRC_BF16 ? launch<T, QK, BS, SRC_BF16, false>(a, t, st) : launch<T, QK, BS, SRC_F16, false>(a, t, st);
+}
+
+}  // namespace
+
+int few(const Few& f, hipStream_t st) {
+    DQ t{nullptr};
+    const int ti = iq_table_index(f.type);
+    if (ti >= 0) {
+        IqDeviceTable tab;
+        const int rc = iq_device_table(ti, &tab, st);
+        if (rc) return rc;
+        t.grid = tab.grid;
+    }
+    FewArgs a{f, 0};
+    switch (f.type) {
+#define SPA_FEW(T, QK, BS)                                 \
+    case T:                                                \
+        a.rowbytes = (int64_t)f.k / QK * BS;               \
+        return pick<T, QK, BS>(a, t, st);
+        SPA_FEW(1, 1, 2) SPA_FEW(30, 1, 2)
+        SPA_FEW(2, 32, 18) SPA_FEW(3, 32, 20) SPA_FEW(6, 32, 22) SPA_FEW(7, 32, 24) SPA_FEW(8, 32, 34)
+        SPA_FEW(10, 256, 84) SPA_FEW(11, 256, 110) SPA_FEW(12, 256, 144) SPA_FEW(13, 256, 176) SPA_FEW(14, 256, 210)
+        SPA_FEW(16, 256, 66) SPA_FEW(17, 256, 74) SPA_FEW(18, 256, 98) SPA_FEW(19, 256, 50) SPA_FEW(20, 32, 18)
+        SPA_FEW(21, 256, 110) SPA_FEW(22, 256, 82) SPA_FEW(23, 256, 136) SPA_FEW(29, 256, 56) SPA_FEW(42, 64, 18)
+#undef SPA_FEW
+        default: return fail(SPA_ERR_TYPE, "weights of type %d are not supported", f.type);
+    }
+}
+
+}  // namespace lin
+}  // namespace spa

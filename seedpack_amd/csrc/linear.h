@@ -1,0 +1,148 @@
+// Products with packed weights: what their kernels share (gemm.hip, few.hip, rows.hip, linear.hip).
+//
+// Numbers. Every sum is held in 32 bits. Where the inputs and the weights have the same 16-bit type
+// their products are exact in float32 and go through that type's matrix instruction. Where they do not
+// (block types, BF16 beside F16) there are two forms:
+//   * many rows: both operands as binary16 with a power of two taken out of each row, so that the row's
+//     largest value lies below 2^15. A BF16 row keeps its values to 2^-39 of its largest (8 of 11 bits
+//     used, 2^-24 the least step); a decoded weight is rounded to 11 bits, an eighth of a BF16
+//     rounding. The powers are added back to the float32 sums as exponents;
+//   * few rows: each value as a sum of two BF16 numbers (16 bits, any exponent), whose products are
+//     summed by two or three BF16 instructions: the matrix unit idles there.
+#pragma once
+
+#include "common.h"
+
+namespace spa {
+namespace lin {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+// the 16-bit types of the products' inputs (SRC_BF16 / SRC_F16)
+__device__ __forceinline__ float wide(uint32_t h, int kind) {
+    if (kind == SRC_BF16) return bf16_to_f32(h);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+__device__ __forceinline__ uint16_t narrow(float v, int kind) {
+    if (kind == SRC_BF16) return __builtin_bit_cast(uint16_t, (__bf16)v);
+    return __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+__device__ __forceinline__ uint32_t narrow2(float a, float b, int kind) {
+    return (uint32_t)narrow(a, kind) | ((uint32_t)narrow(b, kind) << 16);
+}
+
+// v = hi + lo to 2^-17 of v: hi is v cut to BF16 (so that v - hi is exact), lo the rest rounded.
+// Infinities and NaN stay in hi alone.
+__device__ __forceinline__ void split8(const float (&v)[8], bf8& hi, bf8& lo) {
+    u4 h;
+    bf8 l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
+        // a NaN whose payload lies in the cut bits would become an infinity: its quiet bit is set
+        const uint32_t ah = v[2 * i] == v[2 * i] ? a : (a | 0x400000u), bh = v[2 * i + 1] == v[2 * i + 1] ? b : (b | 0x400000u);
+        h[i] = __builtin_amdgcn_perm(bh, ah, 0x07060302u);
+        const bool fa = (a & 0x7f800000u) != 0x7f800000u, fb = (b & 0x7f800000u) != 0x7f800000u;
+        l[2 * i] = (__bf16)(fa ? v[2 * i] - __uint_as_float(a & 0xffff0000u) : 0.f);
+        l[2 * i + 1] = (__bf16)(fb ? v[2 * i + 1] - __uint_as_float(b & 0xffff0000u) : 0.f);
+    }
+    hi = __builtin_bit_cast(bf8, h);
+    lo = l;
+}
+
+// A gate's value and slope. silu: g s(g), s the logistic; gelu in its tanh form,
+// 0.5 g (1 + tanh(t)) = g s(2t), t = sqrt(2/pi) (g + 0.044715 g^3).
+enum Act { ACT_SILU = 0, ACT_GELU = 1 };
+__device__ __forceinline__ float act_logit(float g, int act) {
+    return act == ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+}
+// v/(1+e^-t): where e^-t overflows the quotient is the limit, zero
+__device__ __forceinline__ float act_value(float g, int act) { return g / (1.f + expf(-act_logit(g, act))); }
+__device__ __forceinline__ void act_both(float g, int act, float& value, float& slope) {
+    const float t = act_logit(g, act), p = 1.f / (1.f + expf(-t));
+    // p (1 - p) falls below the least number long before g overflows it: zero times a large g is zero
+    const float dt = act == ACT_SILU ? 1.f : 1.5957691216057308f * (1.f + 0.134145f * g * g);
+    const float q = p / (1.f + expf(t));                     // p (1 - p) without the difference
+    value = g * p;
+    slope = p + (q > 0.f ? g * q * dt : 0.f * g);
+}
+
+// the adapters of a call: low[m][rp] = s_a x[m] A_a^T in float32 (rp = the rank rounded up to 16, zeros
+// beyond it), b the adapters' second matrices
+struct Expand {
+    const float* low;
+    const uint16_t* b;        // [pool][n][rank], the type of the inputs
+    const int32_t* which;     // [m]; a row whose number is outside 0..pool-1 has none
+    int pool, rank, rp, kind;
+    bool wide_b;              // 16-byte loads of b's rows: rank a multiple of 8, b 16-byte aligned
+};
+
+enum GemmOut { OUT_PLAIN = 0, OUT_GATED = 1, OUT_GRAD = 2 };
+
+// sum_k x[m][k] w[n][k] over rows padded to a multiple of 64 (zeros), and what becomes of it
+struct Gemm {
+    int half;                 // SRC_BF16 / SRC_F16: the type of both operands
+    const uint16_t* x;        // [m][k], rows of ldx, 16-byte aligned
+    const uint16_t *w0, *w1;  // [n][k], rows of ldw; w1: the second matrix of OUT_GATED / OUT_GRAD
+    int64_t ldx, ldw;
+    int m, n, k;
+    const int32_t *xe, *we0, *we1;   // powers of two taken out of the rows, or null
+    int kind;                 // type of y and dh
+    uint16_t* y;              // OUT_PLAIN, OUT_GATED: [m][n], rows of ldy
+    int64_t ldy;
+    Expand ex;                // OUT_PLAIN; ex.low null: none
+    int act;
+    const uint16_t* dh;       // OUT_GRAD: [m][n], rows of ldh
+    int64_t ldh;
+    uint16_t* grad;           // OUT_GRAD: [m][2 np]: the gate's gradient, then the up projection's; zeros beyond n
+    int64_t np;
+    const int32_t* ge;        // OUT_GRAD: power of two taken out of each row of grad (binary16), or null
+};
+int gemm(const Gemm& g, hipStream_t st);
+
+// ---- few rows (few.hip)
+struct Few {
+    int type;                 // the weights' ggml type (1 F16, 30 BF16, or a block type)
+    const uint8_t *w0, *w1;   // w1 for the gated form, else null
+    int64_t wbytes;           // bytes of each matrix
+    int n, k;
+    const uint16_t* x;        // [m][k], rows of ldx (a multiple of 8), 16-byte aligned
+    int64_t ldx;
+    int m, kind;
+    uint16_t* y;
+    int64_t ldy;
+    Expand ex;
+    int act;
+};
+constexpr int FEW_ROWS = 64;
+int few(const Few& f, hipStream_t st);
+
+// ---- rows (rows.hip)
+// rows of a 16-bit matrix copied into rows of kp (a multiple of 64), zeros beyond k
+int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, hipStream_t st);
+// the same into binary16 with a power of two taken out of each row (e), optionally the row's 2-norm as it
+// was, and top[0], top[1]: the largest norm (as bits) and power (plus 1024) of any row, raised in place
+int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e,
+              float* norm, uint32_t* top, hipStream_t st);
+// the same from a block type
+int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, uint32_t* top,
+                hipStream_t st);
+// dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (even)
+int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
+                hipStream_t st);
+// the power of two to take out of each row of the gated block's inner gradients
+int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const uint32_t* top,
+                   int32_t* e, hipStream_t st);
+int zero_words(uint32_t* p, int n, hipStream_t st);
+int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st);
+// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]
+int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
+             const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st);
+
+}  // namespace lin
+}  // namespace spa

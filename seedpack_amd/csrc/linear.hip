@@ -1,0 +1,435 @@
+// The products with packed weights behind the C ABI: arguments checked, the form chosen by sizes and types,
+// the workspace laid out. Nothing is allocated and nothing waits; every launch goes to the caller's stream.
+#include "../../include/seedpack_amd.h"
+#include "launch.h"
+#include "linear.h"
+
+namespace spa {
+namespace lin {
+namespace {
+
+int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
+
+// a workspace handed out in pieces of whole 256 bytes; with no memory behind it, only counted
+struct Work {
+    uint8_t* base;
+    uint64_t used = 0;
+    template <typename T> T* take(int64_t n) {
+        T* p = reinterpret_cast<T*>(base + used);
+        used += ((uint64_t)n * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+bool is16(int type) { return type == 1 || type == 30; }
+int kind_of(int type) { return type == 1 ? SRC_F16 : SRC_BF16; }
+
+int check_weight(const char* who, int type, int64_t n, int64_t k) {
+    if (!is16(type) && !type_qk(type)) return fail(SPA_ERR_TYPE, "%s: weights of type %d are not supported", who, type);
+    if (n < 0 || k <= 0 || n > INT32_MAX - 256 || k > (1 << 22))
+        return fail(SPA_ERR_ARG, "%s: bad weight shape %lld x %lld", who, (long long)n, (long long)k);
+    if (!is16(type) && k % type_qk(type))
+        return fail(SPA_ERR_ARG, "%s: row of %lld not a multiple of %d (type %d)", who, (long long)k, type_qk(type), type);
+    return SPA_OK;
+}
+int check_rows(const char* who, int kind, int64_t m, int64_t k, int64_t stride) {
+    if (kind != SPA_SRC_BF16 && kind != SPA_SRC_F16) return fail(SPA_ERR_TYPE, "%s: inputs of kind %d (BF16 and F16 are taken)", who, kind);
+    if (m < 0 || m > INT32_MAX - 256 || stride < k) return fail(SPA_ERR_ARG, "%s: bad shape %lld x %lld, stride %lld", who, (long long)m, (long long)k, (long long)stride);
+    return SPA_OK;
+}
+bool on(const void* p, uintptr_t unit) { return (reinterpret_cast<uintptr_t>(p) & (unit - 1)) == 0; }
+int check_weight_at(const char* who, int type, const void* w) {
+    // 16-bit weights are fetched sixteen bytes at a time; blocks lie at any byte
+    if (is16(type) && !on(w, 16)) return fail(SPA_ERR_ARG, "%s: 16-bit weights not 16-byte aligned", who);
+    return SPA_OK;
+}
+int check_work(const char* who, const void* work, uint64_t have, uint64_t need) {
+    if (need && (!work || !on(work, 256) || have < need))
+        return fail(SPA_ERR_ARG, "%s: needs a 256-byte aligned workspace of %llu bytes, got %llu", who, (unsigned long long)need, (unsigned long long)(work ? have : 0));
+    return SPA_OK;
+}
+int64_t weight_bytes(int type, int64_t n, int64_t k) { return is16(type) ? 2 * n * k : n * (k / type_qk(type)) * type_bs(type); }
+
+// the operands of a product as its kernels take them
+struct Operands {
+    const uint16_t *x = nullptr, *w0 = nullptr, *w1 = nullptr;
+    int64_t ldx = 0, ldw = 0;
+    int half = 0;
+    int32_t *xe = nullptr, *we0 = nullptr, *we1 = nullptr;
+    float* norm = nullptr;
+    uint32_t* top = nullptr;
+};
+
+// Inputs and weights brought into the form of the many-rows product. Where both are of one 16-bit type they
+// are used as they lie, or copied where rows are not whole 128-byte steps at 16-byte addresses; otherwise
+// both become binary16 rows. `run` false only lays out the workspace (for the widest case).
+int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64_t n, int64_t k, int kind, const void* x, int64_t m,
+             int64_t ldx, bool bounds, Operands& o, hipStream_t st) {
+    const int64_t kp = up64(k);
+    const bool same = is16(type) && kind_of(type) == kind;
+    o.half = same ? kind : SRC_F16;
+    uint16_t* xp = wk.take<uint16_t>(m * kp);
+    int rc;
+    if (same) {
+        o.x = (const uint16_t*)x;
+        o.ldx = ldx;
+        if (run && (kp != k || !on(x, 16) || ldx % 8 || ldx > (1 << 22))) {
+            if ((rc = pack_rows((const uint16_t*)x, ldx, m, k, xp, kp, st))) return rc;
+            o.x = xp;
+            o.ldx = kp;
+        }
+        o.w0 = (const uint16_t*)w0;
+        o.w1 = (const uint16_t*)w1;
+        o.ldw = k;
+        if (kp != k) {
+            uint16_t* p0 = wk.take<uint16_t>(n * kp);
+            uint16_t* p1 = w1 ? wk.take<uint16_t>(n * kp) : nullptr;
+            if (run) {
+                if ((rc = pack_rows(o.w0, k, n, k, p0, kp, st))) return rc;
+                if (w1 && (rc = pack_rows(o.w1, k, n, k, p1, kp, st))) return rc;
+            }
+            o.w0 = p0;
+            o.w1 = p1;
+            o.ldw = kp;
+        }
+        return SPA_OK;
+    }
+    o.xe = wk.take<int32_t>(m);
+    if (bounds) {
+        o.norm = wk.take<float>(m);
+        o.top = wk.take<uint32_t>(2);
+    }
+    if (run && o.top && (rc = zero_words(o.top, 2, st))) return rc;
+    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, o.xe, o.norm, nullptr, st))) return rc;
+    o.x = xp;
+    o.ldx = o.ldw = kp;
+    for (int i = 0; i < (w1 ? 2 : 1); ++i) {
+        uint16_t* p = wk.take<uint16_t>(n * kp);
+        int32_t* e = wk.take<int32_t>(n);
+        const void* w = i ? w1 : w0;
+        if (run) {
+            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, e, nullptr, o.top, st)
+                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, e, o.top, st);
+            if (rc) return rc;
+        }
+        (i ? o.w1 : o.w0) = p;
+        (i ? o.we1 : o.we0) = e;
+    }
+    return SPA_OK;
+}
+
+// Few rows: the weights as they lie. Rows are padded where a 16-byte load of x (or of 16-bit weights) or
+// a step of 32 k would not fit; for 16-bit weights that are copied too.
+int few_operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64_t n, int64_t k, const void* x, int64_t m,
+                 int64_t ldx, Few& f, hipStream_t st) {
+    const int64_t kp = (k + 31) / 32 * 32;
+    uint16_t* xp = wk.take<uint16_t>(m * kp);
+    int rc;
+    f.x = (const uint16_t*)x;
+    f.ldx = ldx;
+    if (run && (kp != k || !on(x, 16) || ldx % 8)) {
+        if ((rc = pack_rows(f.x, ldx, m, k, xp, kp, st))) return rc;
+        f.x = xp;
+        f.ldx = kp;
+    }
+    f.w0 = (const uint8_t*)w0;
+    f.w1 = (const uint8_t*)w1;
+    if (kp != k) {                                               // block types have whole steps
+        uint16_t* p0 = wk.take<uint16_t>(n * kp);
+        uint16_t* p1 = w1 ? wk.take<uint16_t>(n * kp) : nullptr;
+        if (run) {
+            if ((rc = pack_rows((const uint16_t*)w0, k, n, k, p0, kp, st))) return rc;
+            if (w1 && (rc = pack_rows((const uint16_t*)w1, k, n, k, p1, kp, st))) return rc;
+        }
+        f.w0 = (const uint8_t*)p0;
+        f.w1 = (const uint8_t*)p1;
+    }
+    f.type = type;
+    f.n = (int)n;
+    f.k = (int)kp;
+    f.m = (int)m;
+    f.wbytes = weight_bytes(type, n, kp);
+    return SPA_OK;
+}
+
+Gemm gemm_of(const Operands& o, int64_t m, int64_t n, int64_t k) {
+    Gemm g{};
+    g.half = o.half;
+    g.x = o.x;
+    g.w0 = o.w0;
+    g.w1 = o.w1;
+    g.ldx = o.ldx;
+    g.ldw = o.ldw;
+    g.m = (int)m;
+    g.n = (int)n;
+    g.k = (int)up64(k);
+    g.xe = o.xe;
+    g.we0 = o.we0;
+    g.we1 = o.we1;
+    return g;
+}
+
+struct Project {
+    int type;
+    const void* w;
+    int64_t n, k;
+    int kind;
+    const void* x;
+    int64_t m, ldx;
+    void* y;
+    int64_t ldy;
+    const void *a, *b;
+    const float* scale;
+    int64_t pool, rank;
+    const int32_t* which;
+};
+
+int project(const Project& p, Work& wk, bool run, hipStream_t st) {
+    Expand ex{};
+    int rc;
+    if (p.pool) {
+        ex.rank = (int)p.rank;
+        ex.rp = (int)((p.rank + 15) / 16 * 16);
+        float* low = wk.take<float>(p.m * ex.rp);
+        ex.low = low;
+        ex.b = (const uint16_t*)p.b;
+        ex.which = p.which;
+        ex.pool = (int)p.pool;
+        ex.kind = p.kind;
+        ex.wide_b = p.rank % 8 == 0 && on(p.b, 16);
+        if (run && (rc = low_rows((const uint16_t*)p.x, p.ldx, p.kind, p.m, p.k, (const uint16_t*)p.a, p.scale, p.which, (int)p.pool,
+                                  (int)p.rank, low, ex.rp, st)))
+            return rc;
+    }
+    if (p.m <= FEW_ROWS) {
+        Few f{};
+        if ((rc = few_operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.x, p.m, p.ldx, f, st)) || !run) return rc;
+        f.kind = p.kind;
+        f.y = (uint16_t*)p.y;
+        f.ldy = p.ldy;
+        f.ex = ex;
+        return few(f, st);
+    }
+    Operands o;
+    if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st)) || !run) return rc;
+    Gemm g = gemm_of(o, p.m, p.n, p.k);
+    g.kind = p.kind;
+    g.y = (uint16_t*)p.y;
+    g.ldy = p.ldy;
+    g.ex = ex;
+    return gemm(g, st);
+}
+
+struct Gated {
+    int type;
+    const void *gate, *up;
+    int64_t n, k;
+    int kind;
+    const void* x;
+    int64_t m, ldx;
+    int act;
+    void* h;
+    int64_t ldh;
+    const void* dh;             // the backward form from here on: dh has rows of ldh too
+    void *dx, *dgate, *dup;
+    int64_t lddx;
+};
+// no pointer of a counted layout is read; the second matrix only has to be there
+const void* const SOME = reinterpret_cast<const void*>(256);
+
+int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
+    int rc;
+    const void* up = run ? p.up : SOME;
+    if (p.m <= FEW_ROWS) {
+        Few f{};
+        if ((rc = few_operands(wk, run, p.type, p.gate, up, p.n, p.k, p.x, p.m, p.ldx, f, st)) || !run) return rc;
+        f.kind = p.kind;
+        f.y = (uint16_t*)p.h;
+        f.ldy = p.ldh;
+        f.act = p.act;
+        return few(f, st);
+    }
+    Operands o;
+    if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st)) || !run) return rc;
+    Gemm g = gemm_of(o, p.m, p.n, p.k);
+    g.kind = p.kind;
+    g.y = (uint16_t*)p.h;
+    g.ldy = p.ldh;
+    g.act = p.act;
+    return gemm(g, st);
+}
+
+// grad = [dG | dU] in one matrix of 2 np columns; dx = grad [Wg; Wu] is then one product over 2 np, with the
+// weights transposed side by side, and the weights' gradients are products over the rows.
+int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w, hipStream_t st) {
+    int rc;
+    const int64_t np = up64(p.n), mp = up64(p.m);
+    Operands o;
+    if ((rc = operands(wk, run, p.type, p.gate, run ? p.up : SOME, p.n, p.k, p.kind, p.x, p.m, p.ldx, true, o, st))) return rc;
+    uint16_t* grad = wk.take<uint16_t>(p.m * 2 * np);
+    int32_t* ge = o.xe ? wk.take<int32_t>(p.m) : nullptr;
+    if (run) {
+        if (ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.top, ge, st))) return rc;
+        Gemm g = gemm_of(o, p.m, p.n, p.k);
+        g.kind = p.kind;
+        g.act = p.act;
+        g.dh = (const uint16_t*)p.dh;
+        g.ldh = p.ldh;
+        g.grad = grad;
+        g.np = np;
+        g.ge = ge;
+        if ((rc = gemm(g, st))) return rc;
+    }
+    if (want_x) {
+        uint16_t* wt = wk.take<uint16_t>(p.k * 2 * np);
+        if (run) {
+            if ((rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, 2 * np, np, st))) return rc;
+            if ((rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, 2 * np, np, st))) return rc;
+            Gemm g{};
+            g.half = o.half;
+            g.x = grad;
+            g.ldx = 2 * np;
+            g.w0 = wt;
+            g.ldw = 2 * np;
+            g.m = (int)p.m;
+            g.n = (int)p.k;
+            g.k = (int)(2 * np);
+            g.xe = ge;
+            g.kind = p.kind;
+            g.y = (uint16_t*)p.dx;
+            g.ldy = p.lddx;
+            if ((rc = gemm(g, st))) return rc;
+        }
+    }
+    if (want_w) {
+        uint16_t* gt = wk.take<uint16_t>(2 * np * mp);
+        uint16_t* xt = wk.take<uint16_t>(p.k * mp);
+        if (run) {
+            if ((rc = transpose16(grad, 2 * np, p.m, 2 * np, gt, mp, mp, st))) return rc;
+            if ((rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, mp, mp, st))) return rc;
+            for (int i = 0; i < 2; ++i) {
+                Gemm g{};
+                g.half = o.half;
+                g.x = gt + (i ? np * mp : 0);
+                g.ldx = mp;
+                g.w0 = xt;
+                g.ldw = mp;
+                g.m = (int)p.n;
+                g.n = (int)p.k;
+                g.k = (int)mp;
+                g.kind = p.kind;
+                g.y = (uint16_t*)(i ? p.dup : p.dgate);
+                g.ldy = p.k;
+                if ((rc = gemm(g, st))) return rc;
+            }
+        }
+    }
+    return SPA_OK;
+}
+
+}  // namespace
+}  // namespace lin
+}  // namespace spa
+
+using namespace spa;
+using namespace spa::lin;
+
+extern "C" uint64_t spa_project_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m, int64_t pool, int64_t rank) {
+    if (check_weight("", type, n, k) || check_rows("", x_kind, m, k, k) || pool < 0 || (pool && rank < 1) || m == 0 || n == 0) return 0;
+    Project p{};
+    p.type = type, p.n = n, p.k = k, p.kind = x_kind, p.m = m, p.ldx = k, p.pool = pool, p.rank = rank;
+    Work wk{nullptr};
+    project(p, wk, false, nullptr);
+    return wk.used;
+}
+
+extern "C" int spa_project(int type, const void* w, int64_t n, int64_t k, int x_kind, const void* x, int64_t m, int64_t x_stride,
+                           void* y, int64_t y_stride, const void* a, const void* b, const float* scale, int64_t pool, int64_t rank,
+                           const int32_t* which, void* work, uint64_t work_bytes, void* stream) {
+    const char* who = "spa_project";
+    int rc;
+    if ((rc = check_weight(who, type, n, k)) || (rc = check_rows(who, x_kind, m, k, x_stride))) return rc;
+    if (y_stride < n) return fail(SPA_ERR_ARG, "%s: output stride %lld for %lld columns", who, (long long)y_stride, (long long)n);
+    if (pool < 0 || pool > INT32_MAX || (pool && (rank < 1 || rank > 256)))
+        return fail(SPA_ERR_ARG, "%s: %lld adapters of rank %lld (1 to 256 are taken)", who, (long long)pool, (long long)rank);
+    if (m == 0 || n == 0) return SPA_OK;
+    if (!w || !x || !y || (pool && (!a || !b || !scale || !which))) return fail(SPA_ERR_ARG, "%s: null pointer", who);
+    if (!on(x, 2) || !on(y, 2) || (pool && (!on(a, 2) || !on(b, 2) || !on(scale, 4) || !on(which, 4))))
+        return fail(SPA_ERR_ARG, "%s: a pointer is not aligned to its elements", who);
+    if ((rc = check_weight_at(who, type, w))) return rc;
+    if ((rc = check_work(who, work, work_bytes, spa_project_work_bytes(type, n, k, x_kind, m, pool, rank)))) return rc;
+    Work wk{(uint8_t*)work};
+    return project(Project{type, w, n, k, x_kind, x, m, x_stride, y, y_stride, a, b, scale, pool, rank, which}, wk, true, (hipStream_t)stream);
+}
+
+namespace {
+int check_act(const char* who, int act) {
+    return act == ACT_SILU || act == ACT_GELU ? SPA_OK : fail(SPA_ERR_ARG, "%s: activation %d", who, act);
+}
+}  // namespace
+
+extern "C" uint64_t spa_gated_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m) {
+    if (check_weight("", type, n, k) || check_rows("", x_kind, m, k, k) || m == 0 || n == 0) return 0;
+    Gated p{};
+    p.type = type, p.n = n, p.k = k, p.kind = x_kind, p.m = m, p.ldx = k;
+    Work wk{nullptr};
+    gated(p, wk, false, nullptr);
+    return wk.used;
+}
+
+extern "C" int spa_gated(int type, const void* gate, const void* up, int64_t n, int64_t k, int x_kind, const void* x, int64_t m,
+                         int64_t x_stride, int act, void* h, int64_t h_stride, void* work, uint64_t work_bytes, void* stream) {
+    const char* who = "spa_gated";
+    int rc;
+    if ((rc = check_weight(who, type, n, k)) || (rc = check_rows(who, x_kind, m, k, x_stride)) || (rc = check_act(who, act))) return rc;
+    if (h_stride < n) return fail(SPA_ERR_ARG, "%s: output stride %lld for %lld columns", who, (long long)h_stride, (long long)n);
+    if (m == 0 || n == 0) return SPA_OK;
+    if (!gate || !up || !x || !h) return fail(SPA_ERR_ARG, "%s: null pointer", who);
+    if (!on(x, 2) || !on(h, 2)) return fail(SPA_ERR_ARG, "%s: a pointer is not aligned to its elements", who);
+    if ((rc = check_weight_at(who, type, gate)) || (rc = check_weight_at(who, type, up))) return rc;
+    if ((rc = check_work(who, work, work_bytes, spa_gated_work_bytes(type, n, k, x_kind, m)))) return rc;
+    Gated p{};
+    p.type = type, p.gate = gate, p.up = up, p.n = n, p.k = k, p.kind = x_kind, p.x = x, p.m = m, p.ldx = x_stride, p.act = act;
+    p.h = h, p.ldh = h_stride;
+    Work wk{(uint8_t*)work};
+    return gated(p, wk, true, (hipStream_t)stream);
+}
+
+extern "C" uint64_t spa_gated_backward_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m, int input_grad, int weight_grads) {
+    if (check_weight("", type, n, k) || check_rows("", x_kind, m, k, k) || m == 0 || n == 0) return 0;
+    Gated p{};
+    p.type = type, p.n = n, p.k = k, p.kind = x_kind, p.m = m, p.ldx = k;
+    Work wk{nullptr};
+    gated_backward(p, wk, false, input_grad != 0, weight_grads != 0, nullptr);
+    return wk.used;
+}
+
+extern "C" int spa_gated_backward(int type, const void* gate, const void* up, int64_t n, int64_t k, int x_kind, const void* x, int64_t m,
+                                  int64_t x_stride, int act, const void* dh, int64_t dh_stride, void* dx, int64_t dx_stride,
+                                  void* dgate, void* dup, void* work, uint64_t work_bytes, void* stream) {
+    const char* who = "spa_gated_backward";
+    int rc;
+    if ((rc = check_weight(who, type, n, k)) || (rc = check_rows(who, x_kind, m, k, x_stride)) || (rc = check_act(who, act))) return rc;
+    if (dh_stride < n || (dx && dx_stride < k)) return fail(SPA_ERR_ARG, "%s: stride %lld for %lld columns, %lld for %lld", who, (long long)dh_stride, (long long)n, (long long)dx_stride, (long long)k);
+    if (!dgate != !dup) return fail(SPA_ERR_ARG, "%s: the gradient of one of the two matrices only", who);
+    if (dgate && !(is16(type) && kind_of(type) == x_kind))
+        return fail(SPA_ERR_TYPE, "%s: gradients of weights of type %d beside inputs of kind %d", who, type, x_kind);
+    if (n > (1 << 21) || m > (1 << 22)) return fail(SPA_ERR_ARG, "%s: %lld rows, %lld weight rows are too many", who, (long long)m, (long long)n);
+    if (!dx && !dgate) return SPA_OK;
+    hipStream_t st = (hipStream_t)stream;
+    if (m == 0 || n == 0) {                                      // sums of nothing
+        if (dx && m && (rc = zero_rows((uint16_t*)dx, dx_stride, m, k, st))) return rc;
+        if (dgate && n && ((rc = zero_rows((uint16_t*)dgate, k, n, k, st)) || (rc = zero_rows((uint16_t*)dup, k, n, k, st)))) return rc;
+        return SPA_OK;
+    }
+    if (!gate || !up || !x || !dh) return fail(SPA_ERR_ARG, "%s: null pointer", who);
+    if (!on(x, 2) || !on(dh, 2) || !on(dx, 2) || !on(dgate, 2) || !on(dup, 2))
+        return fail(SPA_ERR_ARG, "%s: a pointer is not aligned to its elements", who);
+    if ((rc = check_weight_at(who, type, gate)) || (rc = check_weight_at(who, type, up))) return rc;
+    if ((rc = check_work(who, work, work_bytes, spa_gated_backward_work_bytes(type, n, k, x_kind, m, dx != nullptr, dgate != nullptr)))) return rc;
+    Gated p{};
+    p.type = type, p.gate = gate, p.up = up, p.n = n, p.k = k, p.kind = x_kind, p.x = x, p.m = m, p.ldx = x_stride, p.act = act;
+    p.ldh = dh_stride, p.dh = dh, p.dx = dx, p.dgate = dgate, p.dup = dup, p.lddx = dx_stride;
+    Work wk{(uint8_t*)work};
+    return gated_backward(p, wk, true, dx != nullptr, dgate != nullptr, st);
+}

@@ -1,0 +1,217 @@
+// Column sums of squares, per expert or whole: what an importance matrix gathers of a matrix's inputs
+// (llama.cpp's "in_sum2" and "counts"). Bound by reading x once.
+//
+// A workgroup takes 512 columns (8 a lane, 64 lanes) and a run of rows, its four waves every fourth row of
+// it; it joins the waves in LDS and writes one partial row, and a second launch adds the partial rows to the
+// caller's sums in the order of the runs. Sums are float32; no atomics, so a call's result depends on its
+// sizes only. With experts a workgroup belongs to one of them and takes that expert's rows of its run.
+#include "../../include/seedpack_amd.h"
+#include "launch.h"
+#include "linear.h"
+
+namespace spa {
+namespace lin {
+namespace {
+
+constexpr int COLS = 512, IDS = 1024;
+
+template <int KIND>
+__device__ __forceinline__ void add8(const void* __restrict__ x, int64_t at, int64_t left, bool wide8, float (&s)[8], float times) {
+    float v[8];
+    if (wide8 && left >= 8) {
+        load_weights<8>(x, KIND, at, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] = 0.f;
+            if (i < left)
+                v[i] = KIND == SRC_F32 ? static_cast<const float*>(x)[at + i] : wide(static_cast<const uint16_t*>(x)[at + i], KIND);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = fmaf(v[i] * times, v[i], s[i]);
+}
+
+struct Sq {
+    const void* x;
+    int64_t ld, rows, cols, run;      // run: rows of a workgroup
+    const int32_t* which;             // [rows][each], or null
+    int each, experts;
+    float* part;                      // [runs][experts][cols]
+    uint32_t* hits;                   // [runs][experts]
+    float* sums;
+    int64_t* counts;
+    int64_t runs;
+    bool wide8;
+};
+
+template <int KIND>
+__global__ __launch_bounds__(256) void k_squares(const Sq q) {
+    __shared__ float join[3][COLS];
+    __shared__ int list[IDS];
+    __shared__ int times[IDS];
+    __shared__ int wsum[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t tiles = (q.cols + COLS - 1) / COLS;
+    const int64_t c0 = (int64_t)(blockIdx.x % tiles) * COLS + 8 * lane, run = blockIdx.x / tiles;
+    const int e = blockIdx.y;
+    const int64_t r0 = run * q.run, r1 = tmin(q.rows, r0 + q.run), left = q.cols - c0;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    uint32_t hits = 0;
+    if (!q.which) {
+#pragma unroll 4
+        for (int64_t r = r0 + wave; r < r1; r += 4)
+            if (left > 0) add8<KIND>(q.x, r * q.ld + c0, left, q.wide8, s, 1.f);
+    } else {
+        for (int64_t b = r0; b < r1; b += IDS) {
+            // the rows of this expert among the next IDS, in their order: each wave a quarter
+            const int n = (int)tmin<int64_t>(IDS, r1 - b);
+            int have = 0;
+            uint64_t mask[IDS / 256];
+            int mult[IDS / 256];
+#pragma unroll
+            for (int i = 0; i < IDS / 256; ++i) {
+                const int r = wave * (IDS / 4) + i * 64 + lane;
+                int h = 0;
+                if (r < n)
+                    for (int j = 0; j < q.each; ++j) h += q.which[(b + r) * q.each + j] == e;
+                mult[i] = h;
+                mask[i] = __ballot(h > 0);
+                have += __popcll(mask[i]);
+                hits += h;
+            }
+            __syncthreads();
+            if (lane == 0) wsum[wave] = have;
+            __syncthreads();
+            int at = 0, total = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if (w < wave) at += wsum[w];
+                total += wsum[w];
+            }
+#pragma unroll
+            for (int i = 0; i < IDS / 256; ++i) {
+                if (mult[i]) {
+                    const int p = at + __popcll(mask[i] & ((1ull << lane) - 1));
+                    list[p] = wave * (IDS / 4) + i * 64 + lane;
+                    times[p] = mult[i];
+                }
+                at += __popcll(mask[i]);
+            }
+            __syncthreads();
+#pragma unroll 4
+            for (int i = wave; i < total; i += 4)
+                if (left > 0) add8<KIND>(q.x, (b + list[i]) * q.ld + c0, left, q.wide8, s, (float)times[i]);
+        }
+        if (blockIdx.x % tiles == 0) {
+#pragma unroll
+            for (int k = 32; k; k >>= 1) hits += __shfl_xor(hits, k);
+            __syncthreads();
+            if (lane == 0) wsum[wave] = (int)hits;
+            __syncthreads();
+            if (threadIdx.x == 0) q.hits[run * q.experts + e] = (uint32_t)(wsum[0] + wsum[1] + wsum[2] + wsum[3]);
+        }
+    }
+    if (wave) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) join[wave - 1][i * 64 + lane] = s[i];
+    }
+    __syncthreads();
+    if (wave == 0) {
+        float* out = q.part + (run * q.experts + e) * q.cols + c0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = (s[i] + join[0][i * 64 + lane]) + (join[1][i * 64 + lane] + join[2][i * 64 + lane]);
+            if (i < left) out[i] = v;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
+    const int64_t n = (int64_t)q.experts * q.cols;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        float v = 0.f;
+#pragma unroll 8
+        for (int64_t r = 0; r < q.runs; ++r) v += q.part[r * n + i];
+        q.sums[i] += v;
+    }
+    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < q.experts; e += gridDim.x * 256ll) {
+        int64_t c = q.which ? 0 : q.rows;
+        if (q.which)
+            for (int64_t r = 0; r < q.runs; ++r) c += q.hits[r * q.experts + e];
+        q.counts[e] += c;
+    }
+}
+
+// rows of a run: enough workgroups to fill the device (about 1024 of them), at least 16 rows each
+int64_t run_rows(int64_t rows, int64_t cols, int64_t experts) {
+    const int64_t tiles = (cols + COLS - 1) / COLS * experts;
+    const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
+    int64_t run = (rows + runs - 1) / runs;
+    if (run < 16) run = 16;
+    while ((rows + run - 1) / run > 65535) run *= 2;
+    return run;
+}
+uint64_t part_bytes(int64_t runs, int64_t cols, int64_t experts) {
+    return ((uint64_t)runs * experts * cols * 4 + 255) / 256 * 256;
+}
+
+}  // namespace
+}  // namespace lin
+}  // namespace spa
+
+using namespace spa;
+using namespace spa::lin;
+
+extern "C" uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts) {
+    if (rows <= 0 || cols <= 0 || experts < 0) return 0;
+    if (experts == 0) experts = 1;
+    const int64_t run = run_rows(rows, cols, experts), runs = (rows + run - 1) / run;
+    return part_bytes(runs, cols, experts) + ((uint64_t)runs * experts * 4 + 255) / 256 * 256;
+}
+
+extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_t cols, int64_t x_stride, const int32_t* which,
+                               int64_t each, int64_t experts, float* sums, int64_t* counts, void* work, uint64_t work_bytes,
+                               void* stream) {
+    if (src_kind < SPA_SRC_BF16 || src_kind > SPA_SRC_F32) return fail(SPA_ERR_TYPE, "spa_add_squares: source kind %d", src_kind);
+    if (rows < 0 || cols <= 0 || x_stride < cols || rows > INT32_MAX || cols > INT32_MAX)
+        return fail(SPA_ERR_ARG, "spa_add_squares: bad shape %lld x %lld, stride %lld", (long long)rows, (long long)cols, (long long)x_stride);
+    if (which ? (experts < 1 || experts > 65535 || each < 1 || each > 65535) : experts != 0)
+        return fail(SPA_ERR_ARG, "spa_add_squares: %lld experts, %lld for each row", (long long)experts, (long long)each);
+    if (rows == 0) return SPA_OK;
+    if (!x || !sums || !counts) return fail(SPA_ERR_ARG, "spa_add_squares: null pointer");
+    const uintptr_t unit = src_kind == SPA_SRC_F32 ? 3 : 1;
+    if ((reinterpret_cast<uintptr_t>(x) & unit) || (reinterpret_cast<uintptr_t>(which) & 3) || (reinterpret_cast<uintptr_t>(sums) & 3) ||
+        (reinterpret_cast<uintptr_t>(counts) & 7))
+        return fail(SPA_ERR_ARG, "spa_add_squares: a pointer is not aligned to its elements");
+    if (!work || (reinterpret_cast<uintptr_t>(work) & 15) || work_bytes < spa_add_squares_work_bytes(rows, cols, experts))
+        return fail(SPA_ERR_ARG, "spa_add_squares: needs a 16-byte aligned workspace of spa_add_squares_work_bytes bytes");
+    Sq q{};
+    q.x = x;
+    q.ld = x_stride;
+    q.rows = rows;
+    q.cols = cols;
+    q.which = which;
+    q.each = (int)each;
+    q.experts = which ? (int)experts : 1;
+    q.run = run_rows(rows, cols, q.experts);
+    q.runs = (rows + q.run - 1) / q.run;
+    q.part = (float*)work;
+    q.hits = (uint32_t*)((uint8_t*)work + part_bytes(q.runs, cols, q.experts));
+    q.sums = sums;
+    q.counts = counts;
+    const int64_t unit16 = src_kind == SPA_SRC_F32 ? 4 : 8;
+    q.wide8 = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_stride % unit16 == 0;
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t tiles = (cols + COLS - 1) / COLS;
+    if (tiles * q.runs > INT32_MAX) return fail(SPA_ERR_ARG, "spa_add_squares: %lld x %lld is too large", (long long)rows, (long long)cols);
+    const dim3 grid((unsigned)(tiles * q.runs), (unsigned)q.experts);
+    if (src_kind == SPA_SRC_BF16) hipLaunchKernelGGL((k_squares<SRC_BF16>), grid, dim3(256), 0, st, q);
+    else if (src_kind == SPA_SRC_F16) hipLaunchKernelGGL((k_squares<SRC_F16>), grid, dim3(256), 0, st, q);
+    else hipLaunchKernelGGL((k_squares<SRC_F32>), grid, dim3(256), 0, st, q);
+    SPA_HIP_TRY(hipGetLastError());
+    const int64_t groups = ((int64_t)q.experts * cols + 255) / 256;
+    hipLaunchKernelGGL(k_squares_join, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, q);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}

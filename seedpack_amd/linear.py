@@ -1,0 +1,190 @@
+"""Products with packed weights: what a program does with the tensors that this package regrows.
+
+  project         a shared projection beside the low-rank adapters of the requests in a batch
+  gated           the gated half of a feed-forward block, act(x gate^T) * (x up^T)
+  gated_backward  its gradients
+  add_squares     the column sums of squares that an importance matrix is made of
+
+Weights are BF16 or F16 matrices or any of the 20 GGUF block types, as they lie in a file (`Weight`).
+Inputs and outputs are two-dimensional DeviceArrays of BF16 bits (uint16) or float16, row-major; with a
+`*_stride` (in elements) an array's rows may lie further apart than their columns. Every call only queues
+work on `stream` and returns; results are float32 sums rounded once. Scratch comes from the calling
+thread's cache of device blocks, whose work is on one stream (device._Cache), or is given as `work`.
+
+The reference has no counterpart: it makes and packs weights (seedpack/gpuquant.py:284-456) and leaves
+their use to llama.cpp.
+"""
+import numpy as np
+
+from . import device as dev
+from ._lib import check, lib
+from .requant import QFUN
+
+F16, BF16 = 1, 30
+ACT = {"silu": 0, "gelu": 1}
+_KIND = {np.dtype(np.uint16): 0, np.dtype(np.float16): 1, np.dtype(np.float32): 2}
+
+
+class Weight:
+    """a matrix of `rows` output rows of `cols` inputs: ggml type (F16, BF16 or a block type) and its bytes"""
+    __slots__ = ("type", "data", "rows", "cols")
+
+    def __init__(self, ttype, data, rows, cols):
+        if ttype in (F16, BF16):
+            need = 2 * rows * cols
+        elif ttype in QFUN:
+            _, qk, bs = QFUN[ttype]
+            if cols % qk:
+                raise ValueError(f"rows of {cols} weights are not whole blocks of {qk} (type {ttype})")
+            need = rows * (cols // qk) * bs
+        else:
+            raise ValueError(f"unknown ggml type {ttype}")
+        if rows < 0 or cols <= 0:
+            raise ValueError(f"bad shape {rows} x {cols}")
+        if data.nbytes < need:
+            raise ValueError(f"{data.nbytes} bytes hold no {rows} x {cols} weights of type {ttype} ({need} bytes)")
+        self.type, self.data, self.rows, self.cols = ttype, data, rows, cols
+
+
+class Adapters:
+    """a pool of low-rank adapters of one projection: a (count, rank, cols), b (count, rows, rank), both of the
+    inputs' type, scale (count,) float32; number i adds scale[i] x a[i]^T b[i]^T"""
+    __slots__ = ("a", "b", "scale", "count", "rank")
+
+    def __init__(self, a, b, scale):
+        if len(a.shape) != 3 or len(b.shape) != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError(f"adapters of shapes {a.shape} and {b.shape}: (count, rank, cols) and (count, rows, rank) are taken")
+        self.count, self.rank = a.shape[:2]
+        if scale.dtype != np.float32 or scale.size != self.count:
+            raise ValueError(f"{scale.size} scales of {scale.dtype} for {self.count} adapters (float32)")
+        if a.dtype != b.dtype:
+            raise TypeError(f"adapters of two types, {a.dtype} and {b.dtype}")
+        self.a, self.b, self.scale = a, b, scale
+
+
+def _rows(name, a, stride, cols=None):
+    """a 2-D array -> (kind, rows, columns, stride)"""
+    kind = _KIND.get(a.dtype)
+    if kind is None:
+        raise TypeError(f"{name} must be bf16 bits (uint16), float16 or float32, not {a.dtype}")
+    if len(a.shape) != 2 or (cols is not None and a.shape[1] != cols):
+        raise ValueError(f"{name} has shape {a.shape}" + (f", {cols} columns are needed" if cols is not None else ""))
+    m, k = a.shape
+    if stride is None:
+        return kind, m, k, k
+    if stride < k:
+        raise ValueError(f"{name}: rows of {k} at a stride of {stride}")
+    return kind, m, k, stride
+
+
+def _ids(which, rows):
+    if which.dtype != np.int32:
+        raise TypeError(f"row numbers must be int32, not {which.dtype}")
+    if which.shape[0] != rows:
+        raise ValueError(f"{which.shape[0]} row numbers for {rows} rows")
+
+
+def _scratch(n, work):
+    if not n:
+        return None, None, 0
+    if work is None:
+        work = dev.DeviceArray(n, np.uint8)
+    return work, work.ptr, work.nbytes
+
+
+def _out(name, out, m, n, dtype, stride):
+    if out is None:
+        if stride is not None:
+            raise ValueError(f"a stride of {name} needs its array")
+        return dev.DeviceArray((m, n), dtype), n
+    if out.dtype != dtype or out.shape != (m, n):
+        raise ValueError(f"{name} is {out.shape} {out.dtype}, ({m}, {n}) {dtype} is needed")
+    if stride is not None and stride < n:
+        raise ValueError(f"{name}: rows of {n} at a stride of {stride}")
+    return out, n if stride is None else stride
+
+
+def project(x, w, adapters=None, which=None, out=None, x_stride=None, out_stride=None, work=None, stream=None):
+    """x (rows, w.cols) -> (rows, w.rows): x W^T, plus for each row r the adapter which[r] (int32; numbers
+    outside the pool: none)"""
+    kind, m, _, ld = _rows("x", x, x_stride, w.cols)
+    out, ldo = _out("out", out, m, w.rows, x.dtype, out_stride)
+    a = b = scale = ids = None
+    pool = rank = 0
+    if adapters is not None:
+        if which is None:
+            raise ValueError("adapters need the number of each row's adapter")
+        if adapters.a.dtype != x.dtype or adapters.a.shape[2] != w.cols or adapters.b.shape[1] != w.rows:
+            raise ValueError(f"adapters of {adapters.a.dtype} {adapters.a.shape}, {adapters.b.shape} beside {x.dtype} inputs "
+                             f"and a {w.rows} x {w.cols} projection")
+        _ids(which, m)
+        a, b, scale, ids, pool, rank = adapters.a.ptr, adapters.b.ptr, adapters.scale.ptr, which.ptr, adapters.count, adapters.rank
+    L = lib()
+    keep, p, n = _scratch(L.spa_project_work_bytes(w.type, w.rows, w.cols, kind, m, pool, rank), work)
+    check(L.spa_project(w.type, w.data.ptr, w.rows, w.cols, kind, x.ptr, m, ld, out.ptr, ldo, a, b, scale, pool, rank, ids,
+                        p, n, stream))
+    return out
+
+
+def _pair(gate, up, act):
+    if (gate.type, gate.rows, gate.cols) != (up.type, up.rows, up.cols):
+        raise ValueError(f"gate is type {gate.type} {gate.rows} x {gate.cols}, up type {up.type} {up.rows} x {up.cols}")
+    if act not in ACT:
+        raise ValueError(f"unknown activation {act!r}: {sorted(ACT)}")
+    return ACT[act]
+
+
+def gated(x, gate, up, act="silu", out=None, x_stride=None, out_stride=None, work=None, stream=None):
+    """x (rows, cols) -> act(x gate^T) * (x up^T), (rows, gate.rows); act "silu" or "gelu" (tanh form)"""
+    act = _pair(gate, up, act)
+    kind, m, _, ld = _rows("x", x, x_stride, gate.cols)
+    out, ldo = _out("out", out, m, gate.rows, x.dtype, out_stride)
+    L = lib()
+    keep, p, n = _scratch(L.spa_gated_work_bytes(gate.type, gate.rows, gate.cols, kind, m), work)
+    check(L.spa_gated(gate.type, gate.data.ptr, up.data.ptr, gate.rows, gate.cols, kind, x.ptr, m, ld, act, out.ptr, ldo, p, n,
+                      stream))
+    return out
+
+
+def gated_backward(x, gate, up, dh, act="silu", dx=None, dgate=None, dup=None, x_stride=None, dh_stride=None, dx_stride=None,
+                   work=None, stream=None):
+    """the gradients of gated() from dh (rows, gate.rows): written to the arrays given, dx (rows, cols) and / or
+    both of dgate and dup (gate.rows, cols; weights of x's own type only). With none given dx is made.
+    -> (dx, dgate, dup)"""
+    act = _pair(gate, up, act)
+    kind, m, k, ld = _rows("x", x, x_stride, gate.cols)
+    _, mh, _, ldh = _rows("dh", dh, dh_stride, gate.rows)
+    if mh != m or dh.dtype != x.dtype:
+        raise ValueError(f"dh is {dh.shape} {dh.dtype} for x {x.shape} {x.dtype}")
+    if (dgate is None) != (dup is None):
+        raise ValueError("both matrices' gradients or neither")
+    ldx = k
+    if dx is not None or dgate is None:
+        dx, ldx = _out("dx", dx, m, k, x.dtype, dx_stride)
+    if dgate is not None:
+        dgate, _ = _out("dgate", dgate, gate.rows, k, x.dtype, None)
+        dup, _ = _out("dup", dup, gate.rows, k, x.dtype, None)
+    L = lib()
+    keep, p, n = _scratch(L.spa_gated_backward_work_bytes(gate.type, gate.rows, k, kind, m, dx is not None, dgate is not None), work)
+    check(L.spa_gated_backward(gate.type, gate.data.ptr, up.data.ptr, gate.rows, k, kind, x.ptr, m, ld, act, dh.ptr, ldh,
+                               None if dx is None else dx.ptr, ldx, None if dgate is None else dgate.ptr,
+                               None if dup is None else dup.ptr, p, n, stream))
+    return dx, dgate, dup
+
+
+def add_squares(x, sums, counts, which=None, x_stride=None, work=None, stream=None):
+    """x (rows, cols), float32 too: adds the rows' squares to sums (experts, cols) float32 and their numbers to
+    counts (experts,) int64. which (rows, each) int32 holds the experts of each row; without it there is one sum
+    over all rows. An importance matrix is sums / counts (imatrix.load of its "in_sum2" and "counts")."""
+    kind, m, k, ld = _rows("x", x, x_stride)
+    experts = each = 0
+    if which is not None:
+        _ids(which, m)
+        experts, each = counts.size, (which.size // m if m else 1)
+    if sums.dtype != np.float32 or counts.dtype != np.int64 or sums.size != counts.size * k or (which is None and counts.size != 1):
+        raise ValueError(f"sums {sums.shape} {sums.dtype}, counts {counts.shape} {counts.dtype} for {k} columns")
+    L = lib()
+    keep, p, n = _scratch(L.spa_add_squares_work_bytes(m, k, experts), work)
+    check(L.spa_add_squares(x.ptr, kind, m, k, ld, None if which is None else which.ptr, each, experts, sums.ptr, counts.ptr,
+                            p, n, stream))
+    return sums, counts
