@@ -1,0 +1,398 @@
+// The few-rows product for the block types whose weights are scale x code - offset with small whole codes
+// (Q4_0, Q8_0, Q4_K, Q5_K, Q6_K). With w[k] = s c[k] - o over a run of k that shares s and o,
+//     sum_k x[k] w[k] = s sum_k x[k] c[k] - o sum_k x[k]:
+// the codes, not the weights, are the matrix instruction's operand. A code of up to 7 bits becomes a BF16
+// number by putting its bits under the exponent of 128 (0x4300 | c = 128 + c, exact), two codes by one byte
+// permutation; 128 s then goes into o. For F16 the same under 1024 (0x6400 | c). Q8_0's 8 bits are exact as
+// BF16 too, by way of float32. So no weight is rounded, unpacking costs about one instruction a weight
+// instead of the six to eight of decoding to float32 and splitting, and the sums of x alone come from a
+// second instruction with an operand of ones, in the registers where they are needed.
+//
+// A lane holds 8 codes of weight row lane & 15 for a step of 32 k. A wave works alone on units of 256 k: the
+// unit's bytes of its 16 rows go to LDS of its own by 16-byte loads that bypass the registers, each byte
+// once (read lane by lane from memory, 32 bytes of a row at a time, the same lines were fetched again and
+// again: Q8_0 12288 x 4096 took 63 us, Q6_K 151936 x 1024 149 us), and no barrier is needed before the join. The
+// loads of many waves of a compute unit keep the memory busy while others compute.
+// Q6_K's scales cover 16 k, half a step: its tiles take 8 input rows twice, rows 0-7 with the first 16 k and
+// rows 8-15 with the second (zeros elsewhere), so that a lane's sums belong to one scale.
+#include "../../include/seedpack_amd.h"
+#include "few.h"
+#include "launch.h"
+
+namespace spa {
+namespace lin {
+namespace {
+
+// This lane's row of a unit in LDS: 32-bit words at any byte of it, in pairs that lie 4 bytes on. Words at k and at
+// k + 2 (k a multiple of 4) have aligned words and shifts of their own, so that k costs nothing where the caller
+// is unrolled. AL: the row begins at a 16-byte address.
+template <bool AL>
+struct Row {
+    const uint32_t* w[2];
+    uint32_t sh[2];
+    __device__ __forceinline__ void set(const uint8_t* stage, uint32_t mis) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t at = AL ? 0 : mis + 2 * i;
+            w[i] = reinterpret_cast<const uint32_t*>(stage) + (at >> 2);
+            sh[i] = AL ? 2 * i : at & 3;
+        }
+    }
+    __device__ __forceinline__ u2 pair(int k) const {
+        const int i = (k >> 1) & 1;
+        const uint32_t* p = w[i] + (k >> 2);
+        if (AL && i == 0) return u2{p[0], p[1]};
+        const uint32_t a = p[0], b = p[1], c = p[2];
+        return u2{__builtin_amdgcn_alignbyte(b, a, sh[i]), __builtin_amdgcn_alignbyte(c, b, sh[i])};
+    }
+    __device__ __forceinline__ uint32_t word(int k) const {
+        const int i = (k >> 1) & 1;
+        const uint32_t* p = w[i] + (k >> 2);
+        return AL && i == 0 ? p[0] : __builtin_amdgcn_alignbyte(p[1], p[0], sh[i]);
+    }
+    __device__ __forceinline__ uint32_t half(int k) const {       // k even, two bytes
+        if (AL) return (w[0][k >> 2] >> (8 * (k & 2))) & 0xffffu;
+        return word(k) & 0xffffu;
+    }
+};
+__device__ __forceinline__ float half_of(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
+
+// codes of up to 7 bits, four bytes -> four numbers BASE + code
+template <int KIND> constexpr float BASE = KIND == SRC_BF16 ? 128.f : 1024.f;
+template <int KIND>
+__device__ __forceinline__ void put4(uint32_t c, u4& w, int at) {
+    constexpr uint32_t E = KIND == SRC_BF16 ? 0x43434343u : 0x64646464u;
+    w[at] = __builtin_amdgcn_perm(E, c, 0x04010400u);
+    w[at + 1] = __builtin_amdgcn_perm(E, c, 0x04030402u);
+}
+
+// a unit of 256 weights of one row as lane group g (0..3) reads it; step f: codes 32 f + 8 g .. of it
+constexpr int UNIT = 256;
+template <int T> struct Unit;
+
+struct K4 {                                                       // Q4_K / Q5_K scales and offsets
+    uint32_t sc[2], mn[2];
+    float d, dm;
+    __device__ __forceinline__ void set(u4 h) {
+        d = half_of(h[0] & 0xffffu);
+        dm = half_of(h[0] >> 16);
+        sc[0] = h[1] & 0x3f3f3f3fu;
+        mn[0] = h[2] & 0x3f3f3f3fu;
+        sc[1] = (h[3] & 0x0f0f0f0fu) | ((h[1] >> 2) & 0x30303030u);
+        mn[1] = ((h[3] >> 4) & 0x0f0f0f0fu) | ((h[2] >> 2) & 0x30303030u);
+    }
+    template <int KIND> __device__ __forceinline__ void scale(int f, float& s, float& o) const {
+        s = d * (float)((sc[f >> 2] >> (8 * (f & 3))) & 0xffu);
+        o = fmaf(BASE<KIND>, s, dm * (float)((mn[f >> 2] >> (8 * (f & 3))) & 0xffu));
+    }
+};
+template <> struct Unit<12> {                                     // Q4_K: 4 x 32 bytes of two nibbles
+    static constexpr int QK = 256, BS = 144;
+    static constexpr bool HALVES = false;
+    K4 k;
+    template <class R> __device__ __forceinline__ void open(const R& r) { k.set(u4{r.word(0), r.word(4), r.word(8), r.word(12)}); }
+    template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
+        const u2 q = r.pair(16 + 32 * (f >> 1) + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) put4<KIND>((f & 1 ? q[i] >> 4 : q[i]) & 0x0f0f0f0fu, w, 2 * i);
+        k.scale<KIND>(f, s, o);
+    }
+};
+template <> struct Unit<13> {                                     // Q5_K: the same, and bit f of 32 bytes
+    static constexpr int QK = 256, BS = 176;
+    static constexpr bool HALVES = false;
+    K4 k;
+    template <class R> __device__ __forceinline__ void open(const R& r) { k.set(u4{r.word(0), r.word(4), r.word(8), r.word(12)}); }
+    template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
+        const u2 q = r.pair(48 + 32 * (f >> 1) + 8 * g), h = r.pair(16 + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t lo = (f & 1 ? q[i] >> 4 : q[i]) & 0x0f0f0f0fu;
+            put4<KIND>(lo | (((h[i] >> f) & 0x01010101u) << 4), w, 2 * i);
+        }
+        k.scale<KIND>(f, s, o);
+    }
+};
+template <> struct Unit<14> {                                     // Q6_K: per half of 128, 4 quarters of 32
+    static constexpr int QK = 256, BS = 210;
+    static constexpr bool HALVES = true;
+    u4 sc;
+    float d;
+    template <class R> __device__ __forceinline__ void open(const R& r) {
+        sc = u4{r.word(192), r.word(196), r.word(200), r.word(204)};
+        d = half_of(r.half(208));
+    }
+    template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
+        const int h = f >> 2, qd = f & 3;
+        const u2 l = r.pair(64 * h + 32 * (qd & 1) + 8 * g), hi = r.pair(128 + 32 * h + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t c = (qd < 2 ? l[i] : l[i] >> 4) & 0x0f0f0f0fu, b = (hi[i] >> (2 * qd)) & 0x03030303u;
+            put4<KIND>(c | (b << 4), w, 2 * i);
+        }
+        const int byte = (int)(sc[2 * h + (qd >> 1)] << (24 - 16 * (qd & 1) - 8 * (g >> 1))) >> 24;   // scale 8 h + 2 qd + g / 2
+        s = d * (float)byte;
+        o = (BASE<KIND> + 32.f) * s;
+    }
+};
+template <> struct Unit<8> {                                      // Q8_0: blocks of 32 codes of 8 bits
+    static constexpr int QK = 32, BS = 34;
+    static constexpr bool HALVES = false;
+    template <class R> __device__ __forceinline__ void open(const R&) {}
+    template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
+        const u2 q = r.pair(34 * f + 2 + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t c = q[i] ^ 0x80808080u;                // code + 128, 0..255
+            if (KIND == SRC_F16) {
+                put4<KIND>(c, w, 2 * i);
+            } else {
+                const float a = (float)(c & 0xffu), b = (float)((c >> 8) & 0xffu), e = (float)((c >> 16) & 0xffu), h = (float)(c >> 24);
+                w[2 * i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+                w[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(h), __float_as_uint(e), 0x07060302u);
+            }
+        }
+        s = half_of(r.half(34 * f));
+        o = (KIND == SRC_F16 ? 1152.f : 128.f) * s;
+    }
+};
+template <> struct Unit<2> {                                      // Q4_0: blocks of 16 low nibbles, then 16 high ones
+    static constexpr int QK = 32, BS = 18;
+    static constexpr bool HALVES = false;
+    template <class R> __device__ __forceinline__ void open(const R&) {}
+    template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
+        const u2 q = r.pair(18 * f + 2 + 8 * (g & 1));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) put4<KIND>((q[i] >> (g & 2 ? 4 : 0)) & 0x0f0f0f0fu, w, 2 * i);
+        s = half_of(r.half(18 * f));
+        o = (BASE<KIND> + 8.f) * s;
+    }
+};
+
+// a block's bytes where they lie
+struct Bytes {
+    const uint8_t* p;
+    __device__ __forceinline__ uint32_t u8(int k) const { return p[k]; }
+    __device__ __forceinline__ uint32_t u16(int k) const { return u8(k) | (u8(k + 1) << 8); }
+    __device__ __forceinline__ uint32_t u32(int k) const { return u16(k) | (u16(k + 2) << 16); }
+    __device__ __forceinline__ float h(int k) const { return f16_to_f32(u16(k)); }
+};
+// an output's sum term by term: infinite inputs make code and offset sums that cancel to NaN, where the sum over
+// the weights may be infinite (or, with inputs near the largest number, finite)
+template <int T>
+struct Direct {
+    const FewArgs& a;
+    __device__ __forceinline__ float operator()(int s, int m, int n) const {
+        const Few& f = a.f;
+        const uint8_t* w = (s ? f.w1 : f.w0) + (int64_t)n * a.rowbytes;
+        const uint16_t* x = a.rows + (int64_t)m * f.ldx;
+        float sum = 0.f;
+        for (int k = 0; k < f.k; k += 4) {
+            float v[4];
+            const int b = k / Unit<T>::QK;
+            dq4<T>(Bytes{w + (int64_t)b * Unit<T>::BS}, k - b * Unit<T>::QK, DQ{nullptr}, nullptr, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = fmaf(wide(x[k + i], f.kind), v[i], sum);
+        }
+        return sum;
+    }
+};
+
+typedef const __attribute__((address_space(1))) void* gptr;
+typedef __attribute__((address_space(3))) void* lptr;
+
+// The inputs as the matrix instruction takes them: for each step of 32 k and each tile a run of 64 lanes x 8
+// numbers, one contiguous load of a wave. Rows of 4096 numbers lie 8 KB apart, all in the same
+// channel of the L2: sixteen of them fetched side by side took Q8_0 12288 x 4096 with 32 rows 55 us.
+template <bool HALVES>
+__global__ __launch_bounds__(256) void k_fragments(const uint16_t* __restrict__ x, int64_t ldx, int m, int k, uint16_t* __restrict__ out,
+                                                   int tiles) {
+    const int i = blockIdx.x * 256 + threadIdx.x, lane = i & 63, tile = (i >> 6) % tiles, step = (i >> 6) / tiles;
+    if (step * 32 >= k) return;
+    const int row = lane & 15, g = lane >> 4, r = HALVES ? 8 * tile + (row & 7) : 16 * tile + row;
+    u4 v = {0, 0, 0, 0};
+    if (r < m && (!HALVES || (row < 8) == (g < 2))) v = *reinterpret_cast<const u4*>(x + (int64_t)r * ldx + step * 32 + 8 * g);
+    reinterpret_cast<u4*>(out)[i] = v;
+}
+
+// ONE: a single input row, read as it lies. AL: every unit of a row begins at a 16-byte address.
+template <int T, int KIND, int MT, bool ONE, bool TWO, bool AL, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void k_codes(const FewArgs a) {
+    typedef Unit<T> U;
+    constexpr int STEPS = UNIT / 32, MR = ONE ? 1 : 4, AHEAD = MT == 1 ? 8 : (MT == 2 ? 4 : (MT == 4 ? 2 : 1));
+    // 16-byte words of a row's unit, wherever in the first of them it begins
+    constexpr int BYTES = UNIT / U::QK * U::BS, WORDS = AL ? BYTES / 16 : (BYTES + 15 + 15) / 16, LOADS = (16 * WORDS + 63) / 64;
+    constexpr int STAGE = WORDS * 256 + 16, RED = WAVES * (1 + TWO) * MT * 1024, ALL = WAVES * (1 + TWO) * STAGE;
+    static_assert(!AL || BYTES % 16 == 0, "units keep the rows' alignment");
+    __shared__ __align__(16) uint8_t mem[ALL > RED ? ALL : RED];
+    const Few& f = a.f;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+    const int row = lane & 15, g = lane >> 4;
+    uint8_t* stage = mem + wave * (1 + TWO) * STAGE;
+    // word lane of load i: word c of row r, from the row's first byte on
+    uint32_t from[LOADS];
+    bool mine[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int word = i * 64 + lane, r = tmin(word / WORDS, 15), c = word % WORDS;
+        from[i] = (uint32_t)(tmin(n0 + r, f.n - 1) - n0) * (uint32_t)a.rowbytes + 16 * c;
+        mine[i] = word < 16 * WORDS;
+    }
+    // all words of these rows lie inside the matrix, with those that reach past a unit's end
+    const int64_t first = (int64_t)n0 * a.rowbytes, last = (int64_t)tmin(n0 + 16, f.n) * a.rowbytes;
+    const bool inside = AL || (first >= 16 && last + 32 <= f.wbytes);
+    const uint32_t wrow = (uint32_t)(tmin(n0 + row, f.n - 1) - n0) * (uint32_t)a.rowbytes;
+    const bool live = U::HALVES ? row == (g < 2 ? 0 : 8) : row == 0;
+    const uint16_t* xrow = f.x + 8 * g;
+    f4 acc[1 + TWO][MT];
+#pragma unroll
+    for (int s = 0; s <= TWO; ++s)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[s][j] = f4{0, 0, 0, 0};
+    constexpr uint32_t UNITY = KIND == SRC_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    const u4 ones = {UNITY, UNITY, UNITY, UNITY};
+    const f4 zero = {0, 0, 0, 0};
+    const int units = (f.k + UNIT - 1) / UNIT;
+    for (int u = wave; u < units; u += WAVES) {
+        const int have = U::QK == UNIT ? STEPS : tmin(STEPS, (f.k - u * UNIT) / 32);
+        const int64_t at = first + (int64_t)u * BYTES;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the unit before has been read
+#pragma unroll
+        for (int h = 0; h <= TWO; ++h) {
+            const uint8_t* w = h ? f.w1 : f.w0;
+            uint8_t* d = stage + h * STAGE;
+            if (inside && have == STEPS) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const uint8_t* p = w + at + from[i];
+                    if (!AL) p -= (reinterpret_cast<uintptr_t>(p) & 15);
+                    if (mine[i]) __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(d + i * 1024), 16, 0, 0);
+                }
+            } else {                                              // the matrix's own bytes only
+#pragma unroll 1
+                for (int i = lane; i < 16 * WORDS; i += 64) {
+                    const int r = tmin(n0 + i / WORDS, f.n - 1) - n0;
+                    const uint8_t* p = w + at + (int64_t)r * a.rowbytes;
+                    p = p - (reinterpret_cast<uintptr_t>(p) & 15) + 16 * (i % WORDS);
+                    if (p >= w && p + 16 <= w + f.wbytes) {
+                        *reinterpret_cast<u4*>(d + i * 16) = *reinterpret_cast<const u4*>(p);
+                        continue;
+                    }
+#pragma unroll 1
+                    for (int k = 0; k < 16; ++k)
+                        if (p + k >= w && p + k < w + f.wbytes) d[i * 16 + k] = p[k];
+                }
+            }
+        }
+        u4 x0[STEPS];                                             // one tile: all of its unit's inputs on the way too
+        if constexpr (MT == 1) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int k = u * UNIT + 32 * s;
+                if (ONE) x0[s] = live && s < have ? *reinterpret_cast<const u4*>(xrow + k) : u4{0, 0, 0, 0};
+                else if (s < have) x0[s] = reinterpret_cast<const u4*>(f.x)[2 * k + lane];
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        U q[1 + TWO];
+        Row<AL> rows[1 + TWO];
+#pragma unroll
+        for (int h = 0; h <= TWO; ++h) {
+            rows[h].set(stage + h * STAGE + row * WORDS * 16, (uint32_t)(reinterpret_cast<uintptr_t>((h ? f.w1 : f.w0) + at + wrow) & 15));
+            q[h].open(rows[h]);
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if (s >= have) break;
+            f4 sx[MT];
+            u4 x[MT];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                if constexpr (MT == 1) x[j] = x0[s];
+                else x[j] = reinterpret_cast<const u4*>(f.x)[((u * STEPS + s) * MT + j) * 64 + lane];
+                sx[j] = mul16<KIND>(x[j], ones, zero);
+            }
+#pragma unroll
+            for (int h = 0; h <= TWO; ++h) {
+                u4 w;
+                float sc, off;
+                q[h].template step<KIND>(rows[h], s, g, w, sc, off);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const f4 p = mul16<KIND>(x[j], w, zero);
+#pragma unroll
+                    for (int c = 0; c < MR; ++c) acc[h][j][c] = fmaf(sc, p[c], fmaf(-off, sx[j][c], acc[h][j][c]));
+                }
+            }
+            // no more of x ahead of its use than the registers hold
+            if ((s + 1) % AHEAD == 0) asm volatile("" ::: "memory");
+        }
+    }
+    finish<WAVES, MT, TWO, U::HALVES>(f, n0, reinterpret_cast<float*>(mem), acc, Direct<T>{a});
+}
+
+template <int T, int KIND, bool TWO, bool AL>
+int launch(const FewArgs& a, hipStream_t st) {
+    constexpr int HIGH = Unit<T>::HALVES ? 8 : 16;
+    const dim3 grid((unsigned)((a.f.n + 15) / 16));
+    const int tiles = few_tiles(T, a.f.m);
+    // few weight rows fill the device with waves only if more of them share a row's k
+    const bool many = TWO || a.f.n >= 8192;
+    constexpr int MOST = TWO ? 8 : 16;
+#define SPA_CODES(MT, ONE, W) hipLaunchKernelGGL((k_codes<T, KIND, MT, ONE, TWO, AL, W>), grid, dim3(W * 64), 0, st, a)
+    if (a.f.m == 1) {
+        if (many) SPA_CODES(1, true, 8);
+        else SPA_CODES(1, true, MOST);
+    } else if (tiles == 1) {
+        if (many) SPA_CODES(1, false, 8);
+        else SPA_CODES(1, false, MOST);
+    } else if (tiles == 2) {
+        SPA_CODES(2, false, 8);
+    } else if (tiles == 4) {
+        SPA_CODES(4, false, 8);
+    } else if constexpr (HIGH == 8) {
+        SPA_CODES(8, false, 8);
+    }
+#undef SPA_CODES
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+template <int T, int KIND, bool TWO>
+int aligned(const FewArgs& a, hipStream_t st) {
+    if constexpr (UNIT / Unit<T>::QK * Unit<T>::BS % 16 == 0) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(a.f.w0) | reinterpret_cast<uintptr_t>(a.f.w1) | (uintptr_t)a.rowbytes;
+        if ((at & 15) == 0) return launch<T, KIND, TWO, true>(a, st);
+    }
+    return launch<T, KIND, TWO, false>(a, st);
+}
+
+template <int T>
+int pick(const Few& f, uint16_t* frags, hipStream_t st) {
+    FewArgs a{f, (int64_t)f.k / Unit<T>::QK * Unit<T>::BS, f.x};
+    if (f.m > 1) {
+        const int tiles = few_tiles(T, f.m), lanes = tiles * (f.k / 32) * 64;
+        hipLaunchKernelGGL((k_fragments<Unit<T>::HALVES>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, f.x, f.ldx, f.m, f.k,
+                           frags, tiles);
+        SPA_HIP_TRY(hipGetLastError());
+        a.f.x = frags;
+    }
+    if (f.w1) return f.kind == SRC_BF16 ? aligned<T, SRC_BF16, true>(a, st) : aligned<T, SRC_F16, true>(a, st);
+    return f.kind == SRC_BF16 ? aligned<T, SRC_BF16, false>(a, st) : aligned<T, SRC_F16, false>(a, st);
+}
+
+}  // namespace
+
+int few_codes(const Few& f, uint16_t* frags, hipStream_t st) {
+    static_assert(FEW_ROWS == 64, "tiles of up to 64 rows");
+    switch (f.type) {
+        case 2: return pick<2>(f, frags, st);
+        case 8: return pick<8>(f, frags, st);
+        case 12: return pick<12>(f, frags, st);
+        case 13: return pick<13>(f, frags, st);
+        default: return pick<14>(f, frags, st);
+    }
+}
+
+}  // namespace lin
+}  // namespace spa

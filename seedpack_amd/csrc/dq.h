@@ -46,27 +46,36 @@ struct DQ {
 
 // outputs e..e+3 of a block (e a multiple of 4; every type's runs of equal header fields hold a
 // multiple of 4 weights), each by the C code's expression for that element
-template <int T>
-__device__ __forceinline__ void dq4(const Blk& b, int e, const DQ& t, const int8_t* kv, float (&v)[4]);
+template <int T> struct Decode;
+template <int T, class B>
+__device__ __forceinline__ void dq4(const B& b, int e, const DQ& t, const int8_t* kv, float (&v)[4]) {
+    Decode<T>::four(b, e, t, kv, v);
+}
 
-template <> __device__ __forceinline__ void dq4<8>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {     // Q8_0 (:553-567)
+template <> struct Decode<8> {     // Q8_0 (:553-567)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const float d = b.h(0);
     const uint32_t w = b.u32(2 + e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> (8 * i)) * d;
 }
-template <> __device__ __forceinline__ void dq4<2>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {     // Q4_0 (:459-477)
+};
+template <> struct Decode<2> {     // Q4_0 (:459-477)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const float d = b.h(0);
     const uint32_t w = b.u32(2 + (e & 15)) >> (e < 16 ? 0 : 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)((int)((w >> (8 * i)) & 0xF) - 8) * d;
 }
-template <> __device__ __forceinline__ void dq4<3>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {     // Q4_1 (:479-498)
+};
+template <> struct Decode<3> {     // Q4_1 (:479-498)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const float d = b.h(0), m = b.h(2);
     const uint32_t w = b.u32(4 + (e & 15)) >> (e < 16 ? 0 : 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)(int)((w >> (8 * i)) & 0xF) * d + m;
 }
+};
 // Q5_0 / Q5_1: the fifth bit of element e (j = e mod 16) is qh bit j (e < 16) or bit j + 16
 __device__ __forceinline__ uint32_t q5_code(uint32_t w, uint32_t qh, int e, int i) {
     const int j = (e & 15) + i;
@@ -74,25 +83,32 @@ __device__ __forceinline__ uint32_t q5_code(uint32_t w, uint32_t qh, int e, int 
     const uint32_t lo = e < 16 ? ((w >> (8 * i)) & 0x0F) : ((w >> (8 * i + 4)) & 0x0F);
     return lo | xh;
 }
-template <> __device__ __forceinline__ void dq4<6>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {     // Q5_0 (:500-524)
+template <> struct Decode<6> {     // Q5_0 (:500-524)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const float d = b.h(0);
     const uint32_t qh = b.u32(2), w = b.u32(6 + (e & 15));
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)((int)q5_code(w, qh, e, i) - 16) * d;
 }
-template <> __device__ __forceinline__ void dq4<7>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {     // Q5_1 (:526-551)
+};
+template <> struct Decode<7> {     // Q5_1 (:526-551)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const float d = b.h(0), m = b.h(2);
     const uint32_t qh = b.u32(4), w = b.u32(8 + (e & 15));
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)(int)q5_code(w, qh, e, i) * d + m;
 }
-template <> __device__ __forceinline__ void dq4<42>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {    // Q2_0 (:439-457)
+};
+template <> struct Decode<42> {    // Q2_0 (:439-457)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const float d = b.h(0);
     const uint32_t w = b.u8(2 + e / 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)((int)((w >> (2 * i)) & 3) - 1) * d;
 }
-template <> __device__ __forceinline__ void dq4<10>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {    // Q2_K (:961-990)
+};
+template <> struct Decode<10> {    // Q2_K (:961-990)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const int n = e >> 7, r = e & 127, j = r >> 5, part = (r >> 4) & 1, l = r & 15;
     const uint32_t sc = b.u8(n * 8 + 2 * j + part);
     const float dl = b.h(80) * (float)(int)(sc & 0xF), ml = b.h(82) * (float)(int)(sc >> 4);
@@ -100,7 +116,9 @@ template <> __device__ __forceinline__ void dq4<10>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = dl * (float)(int)((w >> (8 * i)) & 3) - ml;
 }
-template <> __device__ __forceinline__ void dq4<11>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {    // Q3_K (:1306-1345)
+};
+template <> struct Decode<11> {    // Q3_K (:1306-1345)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const int n = e >> 7, r = e & 127, j = r >> 5, part = (r >> 4) & 1, l = r & 15;
     const int is = n * 8 + 2 * j + part;
     const uint32_t lo = is < 8 ? (b.u8(96 + is) & 0xF) : (b.u8(96 + is - 8) >> 4);
@@ -114,7 +132,9 @@ template <> __device__ __forceinline__ void dq4<11>(const Blk& b, int e, const D
         v[i] = dl * (float)(q - (hb ? 0 : 4));
     }
 }
-__device__ __forceinline__ void k4_scale_min(const Blk& b, int j, uint32_t& d, uint32_t& m) {   // get_scale_min_k4 (:880-887), scales at byte 4
+};
+template <class B>
+__device__ __forceinline__ void k4_scale_min(const B& b, int j, uint32_t& d, uint32_t& m) {   // get_scale_min_k4 (:880-887), scales at byte 4
     if (j < 4) {
         d = b.u8(4 + j) & 63;
         m = b.u8(4 + j + 4) & 63;
@@ -123,7 +143,8 @@ __device__ __forceinline__ void k4_scale_min(const Blk& b, int j, uint32_t& d, u
         m = (b.u8(4 + j + 4) >> 4) | ((b.u8(4 + j) >> 6) << 4);
     }
 }
-template <> __device__ __forceinline__ void dq4<12>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {    // Q4_K (:1530-1550)
+template <> struct Decode<12> {    // Q4_K (:1530-1550)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const int c = e >> 6, r = e & 63, l = r & 31;
     uint32_t sc, m;
     k4_scale_min(b, 2 * c + (r >> 5), sc, m);
@@ -132,7 +153,9 @@ template <> __device__ __forceinline__ void dq4<12>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = d1 * (float)(int)((w >> (8 * i)) & 0xF) - m1;
 }
-template <> __device__ __forceinline__ void dq4<13>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {    // Q5_K (:1732-1757)
+};
+template <> struct Decode<13> {    // Q5_K (:1732-1757)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const int c = e >> 6, r = e & 63, l = r & 31;
     uint32_t sc, m;
     k4_scale_min(b, 2 * c + (r >> 5), sc, m);
@@ -145,7 +168,9 @@ template <> __device__ __forceinline__ void dq4<13>(const Blk& b, int e, const D
         v[i] = d1 * (float)q - m1;
     }
 }
-template <> __device__ __forceinline__ void dq4<14>(const Blk& b, int e, const DQ&, const int8_t*, float (&v)[4]) {    // Q6_K (:1940-1968)
+};
+template <> struct Decode<14> {    // Q6_K (:1940-1968)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t*, float (&v)[4]) {
     const int n = e >> 7, r = e & 127, qd = r >> 5, l = r & 31, is = l / 16;
     const uint32_t wl = b.u32(n * 64 + l + (qd & 1) * 32) >> (qd < 2 ? 0 : 4), wh = b.u32(128 + n * 32 + l) >> (2 * qd);
     const int sc = (int8_t)b.u8(192 + n * 8 + is + 2 * qd);
@@ -156,7 +181,9 @@ template <> __device__ __forceinline__ void dq4<14>(const Blk& b, int e, const D
         v[i] = ds * (float)((int)(int8_t)(uint8_t)code - 32);
     }
 }
-template <> __device__ __forceinline__ void dq4<16>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ2_XXS (:2489-2513)
+};
+template <> struct Decode<16> {  // IQ2_XXS (:2489-2513)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t a1 = b.u32(2 + 8 * ib + 4);
     const float db = b.h(0) * (0.5f + (float)(a1 >> 28)) * 0.25f;
@@ -165,7 +192,9 @@ template <> __device__ __forceinline__ void dq4<16>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = db * iq2_val(glev(gw, i)) * sgn(s, j0 + i);
 }
-template <> __device__ __forceinline__ void dq4<17>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ2_XS (:2517-2540)
+};
+template <> struct Decode<17> {  // IQ2_XS (:2517-2540)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t sc = b.u8(66 + ib);
     const float db = b.h(0) * (0.5f + (float)((l < 2 ? sc : sc >> 4) & 0xf)) * 0.25f;
@@ -175,7 +204,9 @@ template <> __device__ __forceinline__ void dq4<17>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = db * iq2_val(glev(gw, i)) * sgn(s, j0 + i);
 }
-template <> __device__ __forceinline__ void dq4<22>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ2_S (:2544-2572)
+};
+template <> struct Decode<22> {  // IQ2_S (:2544-2572)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t sc = b.u8(74 + ib);
     const float dl = b.h(0) * (0.5f + (float)((l < 2 ? sc : sc >> 4) & 0xf)) * 0.25f;
@@ -185,7 +216,9 @@ template <> __device__ __forceinline__ void dq4<22>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = dl * iq2_val(glev(gw, i)) * sgn(s, j0 + i);
 }
-template <> __device__ __forceinline__ void dq4<18>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ3_XXS (:2576-2604)
+};
+template <> struct Decode<18> {  // IQ3_XXS (:2576-2604)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t a = b.u32(2 + 64 + 4 * ib);
     const float db = b.h(0) * (0.5f + (float)(a >> 28)) * 0.5f;
@@ -194,7 +227,9 @@ template <> __device__ __forceinline__ void dq4<18>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = db * iq3xxs_val(glev(gw, i)) * sgn(s, j0 + i);
 }
-template <> __device__ __forceinline__ void dq4<21>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ3_S (:2608-2647)
+};
+template <> struct Decode<21> {  // IQ3_S (:2608-2647)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t sc = b.u8(106 + ib / 2);
     const float db = b.h(0) * (float)(1 + 2 * (int)((ib & 1) ? (sc >> 4) : (sc & 0xf)));
@@ -206,7 +241,9 @@ template <> __device__ __forceinline__ void dq4<21>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = db * (float)(2 * glev(gw, i) + 1) * sgn(s, j0 + i);
 }
-template <> __device__ __forceinline__ void dq4<19>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ1_S (:2651-2674)
+};
+template <> struct Decode<19> {  // IQ1_S (:2651-2674)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t qh = b.u16(34 + 2 * ib);
     const float dl = b.h(0) * (float)(2 * (int)((qh >> 12) & 7) + 1);
@@ -215,7 +252,9 @@ template <> __device__ __forceinline__ void dq4<19>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = dl * ((float)(glev(gw, i) - 1) + delta);
 }
-template <> __device__ __forceinline__ void dq4<29>(const Blk& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {  // IQ1_M (:2676-2724)
+};
+template <> struct Decode<29> {  // IQ1_M (:2676-2724)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ& t, const int8_t*, float (&v)[4]) {
     const int ib = e >> 5, l = (e >> 3) & 3, j0 = e & 7;
     const uint32_t s0 = b.u16(48), s1 = b.u16(50), s2 = b.u16(52), s3 = b.u16(54);
     const uint32_t sf = (s0 >> 12) | ((s1 >> 8) & 0x00f0) | ((s2 >> 4) & 0x0f00) | (s3 & 0xf000);
@@ -230,13 +269,17 @@ template <> __device__ __forceinline__ void dq4<29>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = dl * ((float)(glev(gw, i) - 1) + delta);
 }
-template <> __device__ __forceinline__ void dq4<20>(const Blk& b, int e, const DQ&, const int8_t* kv, float (&v)[4]) {  // IQ4_NL (:2726-2742)
+};
+template <> struct Decode<20> {  // IQ4_NL (:2726-2742)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t* kv, float (&v)[4]) {
     const float d = b.h(0);
     const uint32_t w = b.u32(2 + (e & 15)) >> (e < 16 ? 0 : 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = d * (float)kv[(w >> (8 * i)) & 0xf];
 }
-template <> __device__ __forceinline__ void dq4<23>(const Blk& b, int e, const DQ&, const int8_t* kv, float (&v)[4]) {  // IQ4_XS (:2744-2764)
+};
+template <> struct Decode<23> {  // IQ4_XS (:2744-2764)
+template <class B> static __device__ __forceinline__ void four(const B& b, int e, const DQ&, const int8_t* kv, float (&v)[4]) {
     const int ib = e >> 5, r = e & 31;
     const int ls = (int)(((b.u8(4 + ib / 2) >> (4 * (ib % 2))) & 0xf) | (((b.u16(2) >> (2 * ib)) & 3) << 4));
     const float dl = b.h(0) * (float)(ls - 32);
@@ -244,6 +287,7 @@ template <> __device__ __forceinline__ void dq4<23>(const Blk& b, int e, const D
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = dl * (float)kv[(w >> (8 * i)) & 0xf];
 }
+};
 
 }  // namespace
 }  // namespace spa

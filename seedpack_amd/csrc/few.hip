@@ -2,22 +2,14 @@
 // the weights' bytes are the floor. A workgroup of 8 waves computes 16 weight rows (16 of each matrix in the
 // gated form) for all input rows; the waves share k and join their sums in LDS, in the order of the waves.
 #include "../../include/seedpack_amd.h"
-#include "dq.h"
+#include "few.h"
 #include "launch.h"
-#include "linear.h"
 
 namespace spa {
 namespace lin {
 namespace {
 
 constexpr int WAVES = 8, KC = 1024, KW = KC / WAVES;          // k of a chunk, and each wave's part of it
-
-struct FewArgs {
-    Few f;
-    int64_t rowbytes;
-};
-
-__device__ __forceinline__ f4 mul_bf(bf8 a, bf8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // the input rows' fragments of one step of 32 k: row lane & 15 of tile j, k0 + 8 (lane / 16) ..
 template <int MT>
@@ -62,56 +54,9 @@ __device__ __forceinline__ void step(const u4 (&x)[MT], const float (&v)[8], f4 
     }
 }
 
-// joins the waves' sums and writes the outputs: red holds [wave][matrix][tile][16 m][16 n]
-template <int MT, bool TWO>
-__device__ __forceinline__ void finish(const Few& f, int n0, float* red, f4 (&acc)[1 + TWO][MT]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s <= TWO; ++s)
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                red[((wave * (1 + TWO) + s) * MT + j) * 256 + (4 * (lane >> 4) + c) * 16 + (lane & 15)] = acc[s][j][c];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += WAVES * 64) {
-        const int m = i >> 4, n = n0 + (i & 15);
-        if (m >= f.m || n >= f.n) continue;
-        float v = 0.f, u = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            v += red[w * (1 + TWO) * MT * 256 + i];
-            if (TWO) u += red[(w * 2 + 1) * MT * 256 + i];
-        }
-        if (TWO) {
-            v = act_value(v, f.act) * u;
-        } else if (f.ex.low) {
-            const Expand& ex = f.ex;
-            const int a = ex.which[m];
-            if (a >= 0 && a < ex.pool) {
-                const float* z = ex.low + (int64_t)m * ex.rp;
-                const uint16_t* b = ex.b + ((int64_t)a * f.n + n) * ex.rank;
-                float t = 0.f;
-                int r = 0;
-                if (ex.wide_b) {
-                    for (; r < ex.rank; r += 8) {
-                        const u4 h = *reinterpret_cast<const u4*>(b + r);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            t = fmaf(z[r + 2 * c], wide(h[c] & 0xffffu, ex.kind), t);
-                            t = fmaf(z[r + 2 * c + 1], wide(h[c] >> 16, ex.kind), t);
-                        }
-                    }
-                } else {
-                    for (; r < ex.rank; ++r) t = fmaf(z[r], wide(b[r], ex.kind), t);
-                }
-                v += t;
-            }
-        }
-        f.y[(int64_t)m * f.ldy + n] = narrow(v, f.kind);
-    }
-}
+struct Never {                                                   // sums that are not numbers stay so
+    __device__ __forceinline__ float operator()(int, int, int) const { return __builtin_nanf(""); }
+};
 
 // Block types: a chunk of 1024 k of the 16 rows is copied to LDS as it lies (whole 16-byte words around each
 // row's bytes), and each lane decodes 8 weights of its row in a step.
@@ -177,47 +122,54 @@ __global__ __launch_bounds__(WAVES * 64) void k_few(const FewArgs a, DQ t) {
             }
         }
     }
-    finish<MT, TWO>(f, n0, reinterpret_cast<float*>(mem), acc);
+    finish<WAVES, MT, TWO, false>(f, n0, reinterpret_cast<float*>(mem), acc, Never());
 }
 
-// 16-bit weights (rows of a multiple of 32 k, 16-byte aligned): fragments straight from memory
+// 16-bit weights (rows of a multiple of 32 k, 16-byte aligned): fragments straight from memory, the loads of
+// four steps under way at once
 template <int WKIND, int KIND, int MT, bool TWO>
 __global__ __launch_bounds__(WAVES * 64) void k_few16(const FewArgs a) {
     const Few& f = a.f;
     __shared__ float red[WAVES * (1 + TWO) * MT * 256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16;
+    constexpr int U = MT > 2 ? 2 : 4, STEP = WAVES * 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
     const int64_t wrow = (int64_t)tmin(n0 + (lane & 15), f.n - 1) * a.rowbytes + 16 * (lane >> 4);
     f4 acc[1 + TWO][MT];
 #pragma unroll
     for (int s = 0; s <= TWO; ++s)
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[s][j] = f4{0, 0, 0, 0};
-    for (int k = wave * 32; k < f.k; k += WAVES * 32) {
-        u4 x[MT];
-        load_x<MT>(f, k, x);
+    for (int k0 = wave * 32; k0 < f.k; k0 += U * STEP) {
+        u4 x[U][MT], w[U][1 + TWO];
 #pragma unroll
-        for (int h = 0; h <= TWO; ++h) {
-            const u4 w = *reinterpret_cast<const u4*>((h ? f.w1 : f.w0) + wrow + 2 * k);
-            if (WKIND == KIND) {
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * STEP;
+            if (k >= f.k) break;
+            load_x<MT>(f, k, x[u]);
 #pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    if (KIND == SRC_BF16)
-                        acc[h][j] = mul_bf(__builtin_bit_cast(bf8, x[j]), __builtin_bit_cast(bf8, w), acc[h][j]);
-                    else
-                        acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, x[j]), __builtin_bit_cast(hf8, w), acc[h][j], 0, 0, 0);
+            for (int h = 0; h <= TWO; ++h) w[u][h] = *reinterpret_cast<const u4*>((h ? f.w1 : f.w0) + wrow + 2 * k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * STEP >= f.k) break;
+#pragma unroll
+            for (int h = 0; h <= TWO; ++h) {
+                if (WKIND == KIND) {
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) acc[h][j] = mul16<KIND>(x[u][j], w[u][h], acc[h][j]);
+                } else {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[2 * i] = wide(w[u][h][i] & 0xffffu, WKIND);
+                        v[2 * i + 1] = wide(w[u][h][i] >> 16, WKIND);
+                    }
+                    step<KIND, MT>(x[u], v, acc[h]);
                 }
-            } else {
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = wide(w[i] & 0xffffu, WKIND);
-                    v[2 * i + 1] = wide(w[i] >> 16, WKIND);
-                }
-                step<KIND, MT>(x, v, acc[h]);
             }
         }
     }
-    finish<MT, TWO>(f, n0, red, acc);
+    finish<WAVES, MT, TWO, false>(f, n0, red, acc, Never());
 }
 
 template <int T, int QK, int BS, int KIND, bool TWO>
@@ -245,7 +197,7 @@ int pick(const FewArgs& a, DQ t, hipStream_t st) {
 
 }  // namespace
 
-int few(const Few& f, hipStream_t st) {
+int few(const Few& f, uint16_t* frags, hipStream_t st) {
     DQ t{nullptr};
     const int ti = iq_table_index(f.type);
     if (ti >= 0) {
@@ -254,15 +206,16 @@ int few(const Few& f, hipStream_t st) {
         if (rc) return rc;
         t.grid = tab.grid;
     }
-    FewArgs a{f, 0};
+    if (coded(f.type)) return few_codes(f, frags, st);
+    FewArgs a{f, 0, f.x};
     switch (f.type) {
 #define SPA_FEW(T, QK, BS)                                 \
     case T:                                                \
         a.rowbytes = (int64_t)f.k / QK * BS;               \
         return pick<T, QK, BS>(a, t, st);
         SPA_FEW(1, 1, 2) SPA_FEW(30, 1, 2)
-        SPA_FEW(2, 32, 18) SPA_FEW(3, 32, 20) SPA_FEW(6, 32, 22) SPA_FEW(7, 32, 24) SPA_FEW(8, 32, 34)
-        SPA_FEW(10, 256, 84) SPA_FEW(11, 256, 110) SPA_FEW(12, 256, 144) SPA_FEW(13, 256, 176) SPA_FEW(14, 256, 210)
+        SPA_FEW(3, 32, 20) SPA_FEW(6, 32, 22) SPA_FEW(7, 32, 24)
+        SPA_FEW(10, 256, 84) SPA_FEW(11, 256, 110)
         SPA_FEW(16, 256, 66) SPA_FEW(17, 256, 74) SPA_FEW(18, 256, 98) SPA_FEW(19, 256, 50) SPA_FEW(20, 32, 18)
         SPA_FEW(21, 256, 110) SPA_FEW(22, 256, 82) SPA_FEW(23, 256, 136) SPA_FEW(29, 256, 56) SPA_FEW(42, 64, 18)
 #undef SPA_FEW

@@ -120,25 +120,35 @@ struct Few {
     int act;
 };
 constexpr int FEW_ROWS = 64;
-int few(const Few& f, hipStream_t st);
+// frags: scratch of few_fragments numbers
+int few(const Few& f, uint16_t* frags, hipStream_t st);
+// types whose codes go to the matrix unit as they are (codes.hip)
+inline bool coded(int type) { return type == 2 || type == 8 || type == 12 || type == 13 || type == 14; }
+int few_codes(const Few& f, uint16_t* frags, hipStream_t st);
+// tiles of input rows: 16 rows each, or 8 (Q6_K), a power of two of them
+inline int few_tiles(int type, int64_t m) {
+    int t = 1;
+    while (t * (type == 14 ? 8 : 16) < m) t *= 2;
+    return t;
+}
+inline int64_t few_fragments(int type, int64_t m, int64_t kp) { return coded(type) && m > 1 ? few_tiles(type, m) * 16 * kp : 0; }
 
 // ---- rows (rows.hip)
 // rows of a 16-bit matrix copied into rows of kp (a multiple of 64), zeros beyond k
 int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, hipStream_t st);
-// the same into binary16 with a power of two taken out of each row (e), optionally the row's 2-norm as it
-// was, and top[0], top[1]: the largest norm (as bits) and power (plus 1024) of any row, raised in place
+// the same into binary16 with a power of two taken out of each row (e), and the row's 2-norm as it was (or null)
 int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e,
-              float* norm, uint32_t* top, hipStream_t st);
+              float* norm, hipStream_t st);
 // the same from a block type
-int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, uint32_t* top,
+int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, float* norm,
                 hipStream_t st);
 // dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (even)
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
                 hipStream_t st);
-// the power of two to take out of each row of the gated block's inner gradients
-int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const uint32_t* top,
-                   int32_t* e, hipStream_t st);
-int zero_words(uint32_t* p, int n, hipStream_t st);
+// the power of two to take out of each row of the gated block's inner gradients, by the 2-norms of the inputs'
+// rows and of both matrices' rows; top: 8 bytes of scratch
+int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const float* n0,
+                   const int32_t* e0, const float* n1, const int32_t* e1, void* top, int32_t* e, hipStream_t st);
 int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st);
 // low[m][rp] = scale[a] x[m] A_a^T, a = which[m]
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,

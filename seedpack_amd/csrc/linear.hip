@@ -56,8 +56,7 @@ struct Operands {
     int64_t ldx = 0, ldw = 0;
     int half = 0;
     int32_t *xe = nullptr, *we0 = nullptr, *we1 = nullptr;
-    float* norm = nullptr;
-    uint32_t* top = nullptr;
+    float *norm = nullptr, *n0 = nullptr, *n1 = nullptr;
 };
 
 // Inputs and weights brought into the form of the many-rows product. Where both are of one 16-bit type they
@@ -97,10 +96,10 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
     o.xe = wk.take<int32_t>(m);
     if (bounds) {
         o.norm = wk.take<float>(m);
-        o.top = wk.take<uint32_t>(2);
+        o.n0 = wk.take<float>(n);
+        o.n1 = wk.take<float>(n);
     }
-    if (run && o.top && (rc = zero_words(o.top, 2, st))) return rc;
-    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, o.xe, o.norm, nullptr, st))) return rc;
+    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, o.xe, o.norm, st))) return rc;
     o.x = xp;
     o.ldx = o.ldw = kp;
     for (int i = 0; i < (w1 ? 2 : 1); ++i) {
@@ -108,8 +107,8 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
         int32_t* e = wk.take<int32_t>(n);
         const void* w = i ? w1 : w0;
         if (run) {
-            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, e, nullptr, o.top, st)
-                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, e, o.top, st);
+            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, e, i ? o.n1 : o.n0, st)
+                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, e, i ? o.n1 : o.n0, st);
             if (rc) return rc;
         }
         (i ? o.w1 : o.w0) = p;
@@ -121,8 +120,9 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
 // Few rows: the weights as they lie. Rows are padded where a 16-byte load of x (or of 16-bit weights) or
 // a step of 32 k would not fit; for 16-bit weights that are copied too.
 int few_operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64_t n, int64_t k, const void* x, int64_t m,
-                 int64_t ldx, Few& f, hipStream_t st) {
+                 int64_t ldx, Few& f, uint16_t*& frags, hipStream_t st) {
     const int64_t kp = (k + 31) / 32 * 32;
+    frags = wk.take<uint16_t>(few_fragments(type, m, kp));
     uint16_t* xp = wk.take<uint16_t>(m * kp);
     int rc;
     f.x = (const uint16_t*)x;
@@ -203,12 +203,13 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
     }
     if (p.m <= FEW_ROWS) {
         Few f{};
-        if ((rc = few_operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.x, p.m, p.ldx, f, st)) || !run) return rc;
+        uint16_t* frags;
+        if ((rc = few_operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.x, p.m, p.ldx, f, frags, st)) || !run) return rc;
         f.kind = p.kind;
         f.y = (uint16_t*)p.y;
         f.ldy = p.ldy;
         f.ex = ex;
-        return few(f, st);
+        return few(f, frags, st);
     }
     Operands o;
     if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st)) || !run) return rc;
@@ -242,12 +243,13 @@ int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
     const void* up = run ? p.up : SOME;
     if (p.m <= FEW_ROWS) {
         Few f{};
-        if ((rc = few_operands(wk, run, p.type, p.gate, up, p.n, p.k, p.x, p.m, p.ldx, f, st)) || !run) return rc;
+        uint16_t* frags;
+        if ((rc = few_operands(wk, run, p.type, p.gate, up, p.n, p.k, p.x, p.m, p.ldx, f, frags, st)) || !run) return rc;
         f.kind = p.kind;
         f.y = (uint16_t*)p.h;
         f.ldy = p.ldh;
         f.act = p.act;
-        return few(f, st);
+        return few(f, frags, st);
     }
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st)) || !run) return rc;
@@ -267,9 +269,10 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, run ? p.up : SOME, p.n, p.k, p.kind, p.x, p.m, p.ldx, true, o, st))) return rc;
     uint16_t* grad = wk.take<uint16_t>(p.m * 2 * np);
-    int32_t* ge = o.xe ? wk.take<int32_t>(p.m) : nullptr;
+    int32_t* ge = o.norm ? wk.take<int32_t>(p.m) : nullptr;
+    void* top = wk.take<uint8_t>(8);
     if (run) {
-        if (ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.top, ge, st))) return rc;
+        if (ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.n0, o.we0, o.n1, o.we1, top, ge, st))) return rc;
         Gemm g = gemm_of(o, p.m, p.n, p.k);
         g.kind = p.kind;
         g.act = p.act;

@@ -56,14 +56,9 @@ __device__ __forceinline__ int exponent_for(float top) {
     frexpf(top, &e);
     return e - 15;
 }
-__device__ __forceinline__ void raise(uint32_t* top, float norm, int e) {
-    atomicMax(top, __float_as_uint(norm));                        // both are never negative: their order is the integers'
-    atomicMax(top + 1, (uint32_t)(e + 1024));
-}
-
 __global__ __launch_bounds__(256) void k_half_rows(const uint16_t* __restrict__ src, int kind, int64_t ld, int64_t k,
                                                    uint16_t* __restrict__ dst, int64_t kp, int32_t* __restrict__ e_out,
-                                                   float* __restrict__ norm, uint32_t* __restrict__ top, bool wide8) {
+                                                   float* __restrict__ norm, bool wide8) {
     __shared__ float lds[4];
     const int64_t row = blockIdx.x;
     src += row * ld;
@@ -89,12 +84,9 @@ __global__ __launch_bounds__(256) void k_half_rows(const uint16_t* __restrict__ 
         *reinterpret_cast<u4*>(dst + c) = *reinterpret_cast<u4*>(h);
     }
     if (threadIdx.x == 0) e_out[row] = e;
-    if (norm || top) {
-        const float nm = fminf(ldexpf(sqrtf(reduce256<false>(sum, lds)), e), 3e38f);
-        if (threadIdx.x == 0) {
-            if (norm) norm[row] = nm;
-            if (top) raise(top, nm, e);
-        }
+    if (norm) {
+        sum = reduce256<false>(sum, lds);
+        if (threadIdx.x == 0) norm[row] = fminf(ldexpf(sqrtf(sum), e), 3e38f);
     }
 }
 
@@ -132,7 +124,7 @@ __device__ __forceinline__ float block_bound(const uint8_t* b) {
 constexpr int TILE = 4096;
 template <int T, int QK, int BS>
 __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__ src, int64_t k, uint16_t* __restrict__ dst,
-                                                     int64_t kp, int32_t* __restrict__ e_out, uint32_t* __restrict__ top, DQ t,
+                                                     int64_t kp, int32_t* __restrict__ e_out, float* __restrict__ norm, DQ t,
                                                      int align) {
     constexpr int TB = TILE / QK, TBYTES = TB * BS;
     __shared__ __align__(16) uint8_t tile[TBYTES + 16];
@@ -182,9 +174,9 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     }
     for (int64_t c = k + threadIdx.x; c < kp; c += 256) dst[c] = 0;
     if (threadIdx.x == 0) e_out[row] = e;
-    if (top) {
-        const float nm = fminf(ldexpf(sqrtf(reduce256<false>(sum, lds)), e), 3e38f);
-        if (threadIdx.x == 0) raise(top, nm, e);
+    if (norm) {
+        sum = reduce256<false>(sum, lds);
+        if (threadIdx.x == 0) norm[row] = fminf(ldexpf(sqrtf(sum), e), 3e38f);
     }
 }
 
@@ -213,10 +205,43 @@ __global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ 
     }
 }
 
+// the largest 2-norm and the largest power of two of both matrices' rows
+struct Top {
+    float norm;
+    int32_t e;
+};
+__global__ __launch_bounds__(1024) void k_top(const float* n0, const int32_t* e0, const float* n1, const int32_t* e1, int64_t n, Top* top) {
+    __shared__ float ln[16];
+    __shared__ int le[16];
+    float a = 0.f;
+    int e = INT32_MIN;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        a = fmaxf(a, fmaxf(n0[i], n1[i]));
+        e = tmax(e, tmax(e0[i], e1[i]));
+    }
+#pragma unroll
+    for (int s = 32; s; s >>= 1) {
+        a = fmaxf(a, __shfl_xor(a, s));
+        e = tmax(e, __shfl_xor(e, s));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        ln[threadIdx.x >> 6] = a;
+        le[threadIdx.x >> 6] = e;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) {
+            a = fmaxf(a, ln[w]);
+            e = tmax(e, le[w]);
+        }
+        *top = Top{a, e};
+    }
+}
+
 // |dh u act'(g)| and |dh act(g)| are at most 1.13 |dh| |x_m| |w_n| (Cauchy-Schwarz; |act'| <= 1.13,
 // |act(g)| <= |g|). Their row is multiplied by the weights' powers of two, so the largest of those counts too.
 __global__ __launch_bounds__(256) void k_grad_exponents(const uint16_t* __restrict__ dh, int kind, int64_t ld, int64_t n,
-                                                        const float* __restrict__ xnorm, const uint32_t* __restrict__ top,
+                                                        const float* __restrict__ xnorm, const Top* __restrict__ top,
                                                         int32_t* __restrict__ e) {
     __shared__ float lds[4];
     const int64_t row = blockIdx.x;
@@ -224,7 +249,7 @@ __global__ __launch_bounds__(256) void k_grad_exponents(const uint16_t* __restri
     for (int64_t c = threadIdx.x; c < n; c += 256) most = fmaxf(most, size_of(wide(dh[row * ld + c], kind)));
     most = reduce256<true>(most, lds);
     if (threadIdx.x) return;
-    const float a = xnorm[row], b = __uint_as_float(top[0]);
+    const float a = xnorm[row], b = top->norm;
     if (!(most > 0.f) || !(a > 0.f) || !(b > 0.f)) {
         e[row] = 0;
         return;
@@ -233,22 +258,20 @@ __global__ __launch_bounds__(256) void k_grad_exponents(const uint16_t* __restri
     frexpf(most, &em);
     frexpf(a, &ea);
     frexpf(b, &eb);
-    e[row] = em + ea + eb + 1 + ((int)top[1] - 1024) - 15;
-}
-
-__global__ void k_zero(uint32_t* p, int n) {
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0;
+    e[row] = em + ea + eb + 1 + top->e - 15;
 }
 
 __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * k; i += gridDim.x * 256ll) p[i / k * ld + i % k] = 0;
 }
 
-// low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 rows a workgroup. Each of 8 waves takes every eighth step
-// of 32 k; 64 ranks at a time, so that x is read once for the usual ranks. For each adapter among the 16
-// rows the whole tile is multiplied and its own rows are kept.
+// low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 rows a workgroup and one adapter: gridDim.y workgroups
+// take the adapters among the 16 rows in turn, in rising order, most of them finding none. The whole tile is
+// multiplied by the adapter's matrix and its own rows are kept. Each of 8 waves takes every eighth step of
+// 32 k, two steps at a time so that ten loads are under way; 64 ranks at a time, so that x is read once for
+// the usual ranks.
 constexpr int LOW_WAVES = 8;
-template <int KIND>
+template <int KIND, bool WIDE>
 __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restrict__ x, int64_t ldx, int64_t m, int64_t k,
                                                         const uint16_t* __restrict__ a_all, const float* __restrict__ scale,
                                                         const int32_t* __restrict__ which, int pool, int rank,
@@ -259,53 +282,95 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
     const int row = lane & 15, kc = (lane >> 4) * 8;
     const int mine = m0 + row < m ? which[m0 + row] : -1;
     const uint16_t* xr = x + (m0 + row < m ? m0 + row : m - 1) * ldx;
-    // rows without an adapter: zeros
-    for (int i = threadIdx.x; i < 16 * rp; i += LOW_WAVES * 64) {
-        const int64_t mi = m0 + i / rp;
-        if (mi < m) {
-            const int a = which[mi];
-            if (a < 0 || a >= pool) low[mi * rp + i % rp] = 0.f;
+    if (blockIdx.y == 0) {                                        // rows without an adapter: zeros
+        for (int i = threadIdx.x; i < 16 * rp; i += LOW_WAVES * 64) {
+            const int64_t mi = m0 + i / rp;
+            if (mi < m) {
+                const int a = which[mi];
+                if (a < 0 || a >= pool) low[mi * rp + i % rp] = 0.f;
+            }
         }
     }
     int a = -1;
-    for (;;) {
+    for (unsigned turn = 0;; ++turn) {                            // the same in every lane and wave
         int best = mine > a && mine < pool ? mine : INT32_MAX;
 #pragma unroll
         for (int s = 8; s; s >>= 1) best = tmin(best, __shfl_xor(best, s));
         a = __builtin_amdgcn_readfirstlane(best);
-        if (a == INT32_MAX) break;
-        for (int r0 = 0; r0 < rp; r0 += 64) {
-            f4 acc[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-            for (int64_t k0 = wave * 32; k0 < k; k0 += LOW_WAVES * 32) {
-                __align__(16) uint16_t xv[8], av[8];
-                load8(xr, k0 + kc, k, wide_x, xv);
+        if (a == INT32_MAX) return;
+        if (turn == blockIdx.y) break;
+    }
+    const uint16_t* aa = a_all + (int64_t)a * rank * k;
+    for (int r0 = 0; r0 < rp; r0 += 64) {
+        const int tiles = tmin(4, (rp - r0) / 16);
+        const uint16_t* ar[4];
+        f4 acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = r0 + 16 * j + row;                      // ranks beyond the last take its row: they are not kept
+            ar[j] = aa + (int64_t)(r < rank ? r : rank - 1) * k;
+            acc[j] = f4{0, 0, 0, 0};
+        }
+        auto fetch = [&](int64_t k0, u4& xv, u4 (&av)[4]) {
+            if (WIDE) {                                           // rows of whole steps at 16-byte addresses
+                const bool in = k0 < k;
+                xv = in ? *reinterpret_cast<const u4*>(xr + k0 + kc) : u4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    av[j] = in && j < tiles ? *reinterpret_cast<const u4*>(ar[j] + k0 + kc) : u4{0, 0, 0, 0};
+            } else {
+                __align__(16) uint16_t h[8];
+                load8(xr, k0 + kc, k, wide_x, h);
+                xv = *reinterpret_cast<u4*>(h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = r0 + 16 * j + row;
-                    if (r0 + 16 * j >= rp) break;
-                    // ranks beyond the last take its row: they are not kept
-                    load8(a_all + ((int64_t)a * rank + (r < rank ? r : rank - 1)) * k, k0 + kc, k, wide_a, av);
-                    if (KIND == SRC_BF16)
-                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf8*>(xv), *reinterpret_cast<bf8*>(av), acc[j], 0, 0, 0);
-                    else
-                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<hf8*>(xv), *reinterpret_cast<hf8*>(av), acc[j], 0, 0, 0);
+                    if (j < tiles) load8(ar[j], k0 + kc, k, wide_a, h);
+                    av[j] = *reinterpret_cast<u4*>(h);
                 }
             }
-            __syncthreads();
+        };
+        auto mul = [&](u4 xv, const u4 (&av)[4]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) {
+                if (j >= tiles) break;
+                if (KIND == SRC_BF16)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, xv), __builtin_bit_cast(bf8, av[j]), acc[j], 0, 0, 0);
+                else
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, xv), __builtin_bit_cast(hf8, av[j]), acc[j], 0, 0, 0);
+            }
+        };
+        constexpr int STEP = LOW_WAVES * 32;
+        u4 x0, x1, a0[4], a1[4];
+        fetch(wave * 32, x0, a0);
+        fetch(wave * 32 + STEP, x1, a1);
+        for (int64_t k0 = wave * 32; k0 < k; k0 += 2 * STEP) {
+            u4 x2, x3, a2[4], a3[4];
+            fetch(k0 + 2 * STEP, x2, a2);
+            fetch(k0 + 3 * STEP, x3, a3);
+            mul(x0, a0);
+            mul(x1, a1);
+            x0 = x2;
+            x1 = x3;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) part[wave][j][(4 * (lane >> 4) + c) * 16 + row] = acc[j][c];
-            __syncthreads();
-            for (int i = threadIdx.x; i < 1024; i += LOW_WAVES * 64) {
-                const int j = i >> 8, mr = (i >> 4) & 15, r = r0 + 16 * j + (i & 15);
-                const int64_t mi = m0 + mr;
-                if (mi < m && r < rp && which[mi] == a) {
-                    float v = 0.f;
+            for (int j = 0; j < 4; ++j) {
+                a0[j] = a2[j];
+                a1[j] = a3[j];
+            }
+        }
+        __syncthreads();
 #pragma unroll
-                    for (int w = 0; w < LOW_WAVES; ++w) v += part[w][j][i & 255];
-                    low[mi * rp + r] = r < rank ? scale[a] * v : 0.f;
-                }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) part[wave][j][(4 * (lane >> 4) + c) * 16 + row] = acc[j][c];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 1024; i += LOW_WAVES * 64) {
+            const int j = i >> 8, mr = (i >> 4) & 15, r = r0 + 16 * j + (i & 15);
+            const int64_t mi = m0 + mr;
+            if (mi < m && r < rp && which[mi] == a) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < LOW_WAVES; ++w) v += part[w][j][i & 255];
+                low[mi * rp + r] = r < rank ? scale[a] * v : 0.f;
             }
         }
     }
@@ -324,14 +389,13 @@ int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t
 }
 
 int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e,
-              float* norm, uint32_t* top, hipStream_t st) {
-    hipLaunchKernelGGL(k_half_rows, dim3((unsigned)rows), dim3(256), 0, st, src, kind, ld, k, dst, kp, e, norm, top,
-                       aligned8(src, ld));
+              float* norm, hipStream_t st) {
+    hipLaunchKernelGGL(k_half_rows, dim3((unsigned)rows), dim3(256), 0, st, src, kind, ld, k, dst, kp, e, norm, aligned8(src, ld));
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
-int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, uint32_t* top,
+int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, float* norm,
                 hipStream_t st) {
     DQ t{nullptr};
     const int ti = iq_table_index(type);
@@ -346,7 +410,7 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
     switch (type) {
 #define SPA_BLOCKS(T, QK, BS)                                                                                           \
     case T:                                                                                                             \
-        hipLaunchKernelGGL((k_half_blocks<T, QK, BS>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, e, top, t, align); \
+        hipLaunchKernelGGL((k_half_blocks<T, QK, BS>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, e, norm, t, align); \
         break;
         SPA_BLOCKS(2, 32, 18) SPA_BLOCKS(3, 32, 20) SPA_BLOCKS(6, 32, 22) SPA_BLOCKS(7, 32, 24) SPA_BLOCKS(8, 32, 34)
         SPA_BLOCKS(10, 256, 84) SPA_BLOCKS(11, 256, 110) SPA_BLOCKS(12, 256, 144) SPA_BLOCKS(13, 256, 176) SPA_BLOCKS(14, 256, 210)
@@ -367,15 +431,11 @@ int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uin
     return SPA_OK;
 }
 
-int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const uint32_t* top,
-                   int32_t* e, hipStream_t st) {
-    hipLaunchKernelGGL(k_grad_exponents, dim3((unsigned)rows), dim3(256), 0, st, dh, kind, ld, n, xnorm, top, e);
+int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const float* n0,
+                   const int32_t* e0, const float* n1, const int32_t* e1, void* top, int32_t* e, hipStream_t st) {
+    hipLaunchKernelGGL(k_top, dim3(1), dim3(1024), 0, st, n0, e0, n1, e1, n, (Top*)top);
     SPA_HIP_TRY(hipGetLastError());
-    return SPA_OK;
-}
-
-int zero_words(uint32_t* p, int n, hipStream_t st) {
-    hipLaunchKernelGGL(k_zero, dim3(1), dim3(256), 0, st, p, n);
+    hipLaunchKernelGGL(k_grad_exponents, dim3((unsigned)rows), dim3(256), 0, st, dh, kind, ld, n, xnorm, (const Top*)top, e);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
@@ -389,12 +449,18 @@ int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st) 
 
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
              const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st) {
-    const dim3 grid((unsigned)((m + 15) / 16)), block(LOW_WAVES * 64);
-    const bool wx = aligned8(x, ldx), wa = aligned8(a, k);
-    if (kind == SRC_BF16)
-        hipLaunchKernelGGL((k_low<SRC_BF16>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, wx, wa);
-    else
-        hipLaunchKernelGGL((k_low<SRC_F16>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, wx, wa);
+    const dim3 grid((unsigned)((m + 15) / 16), (unsigned)(pool < 16 ? pool : 16)), block(LOW_WAVES * 64);
+    const bool wx = aligned8(x, ldx), wa = aligned8(a, k), whole = wx && wa && k % 32 == 0;
+#define SPA_LOW(KIND, WIDE) \
+    hipLaunchKernelGGL((k_low<KIND, WIDE>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, wx, wa)
+    if (kind == SRC_BF16) {
+        if (whole) SPA_LOW(SRC_BF16, true);
+        else SPA_LOW(SRC_BF16, false);
+    } else {
+        if (whole) SPA_LOW(SRC_F16, true);
+        else SPA_LOW(SRC_F16, false);
+    }
+#undef SPA_LOW
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }

@@ -53,8 +53,9 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
     __shared__ int wsum[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t tiles = (q.cols + COLS - 1) / COLS;
-    const int64_t c0 = (int64_t)(blockIdx.x % tiles) * COLS + 8 * lane, run = blockIdx.x / tiles;
-    const int e = blockIdx.y;
+    // the experts of one piece of x side by side: its second reader finds it in the caches
+    const int e = (int)(blockIdx.x % q.experts);
+    const int64_t piece = blockIdx.x / q.experts, run = piece / tiles, c0 = piece % tiles * COLS + 8 * lane;
     const int64_t r0 = run * q.run, r1 = tmin(q.rows, r0 + q.run), left = q.cols - c0;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     uint32_t hits = 0;
@@ -99,11 +100,11 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
                 at += __popcll(mask[i]);
             }
             __syncthreads();
-#pragma unroll 4
+#pragma unroll 8
             for (int i = wave; i < total; i += 4)
                 if (left > 0) add8<KIND>(q.x, (b + list[i]) * q.ld + c0, left, q.wide8, s, (float)times[i]);
         }
-        if (blockIdx.x % tiles == 0) {
+        if (piece % tiles == 0) {
 #pragma unroll
             for (int k = 32; k; k >>= 1) hits += __shfl_xor(hits, k);
             __syncthreads();
@@ -143,13 +144,18 @@ __global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
     }
 }
 
-// rows of a run: enough workgroups to fill the device (about 1024 of them), at least 16 rows each
-int64_t run_rows(int64_t rows, int64_t cols, int64_t experts) {
+// Rows of a run. Whole: enough workgroups to fill the device (about 1024 of them), at least 16 rows each. By
+// expert: 512 rows, so that an expert which gets most of the rows is still spread over many workgroups
+// (with runs of 8192 rows the first of 64 unlike experts kept 16384 x 4096 busy for 202 us).
+int64_t run_rows(int64_t rows, int64_t cols, int64_t experts, bool by_expert) {
     const int64_t tiles = (cols + COLS - 1) / COLS * experts;
-    const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
-    int64_t run = (rows + runs - 1) / runs;
-    if (run < 16) run = 16;
-    while ((rows + run - 1) / run > 65535) run *= 2;
+    int64_t run = 512;
+    if (!by_expert) {
+        const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
+        run = (rows + runs - 1) / runs;
+        if (run < 16) run = 16;
+    }
+    while ((rows + run - 1) / run * tiles > (1 << 24)) run *= 2;
     return run;
 }
 uint64_t part_bytes(int64_t runs, int64_t cols, int64_t experts) {
@@ -165,8 +171,9 @@ using namespace spa::lin;
 
 extern "C" uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts) {
     if (rows <= 0 || cols <= 0 || experts < 0) return 0;
-    if (experts == 0) experts = 1;
-    const int64_t run = run_rows(rows, cols, experts), runs = (rows + run - 1) / run;
+    const bool by_expert = experts != 0;
+    if (!by_expert) experts = 1;
+    const int64_t run = run_rows(rows, cols, experts, by_expert), runs = (rows + run - 1) / run;
     return part_bytes(runs, cols, experts) + ((uint64_t)runs * experts * 4 + 255) / 256 * 256;
 }
 
@@ -194,7 +201,7 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     q.which = which;
     q.each = (int)each;
     q.experts = which ? (int)experts : 1;
-    q.run = run_rows(rows, cols, q.experts);
+    q.run = run_rows(rows, cols, q.experts, which != nullptr);
     q.runs = (rows + q.run - 1) / q.run;
     q.part = (float*)work;
     q.hits = (uint32_t*)((uint8_t*)work + part_bytes(q.runs, cols, q.experts));
@@ -204,8 +211,8 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     q.wide8 = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_stride % unit16 == 0;
     hipStream_t st = (hipStream_t)stream;
     const int64_t tiles = (cols + COLS - 1) / COLS;
-    if (tiles * q.runs > INT32_MAX) return fail(SPA_ERR_ARG, "spa_add_squares: %lld x %lld is too large", (long long)rows, (long long)cols);
-    const dim3 grid((unsigned)(tiles * q.runs), (unsigned)q.experts);
+    if (tiles * q.runs * q.experts > INT32_MAX) return fail(SPA_ERR_ARG, "spa_add_squares: %lld x %lld is too large", (long long)rows, (long long)cols);
+    const dim3 grid((unsigned)(tiles * q.runs * q.experts));
     if (src_kind == SPA_SRC_BF16) hipLaunchKernelGGL((k_squares<SRC_BF16>), grid, dim3(256), 0, st, q);
     else if (src_kind == SPA_SRC_F16) hipLaunchKernelGGL((k_squares<SRC_F16>), grid, dim3(256), 0, st, q);
     else hipLaunchKernelGGL((k_squares<SRC_F32>), grid, dim3(256), 0, st, q);

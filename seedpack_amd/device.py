@@ -8,6 +8,7 @@ arrays never reach hipFree, which waits for the whole device.
 import bisect
 import collections
 import ctypes
+import math
 import threading
 
 import numpy as np
@@ -148,8 +149,8 @@ class DeviceArray:
 
     def __init__(self, shape, dtype, ptr=None, owner=None):
         self.dtype = np.dtype(dtype)
-        self.shape = tuple(int(s) for s in (shape if isinstance(shape, (tuple, list)) else (shape,)))
-        self.nbytes = int(np.prod(self.shape, dtype=np.int64)) * self.dtype.itemsize
+        self.shape = tuple(map(int, shape)) if isinstance(shape, (tuple, list)) else (int(shape),)
+        self.nbytes = math.prod(self.shape) * self.dtype.itemsize
         self._alloc = None
         if ptr is None:
             dev_id, n = _device_id(), _Cache.size_class(self.nbytes)
