@@ -3,10 +3,11 @@
 //
 // A workgroup computes TN weight rows x TM input rows. Both operands are contiguous along k, so a tile
 // step of 64 k is TN + TM rows of 128 bytes; they go from HBM / L2 straight to LDS (16-byte
-// global_load_lds) into one of two buffers while the other is multiplied. LDS rows are 128 bytes too,
-// their eight 16-byte chunks stored at chunk ^ (row & 7): a fragment read takes the same chunk of 8
-// consecutive rows in a phase, which the exchange spreads over all banks. The exchange is made on the
-// global side (a lane fetches the chunk that belongs at its place).
+// buffer loads into LDS) into one of two buffers while the other is multiplied. LDS rows are 128 bytes too,
+// their eight 16-byte chunks stored at chunk ^ (row / 2 & 7): a fragment read takes the same chunk of 16
+// consecutive rows in a phase, which then lie in 16 different places of the 256 bytes that LDS serves at once
+// (with row & 7, which repeats after 8 rows, half of the LDS cycles were conflicts). The exchange is made on
+// the global side (a lane fetches the chunk that belongs at its place).
 // Weights are the matrix instruction's first operand: a lane then holds four consecutive n of one input
 // row, which leave as one 8-byte store.
 // For the gated forms half of the TN rows are the gate's and half the same rows of the up projection, so
@@ -15,10 +16,15 @@
 #include "launch.h"
 #include "linear.h"
 
+#include <type_traits>
+
 namespace spa {
 namespace lin {
 namespace {
 
+#ifndef SPA_WM
+#define SPA_WM 4
+#endif
 constexpr int BK = 64;
 
 template <int HALF> struct Op;
@@ -34,7 +40,7 @@ template <> struct Op<SRC_F16> {
 };
 __device__ __forceinline__ f16v mul_bf(bf8 a, bf8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-typedef const __attribute__((address_space(1))) void* gptr;
+typedef __amdgpu_buffer_rsrc_t rsrc;
 typedef __attribute__((address_space(3))) void* lptr;
 
 // the least adapter number above `after` among the tile's rows, or INT32_MAX
@@ -52,14 +58,17 @@ __device__ __forceinline__ int next_adapter(const Expand& ex, int m0, int m, int
 }
 
 template <int HALF, int TN, int TM, int WN, int WM, int OUT>
-__global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
+__device__ __forceinline__ void product(const Gemm& g) {
     constexpr int NW = WN * WM;                              // waves
-    constexpr bool TWO = OUT != OUT_PLAIN;
+    constexpr bool TWO = OUT == OUT_GATED || OUT == OUT_GRAD;
     constexpr int TNE = TWO ? TN / 2 : TN;                   // output columns of the tile
     constexpr int FN = TN / WN / 32, FM = TM / WM / 32;      // 32 x 32 fragments of a wave
     constexpr int LOADS = (TN + TM) / 8 / NW;                // 8 rows by one load of a wave
     static_assert((TN + TM) % (8 * NW) == 0 && (!TWO || FN % 2 == 0), "tile shape");
-    __shared__ __align__(16) uint16_t tile[2][(TN + TM) * BK];
+    // a wave's outputs on their way out: its input rows x its columns, rows 16 bytes apart from a power of two
+    constexpr int ROWS = TM / WM, COLS = TN / WN, PITCH = COLS + 8;
+    constexpr int STAGES = 2 * (TN + TM) * BK, OUTS = NW * ROWS * PITCH;
+    __shared__ __align__(16) uint16_t mem[STAGES > OUTS ? STAGES : OUTS];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Tiles are dealt so that each of the 8 XCDs, which take workgroups in turn, has a run of neighbours
@@ -75,29 +84,30 @@ __global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
     const int height = tmin(GROUP, mt - band * GROUP);
     const int m0 = (band * GROUP + in % height) * TM, n0 = in / height * TNE;
 
-    // where this lane fetches from: row lane / 8 of an 8-row load, the chunk that belongs at its place
-    const char* base[LOADS];
+    // where this lane fetches from: row lane / 8 of an 8-row load, the chunk that belongs at its place. Buffer
+    // loads, whose addresses are a wave's base and a lane's 32-bit offset (and whose LDS writes, unlike those of
+    // global loads, do not make the compiler wait for every LDS read at once).
     uint32_t off[LOADS];
-    const int lr = lane >> 3, chunk = (lane & 7) ^ lr;
+    static_assert(NW % 2 == 0, "the parity of an 8-row load is its wave's");
+    const int lr = lane >> 3, chunk = (lane & 7) ^ ((lr >> 1) + 4 * (wave & 1));
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
         const int r0 = (j * NW + wave) * 8;
-        if (r0 < TN) {
-            const bool second = TWO && r0 >= TNE;
-            const int r = tmin(n0 + r0 - (second ? TNE : 0) + lr, g.n - 1) - n0;
-            base[j] = reinterpret_cast<const char*>((second ? g.w1 : g.w0) + (int64_t)n0 * g.ldw);
-            off[j] = (uint32_t)r * (uint32_t)(2 * g.ldw) + 16 * chunk;
-        } else {
-            const int r = tmin(m0 + r0 - TN + lr, g.m - 1) - m0;
-            base[j] = reinterpret_cast<const char*>(g.x + (int64_t)m0 * g.ldx);
-            off[j] = (uint32_t)r * (uint32_t)(2 * g.ldx) + 16 * chunk;
-        }
+        if (r0 < TN) off[j] = (uint32_t)(tmin(n0 + r0 - (TWO && r0 >= TNE ? TNE : 0) + lr, g.n - 1) - n0) * (uint32_t)(2 * g.ldw);
+        else off[j] = (uint32_t)(tmin(m0 + r0 - TN + lr, g.m - 1) - m0) * (uint32_t)(2 * g.ldx);
+        off[j] += 16 * chunk;
     }
-    auto fetch = [&](int buf, int kt) {
+    constexpr int RAW = 0x00027000;                               // a plain buffer of bytes
+    const rsrc rw0 = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.w0 + (int64_t)n0 * g.ldw), 0, -1, RAW);
+    const rsrc rw1 = TWO ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.w1 + (int64_t)n0 * g.ldw), 0, -1, RAW) : rw0;
+    const rsrc rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x + (int64_t)m0 * g.ldx), 0, -1, RAW);
+    auto fetch = [&](int buf, int kt, int j0, int j1) {
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            const char* p = base[j] + (int64_t)kt * (2 * BK);
-            __builtin_amdgcn_global_load_lds((gptr)(p + off[j]), (lptr)(&tile[buf][(j * NW + wave) * 8 * BK]), 16, 0, 0);
+        for (int j = j0; j < j1; ++j) {
+            // a load of all waves lies in one operand
+            static_assert(TNE % (8 * NW) == 0 && TN % (8 * NW) == 0, "tile shape");
+            const rsrc r = j * NW * 8 >= TN ? rx : (TWO && j * NW * 8 >= TNE ? rw1 : rw0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)(mem + buf * (TN + TM) * BK + (j * NW + wave) * 8 * BK), 16, off[j], kt * (2 * BK), 0, 0);
         }
     };
 
@@ -120,54 +130,108 @@ __global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
 #pragma unroll
             for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
 
+    // Fragments are read one part of 16 k ahead of their use. In a tile's last part the other buffer's first
+    // fragments are read: before it, every wave's fetches into that buffer have arrived and every wave has read the
+    // last of this one, so one barrier a tile orders both, and this buffer's next contents, fetched right after
+    // it, have a whole tile's time to arrive.
+    constexpr int PARTS = BK / 16;
+    u4 fa[2][FN], fb[2][FM];
+    auto read = [&](int buf, int part, int to) {
+        const uint16_t* t = mem + buf * (TN + TM) * BK;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+            fa[to][i] = *reinterpret_cast<const u4*>(t + arow[i] * BK + (((2 * part + fk) ^ ((arow[i] >> 1) & 7)) * 8));
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            fb[to][i] = *reinterpret_cast<const u4*>(t + brow[i] * BK + (((2 * part + fk) ^ ((brow[i] >> 1) & 7)) * 8));
+    };
+    // One tile step; N1, N2: there is a next one, and one after that. Fetches, fragment reads and products are
+    // dealt out in turn: a wave whose fetches (eight in a row) or reads queue up would issue no product meanwhile.
+    constexpr int EARLY = LOADS / 2;
+    auto tile_step = [&](int kt, auto n1, auto n2) {
+        constexpr bool N1 = decltype(n1)::value, N2 = decltype(n2)::value;
+        const int buf = kt & 1;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            const bool last = part == PARTS - 1;
+            if (last && N1) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+            }
+            if (!last) read(buf, part + 1, (part + 1) & 1);
+            else if (N1) read(buf ^ 1, 0, 0);
+            if (part == 0 && N1) fetch(buf ^ 1, kt + 1, EARLY, LOADS);
+            if (last && N2) fetch(buf, kt + 2, 0, EARLY);
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = Op<HALF>::mul(fa[part & 1][i], fb[part & 1][j], acc[i][j]);
+#pragma unroll
+            for (int i = 0; i < FN * FM; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
     const int steps = g.k / BK;
-    fetch(0, 0);
+    fetch(0, 0, 0, LOADS);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    for (int kt = 0; kt < steps; ++kt) {
-        const uint16_t* t = tile[kt & 1];
-        // the other buffer's last readers passed the barrier at the end of the step before
-        if (kt + 1 < steps) fetch((kt + 1) & 1, kt + 1);
-#pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-            u4 a[FN], b[FM];
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-                a[i] = *reinterpret_cast<const u4*>(t + arow[i] * BK + (((2 * kk + fk) ^ (arow[i] & 7)) * 8));
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-                b[i] = *reinterpret_cast<const u4*>(t + brow[i] * BK + (((2 * kk + fk) ^ (brow[i] & 7)) * 8));
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-#pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = Op<HALF>::mul(a[i], b[j], acc[i][j]);
-        }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-    }
+    if (steps > 1) fetch(1, 1, 0, EARLY);
+    read(0, 0, 0);
+    for (int kt = 0; kt < steps - 2; ++kt) tile_step(kt, std::true_type(), std::true_type());
+    if (steps > 1) tile_step(steps - 2, std::true_type(), std::false_type());
+    tile_step(steps - 1, std::false_type(), std::false_type());
 
-    // lane: input row (lane & 31) of a fragment; register 4 q + c: weight row 8 q + 4 (lane >> 5) + c
-    const int nw = n0 + wn * (TNE / WN) + 4 * fk;
-    const bool vec = OUT == OUT_GRAD || ((g.ldy & 3) == 0 && (reinterpret_cast<uintptr_t>(g.y) & 7) == 0);
-    if constexpr (OUT == OUT_PLAIN) {
-        if (g.xe || g.we0) {
+    // Lane: input row (lane & 31) of a fragment; register 4 q + c: weight row 8 q + 4 (lane >> 5) + c. Stored as
+    // they lie, a wave would write 16 bytes to each of 32 rows at a time; by way of LDS, which the loop is done with,
+    // it writes (and reads dh) in runs of its columns.
+    const int nw = n0 + wn * (TNE / WN) + 4 * fk, mw = m0 + wm * ROWS;
+    uint16_t* const out = mem + wave * ROWS * PITCH;
+    __builtin_amdgcn_s_barrier();
+    auto place = [&](int j, int i, int q) -> u2& {
+        return *reinterpret_cast<u2*>(out + (32 * j + fr) * PITCH + 32 * i + 8 * q + 4 * fk);
+    };
+    // columns c0.. of the staged rows to or from columns n.. of a matrix, `most` columns wide, eight numbers a lane
+    constexpr int RUN = TNE / WN;
+    auto flush = [&](uint16_t* y, int64_t ld, int c0, int most) {
+        const bool wide16 = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int u = lane; u < ROWS * (RUN / 8); u += 64) {
+            const int r = u / (RUN / 8), c = u % (RUN / 8) * 8, n = n0 + wn * RUN + c;
+            if (mw + r >= g.m || n >= most) continue;
+            uint16_t* p = y + (int64_t)(mw + r) * ld + n;
+            const u4 v = *reinterpret_cast<const u4*>(out + r * PITCH + c0 + c);
+            if (wide16 && n + 8 <= most) {
+                *reinterpret_cast<u4*>(p) = v;
+            } else {
 #pragma unroll
-            for (int j = 0; j < FM; ++j) {
-                const int mi = m0 + brow[j] - TN;
-                const int xe = g.xe && mi < g.m ? g.xe[mi] : 0;
-#pragma unroll
-                for (int i = 0; i < FN; ++i)
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const int ni = nw + 32 * i + 8 * (c >> 2) + (c & 3);
-                        acc[i][j][c] = ldexpf(acc[i][j][c], xe + (g.we0 && ni < g.n ? g.we0[ni] : 0));
-                    }
+                for (int k = 0; k < 8; ++k)
+                    if (n + k < most) p[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
             }
         }
-        if (g.ex.low) {
+    };
+    if constexpr (!TWO) {
+        const bool scaled = g.xe || g.we0;
+        auto unscale = [&](int i, int j, f16v& v) {
+            if (!scaled) return;
+            const int mi = tmin(m0 + brow[j] - TN, g.m - 1), xe = g.xe ? g.xe[mi] : 0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const int ni = tmin(nw + 32 * i + 8 * (c >> 2) + (c & 3), g.n - 1);
+                v[c] = ldexpf(v[c], xe + (g.we0 ? g.we0[ni] : 0));
+            }
+        };
+        if constexpr (OUT == OUT_LOW) {
             // the adapters' second product, one adapter of the tile's rows at a time: rows of another
             // adapter take part with zeros. low is split into two BF16 parts, b into two where it is F16.
             const Expand& ex = g.ex;
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+#pragma unroll
+                for (int i = 0; i < FN; ++i) unscale(i, j, acc[i][j]);
             for (int a = next_adapter<TM>(ex, m0, g.m, -1); a != INT32_MAX; a = next_adapter<TM>(ex, m0, g.m, a)) {
                 const uint16_t* ba = ex.b + (int64_t)a * g.n * ex.rank;
                 for (int r0 = 0; r0 < ex.rp; r0 += 16) {
@@ -218,30 +282,39 @@ __global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int mi = m0 + brow[j] - TN;
-            if (mi >= g.m) continue;
-            uint16_t* y = g.y + (int64_t)mi * g.ldy;
+        for (int j = 0; j < FM; ++j)
 #pragma unroll
-            for (int i = 0; i < FN; ++i)
+            for (int i = 0; i < FN; ++i) {
+                f16v v = acc[i][j];
+                if constexpr (OUT == OUT_PLAIN) unscale(i, j, v);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int ni = nw + 32 * i + 8 * q;
-                    if (vec && ni + 3 < g.n) {
-                        *reinterpret_cast<u2*>(y + ni) = u2{narrow2(acc[i][j][4 * q], acc[i][j][4 * q + 1], g.kind),
-                                                            narrow2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3], g.kind)};
+                for (int q = 0; q < 4; ++q)
+                    place(j, i, q) = u2{narrow2(v[4 * q], v[4 * q + 1], g.kind), narrow2(v[4 * q + 2], v[4 * q + 3], g.kind)};
+            }
+        flush(g.y, g.ldy, 0, g.n);
+    } else {
+        if constexpr (OUT == OUT_GRAD) {                          // dh to where its gate's gradient will lie
+            const bool wide16 = (g.ldh & 7) == 0 && (reinterpret_cast<uintptr_t>(g.dh) & 15) == 0;
+            for (int u = lane; u < ROWS * (RUN / 8); u += 64) {
+                const int r = u / (RUN / 8), c = u % (RUN / 8) * 8, n = n0 + wn * RUN + c;
+                u4 v = {0, 0, 0, 0};
+                if (mw + r < g.m && n < g.n) {
+                    const uint16_t* p = g.dh + (int64_t)(mw + r) * g.ldh + n;
+                    if (wide16 && n + 8 <= g.n) {
+                        v = *reinterpret_cast<const u4*>(p);
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (ni + c < g.n) y[ni + c] = narrow(acc[i][j][4 * q + c], g.kind);
+                        for (int k = 0; k < 8; ++k)
+                            if (n + k < g.n) v[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
                     }
                 }
+                *reinterpret_cast<u4*>(out + r * PITCH + c) = v;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-    } else {
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
-            const int mi = m0 + brow[j] - TN;
-            if (mi >= g.m) continue;
+            const int mi = tmin(m0 + brow[j] - TN, g.m - 1);
             const int xe = g.xe ? g.xe[mi] : 0;
             const int ge = OUT == OUT_GRAD && g.ge ? g.ge[mi] : 0;
 #pragma unroll
@@ -258,47 +331,45 @@ __global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
                         if (g.we0 && ni + c < g.n) { e0[c] = g.we0[ni + c]; e1[c] = g.we1[ni + c]; }
                         if (g.xe || g.we0) { gv[c] = ldexpf(gv[c], xe + e0[c]); uv[c] = ldexpf(uv[c], xe + e1[c]); }
                     }
+                    u2& at = place(j, i, q);
                     if constexpr (OUT == OUT_GATED) {
-                        uint16_t* y = g.y + (int64_t)mi * g.ldy;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) gv[c] = act_value(gv[c], g.act) * uv[c];
-                        if (vec && ni + 3 < g.n) {
-                            *reinterpret_cast<u2*>(y + ni) = u2{narrow2(gv[0], gv[1], g.kind), narrow2(gv[2], gv[3], g.kind)};
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (ni + c < g.n) y[ni + c] = narrow(gv[c], g.kind);
-                        }
                     } else {
-                        // columns n..np-1 are padding of the products that follow: zeros
-                        const uint16_t* dh = g.dh + (int64_t)mi * g.ldh;
+                        const u2 d4 = at;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            float dg = 0.f, du = 0.f;
-                            if (ni + c < g.n) {
-                                const float d = wide(dh[ni + c], g.kind);
-                                float value, slope;
-                                act_both(gv[c], g.act, value, slope);
-                                dg = ldexpf(d * uv[c] * slope, e0[c] - ge);
-                                du = ldexpf(d * value, e1[c] - ge);
-                            }
-                            gv[c] = dg;
-                            uv[c] = du;
+                            // columns n..np-1 are padding of the products that follow: zeros, whatever the sums are
+                            const float d = wide((d4[c >> 1] >> (16 * (c & 1))) & 0xffffu, g.kind);
+                            float value, slope;
+                            act_both(gv[c], g.act, value, slope);
+                            const bool in = ni + c < g.n;
+                            gv[c] = in ? ldexpf(d * uv[c] * slope, e0[c] - ge) : 0.f;
+                            uv[c] = in ? ldexpf(d * value, e1[c] - ge) : 0.f;
                         }
-                        if (ni < g.np) {                        // np is a multiple of 64: whole groups of four
-                            uint16_t* y = g.grad + (int64_t)mi * 2 * g.np + ni;
-                            *reinterpret_cast<u2*>(y) = u2{narrow2(gv[0], gv[1], HALF), narrow2(gv[2], gv[3], HALF)};
-                            *reinterpret_cast<u2*>(y + g.np) = u2{narrow2(uv[0], uv[1], HALF), narrow2(uv[2], uv[3], HALF)};
-                        }
+                        (&at)[RUN / 4] = u2{narrow2(uv[0], uv[1], HALF), narrow2(uv[2], uv[3], HALF)};
                     }
+                    const int kind = OUT == OUT_GRAD ? HALF : g.kind;
+                    at = u2{narrow2(gv[0], gv[1], kind), narrow2(gv[2], gv[3], kind)};
                 }
+        }
+        if constexpr (OUT == OUT_GATED) {
+            flush(g.y, g.ldy, 0, g.n);
+        } else {
+            flush(g.grad, g.ldg, 0, (int)g.np);
+            flush(g.grad + g.np, g.ldg, RUN, (int)g.np);
         }
     }
 }
 
 template <int HALF, int TN, int TM, int WN, int WM, int OUT>
+__global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
+    product<HALF, TN, TM, WN, WM, OUT>(g);
+}
+
+template <int HALF, int TN, int TM, int WN, int WM, int OUT>
 int launch(const Gemm& g, hipStream_t st) {
-    constexpr int TNE = OUT == OUT_PLAIN ? TN : TN / 2;
+    constexpr int TNE = OUT == OUT_PLAIN || OUT == OUT_LOW ? TN : TN / 2;
     const int64_t nt = (g.n + TNE - 1) / TNE, mt = (g.m + TM - 1) / TM;
     if (nt * mt > INT32_MAX) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", g.m, g.n);
     hipLaunchKernelGGL((k_gemm<HALF, TN, TM, WN, WM, OUT>), dim3((unsigned)(nt * mt)), dim3(WN * WM * 64), 0, st, g);
@@ -308,23 +379,23 @@ int launch(const Gemm& g, hipStream_t st) {
 
 template <int HALF, int OUT>
 int pick(const Gemm& g, hipStream_t st) {
-    constexpr int D = OUT == OUT_PLAIN ? 1 : 2;
+    constexpr int D = OUT == OUT_PLAIN || OUT == OUT_LOW ? 1 : 2;
     const int64_t big = (int64_t)((g.n * D + 255) / 256) * ((g.m + 255) / 256);
-    if (big >= 192) return launch<HALF, 256, 256, 2, 4, OUT>(g, st);
+    if (big >= 192) return launch<HALF, 256, 256, 2, SPA_WM, OUT>(g, st);
     if (g.m <= 64) return launch<HALF, 128, 64, 2, 2, OUT>(g, st);
     return launch<HALF, 128, 128, 2, 2, OUT>(g, st);
 }
 
+template <int HALF>
+int form(const Gemm& g, hipStream_t st) {
+    if (g.grad) return pick<HALF, OUT_GRAD>(g, st);
+    if (g.w1) return pick<HALF, OUT_GATED>(g, st);
+    return g.ex.low ? pick<HALF, OUT_LOW>(g, st) : pick<HALF, OUT_PLAIN>(g, st);
+}
+
 }  // namespace
 
-int gemm(const Gemm& g, hipStream_t st) {
-    if (g.half == SRC_BF16) {
-        if (g.grad) return pick<SRC_BF16, OUT_GRAD>(g, st);
-        return g.w1 ? pick<SRC_BF16, OUT_GATED>(g, st) : pick<SRC_BF16, OUT_PLAIN>(g, st);
-    }
-    if (g.grad) return pick<SRC_F16, OUT_GRAD>(g, st);
-    return g.w1 ? pick<SRC_F16, OUT_GATED>(g, st) : pick<SRC_F16, OUT_PLAIN>(g, st);
-}
+int gemm(const Gemm& g, hipStream_t st) { return g.half == SRC_BF16 ? form<SRC_BF16>(g, st) : form<SRC_F16>(g, st); }
 
 }  // namespace lin
 }  // namespace spa

@@ -8,6 +8,8 @@ namespace spa {
 namespace lin {
 namespace {
 
+// rows of the inner matrices lie 128 bytes more than whole steps apart
+constexpr int64_t PAD = 64;
 int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // a workspace handed out in pieces of whole 256 bytes; with no memory behind it, only counted
@@ -268,7 +270,8 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     const int64_t np = up64(p.n), mp = up64(p.m);
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, run ? p.up : SOME, p.n, p.k, p.kind, p.x, p.m, p.ldx, true, o, st))) return rc;
-    uint16_t* grad = wk.take<uint16_t>(p.m * 2 * np);
+    const int64_t ldg = 2 * np + PAD, ldm = mp + PAD;
+    uint16_t* grad = wk.take<uint16_t>(p.m * ldg);
     int32_t* ge = o.norm ? wk.take<int32_t>(p.m) : nullptr;
     void* top = wk.take<uint8_t>(8);
     if (run) {
@@ -280,20 +283,21 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
         g.ldh = p.ldh;
         g.grad = grad;
         g.np = np;
+        g.ldg = ldg;
         g.ge = ge;
         if ((rc = gemm(g, st))) return rc;
     }
     if (want_x) {
-        uint16_t* wt = wk.take<uint16_t>(p.k * 2 * np);
+        uint16_t* wt = wk.take<uint16_t>(p.k * ldg);
         if (run) {
-            if ((rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, 2 * np, np, st))) return rc;
-            if ((rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, 2 * np, np, st))) return rc;
+            if ((rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, ldg, np, st))) return rc;
+            if ((rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, ldg, np, st))) return rc;
             Gemm g{};
             g.half = o.half;
             g.x = grad;
-            g.ldx = 2 * np;
+            g.ldx = ldg;
             g.w0 = wt;
-            g.ldw = 2 * np;
+            g.ldw = ldg;
             g.m = (int)p.m;
             g.n = (int)p.k;
             g.k = (int)(2 * np);
@@ -305,18 +309,18 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
         }
     }
     if (want_w) {
-        uint16_t* gt = wk.take<uint16_t>(2 * np * mp);
-        uint16_t* xt = wk.take<uint16_t>(p.k * mp);
+        uint16_t* gt = wk.take<uint16_t>(2 * np * ldm);
+        uint16_t* xt = wk.take<uint16_t>(p.k * ldm);
         if (run) {
-            if ((rc = transpose16(grad, 2 * np, p.m, 2 * np, gt, mp, mp, st))) return rc;
-            if ((rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, mp, mp, st))) return rc;
+            if ((rc = transpose16(grad, ldg, p.m, 2 * np, gt, ldm, mp, st))) return rc;
+            if ((rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, ldm, mp, st))) return rc;
             for (int i = 0; i < 2; ++i) {
                 Gemm g{};
                 g.half = o.half;
-                g.x = gt + (i ? np * mp : 0);
-                g.ldx = mp;
+                g.x = gt + (i ? np * ldm : 0);
+                g.ldx = ldm;
                 g.w0 = xt;
-                g.ldw = mp;
+                g.ldw = ldm;
                 g.m = (int)p.n;
                 g.n = (int)p.k;
                 g.k = (int)mp;
