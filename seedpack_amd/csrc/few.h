@@ -23,29 +23,6 @@ __device__ __forceinline__ f4 mul16(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
 }
 
-// the adapters' part of output (m, n)
-__device__ __forceinline__ float expand(const Few& f, int m, int n) {
-    const Expand& ex = f.ex;
-    const int a = ex.which[m];
-    if (a < 0 || a >= ex.pool) return 0.f;
-    const float* z = ex.low + (int64_t)m * ex.rp;
-    const uint16_t* b = ex.b + ((int64_t)a * f.n + n) * ex.rank;
-    float t = 0.f;
-    if (ex.wide_b) {
-        for (int r = 0; r < ex.rank; r += 8) {
-            const u4 h = *reinterpret_cast<const u4*>(b + r);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                t = fmaf(z[r + 2 * c], wide(h[c] & 0xffffu, ex.kind), t);
-                t = fmaf(z[r + 2 * c + 1], wide(h[c] >> 16, ex.kind), t);
-            }
-        }
-    } else {
-        for (int r = 0; r < ex.rank; ++r) t = fmaf(z[r], wide(b[r], ex.kind), t);
-    }
-    return t;
-}
-
 // Joins the waves' sums and writes the outputs; red has WAVES (1 + TWO) MT 256 floats. With HALVES a tile is
 // 8 input rows, each as the sum of tile rows m and m + 8. again(matrix, m, n) gives a sum anew, term by
 // term, where the joined one is not a number.
@@ -78,7 +55,7 @@ __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f
         }
         float y;
         if constexpr (TWO) y = act_value(v[0], f.act) * v[1];
-        else y = f.ex.low ? v[0] + expand(f, m, n) : v[0];
+        else y = f.ex.low ? v[0] + expand(f.ex, m, n, f.n) : v[0];
         f.y[(int64_t)m * f.ldy + n] = narrow(y, f.kind);
     }
 }

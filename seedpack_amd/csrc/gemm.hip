@@ -22,9 +22,6 @@ namespace spa {
 namespace lin {
 namespace {
 
-#ifndef SPA_WM
-#define SPA_WM 4
-#endif
 constexpr int BK = 64;
 
 template <int HALF> struct Op;
@@ -43,18 +40,16 @@ __device__ __forceinline__ f16v mul_bf(bf8 a, bf8 b, f16v c) { return __builtin_
 typedef __amdgpu_buffer_rsrc_t rsrc;
 typedef __attribute__((address_space(3))) void* lptr;
 
-// the least adapter number above `after` among the tile's rows, or INT32_MAX
-template <int TM>
-__device__ __forceinline__ int next_adapter(const Expand& ex, int m0, int m, int after) {
+// the least adapter number above `after` among the tile's rows (held by the wave's lanes), or INT32_MAX
+template <int N>
+__device__ __forceinline__ int next_adapter(const int (&ids)[N], int after) {
     int best = INT32_MAX;
-    for (int r = threadIdx.x & 63; r < TM; r += 64) {
-        if (m0 + r >= m) continue;
-        const int a = ex.which[m0 + r];
-        if (a > after && a < ex.pool && a < best) best = a;
-    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (ids[i] > after) best = tmin(best, ids[i]);
 #pragma unroll
     for (int s = 32; s; s >>= 1) best = tmin(best, __shfl_xor(best, s));
-    return best;
+    return __builtin_amdgcn_readfirstlane(best);
 }
 
 template <int HALF, int TN, int TM, int WN, int WM, int OUT>
@@ -67,14 +62,25 @@ __device__ __forceinline__ void product(const Gemm& g) {
     static_assert((TN + TM) % (8 * NW) == 0 && (!TWO || FN % 2 == 0), "tile shape");
     // a wave's outputs on their way out: its input rows x its columns, rows 16 bytes apart from a power of two
     constexpr int ROWS = TM / WM, COLS = TN / WN, PITCH = COLS + 8;
-    constexpr int STAGES = 2 * (TN + TM) * BK, OUTS = NW * ROWS * PITCH;
+    constexpr int STAGES = 2 * (TN + TM) * BK, OUTS = OUT == OUT_PART ? NW * 64 * (COLS + 4) : NW * ROWS * PITCH;
     __shared__ __align__(16) uint16_t mem[STAGES > OUTS ? STAGES : OUTS];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Tiles are dealt so that each of the 8 XCDs, which take workgroups in turn, has a run of neighbours
     // (its L2 then serves their shared rows), and a run covers 8 tiles of input rows per tile of weights.
     const int nt = (g.n + TNE - 1) / TNE, mt = (g.m + TM - 1) / TM, total = nt * mt;
-    int id = blockIdx.x;
+    int id = blockIdx.x, piece = 0, side = 0;
+    const uint16_t* w0 = g.w0;
+    int k0 = 0, steps = g.k / BK;
+    if (OUT == OUT_PART) {                                        // a piece of k of one matrix
+        piece = id / total;
+        id -= piece * total;
+        side = piece / g.pieces;
+        piece -= side * g.pieces;
+        if (side) w0 = g.w1;
+        k0 = steps * piece / g.pieces;
+        steps = steps * (piece + 1) / g.pieces - k0;
+    }
     {
         const int q = total / 8, r = total % 8, xcd = id & 7, at = id >> 3;
         id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
@@ -98,9 +104,9 @@ __device__ __forceinline__ void product(const Gemm& g) {
         off[j] += 16 * chunk;
     }
     constexpr int RAW = 0x00027000;                               // a plain buffer of bytes
-    const rsrc rw0 = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.w0 + (int64_t)n0 * g.ldw), 0, -1, RAW);
-    const rsrc rw1 = TWO ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.w1 + (int64_t)n0 * g.ldw), 0, -1, RAW) : rw0;
-    const rsrc rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x + (int64_t)m0 * g.ldx), 0, -1, RAW);
+    const rsrc rw0 = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(w0 + (int64_t)n0 * g.ldw + k0 * BK), 0, -1, RAW);
+    const rsrc rw1 = TWO ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.w1 + (int64_t)n0 * g.ldw + k0 * BK), 0, -1, RAW) : rw0;
+    const rsrc rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(g.x + (int64_t)m0 * g.ldx + k0 * BK), 0, -1, RAW);
     auto fetch = [&](int buf, int kt, int j0, int j1) {
 #pragma unroll
         for (int j = j0; j < j1; ++j) {
@@ -155,8 +161,7 @@ __device__ __forceinline__ void product(const Gemm& g) {
         for (int part = 0; part < PARTS; ++part) {
             const bool last = part == PARTS - 1;
             if (last && N1) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             if (!last) read(buf, part + 1, (part + 1) & 1);
             else if (N1) read(buf ^ 1, 0, 0);
@@ -175,10 +180,8 @@ __device__ __forceinline__ void product(const Gemm& g) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    const int steps = g.k / BK;
     fetch(0, 0, 0, LOADS);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (steps > 1) fetch(1, 1, 0, EARLY);
     read(0, 0, 0);
     for (int kt = 0; kt < steps - 2; ++kt) tile_step(kt, std::true_type(), std::true_type());
@@ -190,7 +193,7 @@ __device__ __forceinline__ void product(const Gemm& g) {
     // it writes (and reads dh) in runs of its columns.
     const int nw = n0 + wn * (TNE / WN) + 4 * fk, mw = m0 + wm * ROWS;
     uint16_t* const out = mem + wave * ROWS * PITCH;
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     auto place = [&](int j, int i, int q) -> u2& {
         return *reinterpret_cast<u2*>(out + (32 * j + fr) * PITCH + 32 * i + 8 * q + 4 * fk);
     };
@@ -214,17 +217,19 @@ __device__ __forceinline__ void product(const Gemm& g) {
         }
     };
     if constexpr (!TWO) {
-        const bool scaled = g.xe || g.we0;
+        const int32_t* const we = side ? g.we1 : g.we0;
+        const bool scaled = g.xe || we;
+        bool unscaled = false;
         auto unscale = [&](int i, int j, f16v& v) {
-            if (!scaled) return;
+            if (!scaled || unscaled) return;
             const int mi = tmin(m0 + brow[j] - TN, g.m - 1), xe = g.xe ? g.xe[mi] : 0;
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
                 const int ni = tmin(nw + 32 * i + 8 * (c >> 2) + (c & 3), g.n - 1);
-                v[c] = ldexpf(v[c], xe + (g.we0 ? g.we0[ni] : 0));
+                v[c] = ldexpf(v[c], xe + (we ? we[ni] : 0));
             }
         };
-        if constexpr (OUT == OUT_LOW) {
+        if (OUT == OUT_LOW || (OUT == OUT_PART && g.ex.low)) {
             // the adapters' second product, one adapter of the tile's rows at a time: rows of another
             // adapter take part with zeros. low is split into two BF16 parts, b into two where it is F16.
             const Expand& ex = g.ex;
@@ -232,43 +237,71 @@ __device__ __forceinline__ void product(const Gemm& g) {
             for (int j = 0; j < FM; ++j)
 #pragma unroll
                 for (int i = 0; i < FN; ++i) unscale(i, j, acc[i][j]);
-            for (int a = next_adapter<TM>(ex, m0, g.m, -1); a != INT32_MAX; a = next_adapter<TM>(ex, m0, g.m, a)) {
+            unscaled = true;
+            int mine[FM], zrow[FM], brow0[FN];
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const int mi = m0 + brow[j] - TN;
+                zrow[j] = tmin(mi, g.m - 1);
+                mine[j] = mi < g.m ? ex.which[zrow[j]] : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < FN; ++i) brow0[i] = tmin(n0 + arow[i], g.n - 1);
+            // pieces of k share the ranks, 16 at a time. Rows and columns beyond the last are read as the last: they
+            // are not kept.
+            const int first = OUT == OUT_PART ? piece * 16 : 0, stride = OUT == OUT_PART ? g.pieces * 16 : 16;
+            int ids[TM / 64];                                     // those outside the pool as -1
+#pragma unroll
+            for (int i = 0; i < TM / 64; ++i) {
+                const int mi = m0 + 64 * i + lane, a = ex.which[tmin(mi, g.m - 1)];
+                ids[i] = mi < g.m && a < ex.pool ? a : -1;
+            }
+            for (int a = next_adapter(ids, -1); a != INT32_MAX; a = next_adapter(ids, a)) {
                 const uint16_t* ba = ex.b + (int64_t)a * g.n * ex.rank;
-                for (int r0 = 0; r0 < ex.rp; r0 += 16) {
+                for (int r0 = first; r0 < ex.rp; r0 += stride) {
                     const int r = r0 + 8 * fk;
+                    f4 z[FM][2];
+                    u4 h[FN];
+#pragma unroll
+                    for (int j = 0; j < FM; ++j)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) z[j][c] = *reinterpret_cast<const f4*>(ex.low + (int64_t)zrow[j] * ex.rp + r + 4 * c);
+#pragma unroll
+                    for (int i = 0; i < FN; ++i) {
+                        const uint16_t* p = ba + (int64_t)brow0[i] * ex.rank;
+                        if (ex.wide_b) {                          // rank a multiple of 8: eight ranks there or none
+                            h[i] = *reinterpret_cast<const u4*>(p + tmin(r, ex.rank - 8));
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const uint32_t lo = p[tmin(r + 2 * c, ex.rank - 1)], hi = p[tmin(r + 2 * c + 1, ex.rank - 1)];
+                                h[i][c] = lo | (hi << 16);
+                            }
+                        }
+                    }
+                    // ranks beyond the last: low holds zeros there, b's numbers are cleared (they may be infinite)
+#pragma unroll
+                    for (int i = 0; i < FN; ++i)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int left = ex.rank - r - 2 * c;
+                            h[i][c] &= left >= 2 ? 0xffffffffu : (left == 1 ? 0xffffu : 0u);
+                        }
                     bf8 zh[FM], zl[FM];
 #pragma unroll
                     for (int j = 0; j < FM; ++j) {
-                        const int mi = m0 + brow[j] - TN;
-                        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                        if (mi < g.m && ex.which[mi] == a) {
-                            const f4* z = reinterpret_cast<const f4*>(ex.low + (int64_t)mi * ex.rp + r);
+                        float v[8];
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) v[c] = z[c >> 2][c & 3];
-                        }
+                        for (int c = 0; c < 8; ++c) v[c] = mine[j] == a ? z[j][c >> 2][c & 3] : 0.f;
                         split8(v, zh[j], zl[j]);
                     }
 #pragma unroll
                     for (int i = 0; i < FN; ++i) {
-                        const int ni = n0 + arow[i];
-                        uint16_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                        if (ni < g.n && r < ex.rank) {
-                            const uint16_t* p = ba + (int64_t)ni * ex.rank + r;
-                            if (ex.wide_b) {
-                                *reinterpret_cast<u4*>(h) = *reinterpret_cast<const u4*>(p);
-                            } else {
-#pragma unroll
-                                for (int c = 0; c < 8; ++c)
-                                    if (r + c < ex.rank) h[c] = p[c];
-                            }
-                        }
-                        bf8 bh, bl;
-                        if (ex.kind == SRC_BF16) {
-                            bh = __builtin_bit_cast(bf8, *reinterpret_cast<u4*>(h));
-                        } else {
+                        bf8 bh = __builtin_bit_cast(bf8, h[i]), bl;
+                        if (ex.kind != SRC_BF16) {
                             float v[8];
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) v[c] = wide(h[c], SRC_F16);
+                            for (int c = 0; c < 8; ++c) v[c] = wide((h[i][c >> 1] >> (16 * (c & 1))) & 0xffffu, SRC_F16);
                             split8(v, bh, bl);
                         }
 #pragma unroll
@@ -281,12 +314,45 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 }
             }
         }
+        if constexpr (OUT == OUT_PART) {
+            // float32 sums, 32 input rows at a time through the wave's staging place
+            float* const stage = reinterpret_cast<float*>(mem) + wave * 32 * (COLS + 4);
+            float* const part = g.part + ((int64_t)(side * g.pieces + piece) * g.m) * g.n;
+            const bool wide16 = (g.n & 3) == 0;
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    f16v v = acc[i][j];
+                    unscale(i, j, v);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f4*>(stage + fr * (COLS + 4) + 32 * i + 8 * q + 4 * fk) = f4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                for (int u = lane; u < 32 * (COLS / 4); u += 64) {
+                    const int r = u / (COLS / 4), c = u % (COLS / 4) * 4, n = n0 + wn * COLS + c, mi = mw + 32 * j + r;
+                    if (mi >= g.m || n >= g.n) continue;
+                    const f4 v = *reinterpret_cast<const f4*>(stage + r * (COLS + 4) + c);
+                    float* p = part + (int64_t)mi * g.n + n;
+                    if (wide16) {
+                        *reinterpret_cast<f4*>(p) = v;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (n + k < g.n) p[k] = v[k];
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < FM; ++j)
 #pragma unroll
             for (int i = 0; i < FN; ++i) {
                 f16v v = acc[i][j];
-                if constexpr (OUT == OUT_PLAIN) unscale(i, j, v);
+                unscale(i, j, v);
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     place(j, i, q) = u2{narrow2(v[4 * q], v[4 * q + 1], g.kind), narrow2(v[4 * q + 2], v[4 * q + 3], g.kind)};
@@ -369,21 +435,117 @@ __global__ __launch_bounds__(WN * WM * 64) void k_gemm(const Gemm g) {
 
 template <int HALF, int TN, int TM, int WN, int WM, int OUT>
 int launch(const Gemm& g, hipStream_t st) {
-    constexpr int TNE = OUT == OUT_PLAIN || OUT == OUT_LOW ? TN : TN / 2;
+    constexpr int TNE = OUT == OUT_GATED || OUT == OUT_GRAD ? TN / 2 : TN;
     const int64_t nt = (g.n + TNE - 1) / TNE, mt = (g.m + TM - 1) / TM;
-    if (nt * mt > INT32_MAX) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", g.m, g.n);
-    hipLaunchKernelGGL((k_gemm<HALF, TN, TM, WN, WM, OUT>), dim3((unsigned)(nt * mt)), dim3(WN * WM * 64), 0, st, g);
+    const int64_t groups = nt * mt * (OUT == OUT_PART ? g.pieces * (g.w1 ? 2 : 1) : 1);
+    if (groups > INT32_MAX) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", g.m, g.n);
+    hipLaunchKernelGGL((k_gemm<HALF, TN, TM, WN, WM, OUT>), dim3((unsigned)groups), dim3(WN * WM * 64), 0, st, g);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
+// The pieces of k joined in their order, and what the one-launch forms do with the sums. Four columns a lane.
+template <int OUT>
+__global__ __launch_bounds__(256) void k_join(const Gemm g) {
+    constexpr bool TWO = OUT == OUT_GATED || OUT == OUT_GRAD;
+    const int width = OUT == OUT_GRAD ? (int)g.np : g.n, per = (width + 3) / 4;
+    const int64_t total = (int64_t)g.m * per, size = (int64_t)g.m * g.n;
+    const bool wide16 = (g.n & 3) == 0;
+    for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < total; at += gridDim.x * 256ll) {
+        const int m = (int)(at / per), n = (int)(at - (int64_t)m * per) * 4;
+        float v[1 + TWO][4];
+#pragma unroll
+        for (int s = 0; s <= TWO; ++s) {
+            const float* p = g.part + s * g.pieces * size + (int64_t)m * g.n + n;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[s][c] = 0.f;
+            for (int i = 0; i < g.pieces; ++i, p += size) {
+                if (wide16 && n < g.n) {
+                    const f4 a = *reinterpret_cast<const f4*>(p);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[s][c] += a[c];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (n + c < g.n) v[s][c] += p[c];
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int ni = n + c;
+            float a = v[0][c];
+            if constexpr (OUT == OUT_GRAD) {
+                float value = 0.f, slope = 0.f, d = 0.f;
+                if (ni < g.n) {
+                    act_both(a, g.act, value, slope);
+                    d = wide(g.dh[(int64_t)m * g.ldh + ni], g.kind);
+                }
+                const int ge = g.ge ? g.ge[m] : 0;
+                const int e0 = g.we0 && ni < g.n ? g.we0[ni] : 0, e1 = g.we1 && ni < g.n ? g.we1[ni] : 0;
+                const float u = v[1][c];
+                if (ni < width) {
+                    uint16_t* y = g.grad + (int64_t)m * g.ldg + ni;
+                    y[0] = narrow(ni < g.n ? ldexpf(d * u * slope, e0 - ge) : 0.f, g.half);
+                    y[g.np] = narrow(ni < g.n ? ldexpf(d * value, e1 - ge) : 0.f, g.half);
+                }
+            } else if (ni < g.n) {
+                if constexpr (OUT == OUT_GATED) a = act_value(a, g.act) * v[1][c];
+                g.y[(int64_t)m * g.ldy + ni] = narrow(a, g.kind);
+            }
+        }
+    }
+}
+
+// What a product takes: a tile of 256 x 256 is a third faster for its work than two of 128 x 128 on a compute unit,
+// but the device has 256 units and waits for its last round. Times of 64 k of a round, in units of 1/100 us on one
+// MI355X: 256 x 256 one to a unit 170; 128 x 128 two to a unit 100, alone on it 85. In pieces of k with too
+// few tiles: each adds 8 bytes of traffic an output and matrix (about 5 TB/s) and the joining launch.
+struct Plan {
+    bool big;
+    int pieces;
+};
+Plan plan(const Gemm& g) {
+    const bool two = g.w1 != nullptr;
+    const int64_t steps = g.k / BK, m = g.m, n = g.n;
+    const int64_t nb = (n * (two ? 2 : 1) + 255) / 256 * ((m + 255) / 256), ns = (n * (two ? 2 : 1) + 127) / 128 * ((m + 127) / 128);
+    auto small = [](int64_t tiles, int64_t st) { return tiles <= 256 ? st * 85 : (tiles + 511) / 512 * st * 100; };
+    Plan best{true, 1};
+    int64_t cost = (nb + 255) / 256 * steps * 170;
+    if (small(ns, steps) < cost) {
+        best = Plan{false, 1};
+        cost = small(ns, steps);
+    }
+    for (int p = 2; p <= g.most && p * 4 <= steps; ++p) {
+        const int64_t st = (steps + p - 1) / p, join = 600 + (int64_t)(m * n * (two ? 2 : 1) * 8 * p / 50000);
+        // in pieces the two matrices are products of their own
+        const int64_t b = (n + 255) / 256 * (two ? 2 : 1) * ((m + 255) / 256) * p, s = (n + 127) / 128 * (two ? 2 : 1) * ((m + 127) / 128) * p;
+        if ((b + 255) / 256 * st * 170 + join < cost) {
+            best = Plan{true, p};
+            cost = (b + 255) / 256 * st * 170 + join;
+        }
+        if (small(s, st) + join < cost) {
+            best = Plan{false, p};
+            cost = small(s, st) + join;
+        }
+    }
+    return best;
+}
+
 template <int HALF, int OUT>
 int pick(const Gemm& g, hipStream_t st) {
-    constexpr int D = OUT == OUT_PLAIN || OUT == OUT_LOW ? 1 : 2;
-    const int64_t big = (int64_t)((g.n * D + 255) / 256) * ((g.m + 255) / 256);
-    if (big >= 192) return launch<HALF, 256, 256, 2, SPA_WM, OUT>(g, st);
-    if (g.m <= 64) return launch<HALF, 128, 64, 2, 2, OUT>(g, st);
-    return launch<HALF, 128, 128, 2, 2, OUT>(g, st);
+    const Plan p = plan(g);
+    if (p.pieces > 1) {
+        Gemm q = g;
+        q.pieces = p.pieces;
+        const int rc = p.big ? launch<HALF, 256, 256, 2, 4, OUT_PART>(q, st) : launch<HALF, 128, 128, 2, 2, OUT_PART>(q, st);
+        if (rc) return rc;
+        const int64_t groups = ((int64_t)g.m * ((OUT == OUT_GRAD ? g.np : g.n) + 3) / 4 + 255) / 256;
+        hipLaunchKernelGGL((k_join<OUT>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, st, q);
+        SPA_HIP_TRY(hipGetLastError());
+        return SPA_OK;
+    }
+    return p.big ? launch<HALF, 256, 256, 2, 4, OUT>(g, st) : launch<HALF, 128, 128, 2, 2, OUT>(g, st);
 }
 
 template <int HALF>
@@ -394,6 +556,13 @@ int form(const Gemm& g, hipStream_t st) {
 }
 
 }  // namespace
+
+int64_t gemm_part(const Gemm& g) {
+    Gemm q = g;
+    q.most = GEMM_PIECES;
+    const Plan p = plan(q);
+    return p.pieces > 1 ? (int64_t)p.pieces * (g.w1 ? 2 : 1) * g.m * g.n : 0;
+}
 
 int gemm(const Gemm& g, hipStream_t st) { return g.half == SRC_BF16 ? form<SRC_BF16>(g, st) : form<SRC_F16>(g, st); }
 

@@ -91,8 +91,31 @@ struct Expand {
     bool wide_b;              // 16-byte loads of b's rows: rank a multiple of 8, b 16-byte aligned
 };
 
-// OUT_LOW: plain, and the adapters' second product
-enum GemmOut { OUT_PLAIN = 0, OUT_GATED = 1, OUT_GRAD = 2, OUT_LOW = 3 };
+// the adapters' part of output (m, n) of `count` columns
+__device__ __forceinline__ float expand(const Expand& ex, int m, int n, int count) {
+    const int a = ex.which[m];
+    if (a < 0 || a >= ex.pool) return 0.f;
+    const float* z = ex.low + (int64_t)m * ex.rp;
+    const uint16_t* b = ex.b + ((int64_t)a * count + n) * ex.rank;
+    float t = 0.f;
+    if (ex.wide_b) {
+        for (int r = 0; r < ex.rank; r += 8) {
+            const u4 h = *reinterpret_cast<const u4*>(b + r);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                t = fmaf(z[r + 2 * c], wide(h[c] & 0xffffu, ex.kind), t);
+                t = fmaf(z[r + 2 * c + 1], wide(h[c] >> 16, ex.kind), t);
+            }
+        }
+    } else {
+        for (int r = 0; r < ex.rank; ++r) t = fmaf(z[r], wide(b[r], ex.kind), t);
+    }
+    return t;
+}
+
+// OUT_PART: a piece of k in float32 (joined by a launch of its own into any of the others); OUT_LOW: plain, and the adapters' second product
+enum GemmOut { OUT_PLAIN = 0, OUT_GATED = 1, OUT_GRAD = 2, OUT_LOW = 3, OUT_PART = 4 };
+constexpr int GEMM_PIECES = 16;
 
 // sum_k x[m][k] w[n][k] over rows padded to a multiple of 64 (zeros), and what becomes of it
 struct Gemm {
@@ -112,7 +135,13 @@ struct Gemm {
     uint16_t* grad;           // OUT_GRAD: [m][2 np], the gate's gradient, then the up projection's; zeros beyond n
     int64_t np, ldg;          // its halves' width and its rows' distance
     const int32_t* ge;        // OUT_GRAD: power of two taken out of each row of grad (binary16), or null
+    // pieces of k: the most that there may be (1: none), scratch of gemm_part() numbers for their sums
+    // [matrix][piece][m][n], and how many there are
+    int most;
+    float* part;
+    int pieces;
 };
+int64_t gemm_part(const Gemm& g);
 int gemm(const Gemm& g, hipStream_t st);
 
 // ---- few rows (few.hip)
@@ -152,7 +181,7 @@ int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k
 // the same from a block type
 int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, float* norm,
                 hipStream_t st);
-// dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (even)
+// dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (rp and ldd multiples of 8)
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
                 hipStream_t st);
 // the power of two to take out of each row of the gated block's inner gradients, by the 2-norms of the inputs'
@@ -160,7 +189,8 @@ int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uin
 int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const float* n0,
                    const int32_t* e0, const float* n1, const int32_t* e1, void* top, int32_t* e, hipStream_t st);
 int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st);
-// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]
+// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]; low has room for low_pieces() of it
+inline int low_pieces(int64_t m, int64_t k) { return m > 256 && k >= 2048 ? 4 : 1; }
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
              const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st);
 

@@ -171,6 +171,14 @@ Gemm gemm_of(const Operands& o, int64_t m, int64_t n, int64_t k) {
     return g;
 }
 
+// the product with scratch for its pieces of k
+int multiply(Gemm& g, Work& wk, bool run, hipStream_t st) {
+    const int64_t part = gemm_part(g);
+    g.part = wk.take<float>(part);
+    g.most = part ? GEMM_PIECES : 1;
+    return run ? gemm(g, st) : SPA_OK;
+}
+
 struct Project {
     int type;
     const void* w;
@@ -192,7 +200,7 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
     if (p.pool) {
         ex.rank = (int)p.rank;
         ex.rp = (int)((p.rank + 15) / 16 * 16);
-        float* low = wk.take<float>(p.m * ex.rp);
+        float* low = wk.take<float>(p.m * ex.rp * low_pieces(p.m, p.k));
         ex.low = low;
         ex.b = (const uint16_t*)p.b;
         ex.which = p.which;
@@ -214,13 +222,13 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
         return few(f, frags, st);
     }
     Operands o;
-    if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st)) || !run) return rc;
+    if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
     Gemm g = gemm_of(o, p.m, p.n, p.k);
     g.kind = p.kind;
     g.y = (uint16_t*)p.y;
     g.ldy = p.ldy;
     g.ex = ex;
-    return gemm(g, st);
+    return multiply(g, wk, run, st);
 }
 
 struct Gated {
@@ -254,13 +262,13 @@ int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
         return few(f, frags, st);
     }
     Operands o;
-    if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st)) || !run) return rc;
+    if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
     Gemm g = gemm_of(o, p.m, p.n, p.k);
     g.kind = p.kind;
     g.y = (uint16_t*)p.h;
     g.ldy = p.ldh;
     g.act = p.act;
-    return gemm(g, st);
+    return multiply(g, wk, run, st);
 }
 
 // grad = [dG | dU] in one matrix of 2 np columns; dx = grad [Wg; Wu] is then one product over 2 np, with the
@@ -274,8 +282,9 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     uint16_t* grad = wk.take<uint16_t>(p.m * ldg);
     int32_t* ge = o.norm ? wk.take<int32_t>(p.m) : nullptr;
     void* top = wk.take<uint8_t>(8);
-    if (run) {
-        if (ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.n0, o.we0, o.n1, o.we1, top, ge, st))) return rc;
+    if (run && ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.n0, o.we0, o.n1, o.we1, top, ge, st)))
+        return rc;
+    {
         Gemm g = gemm_of(o, p.m, p.n, p.k);
         g.kind = p.kind;
         g.act = p.act;
@@ -285,50 +294,44 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
         g.np = np;
         g.ldg = ldg;
         g.ge = ge;
-        if ((rc = gemm(g, st))) return rc;
+        if ((rc = multiply(g, wk, run, st))) return rc;
     }
     if (want_x) {
         uint16_t* wt = wk.take<uint16_t>(p.k * ldg);
-        if (run) {
-            if ((rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, ldg, np, st))) return rc;
-            if ((rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, ldg, np, st))) return rc;
-            Gemm g{};
-            g.half = o.half;
-            g.x = grad;
-            g.ldx = ldg;
-            g.w0 = wt;
-            g.ldw = ldg;
-            g.m = (int)p.m;
-            g.n = (int)p.k;
-            g.k = (int)(2 * np);
-            g.xe = ge;
-            g.kind = p.kind;
-            g.y = (uint16_t*)p.dx;
-            g.ldy = p.lddx;
-            if ((rc = gemm(g, st))) return rc;
-        }
+        if (run && (rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, ldg, np, st))) return rc;
+        if (run && (rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, ldg, np, st))) return rc;
+        Gemm g{};
+        g.half = o.half;
+        g.x = grad;
+        g.w0 = wt;
+        g.ldx = g.ldw = ldg;
+        g.m = (int)p.m;
+        g.n = (int)p.k;
+        g.k = (int)(2 * np);
+        g.xe = ge;
+        g.kind = p.kind;
+        g.y = (uint16_t*)p.dx;
+        g.ldy = p.lddx;
+        if ((rc = multiply(g, wk, run, st))) return rc;
     }
     if (want_w) {
         uint16_t* gt = wk.take<uint16_t>(2 * np * ldm);
         uint16_t* xt = wk.take<uint16_t>(p.k * ldm);
-        if (run) {
-            if ((rc = transpose16(grad, ldg, p.m, 2 * np, gt, ldm, mp, st))) return rc;
-            if ((rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, ldm, mp, st))) return rc;
-            for (int i = 0; i < 2; ++i) {
-                Gemm g{};
-                g.half = o.half;
-                g.x = gt + (i ? np * ldm : 0);
-                g.ldx = ldm;
-                g.w0 = xt;
-                g.ldw = ldm;
-                g.m = (int)p.n;
-                g.n = (int)p.k;
-                g.k = (int)mp;
-                g.kind = p.kind;
-                g.y = (uint16_t*)(i ? p.dup : p.dgate);
-                g.ldy = p.k;
-                if ((rc = gemm(g, st))) return rc;
-            }
+        if (run && (rc = transpose16(grad, ldg, p.m, 2 * np, gt, ldm, mp, st))) return rc;
+        if (run && (rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, ldm, mp, st))) return rc;
+        for (int i = 0; i < 2; ++i) {
+            Gemm g{};
+            g.half = o.half;
+            g.x = gt + (i ? np * ldm : 0);
+            g.w0 = xt;
+            g.ldx = g.ldw = ldm;
+            g.m = (int)p.n;
+            g.n = (int)p.k;
+            g.k = (int)mp;
+            g.kind = p.kind;
+            g.y = (uint16_t*)(i ? p.dup : p.dgate);
+            g.ldy = p.k;
+            if ((rc = multiply(g, wk, run, st))) return rc;
         }
     }
     return SPA_OK;

@@ -11,13 +11,16 @@ namespace lin {
 namespace {
 
 // eight elements from k on, zeros from n on; wide: the address is 16-byte aligned wherever k + 8 <= n
-__device__ __forceinline__ void load8(const uint16_t* row, int64_t k, int64_t n, bool wide8, uint16_t (&h)[8]) {
+__device__ __forceinline__ void load8(const uint16_t* row, int64_t k, int64_t n, bool wide8, u4& v) {
     if (wide8 && k + 8 <= n) {
-        *reinterpret_cast<u4*>(h) = *reinterpret_cast<const u4*>(row + k);
+        v = *reinterpret_cast<const u4*>(row + k);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = k + i < n ? row[k + i] : 0;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = k + 2 * i < n ? row[k + 2 * i] : 0, b = k + 2 * i + 1 < n ? row[k + 2 * i + 1] : 0;
+        v[i] = a | (b << 16);
+    }
 }
 
 __global__ __launch_bounds__(256) void k_pack(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t k,
@@ -25,9 +28,9 @@ __global__ __launch_bounds__(256) void k_pack(const uint16_t* __restrict__ src, 
     const int64_t per = kp / 8, total = rows * per;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const int64_t r = i / per, c = (i - r * per) * 8;
-        __align__(16) uint16_t h[8];
+        u4 h;
         load8(src + r * ld, c, k, wide8, h);
-        *reinterpret_cast<u4*>(dst + r * kp + c) = *reinterpret_cast<u4*>(h);
+        *reinterpret_cast<u4*>(dst + r * kp + c) = h;
     }
 }
 
@@ -65,23 +68,24 @@ __global__ __launch_bounds__(256) void k_half_rows(const uint16_t* __restrict__ 
     dst += row * kp;
     float most = 0.f;
     for (int64_t c = threadIdx.x * 8; c < k; c += 2048) {
-        __align__(16) uint16_t h[8];
+        u4 h;
         load8(src, c, k, wide8, h);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, size_of(wide(h[i], kind)));
+        for (int i = 0; i < 4; ++i)
+            most = fmaxf(most, fmaxf(size_of(wide(h[i] & 0xffffu, kind)), size_of(wide(h[i] >> 16, kind))));
     }
     const int e = exponent_for(reduce256<true>(most, lds));
     float sum = 0.f;
     for (int64_t c = threadIdx.x * 8; c < kp; c += 2048) {
-        __align__(16) uint16_t h[8];
+        u4 h;
         load8(src, c, k, wide8, h);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = ldexpf(wide(h[i], kind), -e);
-            sum = fmaf(size_of(v), size_of(v), sum);
-            h[i] = narrow(v, SRC_F16);
+        for (int i = 0; i < 4; ++i) {
+            const float a = ldexpf(wide(h[i] & 0xffffu, kind), -e), b = ldexpf(wide(h[i] >> 16, kind), -e);
+            sum = fmaf(size_of(a), size_of(a), fmaf(size_of(b), size_of(b), sum));
+            h[i] = narrow2(a, b, SRC_F16);
         }
-        *reinterpret_cast<u4*>(dst + c) = *reinterpret_cast<u4*>(h);
+        *reinterpret_cast<u4*>(dst + c) = h;
     }
     if (threadIdx.x == 0) e_out[row] = e;
     if (norm) {
@@ -180,28 +184,34 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     }
 }
 
-// 64 x 64 tiles through LDS: read along a row's columns, written along a column's rows
+// 64 x 64 tiles through LDS: read along a row's columns, written along a column's rows, eight numbers a lane both
+// ways. WIDE: whole groups of eight at 16-byte addresses on the reading side.
+template <bool WIDE>
 __global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
                                                    uint16_t* __restrict__ dst, int64_t ldd, int64_t rp, int64_t tiles_c) {
-    __shared__ uint16_t t[64][66];
+    __shared__ uint16_t t[64][66];                                // 33 words a row: a column's reads meet few banks twice
     const int64_t r0 = blockIdx.x / tiles_c * 64, c0 = blockIdx.x % tiles_c * 64;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int u = i * 256 + threadIdx.x, r = u >> 5, c = (u & 31) * 2;
+    for (int i = 0; i < 2; ++i) {
+        const int u = i * 256 + threadIdx.x, r = u >> 3, c = (u & 7) * 8;
         const int64_t R = r0 + r, C = c0 + c;
-        uint16_t a = 0, b = 0;
-        if (R < rows && C < cols) a = src[R * ld + C];
-        if (R < rows && C + 1 < cols) b = src[R * ld + C + 1];
-        t[r][c] = a;
-        t[r][c + 1] = b;
+        u4 v = {0, 0, 0, 0};
+        if (R < rows && C < cols) load8(src + R * ld, C, cols, WIDE, v);
+        uint32_t* p = reinterpret_cast<uint32_t*>(&t[r][c]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = v[k];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int u = i * 256 + threadIdx.x, c = u >> 5, r = (u & 31) * 2;
+    for (int i = 0; i < 2; ++i) {
+        const int u = i * 256 + threadIdx.x, c = u >> 3, r = (u & 7) * 8;
         const int64_t R = r0 + r, C = c0 + c;
-        if (C < cols && R < rp)                                   // rp is even
-            *reinterpret_cast<uint32_t*>(dst + C * ldd + R) = (uint32_t)t[r][c] | ((uint32_t)t[r + 1][c] << 16);
+        if (C < cols && R < rp) {                                 // rp and ldd are multiples of 8, dst 16-byte aligned
+            u4 v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (uint32_t)t[r + 2 * k][c] | ((uint32_t)t[r + 2 * k + 1][c] << 16);
+            *reinterpret_cast<u4*>(dst + C * ldd + R) = v;
+        }
     }
 }
 
@@ -265,25 +275,33 @@ __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * k; i += gridDim.x * 256ll) p[i / k * ld + i % k] = 0;
 }
 
-// low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 rows a workgroup and one adapter: gridDim.y workgroups
-// take the adapters among the 16 rows in turn, in rising order, most of them finding none. The whole tile is
-// multiplied by the adapter's matrix and its own rows are kept. Each of 8 waves takes every eighth step of
-// 32 k, two steps at a time so that ten loads are under way; 64 ranks at a time, so that x is read once for
-// the usual ranks.
-constexpr int LOW_WAVES = 8;
-template <int KIND, bool WIDE>
+// low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 MT rows a workgroup and one adapter: gridDim.y workgroups take
+// the adapters among the rows in turn, in rising order, most of them finding none. The whole tile is
+// multiplied by the adapter's matrix and its own rows are kept. The 16 waves take 64 k (a line of each row)
+// in turn, the loads of 128 k under way at once; 64 ranks at a time, so that x is read once for the usual ranks.
+// Many rows: gridDim.z workgroups share k, each writing its sums to a place of its own in `low`, and k_low_join
+// adds them in their order.
+constexpr int LOW_WAVES = 16;
+template <int KIND, bool WIDE, int MT>
 __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restrict__ x, int64_t ldx, int64_t m, int64_t k,
                                                         const uint16_t* __restrict__ a_all, const float* __restrict__ scale,
                                                         const int32_t* __restrict__ which, int pool, int rank,
                                                         float* __restrict__ low, int rp, bool wide_x, bool wide_a) {
     __shared__ float part[LOW_WAVES][4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t m0 = (int64_t)blockIdx.x * 16;
+    const int64_t m0 = (int64_t)blockIdx.x * 16 * MT;
     const int row = lane & 15, kc = (lane >> 4) * 8;
-    const int mine = m0 + row < m ? which[m0 + row] : -1;
-    const uint16_t* xr = x + (m0 + row < m ? m0 + row : m - 1) * ldx;
+    int mine[MT];
+    const uint16_t* xr[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t mi = m0 + 16 * t + row;
+        mine[t] = mi < m ? which[mi] : -1;
+        xr[t] = x + (mi < m ? mi : m - 1) * ldx;
+    }
+    low += blockIdx.z * m * rp;
     if (blockIdx.y == 0) {                                        // rows without an adapter: zeros
-        for (int i = threadIdx.x; i < 16 * rp; i += LOW_WAVES * 64) {
+        for (int i = threadIdx.x; i < 16 * MT * rp; i += LOW_WAVES * 64) {
             const int64_t mi = m0 + i / rp;
             if (mi < m) {
                 const int a = which[mi];
@@ -293,79 +311,80 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
     }
     int a = -1;
     for (unsigned turn = 0;; ++turn) {                            // the same in every lane and wave
-        int best = mine > a && mine < pool ? mine : INT32_MAX;
+        int best = INT32_MAX;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (mine[t] > a && mine[t] < pool) best = tmin(best, mine[t]);
 #pragma unroll
         for (int s = 8; s; s >>= 1) best = tmin(best, __shfl_xor(best, s));
         a = __builtin_amdgcn_readfirstlane(best);
         if (a == INT32_MAX) return;
         if (turn == blockIdx.y) break;
     }
+    const int64_t lines = (k + 63) / 64, l0 = lines * blockIdx.z / gridDim.z, l1 = lines * (blockIdx.z + 1) / gridDim.z;
+    const int64_t turned = l1 > l0 ? (int64_t)blockIdx.x * 5 % (l1 - l0) : 0;
     const uint16_t* aa = a_all + (int64_t)a * rank * k;
     for (int r0 = 0; r0 < rp; r0 += 64) {
         const int tiles = tmin(4, (rp - r0) / 16);
         const uint16_t* ar[4];
-        f4 acc[4];
+        f4 acc[MT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int r = r0 + 16 * j + row;                      // ranks beyond the last take its row: they are not kept
             ar[j] = aa + (int64_t)(r < rank ? r : rank - 1) * k;
-            acc[j] = f4{0, 0, 0, 0};
-        }
-        auto fetch = [&](int64_t k0, u4& xv, u4 (&av)[4]) {
-            if (WIDE) {                                           // rows of whole steps at 16-byte addresses
-                const bool in = k0 < k;
-                xv = in ? *reinterpret_cast<const u4*>(xr + k0 + kc) : u4{0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    av[j] = in && j < tiles ? *reinterpret_cast<const u4*>(ar[j] + k0 + kc) : u4{0, 0, 0, 0};
-            } else {
-                __align__(16) uint16_t h[8];
-                load8(xr, k0 + kc, k, wide_x, h);
-                xv = *reinterpret_cast<u4*>(h);
+            for (int t = 0; t < MT; ++t) acc[t][j] = f4{0, 0, 0, 0};
+        }
+        constexpr int U = MT == 1 ? 4 : 2;                        // steps of 32 k at once
+        for (int64_t l = wave; l < l1 - l0; l += LOW_WAVES * (U / 2)) {
+            u4 xv[U][MT], av[U][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                // workgroups begin at different lines: rows of a power of two apart lie in few memory channels
+                const int64_t i = l + LOW_WAVES * (u / 2), at = l0 + (i + turned < l1 - l0 ? i + turned : i + turned - (l1 - l0));
+                const int64_t k0 = at * 64 + 32 * (u % 2) + kc;
+                const bool in = i < l1 - l0 && k0 < k;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    xv[u][t] = u4{0, 0, 0, 0};
+                    if (in) {
+                        if (WIDE) xv[u][t] = *reinterpret_cast<const u4*>(xr[t] + k0);   // rows of whole steps at 16-byte addresses
+                        else load8(xr[t], k0, k, wide_x, xv[u][t]);
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (j < tiles) load8(ar[j], k0 + kc, k, wide_a, h);
-                    av[j] = *reinterpret_cast<u4*>(h);
+                    av[u][j] = u4{0, 0, 0, 0};
+                    if (in && j < tiles) {
+                        if (WIDE) av[u][j] = *reinterpret_cast<const u4*>(ar[j] + k0);
+                        else load8(ar[j], k0, k, wide_a, av[u][j]);
+                    }
                 }
             }
-        };
-        auto mul = [&](u4 xv, const u4 (&av)[4]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j >= tiles) break;
-                if (KIND == SRC_BF16)
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, xv), __builtin_bit_cast(bf8, av[j]), acc[j], 0, 0, 0);
-                else
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, xv), __builtin_bit_cast(hf8, av[j]), acc[j], 0, 0, 0);
-            }
-        };
-        constexpr int STEP = LOW_WAVES * 32;
-        u4 x0, x1, a0[4], a1[4];
-        fetch(wave * 32, x0, a0);
-        fetch(wave * 32 + STEP, x1, a1);
-        for (int64_t k0 = wave * 32; k0 < k; k0 += 2 * STEP) {
-            u4 x2, x3, a2[4], a3[4];
-            fetch(k0 + 2 * STEP, x2, a2);
-            fetch(k0 + 3 * STEP, x3, a3);
-            mul(x0, a0);
-            mul(x1, a1);
-            x0 = x2;
-            x1 = x3;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                a0[j] = a2[j];
-                a1[j] = a3[j];
-            }
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= tiles) break;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        if (KIND == SRC_BF16)
+                            acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, xv[u][t]), __builtin_bit_cast(bf8, av[u][j]), acc[t][j], 0, 0, 0);
+                        else
+                            acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, xv[u][t]), __builtin_bit_cast(hf8, av[u][j]), acc[t][j], 0, 0, 0);
+                    }
+                }
         }
-        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int t = 0; t < MT; ++t) {
+            __syncthreads();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) part[wave][j][(4 * (lane >> 4) + c) * 16 + row] = acc[j][c];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 1024; i += LOW_WAVES * 64) {
-            const int j = i >> 8, mr = (i >> 4) & 15, r = r0 + 16 * j + (i & 15);
-            const int64_t mi = m0 + mr;
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) part[wave][j][(4 * (lane >> 4) + c) * 16 + row] = acc[t][j][c];
+            __syncthreads();
+            const int i = threadIdx.x, j = i >> 8, mr = (i >> 4) & 15, r = r0 + 16 * j + (i & 15);
+            const int64_t mi = m0 + 16 * t + mr;
             if (mi < m && r < rp && which[mi] == a) {
                 float v = 0.f;
 #pragma unroll
@@ -373,6 +392,14 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
                 low[mi * rp + r] = r < rank ? scale[a] * v : 0.f;
             }
         }
+    }
+}
+
+__global__ __launch_bounds__(256) void k_low_join(float* low, int64_t n, int pieces) {
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        float v = low[i];
+        for (int p = 1; p < pieces; ++p) v += low[p * n + i];
+        low[i] = v;
     }
 }
 
@@ -426,7 +453,8 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
                 hipStream_t st) {
     const int64_t tr = (rp + 63) / 64, tc = (cols + 63) / 64;
-    hipLaunchKernelGGL(k_transpose, dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
+    if (aligned8(src, ld)) hipLaunchKernelGGL((k_transpose<true>), dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
+    else hipLaunchKernelGGL((k_transpose<false>), dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
@@ -449,19 +477,32 @@ int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st) 
 
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
              const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st) {
-    const dim3 grid((unsigned)((m + 15) / 16), (unsigned)(pool < 16 ? pool : 16)), block(LOW_WAVES * 64);
+    const int pieces = low_pieces(m, k);
+    const int64_t rows = pieces > 1 ? 32 : 16;
+    const dim3 grid((unsigned)((m + rows - 1) / rows), (unsigned)(pool < rows ? pool : rows), (unsigned)pieces), block(LOW_WAVES * 64);
     const bool wx = aligned8(x, ldx), wa = aligned8(a, k), whole = wx && wa && k % 32 == 0;
-#define SPA_LOW(KIND, WIDE) \
-    hipLaunchKernelGGL((k_low<KIND, WIDE>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, wx, wa)
+#define SPA_LOW(KIND, WIDE, MT) \
+    hipLaunchKernelGGL((k_low<KIND, WIDE, MT>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, wx, wa)
+#define SPA_LOW_ROWS(KIND, WIDE)                \
+    do {                                        \
+        if (rows == 32) SPA_LOW(KIND, WIDE, 2); \
+        else SPA_LOW(KIND, WIDE, 1);            \
+    } while (0)
     if (kind == SRC_BF16) {
-        if (whole) SPA_LOW(SRC_BF16, true);
-        else SPA_LOW(SRC_BF16, false);
+        if (whole) SPA_LOW_ROWS(SRC_BF16, true);
+        else SPA_LOW_ROWS(SRC_BF16, false);
     } else {
-        if (whole) SPA_LOW(SRC_F16, true);
-        else SPA_LOW(SRC_F16, false);
+        if (whole) SPA_LOW_ROWS(SRC_F16, true);
+        else SPA_LOW_ROWS(SRC_F16, false);
     }
+#undef SPA_LOW_ROWS
 #undef SPA_LOW
     SPA_HIP_TRY(hipGetLastError());
+    if (pieces > 1) {
+        const int64_t n = m * rp, groups = (n + 255) / 256;
+        hipLaunchKernelGGL(k_low_join, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, low, n, pieces);
+        SPA_HIP_TRY(hipGetLastError());
+    }
     return SPA_OK;
 }
 

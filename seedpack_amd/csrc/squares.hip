@@ -45,7 +45,7 @@ struct Sq {
     bool wide8;
 };
 
-template <int KIND>
+template <int KIND, bool SPLIT>
 __global__ __launch_bounds__(256) void k_squares(const Sq q) {
     __shared__ float join[3][COLS];
     __shared__ int list[IDS];
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
     const int64_t r0 = run * q.run, r1 = tmin(q.rows, r0 + q.run), left = q.cols - c0;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     uint32_t hits = 0;
-    if (!q.which) {
+    if constexpr (!SPLIT) {
 #pragma unroll 4
         for (int64_t r = r0 + wave; r < r1; r += 4)
             if (left > 0) add8<KIND>(q.x, r * q.ld + c0, left, q.wide8, s, 1.f);
@@ -100,9 +100,25 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
                 at += __popcll(mask[i]);
             }
             __syncthreads();
-#pragma unroll 8
-            for (int i = wave; i < total; i += 4)
-                if (left > 0) add8<KIND>(q.x, (b + list[i]) * q.ld + c0, left, q.wide8, s, (float)times[i]);
+            if (q.wide8 && left >= 8) {
+                for (int i = wave; i < total; i += 32) {          // eight rows' loads under way at once
+                    float v[8][8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) load_weights<8>(q.x, KIND, (b + list[tmin(i + 4 * u, total - 1)]) * q.ld + c0, v[u]);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const bool in = i + 4 * u < total;
+                        const float t = in ? (float)times[i + 4 * u] : 0.f;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const float w = in ? v[u][c] : 0.f;
+                            s[c] = fmaf(w * t, w, s[c]);
+                        }
+                    }
+                }
+            } else if (left > 0) {
+                for (int i = wave; i < total; i += 4) add8<KIND>(q.x, (b + list[i]) * q.ld + c0, left, q.wide8, s, (float)times[i]);
+            }
         }
         if (piece % tiles == 0) {
 #pragma unroll
@@ -145,11 +161,11 @@ __global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
 }
 
 // Rows of a run. Whole: enough workgroups to fill the device (about 1024 of them), at least 16 rows each. By
-// expert: 512 rows, so that an expert which gets most of the rows is still spread over many workgroups
+// expert: 1024 rows, so that an expert which gets most of the rows is still spread over many workgroups
 // (with runs of 8192 rows the first of 64 unlike experts kept 16384 x 4096 busy for 202 us).
 int64_t run_rows(int64_t rows, int64_t cols, int64_t experts, bool by_expert) {
     const int64_t tiles = (cols + COLS - 1) / COLS * experts;
-    int64_t run = 512;
+    int64_t run = IDS;
     if (!by_expert) {
         const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
         run = (rows + runs - 1) / runs;
@@ -213,9 +229,15 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     const int64_t tiles = (cols + COLS - 1) / COLS;
     if (tiles * q.runs * q.experts > INT32_MAX) return fail(SPA_ERR_ARG, "spa_add_squares: %lld x %lld is too large", (long long)rows, (long long)cols);
     const dim3 grid((unsigned)(tiles * q.runs * q.experts));
-    if (src_kind == SPA_SRC_BF16) hipLaunchKernelGGL((k_squares<SRC_BF16>), grid, dim3(256), 0, st, q);
-    else if (src_kind == SPA_SRC_F16) hipLaunchKernelGGL((k_squares<SRC_F16>), grid, dim3(256), 0, st, q);
-    else hipLaunchKernelGGL((k_squares<SRC_F32>), grid, dim3(256), 0, st, q);
+#define SPA_SQUARES(KIND)                                                                                   \
+    do {                                                                                                    \
+        if (which) hipLaunchKernelGGL((k_squares<KIND, true>), grid, dim3(256), 0, st, q);                  \
+        else hipLaunchKernelGGL((k_squares<KIND, false>), grid, dim3(256), 0, st, q);                       \
+    } while (0)
+    if (src_kind == SPA_SRC_BF16) SPA_SQUARES(SRC_BF16);
+    else if (src_kind == SPA_SRC_F16) SPA_SQUARES(SRC_F16);
+    else SPA_SQUARES(SRC_F32);
+#undef SPA_SQUARES
     SPA_HIP_TRY(hipGetLastError());
     const int64_t groups = ((int64_t)q.experts * cols + 255) / 256;
     hipLaunchKernelGGL(k_squares_join, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, q);
