@@ -369,7 +369,7 @@ int aligned(const FewArgs& a, hipStream_t st) {
 
 template <int T>
 int pick(const Few& f, uint16_t* frags, hipStream_t st) {
-    FewArgs a{f, (int64_t)f.k / Unit<T>::QK * Unit<T>::BS, f.x};
+    FewArgs a{f, f.rowbytes, f.x};
     if (f.m > 1) {
         const int tiles = few_tiles(T, f.m), lanes = tiles * (f.k / 32) * 64;
         hipLaunchKernelGGL((k_fragments<Unit<T>::HALVES>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, f.x, f.ldx, f.m, f.k,

@@ -125,15 +125,18 @@ __global__ __launch_bounds__(WAVES * 64) void k_few(const FewArgs a, DQ t) {
     finish<WAVES, MT, TWO, false>(f, n0, reinterpret_cast<float*>(mem), acc, Never());
 }
 
-// 16-bit weights (rows of a multiple of 32 k, 16-byte aligned): fragments straight from memory, the loads of
-// four steps under way at once
-template <int WKIND, int KIND, int MT, bool TWO>
-__global__ __launch_bounds__(WAVES * 64) void k_few16(const FewArgs a) {
+// 16-bit weights: fragments straight from memory, the loads of four steps under way at once. LINED: rows of whole
+// steps at 16-byte addresses. Other rows begin at any number: their 16-byte loads cross words, and the step that
+// reaches past a row's end is read number by number, with zeros (the inputs hold zeros there too, but the next
+// row's weights may be infinite).
+template <int WKIND, int KIND, int MT, bool TWO, bool LINED, int W>
+__global__ __launch_bounds__(W * 64) void k_few16(const FewArgs a) {
     const Few& f = a.f;
-    __shared__ float red[WAVES * (1 + TWO) * MT * 256];
-    constexpr int U = MT > 2 ? 2 : 4, STEP = WAVES * 32;
+    __shared__ float red[W * (1 + TWO) * MT * 256];
+    constexpr int U = MT > 2 ? 2 : 4, STEP = W * 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
-    const int64_t wrow = (int64_t)tmin(n0 + (lane & 15), f.n - 1) * a.rowbytes + 16 * (lane >> 4);
+    const int kl = 8 * (lane >> 4), cols = (int)(a.rowbytes / 2);
+    const int64_t wrow = (int64_t)tmin(n0 + (lane & 15), f.n - 1) * a.rowbytes;
     f4 acc[1 + TWO][MT];
 #pragma unroll
     for (int s = 0; s <= TWO; ++s)
@@ -147,7 +150,21 @@ __global__ __launch_bounds__(WAVES * 64) void k_few16(const FewArgs a) {
             if (k >= f.k) break;
             load_x<MT>(f, k, x[u]);
 #pragma unroll
-            for (int h = 0; h <= TWO; ++h) w[u][h] = *reinterpret_cast<const u4*>((h ? f.w1 : f.w0) + wrow + 2 * k);
+            for (int h = 0; h <= TWO; ++h) {
+                const uint8_t* p = (h ? f.w1 : f.w0) + wrow + 2 * (k + kl);
+                if (LINED) {
+                    w[u][h] = *reinterpret_cast<const u4*>(p);
+                } else if (k + 32 <= cols) {
+                    __builtin_memcpy(&w[u][h], p, 16);
+                } else {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t lo = k + kl + 2 * i < cols ? q[2 * i] : 0, hi = k + kl + 2 * i + 1 < cols ? q[2 * i + 1] : 0;
+                        w[u][h][i] = lo | (hi << 16);
+                    }
+                }
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -169,7 +186,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_few16(const FewArgs a) {
             }
         }
     }
-    finish<WAVES, MT, TWO, false>(f, n0, red, acc, Never());
+    finish<W, MT, TWO, false>(f, n0, red, acc, Never());
 }
 
 template <int T, int QK, int BS, int KIND, bool TWO>
@@ -177,9 +194,23 @@ int launch(const FewArgs& a, DQ t, hipStream_t st) {
     const dim3 grid((unsigned)((a.f.n + 15) / 16)), block(WAVES * 64);
     if constexpr (T == 1 || T == 30) {
         constexpr int WK = T == 1 ? SRC_F16 : SRC_BF16;
-        if (a.f.m <= 16) hipLaunchKernelGGL((k_few16<WK, KIND, 1, TWO>), grid, block, 0, st, a);
-        else if (a.f.m <= 32) hipLaunchKernelGGL((k_few16<WK, KIND, 2, TWO>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_few16<WK, KIND, 4, TWO>), grid, block, 0, st, a);
+        const bool lined = a.rowbytes == 2 * (int64_t)a.f.k && ((reinterpret_cast<uintptr_t>(a.f.w0) | reinterpret_cast<uintptr_t>(a.f.w1)) & 15) == 0;
+        // few weight rows fill the device with waves only if more of them share a row's k (one row of 4060 x 5795
+        // with 8 waves: 80 us)
+#define SPA_FEW16(MT, W)                                                                                    \
+    do {                                                                                                    \
+        if (lined) hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, true, W>), grid, dim3(W * 64), 0, st, a); \
+        else hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, false, W>), grid, dim3(W * 64), 0, st, a);      \
+    } while (0)
+        if (a.f.m <= 16) {
+            if (a.f.n < 8192) SPA_FEW16(1, 16);
+            else SPA_FEW16(1, 8);
+        } else if (a.f.m <= 32) {
+            SPA_FEW16(2, 8);
+        } else {
+            SPA_FEW16(4, 8);
+        }
+#undef SPA_FEW16
     } else {
         if (a.f.m <= 16) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 1, TWO>), grid, block, 0, st, a, t);
         else if (a.f.m <= 32) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 2, TWO>), grid, block, 0, st, a, t);
@@ -211,7 +242,7 @@ int few(const Few& f, uint16_t* frags, hipStream_t st) {
     switch (f.type) {
 #define SPA_FEW(T, QK, BS)                                 \
     case T:                                                \
-        a.rowbytes = (int64_t)f.k / QK * BS;               \
+        a.rowbytes = f.rowbytes;                           \
         return pick<T, QK, BS>(a, t, st);
         SPA_FEW(1, 1, 2) SPA_FEW(30, 1, 2)
         SPA_FEW(3, 32, 20) SPA_FEW(6, 32, 22) SPA_FEW(7, 32, 24)

@@ -497,37 +497,28 @@ __global__ __launch_bounds__(256) void k_join(const Gemm g) {
     }
 }
 
-// What a product takes: a tile of 256 x 256 is a third faster for its work than two of 128 x 128 on a compute unit,
+// What a product takes: a tile of 256 x 256 is half again as fast as two of 128 x 128 on a compute unit,
 // but the device has 256 units and waits for its last round. Times of 64 k of a round, in units of 1/100 us on one
-// MI355X: 256 x 256 one to a unit 170; 128 x 128 two to a unit 100, alone on it 85. In pieces of k with too
+// MI355X: 256 x 256 one to a unit 170; 128 x 128 two to a unit 126, alone on it 85. In pieces of k with too
 // few tiles: each adds 8 bytes of traffic an output and matrix (about 5 TB/s) and the joining launch.
 struct Plan {
     bool big;
     int pieces;
+    int64_t cost;
 };
 Plan plan(const Gemm& g) {
     const bool two = g.w1 != nullptr;
     const int64_t steps = g.k / BK, m = g.m, n = g.n;
     const int64_t nb = (n * (two ? 2 : 1) + 255) / 256 * ((m + 255) / 256), ns = (n * (two ? 2 : 1) + 127) / 128 * ((m + 127) / 128);
-    auto small = [](int64_t tiles, int64_t st) { return tiles <= 256 ? st * 85 : (tiles + 511) / 512 * st * 100; };
-    Plan best{true, 1};
-    int64_t cost = (nb + 255) / 256 * steps * 170;
-    if (small(ns, steps) < cost) {
-        best = Plan{false, 1};
-        cost = small(ns, steps);
-    }
+    auto small = [](int64_t tiles, int64_t st) { return tiles <= 256 ? st * 85 : (tiles + 511) / 512 * st * 126; };
+    Plan best{true, 1, (nb + 255) / 256 * steps * 170};
+    if (small(ns, steps) < best.cost) best = Plan{false, 1, small(ns, steps)};
     for (int p = 2; p <= g.most && p * 4 <= steps; ++p) {
         const int64_t st = (steps + p - 1) / p, join = 600 + (int64_t)(m * n * (two ? 2 : 1) * 8 * p / 50000);
         // in pieces the two matrices are products of their own
         const int64_t b = (n + 255) / 256 * (two ? 2 : 1) * ((m + 255) / 256) * p, s = (n + 127) / 128 * (two ? 2 : 1) * ((m + 127) / 128) * p;
-        if ((b + 255) / 256 * st * 170 + join < cost) {
-            best = Plan{true, p};
-            cost = (b + 255) / 256 * st * 170 + join;
-        }
-        if (small(s, st) + join < cost) {
-            best = Plan{false, p};
-            cost = small(s, st) + join;
-        }
+        if ((b + 255) / 256 * st * 170 + join < best.cost) best = Plan{true, p, (b + 255) / 256 * st * 170 + join};
+        if (small(s, st) + join < best.cost) best = Plan{false, p, small(s, st) + join};
     }
     return best;
 }
@@ -562,6 +553,16 @@ int64_t gemm_part(const Gemm& g) {
     q.most = GEMM_PIECES;
     const Plan p = plan(q);
     return p.pieces > 1 ? (int64_t)p.pieces * (g.w1 ? 2 : 1) * g.m * g.n : 0;
+}
+
+int64_t gemm_cost(const Gemm& g) {
+    Gemm q = g;
+    q.most = GEMM_PIECES;
+    return plan(q).cost;
+}
+
+int gemm_pieces(const Gemm& g, hipStream_t st) {
+    return g.half == SRC_BF16 ? launch<SRC_BF16, 128, 128, 2, 2, OUT_PART>(g, st) : launch<SRC_F16, 128, 128, 2, 2, OUT_PART>(g, st);
 }
 
 int gemm(const Gemm& g, hipStream_t st) { return g.half == SRC_BF16 ? form<SRC_BF16>(g, st) : form<SRC_F16>(g, st); }

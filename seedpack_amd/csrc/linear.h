@@ -108,7 +108,13 @@ __device__ __forceinline__ float expand(const Expand& ex, int m, int n, int coun
             }
         }
     } else {
-        for (int r = 0; r < ex.rank; ++r) t = fmaf(z[r], wide(b[r], ex.kind), t);
+        for (int r = 0; r < ex.rank; r += 8) {                    // eight loads at once; those beyond the last are dropped
+            uint16_t h[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) h[c] = b[tmin(r + c, ex.rank - 1)];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) t = r + c < ex.rank ? fmaf(z[r + c], wide(h[c], ex.kind), t) : t;
+        }
     }
     return t;
 }
@@ -142,6 +148,10 @@ struct Gemm {
     int pieces;
 };
 int64_t gemm_part(const Gemm& g);
+// what a product is expected to take, in hundredths of a microsecond
+int64_t gemm_cost(const Gemm& g);
+// the pieces alone, left in part as [piece][m][n]; g.pieces of them
+int gemm_pieces(const Gemm& g, hipStream_t st);
 int gemm(const Gemm& g, hipStream_t st);
 
 // ---- few rows (few.hip)
@@ -149,7 +159,8 @@ struct Few {
     int type;                 // the weights' ggml type (1 F16, 30 BF16, or a block type)
     const uint8_t *w0, *w1;   // w1 for the gated form, else null
     int64_t wbytes;           // bytes of each matrix
-    int n, k;
+    int64_t rowbytes;         // and of a row of it
+    int n, k;                 // k: whole steps of 32, x zero beyond the weights' own
     const uint16_t* x;        // [m][k], rows of ldx (a multiple of 8), 16-byte aligned
     int64_t ldx;
     int m, kind;
@@ -175,11 +186,11 @@ inline int64_t few_fragments(int type, int64_t m, int64_t kp) { return coded(typ
 // ---- rows (rows.hip)
 // rows of a 16-bit matrix copied into rows of kp (a multiple of 64), zeros beyond k
 int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, hipStream_t st);
-// the same into binary16 with a power of two taken out of each row (e), and the row's 2-norm as it was (or null)
-int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e,
+// the same into binary16, rows of ldd, with a power of two taken out of each row (e), and the row's 2-norm as it was (or null)
+int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e,
               float* norm, hipStream_t st);
 // the same from a block type
-int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, float* norm,
+int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e, float* norm,
                 hipStream_t st);
 // dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (rp and ldd multiples of 8)
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
@@ -189,10 +200,13 @@ int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uin
 int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const float* n0,
                    const int32_t* e0, const float* n1, const int32_t* e1, void* top, int32_t* e, hipStream_t st);
 int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st);
-// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]; low has room for low_pieces() of it
-inline int low_pieces(int64_t m, int64_t k) { return m > 256 && k >= 2048 ? 4 : 1; }
+// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
              const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st);
+
+// the same from the pieces of x [A_0; A_1; ..]^T (gemm_pieces)
+int low_pick(const float* part, int pieces, const float* scale, const int32_t* which, int64_t m, int pool, int rank, float* low, int rp,
+             hipStream_t st);
 
 }  // namespace lin
 }  // namespace spa

@@ -8,7 +8,8 @@ namespace spa {
 namespace lin {
 namespace {
 
-// rows of the inner matrices lie 128 bytes more than whole steps apart
+// Rows of the inner matrices lie 128 bytes more than whole steps apart: at powers of two, the rows of a tile share few
+// of the memory's channels (4096 x 4096 x 24576: 660 to 616 us)
 constexpr int64_t PAD = 64;
 int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 
@@ -69,7 +70,8 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
     const int64_t kp = up64(k);
     const bool same = is16(type) && kind_of(type) == kind;
     o.half = same ? kind : SRC_F16;
-    uint16_t* xp = wk.take<uint16_t>(m * kp);
+    const int64_t ldd = same ? kp : kp + PAD;
+    uint16_t* xp = wk.take<uint16_t>(m * ldd);
     int rc;
     if (same) {
         o.x = (const uint16_t*)x;
@@ -101,16 +103,16 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
         o.n0 = wk.take<float>(n);
         o.n1 = wk.take<float>(n);
     }
-    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, o.xe, o.norm, st))) return rc;
+    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, ldd, o.xe, o.norm, st))) return rc;
     o.x = xp;
-    o.ldx = o.ldw = kp;
+    o.ldx = o.ldw = ldd;
     for (int i = 0; i < (w1 ? 2 : 1); ++i) {
-        uint16_t* p = wk.take<uint16_t>(n * kp);
+        uint16_t* p = wk.take<uint16_t>(n * ldd);
         int32_t* e = wk.take<int32_t>(n);
         const void* w = i ? w1 : w0;
         if (run) {
-            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, e, i ? o.n1 : o.n0, st)
-                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, e, i ? o.n1 : o.n0, st);
+            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, ldd, e, i ? o.n1 : o.n0, st)
+                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, ldd, e, i ? o.n1 : o.n0, st);
             if (rc) return rc;
         }
         (i ? o.w1 : o.w0) = p;
@@ -119,8 +121,8 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
     return SPA_OK;
 }
 
-// Few rows: the weights as they lie. Rows are padded where a 16-byte load of x (or of 16-bit weights) or
-// a step of 32 k would not fit; for 16-bit weights that are copied too.
+// Few rows: the weights as they lie. The inputs are copied where their rows are not whole steps of 32 at 16-byte
+// addresses.
 int few_operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64_t n, int64_t k, const void* x, int64_t m,
                  int64_t ldx, Few& f, uint16_t*& frags, hipStream_t st) {
     const int64_t kp = (k + 31) / 32 * 32;
@@ -136,21 +138,12 @@ int few_operands(Work& wk, bool run, int type, const void* w0, const void* w1, i
     }
     f.w0 = (const uint8_t*)w0;
     f.w1 = (const uint8_t*)w1;
-    if (kp != k) {                                               // block types have whole steps
-        uint16_t* p0 = wk.take<uint16_t>(n * kp);
-        uint16_t* p1 = w1 ? wk.take<uint16_t>(n * kp) : nullptr;
-        if (run) {
-            if ((rc = pack_rows((const uint16_t*)w0, k, n, k, p0, kp, st))) return rc;
-            if (w1 && (rc = pack_rows((const uint16_t*)w1, k, n, k, p1, kp, st))) return rc;
-        }
-        f.w0 = (const uint8_t*)p0;
-        f.w1 = (const uint8_t*)p1;
-    }
     f.type = type;
     f.n = (int)n;
     f.k = (int)kp;
     f.m = (int)m;
-    f.wbytes = weight_bytes(type, n, kp);
+    f.wbytes = weight_bytes(type, n, k);
+    f.rowbytes = weight_bytes(type, 1, k);
     return SPA_OK;
 }
 
@@ -194,33 +187,85 @@ struct Project {
     const int32_t* which;
 };
 
+// Many rows' first products as one product with every adapter of the pool, where it is small enough that
+// the rows' other adapters cost less than reading x a few lanes at a time (2053 rows of 12288, 4 adapters of rank
+// 64: 55 us row by row): 128 x 128 tiles in pieces of k that fill the device.
+int64_t low_as_product(const Project& p) {
+    const int64_t width = p.pool * p.rank;
+    if (p.m <= 256 || width > 1024 || p.k % 64 || p.k < 2048) return 0;
+    const int64_t tiles = (p.m + 127) / 128 * ((width + 127) / 128), pieces = tiles < 256 ? 256 / tiles : 1;
+    return pieces < p.k / 256 ? pieces : p.k / 256;
+}
+
+// rows beyond whole tiles that the few-rows form takes, because the tiles they would need cost more: its weights at
+// about 2 TB/s and two launches. The types whose few-rows form decodes in registers are left out.
+int64_t tail_rows(const Gemm& g, int type) {
+    if (!coded(type) && !is16(type)) return 0;
+    const int64_t bytes = weight_bytes(type, g.n, g.k) * (g.w1 ? 2 : 1), extra = 1500 + bytes / 20000;
+    int64_t best = 0, cost = gemm_cost(g);
+    for (int tile = 256; tile >= 128; tile /= 2) {
+        const int t = g.m % tile;
+        if (t == 0 || t > 16 || t == g.m) continue;
+        Gemm q = g;
+        q.m = g.m - t;
+        if (gemm_cost(q) + extra < cost) {
+            best = t;
+            cost = gemm_cost(q) + extra;
+        }
+    }
+    return best;
+}
+
 int project(const Project& p, Work& wk, bool run, hipStream_t st) {
     Expand ex{};
     int rc;
     if (p.pool) {
         ex.rank = (int)p.rank;
         ex.rp = (int)((p.rank + 15) / 16 * 16);
-        float* low = wk.take<float>(p.m * ex.rp * low_pieces(p.m, p.k));
+        float* low = wk.take<float>(p.m * ex.rp);
         ex.low = low;
         ex.b = (const uint16_t*)p.b;
         ex.which = p.which;
         ex.pool = (int)p.pool;
         ex.kind = p.kind;
         ex.wide_b = p.rank % 8 == 0 && on(p.b, 16);
-        if (run && (rc = low_rows((const uint16_t*)p.x, p.ldx, p.kind, p.m, p.k, (const uint16_t*)p.a, p.scale, p.which, (int)p.pool,
-                                  (int)p.rank, low, ex.rp, st)))
+        const int64_t pieces = low_as_product(p);
+        float* part = wk.take<float>(pieces * p.m * p.pool * p.rank);
+        if (run && pieces && on(p.x, 16) && on(p.a, 16) && p.ldx % 8 == 0 && p.ldx <= (1 << 22)) {
+            Gemm g{};
+            g.half = p.kind;
+            g.x = (const uint16_t*)p.x;
+            g.ldx = p.ldx;
+            g.w0 = (const uint16_t*)p.a;
+            g.ldw = p.k;
+            g.m = (int)p.m;
+            g.n = (int)(p.pool * p.rank);
+            g.k = (int)p.k;
+            g.part = part;
+            g.pieces = (int)pieces;
+            if ((rc = gemm_pieces(g, st))) return rc;
+            if ((rc = low_pick(part, (int)pieces, p.scale, p.which, p.m, (int)p.pool, (int)p.rank, low, ex.rp, st))) return rc;
+        } else if (run && (rc = low_rows((const uint16_t*)p.x, p.ldx, p.kind, p.m, p.k, (const uint16_t*)p.a, p.scale, p.which,
+                                         (int)p.pool, (int)p.rank, low, ex.rp, st))) {
             return rc;
+        }
     }
-    if (p.m <= FEW_ROWS) {
+    auto few_rows = [&](int64_t from, int64_t m) {
         Few f{};
         uint16_t* frags;
-        if ((rc = few_operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.x, p.m, p.ldx, f, frags, st)) || !run) return rc;
+        const int r = few_operands(wk, run, p.type, p.w, nullptr, p.n, p.k, (const uint16_t*)p.x + from * p.ldx, m, p.ldx, f, frags, st);
+        if (r || !run) return r;
         f.kind = p.kind;
-        f.y = (uint16_t*)p.y;
+        f.y = (uint16_t*)p.y + from * p.ldy;
         f.ldy = p.ldy;
         f.ex = ex;
+        if (ex.low) {
+            f.ex.low += from * ex.rp;
+            f.ex.which += from;
+        }
         return few(f, frags, st);
-    }
+    };
+    if (p.m <= FEW_ROWS) return few_rows(0, p.m);
     Operands o;
     if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
     Gemm g = gemm_of(o, p.m, p.n, p.k);
@@ -228,7 +273,10 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
     g.y = (uint16_t*)p.y;
     g.ldy = p.ldy;
     g.ex = ex;
-    return multiply(g, wk, run, st);
+    const int64_t tail = tail_rows(g, p.type);
+    g.m -= (int)tail;
+    if ((rc = multiply(g, wk, run, st))) return rc;
+    return tail ? few_rows(p.m - tail, tail) : SPA_OK;
 }
 
 struct Gated {
@@ -251,16 +299,18 @@ const void* const SOME = reinterpret_cast<const void*>(256);
 int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
     int rc;
     const void* up = run ? p.up : SOME;
-    if (p.m <= FEW_ROWS) {
+    auto few_rows = [&](int64_t from, int64_t m) {
         Few f{};
         uint16_t* frags;
-        if ((rc = few_operands(wk, run, p.type, p.gate, up, p.n, p.k, p.x, p.m, p.ldx, f, frags, st)) || !run) return rc;
+        const int r = few_operands(wk, run, p.type, p.gate, up, p.n, p.k, (const uint16_t*)p.x + from * p.ldx, m, p.ldx, f, frags, st);
+        if (r || !run) return r;
         f.kind = p.kind;
-        f.y = (uint16_t*)p.h;
+        f.y = (uint16_t*)p.h + from * p.ldh;
         f.ldy = p.ldh;
         f.act = p.act;
         return few(f, frags, st);
-    }
+    };
+    if (p.m <= FEW_ROWS) return few_rows(0, p.m);
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
     Gemm g = gemm_of(o, p.m, p.n, p.k);
@@ -268,7 +318,10 @@ int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
     g.y = (uint16_t*)p.h;
     g.ldy = p.ldh;
     g.act = p.act;
-    return multiply(g, wk, run, st);
+    const int64_t tail = tail_rows(g, p.type);
+    g.m -= (int)tail;
+    if ((rc = multiply(g, wk, run, st))) return rc;
+    return tail ? few_rows(p.m - tail, tail) : SPA_OK;
 }
 
 // grad = [dG | dU] in one matrix of 2 np columns; dx = grad [Wg; Wu] is then one product over 2 np, with the

@@ -10,10 +10,10 @@ namespace spa {
 namespace lin {
 namespace {
 
-// eight elements from k on, zeros from n on; wide: the address is 16-byte aligned wherever k + 8 <= n
-__device__ __forceinline__ void load8(const uint16_t* row, int64_t k, int64_t n, bool wide8, u4& v) {
-    if (wide8 && k + 8 <= n) {
-        v = *reinterpret_cast<const u4*>(row + k);
+// eight elements from k on, zeros from n on. The address may be any element's: gfx950 loads 16 bytes from any byte.
+__device__ __forceinline__ void load8(const uint16_t* row, int64_t k, int64_t n, u4& v) {
+    if (k + 8 <= n) {
+        __builtin_memcpy(&v, row + k, 16);
         return;
     }
 #pragma unroll
@@ -24,19 +24,19 @@ __device__ __forceinline__ void load8(const uint16_t* row, int64_t k, int64_t n,
 }
 
 __global__ __launch_bounds__(256) void k_pack(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t k,
-                                              uint16_t* __restrict__ dst, int64_t kp, bool wide8) {
+                                              uint16_t* __restrict__ dst, int64_t kp) {
     const int64_t per = kp / 8, total = rows * per;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const int64_t r = i / per, c = (i - r * per) * 8;
         u4 h;
-        load8(src + r * ld, c, k, wide8, h);
+        load8(src + r * ld, c, k, h);
         *reinterpret_cast<u4*>(dst + r * kp + c) = h;
     }
 }
 
 // a workgroup's largest or total float, the same in every lane; in an order of its own shape only
-template <bool MAX>
-__device__ __forceinline__ float reduce256(float v, float* lds) {
+template <bool MAX, int LANES = 256>
+__device__ __forceinline__ float reduce(float v, float* lds) {
 #pragma unroll
     for (int s = 32; s; s >>= 1) {
         const float o = __shfl_xor(v, s);
@@ -45,7 +45,10 @@ __device__ __forceinline__ float reduce256(float v, float* lds) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    return MAX ? fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])) : (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < LANES / 64; ++w) v = MAX ? fmaxf(v, lds[w]) : v + lds[w];
+    return v;
 }
 
 __device__ __forceinline__ float size_of(float v) {              // |v|, zero for infinities and NaN
@@ -59,26 +62,42 @@ __device__ __forceinline__ int exponent_for(float top) {
     frexpf(top, &e);
     return e - 15;
 }
-__global__ __launch_bounds__(256) void k_half_rows(const uint16_t* __restrict__ src, int kind, int64_t ld, int64_t k,
-                                                   uint16_t* __restrict__ dst, int64_t kp, int32_t* __restrict__ e_out,
-                                                   float* __restrict__ norm, bool wide8) {
-    __shared__ float lds[4];
+// A row of up to KEEP numbers a lane stays in registers between the search for its largest and its conversion;
+// KEEP = 0: any row, read twice.
+template <int KEEP, int LANES>
+__global__ __launch_bounds__(LANES) void k_half_rows(const uint16_t* __restrict__ src, int kind, int64_t ld, int64_t k,
+                                                   uint16_t* __restrict__ dst, int64_t kp, int64_t ldd, int32_t* __restrict__ e_out,
+                                                   float* __restrict__ norm) {
+    __shared__ float lds[LANES / 64];
     const int64_t row = blockIdx.x;
     src += row * ld;
-    dst += row * kp;
+    dst += row * ldd;
     float most = 0.f;
-    for (int64_t c = threadIdx.x * 8; c < k; c += 2048) {
-        u4 h;
-        load8(src, c, k, wide8, h);
+    u4 held[KEEP ? KEEP / 8 : 1];
+    auto largest = [&](const u4& h) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             most = fmaxf(most, fmaxf(size_of(wide(h[i] & 0xffffu, kind)), size_of(wide(h[i] >> 16, kind))));
+    };
+    if constexpr (KEEP != 0) {
+#pragma unroll
+        for (int t = 0; t < KEEP / 8; ++t) {
+            const int64_t c = t * (8 * LANES) + threadIdx.x * 8;
+            held[t] = u4{0, 0, 0, 0};
+            if (c < k) load8(src, c, k, held[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < KEEP / 8; ++t) largest(held[t]);
+    } else {
+        for (int64_t c = threadIdx.x * 8; c < k; c += 8 * LANES) {
+            u4 h;
+            load8(src, c, k, h);
+            largest(h);
+        }
     }
-    const int e = exponent_for(reduce256<true>(most, lds));
+    const int e = exponent_for(reduce<true, LANES>(most, lds));
     float sum = 0.f;
-    for (int64_t c = threadIdx.x * 8; c < kp; c += 2048) {
-        u4 h;
-        load8(src, c, k, wide8, h);
+    auto convert = [&](int64_t c, u4 h) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float a = ldexpf(wide(h[i] & 0xffffu, kind), -e), b = ldexpf(wide(h[i] >> 16, kind), -e);
@@ -86,10 +105,23 @@ __global__ __launch_bounds__(256) void k_half_rows(const uint16_t* __restrict__ 
             h[i] = narrow2(a, b, SRC_F16);
         }
         *reinterpret_cast<u4*>(dst + c) = h;
+    };
+    if constexpr (KEEP != 0) {
+#pragma unroll
+        for (int t = 0; t < KEEP / 8; ++t) {
+            const int64_t c = t * (8 * LANES) + threadIdx.x * 8;
+            if (c < kp) convert(c, held[t]);
+        }
+    } else {
+        for (int64_t c = threadIdx.x * 8; c < kp; c += 8 * LANES) {
+            u4 h;
+            load8(src, c, k, h);
+            convert(c, h);
+        }
     }
     if (threadIdx.x == 0) e_out[row] = e;
     if (norm) {
-        sum = reduce256<false>(sum, lds);
+        sum = reduce<false, LANES>(sum, lds);
         if (threadIdx.x == 0) norm[row] = fminf(ldexpf(sqrtf(sum), e), 3e38f);
     }
 }
@@ -125,10 +157,11 @@ __device__ __forceinline__ float block_bound(const uint8_t* b) {
     }
 }
 
-constexpr int TILE = 4096;
-template <int T, int QK, int BS>
+// A row's blocks go to LDS, TILE weights at a time; a row of one tile is there before its headers are looked at, so
+// that its bytes are waited for once. Longer rows: the headers from memory first.
+template <int T, int QK, int BS, int TILE>
 __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__ src, int64_t k, uint16_t* __restrict__ dst,
-                                                     int64_t kp, int32_t* __restrict__ e_out, float* __restrict__ norm, DQ t,
+                                                     int64_t kp, int64_t ldd, int32_t* __restrict__ e_out, float* __restrict__ norm, DQ t,
                                                      int align) {
     constexpr int TB = TILE / QK, TBYTES = TB * BS;
     __shared__ __align__(16) uint8_t tile[TBYTES + 16];
@@ -139,15 +172,10 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     }
     const int64_t row = blockIdx.x, nb = k / QK;
     src += row * nb * BS;
-    dst += row * kp;
-    float most = 0.f;
-    for (int64_t b = threadIdx.x; b < nb; b += 256) most = fmaxf(most, block_bound<T>(src + b * BS));
-    const int e = exponent_for(reduce256<true>(most, lds));
-    float sum = 0.f;
-    for (int64_t b0 = 0; b0 < nb; b0 += TB) {
-        const int n = (int)(nb - b0 < TB ? nb - b0 : TB), bytes = n * BS;
+    dst += row * ldd;
+    auto stage = [&](int64_t b0, int n) {
+        const int bytes = n * BS;
         const uint8_t* s = src + b0 * BS;
-        __syncthreads();
         int done = 0;
         if (align >= 16) {
             for (int u = threadIdx.x; u < (bytes >> 4); u += 256)
@@ -164,6 +192,19 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
         }
         for (int u = done + threadIdx.x; u < bytes; u += 256) tile[u] = s[u];
         __syncthreads();
+    };
+    const bool one = nb <= TB;
+    if (one) stage(0, (int)nb);
+    float most = 0.f;
+    for (int64_t b = threadIdx.x; b < nb; b += 256) most = fmaxf(most, block_bound<T>((one ? tile : src) + b * BS));
+    const int e = exponent_for(reduce<true>(most, lds));
+    float sum = 0.f;
+    for (int64_t b0 = 0; b0 < nb; b0 += TB) {
+        const int n = (int)(nb - b0 < TB ? nb - b0 : TB);
+        if (!one) {
+            __syncthreads();
+            stage(b0, n);
+        }
         for (int q = threadIdx.x; q < n * (QK / 4); q += 256) {
             const int o = q * 4, blk = o / QK;
             float v[4];
@@ -179,14 +220,13 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     for (int64_t c = k + threadIdx.x; c < kp; c += 256) dst[c] = 0;
     if (threadIdx.x == 0) e_out[row] = e;
     if (norm) {
-        sum = reduce256<false>(sum, lds);
+        sum = reduce<false>(sum, lds);
         if (threadIdx.x == 0) norm[row] = fminf(ldexpf(sqrtf(sum), e), 3e38f);
     }
 }
 
 // 64 x 64 tiles through LDS: read along a row's columns, written along a column's rows, eight numbers a lane both
-// ways. WIDE: whole groups of eight at 16-byte addresses on the reading side.
-template <bool WIDE>
+// ways.
 __global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
                                                    uint16_t* __restrict__ dst, int64_t ldd, int64_t rp, int64_t tiles_c) {
     __shared__ uint16_t t[64][66];                                // 33 words a row: a column's reads meet few banks twice
@@ -196,7 +236,7 @@ __global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ 
         const int u = i * 256 + threadIdx.x, r = u >> 3, c = (u & 7) * 8;
         const int64_t R = r0 + r, C = c0 + c;
         u4 v = {0, 0, 0, 0};
-        if (R < rows && C < cols) load8(src + R * ld, C, cols, WIDE, v);
+        if (R < rows && C < cols) load8(src + R * ld, C, cols, v);
         uint32_t* p = reinterpret_cast<uint32_t*>(&t[r][c]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) p[k] = v[k];
@@ -256,8 +296,14 @@ __global__ __launch_bounds__(256) void k_grad_exponents(const uint16_t* __restri
     __shared__ float lds[4];
     const int64_t row = blockIdx.x;
     float most = 0.f;
-    for (int64_t c = threadIdx.x; c < n; c += 256) most = fmaxf(most, size_of(wide(dh[row * ld + c], kind)));
-    most = reduce256<true>(most, lds);
+    for (int64_t c = threadIdx.x * 8; c < n; c += 2048) {
+        u4 h;
+        load8(dh + row * ld, c, n, h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            most = fmaxf(most, fmaxf(size_of(wide(h[i] & 0xffffu, kind)), size_of(wide(h[i] >> 16, kind))));
+    }
+    most = reduce<true>(most, lds);
     if (threadIdx.x) return;
     const float a = xnorm[row], b = top->norm;
     if (!(most > 0.f) || !(a > 0.f) || !(b > 0.f)) {
@@ -279,14 +325,12 @@ __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
 // the adapters among the rows in turn, in rising order, most of them finding none. The whole tile is
 // multiplied by the adapter's matrix and its own rows are kept. The 16 waves take 64 k (a line of each row)
 // in turn, the loads of 128 k under way at once; 64 ranks at a time, so that x is read once for the usual ranks.
-// Many rows: gridDim.z workgroups share k, each writing its sums to a place of its own in `low`, and k_low_join
-// adds them in their order.
 constexpr int LOW_WAVES = 16;
-template <int KIND, bool WIDE, int MT>
+template <int KIND, int MT>
 __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restrict__ x, int64_t ldx, int64_t m, int64_t k,
                                                         const uint16_t* __restrict__ a_all, const float* __restrict__ scale,
                                                         const int32_t* __restrict__ which, int pool, int rank,
-                                                        float* __restrict__ low, int rp, bool wide_x, bool wide_a) {
+                                                        float* __restrict__ low, int rp) {
     __shared__ float part[LOW_WAVES][4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t m0 = (int64_t)blockIdx.x * 16 * MT;
@@ -299,7 +343,6 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
         mine[t] = mi < m ? which[mi] : -1;
         xr[t] = x + (mi < m ? mi : m - 1) * ldx;
     }
-    low += blockIdx.z * m * rp;
     if (blockIdx.y == 0) {                                        // rows without an adapter: zeros
         for (int i = threadIdx.x; i < 16 * MT * rp; i += LOW_WAVES * 64) {
             const int64_t mi = m0 + i / rp;
@@ -321,8 +364,7 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
         if (a == INT32_MAX) return;
         if (turn == blockIdx.y) break;
     }
-    const int64_t lines = (k + 63) / 64, l0 = lines * blockIdx.z / gridDim.z, l1 = lines * (blockIdx.z + 1) / gridDim.z;
-    const int64_t turned = l1 > l0 ? (int64_t)blockIdx.x * 5 % (l1 - l0) : 0;
+    const int64_t lines = (k + 63) / 64, turned = (int64_t)blockIdx.x * 5 % lines;
     const uint16_t* aa = a_all + (int64_t)a * rank * k;
     for (int r0 = 0; r0 < rp; r0 += 64) {
         const int tiles = tmin(4, (rp - r0) / 16);
@@ -336,29 +378,23 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
             for (int t = 0; t < MT; ++t) acc[t][j] = f4{0, 0, 0, 0};
         }
         constexpr int U = MT == 1 ? 4 : 2;                        // steps of 32 k at once
-        for (int64_t l = wave; l < l1 - l0; l += LOW_WAVES * (U / 2)) {
+        for (int64_t l = wave; l < lines; l += LOW_WAVES * (U / 2)) {
             u4 xv[U][MT], av[U][4];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 // workgroups begin at different lines: rows of a power of two apart lie in few memory channels
-                const int64_t i = l + LOW_WAVES * (u / 2), at = l0 + (i + turned < l1 - l0 ? i + turned : i + turned - (l1 - l0));
+                const int64_t i = l + LOW_WAVES * (u / 2), at = i + turned < lines ? i + turned : i + turned - lines;
                 const int64_t k0 = at * 64 + 32 * (u % 2) + kc;
-                const bool in = i < l1 - l0 && k0 < k;
+                const bool in = i < lines && k0 < k;
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     xv[u][t] = u4{0, 0, 0, 0};
-                    if (in) {
-                        if (WIDE) xv[u][t] = *reinterpret_cast<const u4*>(xr[t] + k0);   // rows of whole steps at 16-byte addresses
-                        else load8(xr[t], k0, k, wide_x, xv[u][t]);
-                    }
+                    if (in) load8(xr[t], k0, k, xv[u][t]);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     av[u][j] = u4{0, 0, 0, 0};
-                    if (in && j < tiles) {
-                        if (WIDE) av[u][j] = *reinterpret_cast<const u4*>(ar[j] + k0);
-                        else load8(ar[j], k0, k, wide_a, av[u][j]);
-                    }
+                    if (in && j < tiles) load8(ar[j], k0, k, av[u][j]);
                 }
             }
 #pragma unroll
@@ -395,34 +431,44 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
     }
 }
 
-__global__ __launch_bounds__(256) void k_low_join(float* low, int64_t n, int pieces) {
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-        float v = low[i];
-        for (int p = 1; p < pieces; ++p) v += low[p * n + i];
+// the row's own adapter out of the products with all of them: part [piece][m][pool rank]
+__global__ __launch_bounds__(256) void k_low_pick(const float* __restrict__ part, int pieces, const float* __restrict__ scale,
+                                                  const int32_t* __restrict__ which, int64_t m, int pool, int rank, float* __restrict__ low,
+                                                  int rp) {
+    const int64_t width = (int64_t)pool * rank, size = m * width;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * rp; i += gridDim.x * 256ll) {
+        const int64_t mi = i / rp;
+        const int r = (int)(i - mi * rp), a = which[mi];
+        float v = 0.f;
+        if (r < rank && a >= 0 && a < pool) {
+            const float* p = part + mi * width + (int64_t)a * rank + r;
+            for (int j = 0; j < pieces; ++j) v += p[j * size];
+            v *= scale[a];
+        }
         low[i] = v;
     }
 }
-
-bool aligned8(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
 }  // namespace
 
 int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, hipStream_t st) {
     const int64_t groups = (rows * (kp / 8) + 255) / 256;
-    hipLaunchKernelGGL(k_pack, dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(256), 0, st, src, ld, rows, k, dst, kp,
-                       aligned8(src, ld));
+    hipLaunchKernelGGL(k_pack, dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(256), 0, st, src, ld, rows, k, dst, kp);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
-int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e,
+int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e,
               float* norm, hipStream_t st) {
-    hipLaunchKernelGGL(k_half_rows, dim3((unsigned)rows), dim3(256), 0, st, src, kind, ld, k, dst, kp, e, norm, aligned8(src, ld));
+    const dim3 grid((unsigned)rows);
+    if (kp <= 4096) hipLaunchKernelGGL((k_half_rows<16, 256>), grid, dim3(256), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm);
+    else if (kp <= 16384) hipLaunchKernelGGL((k_half_rows<16, 1024>), grid, dim3(1024), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm);
+    else hipLaunchKernelGGL((k_half_rows<0, 1024>), grid, dim3(1024), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
-int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int32_t* e, float* norm,
+int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e, float* norm,
                 hipStream_t st) {
     DQ t{nullptr};
     const int ti = iq_table_index(type);
@@ -437,7 +483,8 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
     switch (type) {
 #define SPA_BLOCKS(T, QK, BS)                                                                                           \
     case T:                                                                                                             \
-        hipLaunchKernelGGL((k_half_blocks<T, QK, BS>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, e, norm, t, align); \
+        if (k <= 4096) hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 4096>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, t, align); \
+        else hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 16384>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, t, align); \
         break;
         SPA_BLOCKS(2, 32, 18) SPA_BLOCKS(3, 32, 20) SPA_BLOCKS(6, 32, 22) SPA_BLOCKS(7, 32, 24) SPA_BLOCKS(8, 32, 34)
         SPA_BLOCKS(10, 256, 84) SPA_BLOCKS(11, 256, 110) SPA_BLOCKS(12, 256, 144) SPA_BLOCKS(13, 256, 176) SPA_BLOCKS(14, 256, 210)
@@ -453,8 +500,7 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
                 hipStream_t st) {
     const int64_t tr = (rp + 63) / 64, tc = (cols + 63) / 64;
-    if (aligned8(src, ld)) hipLaunchKernelGGL((k_transpose<true>), dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
-    else hipLaunchKernelGGL((k_transpose<false>), dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
+    hipLaunchKernelGGL(k_transpose, dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
@@ -477,32 +523,27 @@ int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st) 
 
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
              const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st) {
-    const int pieces = low_pieces(m, k);
-    const int64_t rows = pieces > 1 ? 32 : 16;
-    const dim3 grid((unsigned)((m + rows - 1) / rows), (unsigned)(pool < rows ? pool : rows), (unsigned)pieces), block(LOW_WAVES * 64);
-    const bool wx = aligned8(x, ldx), wa = aligned8(a, k), whole = wx && wa && k % 32 == 0;
-#define SPA_LOW(KIND, WIDE, MT) \
-    hipLaunchKernelGGL((k_low<KIND, WIDE, MT>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, wx, wa)
-#define SPA_LOW_ROWS(KIND, WIDE)                \
-    do {                                        \
-        if (rows == 32) SPA_LOW(KIND, WIDE, 2); \
-        else SPA_LOW(KIND, WIDE, 1);            \
-    } while (0)
+    const int64_t rows = m > 256 ? 32 : 16;
+    const dim3 grid((unsigned)((m + rows - 1) / rows), (unsigned)(pool < rows ? pool : rows)), block(LOW_WAVES * 64);
+#define SPA_LOW(KIND, MT) \
+    hipLaunchKernelGGL((k_low<KIND, MT>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp)
     if (kind == SRC_BF16) {
-        if (whole) SPA_LOW_ROWS(SRC_BF16, true);
-        else SPA_LOW_ROWS(SRC_BF16, false);
+        if (rows == 32) SPA_LOW(SRC_BF16, 2);
+        else SPA_LOW(SRC_BF16, 1);
     } else {
-        if (whole) SPA_LOW_ROWS(SRC_F16, true);
-        else SPA_LOW_ROWS(SRC_F16, false);
+        if (rows == 32) SPA_LOW(SRC_F16, 2);
+        else SPA_LOW(SRC_F16, 1);
     }
-#undef SPA_LOW_ROWS
 #undef SPA_LOW
     SPA_HIP_TRY(hipGetLastError());
-    if (pieces > 1) {
-        const int64_t n = m * rp, groups = (n + 255) / 256;
-        hipLaunchKernelGGL(k_low_join, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, low, n, pieces);
-        SPA_HIP_TRY(hipGetLastError());
-    }
+    return SPA_OK;
+}
+
+int low_pick(const float* part, int pieces, const float* scale, const int32_t* which, int64_t m, int pool, int rank, float* low, int rp,
+             hipStream_t st) {
+    const int64_t groups = (m * rp + 255) / 256;
+    hipLaunchKernelGGL(k_low_pick, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, part, pieces, scale, which, m, pool, rank, low, rp);
+    SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 

@@ -15,18 +15,25 @@ namespace {
 
 constexpr int COLS = 512, IDS = 1024;
 
+// Column i of a lane's eight: eight in a row where rows lie at 16-byte addresses, else every 64th, so that a wave's
+// loads of one number a lane still are runs of memory.
+__device__ __forceinline__ int column(int lane, int i, bool wide8) { return wide8 ? 8 * lane + i : lane + 64 * i; }
+
 template <int KIND>
 __device__ __forceinline__ void add8(const void* __restrict__ x, int64_t at, int64_t left, bool wide8, float (&s)[8], float times) {
+    // at, left: the lane's first number, and the columns from there on
     float v[8];
     if (wide8 && left >= 8) {
         load_weights<8>(x, KIND, at, v);
     } else {
+        // columns beyond the last are read as the last and dropped: no load waits for a branch
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[i] = 0.f;
-            if (i < left)
-                v[i] = KIND == SRC_F32 ? static_cast<const float*>(x)[at + i] : wide(static_cast<const uint16_t*>(x)[at + i], KIND);
+            const int64_t c = wide8 ? i : 64 * i, in = at + (c < left ? c : left - 1);
+            v[i] = KIND == SRC_F32 ? static_cast<const float*>(x)[in] : wide(static_cast<const uint16_t*>(x)[in], KIND);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (wide8 ? i : 64 * i) < left ? v[i] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = fmaf(v[i] * times, v[i], s[i]);
@@ -55,14 +62,19 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
     const int64_t tiles = (q.cols + COLS - 1) / COLS;
     // the experts of one piece of x side by side: its second reader finds it in the caches
     const int e = (int)(blockIdx.x % q.experts);
-    const int64_t piece = blockIdx.x / q.experts, run = piece / tiles, c0 = piece % tiles * COLS + 8 * lane;
+    const int64_t piece = blockIdx.x / q.experts, run = piece / tiles, c0 = piece % tiles * COLS + column(lane, 0, q.wide8);
     const int64_t r0 = run * q.run, r1 = tmin(q.rows, r0 + q.run), left = q.cols - c0;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     uint32_t hits = 0;
     if constexpr (!SPLIT) {
-#pragma unroll 4
-        for (int64_t r = r0 + wave; r < r1; r += 4)
-            if (left > 0) add8<KIND>(q.x, r * q.ld + c0, left, q.wide8, s, 1.f);
+        if (left > 0) {
+            int64_t r = r0 + wave;
+            for (; r + 12 < r1; r += 16) {                        // four rows' loads under way at once
+#pragma unroll
+                for (int u = 0; u < 4; ++u) add8<KIND>(q.x, (r + 4 * u) * q.ld + c0, left, q.wide8, s, 1.f);
+            }
+            for (; r < r1; r += 4) add8<KIND>(q.x, r * q.ld + c0, left, q.wide8, s, 1.f);
+        }
     } else {
         for (int64_t b = r0; b < r1; b += IDS) {
             // the rows of this expert among the next IDS, in their order: each wave a quarter
@@ -126,7 +138,11 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
             __syncthreads();
             if (lane == 0) wsum[wave] = (int)hits;
             __syncthreads();
-            if (threadIdx.x == 0) q.hits[run * q.experts + e] = (uint32_t)(wsum[0] + wsum[1] + wsum[2] + wsum[3]);
+            if (threadIdx.x == 0) {
+                const int n = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+                if (q.runs == 1) q.counts[e] += n;
+                else q.hits[run * q.experts + e] = (uint32_t)n;
+            }
         }
     }
     if (wave) {
@@ -135,21 +151,34 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
     }
     __syncthreads();
     if (wave == 0) {
-        float* out = q.part + (run * q.experts + e) * q.cols + c0;
+        float* out = (q.runs == 1 ? q.sums + e * q.cols : q.part + (run * q.experts + e) * q.cols) + c0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float v = (s[i] + join[0][i * 64 + lane]) + (join[1][i * 64 + lane] + join[2][i * 64 + lane]);
-            if (i < left) out[i] = v;
+            const int c = column(lane, i, q.wide8) - column(lane, 0, q.wide8);
+            float v = (s[i] + join[0][i * 64 + lane]) + (join[1][i * 64 + lane] + join[2][i * 64 + lane]);
+            if (c >= left) continue;
+            if (q.runs == 1) v = out[c] + v;                      // nothing to join: straight to the caller's sums
+            out[c] = v;
         }
     }
+    if (!SPLIT && q.runs == 1 && blockIdx.x == 0 && threadIdx.x == 0) q.counts[0] += q.rows;
 }
 
+// 32 sums a workgroup, eight lanes to each: every eighth run in turn, the eight then in their order
 __global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
-    const int64_t n = (int64_t)q.experts * q.cols;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-        float v = 0.f;
+    __shared__ float lds[8][32];
+    const int64_t n = (int64_t)q.experts * q.cols, i = blockIdx.x * 32ll + (threadIdx.x & 31);
+    const int g = threadIdx.x >> 5;
+    float v = 0.f;
+    if (i < n) {
 #pragma unroll 8
-        for (int64_t r = 0; r < q.runs; ++r) v += q.part[r * n + i];
+        for (int64_t r = g; r < q.runs; r += 8) v += q.part[r * n + i];
+    }
+    lds[g][threadIdx.x & 31] = v;
+    __syncthreads();
+    if (g == 0 && i < n) {
+#pragma unroll
+        for (int j = 1; j < 8; ++j) v += lds[j][threadIdx.x];
         q.sums[i] += v;
     }
     for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < q.experts; e += gridDim.x * 256ll) {
@@ -165,11 +194,12 @@ __global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
 // (with runs of 8192 rows the first of 64 unlike experts kept 16384 x 4096 busy for 202 us).
 int64_t run_rows(int64_t rows, int64_t cols, int64_t experts, bool by_expert) {
     const int64_t tiles = (cols + COLS - 1) / COLS * experts;
-    int64_t run = IDS;
+    int64_t run = rows < IDS ? rows : IDS;
     if (!by_expert) {
         const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
         run = (rows + runs - 1) / runs;
         if (run < 16) run = 16;
+        if (rows <= 128) run = rows;                              // one launch
     }
     while ((rows + run - 1) / run * tiles > (1 << 24)) run *= 2;
     return run;
@@ -190,6 +220,7 @@ extern "C" uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64
     const bool by_expert = experts != 0;
     if (!by_expert) experts = 1;
     const int64_t run = run_rows(rows, cols, experts, by_expert), runs = (rows + run - 1) / run;
+    if (runs == 1) return 0;
     return part_bytes(runs, cols, experts) + ((uint64_t)runs * experts * 4 + 255) / 256 * 256;
 }
 
@@ -207,7 +238,8 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     if ((reinterpret_cast<uintptr_t>(x) & unit) || (reinterpret_cast<uintptr_t>(which) & 3) || (reinterpret_cast<uintptr_t>(sums) & 3) ||
         (reinterpret_cast<uintptr_t>(counts) & 7))
         return fail(SPA_ERR_ARG, "spa_add_squares: a pointer is not aligned to its elements");
-    if (!work || (reinterpret_cast<uintptr_t>(work) & 15) || work_bytes < spa_add_squares_work_bytes(rows, cols, experts))
+    const uint64_t need = spa_add_squares_work_bytes(rows, cols, experts);
+    if (need && (!work || (reinterpret_cast<uintptr_t>(work) & 15) || work_bytes < need))
         return fail(SPA_ERR_ARG, "spa_add_squares: needs a 16-byte aligned workspace of spa_add_squares_work_bytes bytes");
     Sq q{};
     q.x = x;
@@ -239,8 +271,10 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     else SPA_SQUARES(SRC_F32);
 #undef SPA_SQUARES
     SPA_HIP_TRY(hipGetLastError());
-    const int64_t groups = ((int64_t)q.experts * cols + 255) / 256;
-    hipLaunchKernelGGL(k_squares_join, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, q);
+    if (q.runs == 1) return SPA_OK;
+    const int64_t groups = ((int64_t)q.experts * cols + 31) / 32;
+    if (groups > INT32_MAX) return fail(SPA_ERR_ARG, "spa_add_squares: %lld experts x %lld is too large", (long long)q.experts, (long long)cols);
+    hipLaunchKernelGGL(k_squares_join, dim3((unsigned)groups), dim3(256), 0, st, q);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }

@@ -8,12 +8,16 @@
 Weights are BF16 or F16 matrices or any of the 20 GGUF block types, as they lie in a file (`Weight`).
 Inputs and outputs are two-dimensional DeviceArrays of BF16 bits (uint16) or float16, row-major; with a
 `*_stride` (in elements) an array's rows may lie further apart than their columns. Every call only queues
-work on `stream` and returns; results are float32 sums rounded once. Scratch comes from the calling
-thread's cache of device blocks, whose work is on one stream (device._Cache), or is given as `work`.
+work on `stream` and returns; results are float32 sums rounded once. A call's scratch is the calling thread's
+own for that device and stream, kept between calls (`release` gives it back), or is given as `work`. Arrays
+that a call makes for its results come from the thread's cache of device blocks, whose work is on one stream
+(device._Cache): a thread that uses several gives its own.
 
 The reference has no counterpart: it makes and packs weights (seedpack/gpuquant.py:284-456) and leaves
 their use to llama.cpp.
 """
+import threading
+
 import numpy as np
 
 from . import device as dev
@@ -84,12 +88,30 @@ def _ids(which, rows):
         raise ValueError(f"{which.shape[0]} row numbers for {rows} rows")
 
 
-def _scratch(n, work):
+_kept = threading.local()
+
+
+def _scratch(n, work, stream):
+    """the call's workspace: the one given, or this thread's own for the device and stream, kept for its next calls
+    there. One that has to grow waits for the stream once, so that work still queued on the old block is done.
+    -> (what keeps it alive, pointer, bytes)"""
     if not n:
         return None, None, 0
     if work is None:
-        work = dev.DeviceArray(n, np.uint8)
+        blocks, key = _kept.__dict__, (dev.current_device(), stream)
+        work = blocks.get(key)
+        if work is None or work.nbytes < n:
+            if work is not None:
+                check(lib().spa_stream_synchronize(stream))
+            work = blocks[key] = dev.DeviceArray(max(n, 1 << 20), np.uint8)
     return work, work.ptr, work.nbytes
+
+
+def release():
+    """gives this thread's workspaces back to the cache of device blocks, after waiting for their work"""
+    for _, stream in list(_kept.__dict__):
+        check(lib().spa_stream_synchronize(stream))
+    _kept.__dict__.clear()
 
 
 def _out(name, out, m, n, dtype, stride):
@@ -120,7 +142,7 @@ def project(x, w, adapters=None, which=None, out=None, x_stride=None, out_stride
         _ids(which, m)
         a, b, scale, ids, pool, rank = adapters.a.ptr, adapters.b.ptr, adapters.scale.ptr, which.ptr, adapters.count, adapters.rank
     L = lib()
-    keep, p, n = _scratch(L.spa_project_work_bytes(w.type, w.rows, w.cols, kind, m, pool, rank), work)
+    keep, p, n = _scratch(L.spa_project_work_bytes(w.type, w.rows, w.cols, kind, m, pool, rank), work, stream)
     check(L.spa_project(w.type, w.data.ptr, w.rows, w.cols, kind, x.ptr, m, ld, out.ptr, ldo, a, b, scale, pool, rank, ids,
                         p, n, stream))
     return out
@@ -140,7 +162,7 @@ def gated(x, gate, up, act="silu", out=None, x_stride=None, out_stride=None, wor
     kind, m, _, ld = _rows("x", x, x_stride, gate.cols)
     out, ldo = _out("out", out, m, gate.rows, x.dtype, out_stride)
     L = lib()
-    keep, p, n = _scratch(L.spa_gated_work_bytes(gate.type, gate.rows, gate.cols, kind, m), work)
+    keep, p, n = _scratch(L.spa_gated_work_bytes(gate.type, gate.rows, gate.cols, kind, m), work, stream)
     check(L.spa_gated(gate.type, gate.data.ptr, up.data.ptr, gate.rows, gate.cols, kind, x.ptr, m, ld, act, out.ptr, ldo, p, n,
                       stream))
     return out
@@ -165,7 +187,7 @@ def gated_backward(x, gate, up, dh, act="silu", dx=None, dgate=None, dup=None, x
         dgate, _ = _out("dgate", dgate, gate.rows, k, x.dtype, None)
         dup, _ = _out("dup", dup, gate.rows, k, x.dtype, None)
     L = lib()
-    keep, p, n = _scratch(L.spa_gated_backward_work_bytes(gate.type, gate.rows, k, kind, m, dx is not None, dgate is not None), work)
+    keep, p, n = _scratch(L.spa_gated_backward_work_bytes(gate.type, gate.rows, k, kind, m, dx is not None, dgate is not None), work, stream)
     check(L.spa_gated_backward(gate.type, gate.data.ptr, up.data.ptr, gate.rows, k, kind, x.ptr, m, ld, act, dh.ptr, ldh,
                                None if dx is None else dx.ptr, ldx, None if dgate is None else dgate.ptr,
                                None if dup is None else dup.ptr, p, n, stream))
@@ -184,7 +206,7 @@ def add_squares(x, sums, counts, which=None, x_stride=None, work=None, stream=No
     if sums.dtype != np.float32 or counts.dtype != np.int64 or sums.size != counts.size * k or (which is None and counts.size != 1):
         raise ValueError(f"sums {sums.shape} {sums.dtype}, counts {counts.shape} {counts.dtype} for {k} columns")
     L = lib()
-    keep, p, n = _scratch(L.spa_add_squares_work_bytes(m, k, experts), work)
+    keep, p, n = _scratch(L.spa_add_squares_work_bytes(m, k, experts), work, stream)
     check(L.spa_add_squares(x.ptr, kind, m, k, ld, None if which is None else which.ptr, each, experts, sums.ptr, counts.ptr,
                             p, n, stream))
     return sums, counts

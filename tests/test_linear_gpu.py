@@ -491,6 +491,61 @@ def test_add_squares_gathers_an_importance():
     close(linear.project(up(x[:70]), linear.Weight(12, blocks, 64, 512)).to_host(), y, slack(total, 512), BF16)
 
 
+@pytest.mark.parametrize("m,n,k", [(4100, 2100, 192), (2100, 4100, 128), (300, 2053, 1024), (700, 130, 2112)])
+@pytest.mark.parametrize("t,kind", [(linear.BF16, BF16), (8, BF16), (8, F16)])
+def test_project_tiles(t, kind, m, n, k):
+    """enough outputs for the large tiles, and few enough for pieces of k; both ragged, with adapters"""
+    g = rng(31, t, m)
+    w, w64 = weights(g, t, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    ad, a, b, s = adapters(g, 3, 20, n, k, kind)
+    which = np.sort(g.integers(-1, 3, m)).astype(np.int32)
+    y, total = x64 @ w64.T, np.abs(x64) @ np.abs(w64.T)
+    for i in range(3):
+        at = which == i
+        y[at] += float(s[i]) * ((x64[at] @ a[i].T) @ b[i].T)
+        total[at] += float(s[i]) * ((np.abs(x64[at]) @ np.abs(a[i].T)) @ np.abs(b[i].T))
+    close(linear.project(up(x), w, ad, up(which)).to_host(), y, slack(total, k + 20), kind)
+    y, total = project64(x64, w64)
+    close(linear.project(up(x), w).to_host(), y, slack(total, k), kind)
+
+
+@pytest.mark.parametrize("m,n,k", [(2100, 2060, 128), (300, 700, 1024), (150, 200, 2048)])
+@pytest.mark.parametrize("t,kind", [(linear.BF16, BF16), (12, BF16)])
+def test_gated_tiles(t, kind, m, n, k):
+    g = rng(32, t, m)
+    k = -(-k // 256) * 256 if t == 12 else k
+    gate, g64 = weights(g, t, n, k)
+    upw, u64 = weights(g, t, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    h, off = gated64(x64, g64, u64, "silu", k)
+    close(linear.gated(up(x), gate, upw).to_host(), h, off, kind)
+    dh = store(g.normal(0, 0.1, (m, n)), kind)
+    want, off = gated_backward64(x64, g64, u64, wide(dh), "silu", k, UNIT[BF16] if t == linear.BF16 else 2.0 ** -11)["dx"]
+    if t == 12:
+        top = max(np.linalg.norm(g64, axis=1).max(), np.linalg.norm(u64, axis=1).max())
+        floor = 2.0 ** -20 * 1.13 * np.abs(wide(dh)).max(1) * np.linalg.norm(x64, axis=1) * top
+        off = off + floor[:, None] * (np.abs(g64).sum(0) + np.abs(u64).sum(0))[None]
+    close(linear.gated_backward(up(x), gate, upw, up(dh))[0].to_host(), want, off, kind)
+
+
+def test_project_last_rows_and_long_adapters():
+    """five rows beyond whole tiles, which the few-rows form takes, and adapters' first products as one product:
+    all of the last rows and a sample of the others, a sample of the columns"""
+    g = rng(33)
+    m, n, k, pool, rank = 2053, 4096, 12288, 4, 64
+    b, w64 = random_blocks(g, 12, 256, k)                 # 16 times the same 256 rows
+    w = linear.Weight(12, up(np.tile(b, 16)), n, k)
+    x, x64 = inputs(g, m, k, BF16)
+    ad, a, bb, s = adapters(g, pool, rank, n, k, BF16)
+    which = np.sort(g.integers(-1, pool, m)).astype(np.int32)
+    rows = np.concatenate([np.arange(0, m - 16, 97), np.arange(m - 16, m)])
+    cols = np.arange(0, n, 37)
+    y, total = project64(x64[rows], w64[cols % 256], a, bb[:, cols], s, which[rows])
+    got = linear.project(up(x), w, ad, up(which)).to_host()
+    close(np.ascontiguousarray(got[rows][:, cols]), y, slack(total, k + rank), BF16)
+
+
 def test_streams_and_repeats():
     """work on a stream of its own; the same call twice gives the same bits"""
     g = rng(30)
