@@ -201,25 +201,11 @@ struct Direct {
 typedef const __attribute__((address_space(1))) void* gptr;
 typedef __attribute__((address_space(3))) void* lptr;
 
-// The inputs as the matrix instruction takes them: for each step of 32 k and each tile a run of 64 lanes x 8
-// numbers, one contiguous load of a wave. Rows of 4096 numbers lie 8 KB apart, all in the same
-// channel of the L2: sixteen of them fetched side by side took Q8_0 12288 x 4096 with 32 rows 55 us.
-template <bool HALVES>
-__global__ __launch_bounds__(256) void k_fragments(const uint16_t* __restrict__ x, int64_t ldx, int m, int k, uint16_t* __restrict__ out,
-                                                   int tiles) {
-    const int i = blockIdx.x * 256 + threadIdx.x, lane = i & 63, tile = (i >> 6) % tiles, step = (i >> 6) / tiles;
-    if (step * 32 >= k) return;
-    const int row = lane & 15, g = lane >> 4, r = HALVES ? 8 * tile + (row & 7) : 16 * tile + row;
-    u4 v = {0, 0, 0, 0};
-    if (r < m && (!HALVES || (row < 8) == (g < 2))) v = *reinterpret_cast<const u4*>(x + (int64_t)r * ldx + step * 32 + 8 * g);
-    reinterpret_cast<u4*>(out)[i] = v;
-}
-
-// ONE: a single input row, read as it lies. AL: every unit of a row begins at a 16-byte address.
-template <int T, int KIND, int MT, bool ONE, bool TWO, bool AL, int WAVES>
+// MT = 1: the inputs are read as they lie, and MR of a lane's four sums count. More tiles: as fragments. AL: every unit of a row begins at a 16-byte address.
+template <int T, int KIND, int MT, int MR, bool TWO, bool AL, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void k_codes(const FewArgs a) {
     typedef Unit<T> U;
-    constexpr int STEPS = UNIT / 32, MR = ONE ? 1 : 4, AHEAD = MT == 1 ? 8 : (MT == 2 ? 4 : (MT == 4 ? 2 : 1));
+    constexpr int STEPS = UNIT / 32, AHEAD = MT == 1 ? 8 : (MT == 2 ? 4 : (MT == 4 ? 2 : 1));
     // 16-byte words of a row's unit, wherever in the first of them it begins
     constexpr int BYTES = UNIT / U::QK * U::BS, WORDS = AL ? BYTES / 16 : (BYTES + 15 + 15) / 16, LOADS = (16 * WORDS + 63) / 64;
     constexpr int STAGE = WORDS * 256 + 16, RED = WAVES * (1 + TWO) * MT * 1024, ALL = WAVES * (1 + TWO) * STAGE;
@@ -242,8 +228,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_codes(const FewArgs a) {
     const int64_t first = (int64_t)n0 * a.rowbytes, last = (int64_t)tmin(n0 + 16, f.n) * a.rowbytes;
     const bool inside = AL || (first >= 16 && last + 32 <= f.wbytes);
     const uint32_t wrow = (uint32_t)(tmin(n0 + row, f.n - 1) - n0) * (uint32_t)a.rowbytes;
-    const bool live = U::HALVES ? row == (g < 2 ? 0 : 8) : row == 0;
-    const uint16_t* xrow = f.x + 8 * g;
+    const int own = U::HALVES ? row & 7 : row;
+    const bool live = own < f.m && (!U::HALVES || (row < 8) == (g < 2));
+    const uint16_t* xrow = f.x + (live ? own * f.ldx : 0) + 8 * g;
     f4 acc[1 + TWO][MT];
 #pragma unroll
     for (int s = 0; s <= TWO; ++s)
@@ -289,8 +276,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_codes(const FewArgs a) {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 const int k = u * UNIT + 32 * s;
-                if (ONE) x0[s] = live && s < have ? *reinterpret_cast<const u4*>(xrow + k) : u4{0, 0, 0, 0};
-                else if (s < have) x0[s] = reinterpret_cast<const u4*>(f.x)[2 * k + lane];
+                x0[s] = live && s < have ? *reinterpret_cast<const u4*>(xrow + k) : u4{0, 0, 0, 0};
             }
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -336,23 +322,25 @@ int launch(const FewArgs& a, hipStream_t st) {
     constexpr int HIGH = Unit<T>::HALVES ? 8 : 16;
     const dim3 grid((unsigned)((a.f.n + 15) / 16));
     const int tiles = few_tiles(T, a.f.m);
-    // few weight rows fill the device with waves only if more of them share a row's k
-    const bool many = TWO || a.f.n >= 8192;
+    // A wave has at least one unit of k to itself (151936 x 1024 with 3 rows: 8 waves, half of them idle, 54 us, 4 waves 34);
+    // few weight rows fill the device with waves only if more of them
+    // share a row's k.
+    const int units = (a.f.k + UNIT - 1) / UNIT;
+    const bool many = TWO || a.f.n >= 8192, low = units <= 4 && a.f.n >= 4096;
     constexpr int MOST = TWO ? 8 : 16;
-#define SPA_CODES(MT, ONE, W) hipLaunchKernelGGL((k_codes<T, KIND, MT, ONE, TWO, AL, W>), grid, dim3(W * 64), 0, st, a)
-    if (a.f.m == 1) {
-        if (many) SPA_CODES(1, true, 8);
-        else SPA_CODES(1, true, MOST);
-    } else if (tiles == 1) {
-        if (many) SPA_CODES(1, false, 8);
-        else SPA_CODES(1, false, MOST);
-    } else if (tiles == 2) {
-        SPA_CODES(2, false, 8);
-    } else if (tiles == 4) {
-        SPA_CODES(4, false, 8);
-    } else if constexpr (HIGH == 8) {
-        SPA_CODES(8, false, 8);
-    }
+#define SPA_CODES(MT, MR, W) hipLaunchKernelGGL((k_codes<T, KIND, MT, MR, TWO, AL, W>), grid, dim3(W * 64), 0, st, a)
+#define SPA_CODES_ONE(MR)               \
+    do {                                \
+        if (low) SPA_CODES(1, MR, 4);   \
+        else if (many) SPA_CODES(1, MR, 8); \
+        else SPA_CODES(1, MR, MOST);    \
+    } while (0)
+    if (a.f.m == 1) SPA_CODES_ONE(1);
+    else if (tiles == 1) SPA_CODES_ONE(4);
+    else if (tiles == 2) SPA_CODES(2, 4, 8);
+    else if (tiles == 4) SPA_CODES(4, 4, 8);
+    else if constexpr (HIGH == 8) SPA_CODES(8, 4, 8);
+#undef SPA_CODES_ONE
 #undef SPA_CODES
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
@@ -370,11 +358,9 @@ int aligned(const FewArgs& a, hipStream_t st) {
 template <int T>
 int pick(const Few& f, uint16_t* frags, hipStream_t st) {
     FewArgs a{f, f.rowbytes, f.x};
-    if (f.m > 1) {
-        const int tiles = few_tiles(T, f.m), lanes = tiles * (f.k / 32) * 64;
-        hipLaunchKernelGGL((k_fragments<Unit<T>::HALVES>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, f.x, f.ldx, f.m, f.k,
-                           frags, tiles);
-        SPA_HIP_TRY(hipGetLastError());
+    if (few_tiles(T, f.m) > 1) {
+        const int rc = fragments<Unit<T>::HALVES>(f, few_tiles(T, f.m), frags, st);
+        if (rc) return rc;
         a.f.x = frags;
     }
     if (f.w1) return f.kind == SRC_BF16 ? aligned<T, SRC_BF16, true>(a, st) : aligned<T, SRC_F16, true>(a, st);

@@ -148,7 +148,12 @@ __global__ __launch_bounds__(W * 64) void k_few16(const FewArgs a) {
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * STEP;
             if (k >= f.k) break;
-            load_x<MT>(f, k, x[u]);
+            if constexpr (MT == 1) {
+                load_x<MT>(f, k, x[u]);
+            } else {                                              // as fragments
+#pragma unroll
+                for (int j = 0; j < MT; ++j) x[u][j] = reinterpret_cast<const u4*>(f.x)[(k / 32 * MT + j) * 64 + lane];
+            }
 #pragma unroll
             for (int h = 0; h <= TWO; ++h) {
                 const uint8_t* p = (h ? f.w1 : f.w0) + wrow + 2 * (k + kl);
@@ -190,10 +195,17 @@ __global__ __launch_bounds__(W * 64) void k_few16(const FewArgs a) {
 }
 
 template <int T, int QK, int BS, int KIND, bool TWO>
-int launch(const FewArgs& a, DQ t, hipStream_t st) {
-    const dim3 grid((unsigned)((a.f.n + 15) / 16)), block(WAVES * 64);
+int launch(const FewArgs& given, DQ t, uint16_t* frags, hipStream_t st) {
+    const dim3 grid((unsigned)((given.f.n + 15) / 16)), block(WAVES * 64);
     if constexpr (T == 1 || T == 30) {
         constexpr int WK = T == 1 ? SRC_F16 : SRC_BF16;
+        FewArgs a = given;
+        const int tiles = few_tiles(T, a.f.m);
+        if (tiles > 1) {
+            const int rc = fragments<false>(a.f, tiles, frags, st);
+            if (rc) return rc;
+            a.f.x = frags;
+        }
         const bool lined = a.rowbytes == 2 * (int64_t)a.f.k && ((reinterpret_cast<uintptr_t>(a.f.w0) | reinterpret_cast<uintptr_t>(a.f.w1)) & 15) == 0;
         // few weight rows fill the device with waves only if more of them share a row's k (one row of 4060 x 5795
         // with 8 waves: 80 us)
@@ -212,18 +224,18 @@ int launch(const FewArgs& a, DQ t, hipStream_t st) {
         }
 #undef SPA_FEW16
     } else {
-        if (a.f.m <= 16) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 1, TWO>), grid, block, 0, st, a, t);
-        else if (a.f.m <= 32) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 2, TWO>), grid, block, 0, st, a, t);
-        else hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 4, TWO>), grid, block, 0, st, a, t);
+        if (given.f.m <= 16) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 1, TWO>), grid, block, 0, st, given, t);
+        else if (given.f.m <= 32) hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 2, TWO>), grid, block, 0, st, given, t);
+        else hipLaunchKernelGGL((k_few<T, QK, BS, KIND, 4, TWO>), grid, block, 0, st, given, t);
     }
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
 template <int T, int QK, int BS>
-int pick(const FewArgs& a, DQ t, hipStream_t st) {
-    if (a.f.w1) return a.f.kind == SRC_BF16 ? launch<T, QK, BS, SRC_BF16, true>(a, t, st) : launch<T, QK, BS, SRC_F16, true>(a, t, st);
-    return a.f.kind == SRC_BF16 ? launch<T, QK, BS, SRC_BF16, false>(a, t, st) : launch<T, QK, BS, SRC_F16, false>(a, t, st);
+int pick(const FewArgs& a, DQ t, uint16_t* frags, hipStream_t st) {
+    if (a.f.w1) return a.f.kind == SRC_BF16 ? launch<T, QK, BS, SRC_BF16, true>(a, t, frags, st) : launch<T, QK, BS, SRC_F16, true>(a, t, frags, st);
+    return a.f.kind == SRC_BF16 ? launch<T, QK, BS, SRC_BF16, false>(a, t, frags, st) : launch<T, QK, BS, SRC_F16, false>(a, t, frags, st);
 }
 
 }  // namespace
@@ -243,7 +255,7 @@ int few(const Few& f, uint16_t* frags, hipStream_t st) {
 #define SPA_FEW(T, QK, BS)                                 \
     case T:                                                \
         a.rowbytes = f.rowbytes;                           \
-        return pick<T, QK, BS>(a, t, st);
+        return pick<T, QK, BS>(a, t, frags, st);
         SPA_FEW(1, 1, 2) SPA_FEW(30, 1, 2)
         SPA_FEW(3, 32, 20) SPA_FEW(6, 32, 22) SPA_FEW(7, 32, 24)
         SPA_FEW(10, 256, 84) SPA_FEW(11, 256, 110)

@@ -181,7 +181,12 @@ inline int few_tiles(int type, int64_t m) {
     while (t * (type == 14 ? 8 : 16) < m) t *= 2;
     return t;
 }
-inline int64_t few_fragments(int type, int64_t m, int64_t kp) { return coded(type) && m > 1 ? few_tiles(type, m) * 16 * kp : 0; }
+inline int64_t few_fragments(int type, int64_t m, int64_t kp) {
+    return (coded(type) || type == 1 || type == 30) && few_tiles(type, m) > 1 ? few_tiles(type, m) * 16 * kp : 0;
+}
+// the most rows that take the few-rows form, FEW_ROWS at a time: where codes are cheap to unpack twice is less than
+// decoding the weights for the many-rows form (Q8_0 12288 x 4096: 28 us for 64 rows, 68 for 65 in the other form)
+inline int64_t few_limit(int type) { return coded(type) && type != 14 ? 2 * FEW_ROWS : FEW_ROWS; }
 
 // ---- rows (rows.hip)
 // rows of a 16-bit matrix copied into rows of kp (a multiple of 64), zeros beyond k

@@ -265,7 +265,11 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
         }
         return few(f, frags, st);
     };
-    if (p.m <= FEW_ROWS) return few_rows(0, p.m);
+    if (p.m <= few_limit(p.type)) {
+        for (int64_t at = 0; at < p.m; at += FEW_ROWS)
+            if ((rc = few_rows(at, p.m - at < FEW_ROWS ? p.m - at : FEW_ROWS))) return rc;
+        return SPA_OK;
+    }
     Operands o;
     if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
     Gemm g = gemm_of(o, p.m, p.n, p.k);
@@ -310,7 +314,11 @@ int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
         f.act = p.act;
         return few(f, frags, st);
     };
-    if (p.m <= FEW_ROWS) return few_rows(0, p.m);
+    if (p.m <= few_limit(p.type)) {
+        for (int64_t at = 0; at < p.m; at += FEW_ROWS)
+            if ((rc = few_rows(at, p.m - at < FEW_ROWS ? p.m - at : FEW_ROWS))) return rc;
+        return SPA_OK;
+    }
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
     Gemm g = gemm_of(o, p.m, p.n, p.k);

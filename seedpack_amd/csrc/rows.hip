@@ -324,14 +324,16 @@ __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
 // low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 MT rows a workgroup and one adapter: gridDim.y workgroups take
 // the adapters among the rows in turn, in rising order, most of them finding none. The whole tile is
 // multiplied by the adapter's matrix and its own rows are kept. The 16 waves take 64 k (a line of each row)
-// in turn, the loads of 128 k under way at once; 64 ranks at a time, so that x is read once for the usual ranks.
+// in turn, the loads of 128 or 256 k under way at once; up to 64 ranks at a time, so that x is read once for the
+// usual ranks.
 constexpr int LOW_WAVES = 16;
-template <int KIND, int MT>
+template <int KIND, int MT, int TILES>
 __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restrict__ x, int64_t ldx, int64_t m, int64_t k,
                                                         const uint16_t* __restrict__ a_all, const float* __restrict__ scale,
                                                         const int32_t* __restrict__ which, int pool, int rank,
                                                         float* __restrict__ low, int rp) {
-    __shared__ float part[LOW_WAVES][4][256];
+    __shared__ float part[LOW_WAVES][TILES][256];
+    __shared__ int ids[16 * MT];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t m0 = (int64_t)blockIdx.x * 16 * MT;
     const int row = lane & 15, kc = (lane >> 4) * 8;
@@ -343,6 +345,7 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
         mine[t] = mi < m ? which[mi] : -1;
         xr[t] = x + (mi < m ? mi : m - 1) * ldx;
     }
+    for (int i = threadIdx.x; i < 16 * MT; i += LOW_WAVES * 64) ids[i] = m0 + i < m ? which[m0 + i] : -1;
     if (blockIdx.y == 0) {                                        // rows without an adapter: zeros
         for (int i = threadIdx.x; i < 16 * MT * rp; i += LOW_WAVES * 64) {
             const int64_t mi = m0 + i / rp;
@@ -366,20 +369,21 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
     }
     const int64_t lines = (k + 63) / 64, turned = (int64_t)blockIdx.x * 5 % lines;
     const uint16_t* aa = a_all + (int64_t)a * rank * k;
-    for (int r0 = 0; r0 < rp; r0 += 64) {
-        const int tiles = tmin(4, (rp - r0) / 16);
-        const uint16_t* ar[4];
-        f4 acc[MT][4];
+    const float sa = scale[a];
+    for (int r0 = 0; r0 < rp; r0 += 16 * TILES) {
+        const int tiles = tmin(TILES, (rp - r0) / 16);
+        const uint16_t* ar[TILES];
+        f4 acc[MT][TILES];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < TILES; ++j) {
             const int r = r0 + 16 * j + row;                      // ranks beyond the last take its row: they are not kept
             ar[j] = aa + (int64_t)(r < rank ? r : rank - 1) * k;
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t][j] = f4{0, 0, 0, 0};
         }
-        constexpr int U = MT == 1 ? 4 : 2;                        // steps of 32 k at once
+        constexpr int U = TILES == 1 ? 8 : (MT == 1 ? 4 : 2);                        // steps of 32 k at once
         for (int64_t l = wave; l < lines; l += LOW_WAVES * (U / 2)) {
-            u4 xv[U][MT], av[U][4];
+            u4 xv[U][MT], av[U][TILES];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 // workgroups begin at different lines: rows of a power of two apart lie in few memory channels
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
                     if (in) load8(xr[t], k0, k, xv[u][t]);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < TILES; ++j) {
                     av[u][j] = u4{0, 0, 0, 0};
                     if (in && j < tiles) load8(ar[j], k0, k, av[u][j]);
                 }
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < TILES; ++j) {
                     if (j >= tiles) break;
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
@@ -415,17 +419,17 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
         for (int t = 0; t < MT; ++t) {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < TILES; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) part[wave][j][(4 * (lane >> 4) + c) * 16 + row] = acc[t][j][c];
             __syncthreads();
             const int i = threadIdx.x, j = i >> 8, mr = (i >> 4) & 15, r = r0 + 16 * j + (i & 15);
             const int64_t mi = m0 + 16 * t + mr;
-            if (mi < m && r < rp && which[mi] == a) {
+            if (j < TILES && mi < m && r < rp && ids[16 * t + mr] == a) {
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < LOW_WAVES; ++w) v += part[w][j][i & 255];
-                low[mi * rp + r] = r < rank ? scale[a] * v : 0.f;
+                low[mi * rp + r] = r < rank ? sa * v : 0.f;
             }
         }
     }
@@ -525,15 +529,17 @@ int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, con
              const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st) {
     const int64_t rows = m > 256 ? 32 : 16;
     const dim3 grid((unsigned)((m + rows - 1) / rows), (unsigned)(pool < rows ? pool : rows)), block(LOW_WAVES * 64);
-#define SPA_LOW(KIND, MT) \
-    hipLaunchKernelGGL((k_low<KIND, MT>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp)
-    if (kind == SRC_BF16) {
-        if (rows == 32) SPA_LOW(SRC_BF16, 2);
-        else SPA_LOW(SRC_BF16, 1);
-    } else {
-        if (rows == 32) SPA_LOW(SRC_F16, 2);
-        else SPA_LOW(SRC_F16, 1);
-    }
+#define SPA_LOW(KIND, MT, TILES) \
+    hipLaunchKernelGGL((k_low<KIND, MT, TILES>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp)
+#define SPA_LOW_ROWS(KIND)                                  \
+    do {                                                    \
+        if (rows == 32) SPA_LOW(KIND, 2, 4);                \
+        else if (rp <= 16) SPA_LOW(KIND, 1, 1);             \
+        else SPA_LOW(KIND, 1, 4);                           \
+    } while (0)
+    if (kind == SRC_BF16) SPA_LOW_ROWS(SRC_BF16);
+    else SPA_LOW_ROWS(SRC_F16);
+#undef SPA_LOW_ROWS
 #undef SPA_LOW
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;

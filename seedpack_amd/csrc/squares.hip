@@ -13,14 +13,14 @@ namespace spa {
 namespace lin {
 namespace {
 
-constexpr int COLS = 512, IDS = 1024;
+constexpr int COLS = 512, PAIRS = 2048, RUN = 1024;
 
 // Column i of a lane's eight: eight in a row where rows lie at 16-byte addresses, else every 64th, so that a wave's
 // loads of one number a lane still are runs of memory.
 __device__ __forceinline__ int column(int lane, int i, bool wide8) { return wide8 ? 8 * lane + i : lane + 64 * i; }
 
 template <int KIND>
-__device__ __forceinline__ void add8(const void* __restrict__ x, int64_t at, int64_t left, bool wide8, float (&s)[8], float times) {
+__device__ __forceinline__ void add8(const void* __restrict__ x, int64_t at, int64_t left, bool wide8, float (&s)[8]) {
     // at, left: the lane's first number, and the columns from there on
     float v[8];
     if (wide8 && left >= 8) {
@@ -36,7 +36,7 @@ __device__ __forceinline__ void add8(const void* __restrict__ x, int64_t at, int
         for (int i = 0; i < 8; ++i) v[i] = (wide8 ? i : 64 * i) < left ? v[i] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = fmaf(v[i] * times, v[i], s[i]);
+    for (int i = 0; i < 8; ++i) s[i] = fmaf(v[i], v[i], s[i]);
 }
 
 struct Sq {
@@ -55,14 +55,15 @@ struct Sq {
 template <int KIND, bool SPLIT>
 __global__ __launch_bounds__(256) void k_squares(const Sq q) {
     __shared__ float join[3][COLS];
-    __shared__ int list[IDS];
-    __shared__ int times[IDS];
+    __shared__ int list[PAIRS];
     __shared__ int wsum[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t tiles = (q.cols + COLS - 1) / COLS;
-    // the experts of one piece of x side by side: its second reader finds it in the caches
-    const int e = (int)(blockIdx.x % q.experts);
-    const int64_t piece = blockIdx.x / q.experts, run = piece / tiles, c0 = piece % tiles * COLS + column(lane, 0, q.wide8);
+    // one expert after another: those with most rows tend to be the first numbers, and the rows under way lie all over x
+    // (an expert of each piece in turn, so that its second reader finds it in the caches: 131 instead of 65 us)
+    const int64_t pieces = gridDim.x / q.experts;
+    const int e = (int)(blockIdx.x / pieces);
+    const int64_t piece = blockIdx.x % pieces, run = piece / tiles, c0 = piece % tiles * COLS + column(lane, 0, q.wide8);
     const int64_t r0 = run * q.run, r1 = tmin(q.rows, r0 + q.run), left = q.cols - c0;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     uint32_t hits = 0;
@@ -71,27 +72,28 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
             int64_t r = r0 + wave;
             for (; r + 12 < r1; r += 16) {                        // four rows' loads under way at once
 #pragma unroll
-                for (int u = 0; u < 4; ++u) add8<KIND>(q.x, (r + 4 * u) * q.ld + c0, left, q.wide8, s, 1.f);
+                for (int u = 0; u < 4; ++u) add8<KIND>(q.x, (r + 4 * u) * q.ld + c0, left, q.wide8, s);
             }
-            for (; r < r1; r += 4) add8<KIND>(q.x, r * q.ld + c0, left, q.wide8, s, 1.f);
+            for (; r < r1; r += 4) add8<KIND>(q.x, r * q.ld + c0, left, q.wide8, s);
         }
     } else {
-        for (int64_t b = r0; b < r1; b += IDS) {
-            // the rows of this expert among the next IDS, in their order: each wave a quarter
-            const int n = (int)tmin<int64_t>(IDS, r1 - b);
-            int have = 0;
-            uint64_t mask[IDS / 256];
-            int mult[IDS / 256];
+        // (row, expert) pairs, PAIRS at a time: those of this expert listed in their order, each wave a quarter
+        const int64_t p1 = r1 * q.each;
+        for (int64_t p0 = r0 * q.each; p0 < p1; p0 += PAIRS) {
+            constexpr int N = PAIRS / 256;
+            int id[N];
 #pragma unroll
-            for (int i = 0; i < IDS / 256; ++i) {
-                const int r = wave * (IDS / 4) + i * 64 + lane;
-                int h = 0;
-                if (r < n)
-                    for (int j = 0; j < q.each; ++j) h += q.which[(b + r) * q.each + j] == e;
-                mult[i] = h;
-                mask[i] = __ballot(h > 0);
+            for (int i = 0; i < N; ++i) {
+                const int64_t at = p0 + wave * (PAIRS / 4) + i * 64 + lane;
+                id[i] = q.which[tmin(at, p1 - 1)];
+                if (at >= p1) id[i] = -1;
+            }
+            uint64_t mask[N];
+            int have = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                mask[i] = __ballot(id[i] == e);
                 have += __popcll(mask[i]);
-                hits += h;
             }
             __syncthreads();
             if (lane == 0) wsum[wave] = have;
@@ -102,47 +104,45 @@ __global__ __launch_bounds__(256) void k_squares(const Sq q) {
                 if (w < wave) at += wsum[w];
                 total += wsum[w];
             }
+            hits += total;
 #pragma unroll
-            for (int i = 0; i < IDS / 256; ++i) {
-                if (mult[i]) {
-                    const int p = at + __popcll(mask[i] & ((1ull << lane) - 1));
-                    list[p] = wave * (IDS / 4) + i * 64 + lane;
-                    times[p] = mult[i];
+            for (int i = 0; i < N; ++i) {
+                if (id[i] == e) {
+                    const int64_t pair = p0 + wave * (PAIRS / 4) + i * 64 + lane;
+                    list[at + __popcll(mask[i] & ((1ull << lane) - 1))] = (int)(r0 + (uint32_t)(pair - r0 * q.each) / (uint32_t)q.each);
                 }
                 at += __popcll(mask[i]);
             }
             __syncthreads();
             if (q.wide8 && left >= 8) {
-                for (int i = wave; i < total; i += 32) {          // eight rows' loads under way at once
-                    float v[8][8];
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) load_weights<8>(q.x, KIND, (b + list[tmin(i + 4 * u, total - 1)]) * q.ld + c0, v[u]);
+                for (int i = wave; i < total; i += 32) {          // eight rows' loads under way at once, as they lie
+                    u4 raw[8][KIND == SRC_F32 ? 2 : 1];
 #pragma unroll
                     for (int u = 0; u < 8; ++u) {
-                        const bool in = i + 4 * u < total;
-                        const float t = in ? (float)times[i + 4 * u] : 0.f;
+                        const int64_t at = (int64_t)list[tmin(i + 4 * u, total - 1)] * q.ld + c0;
+                        const u4* p = KIND == SRC_F32 ? reinterpret_cast<const u4*>(static_cast<const float*>(q.x) + at)
+                                                      : reinterpret_cast<const u4*>(static_cast<const uint16_t*>(q.x) + at);
+                        raw[u][0] = p[0];
+                        if (KIND == SRC_F32) raw[u][KIND == SRC_F32] = p[1];
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (i + 4 * u >= total) break;
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
-                            const float w = in ? v[u][c] : 0.f;
-                            s[c] = fmaf(w * t, w, s[c]);
+                            const float v = KIND == SRC_F32 ? __uint_as_float(raw[u][(KIND == SRC_F32) * (c >> 2)][c & 3])
+                                                            : wide((raw[u][0][c >> 1] >> (16 * (c & 1))) & 0xffffu, KIND);
+                            s[c] = fmaf(v, v, s[c]);
                         }
                     }
                 }
             } else if (left > 0) {
-                for (int i = wave; i < total; i += 4) add8<KIND>(q.x, (b + list[i]) * q.ld + c0, left, q.wide8, s, (float)times[i]);
+                for (int i = wave; i < total; i += 4) add8<KIND>(q.x, (int64_t)list[i] * q.ld + c0, left, q.wide8, s);
             }
         }
-        if (piece % tiles == 0) {
-#pragma unroll
-            for (int k = 32; k; k >>= 1) hits += __shfl_xor(hits, k);
-            __syncthreads();
-            if (lane == 0) wsum[wave] = (int)hits;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const int n = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-                if (q.runs == 1) q.counts[e] += n;
-                else q.hits[run * q.experts + e] = (uint32_t)n;
-            }
+        if (piece % tiles == 0 && threadIdx.x == 0) {
+            if (q.runs == 1) q.counts[e] += hits;
+            else q.hits[run * q.experts + e] = hits;
         }
     }
     if (wave) {
@@ -189,17 +189,18 @@ __global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
     }
 }
 
-// Rows of a run. Whole: enough workgroups to fill the device (about 1024 of them), at least 16 rows each. By
-// expert: 1024 rows, so that an expert which gets most of the rows is still spread over many workgroups
-// (with runs of 8192 rows the first of 64 unlike experts kept 16384 x 4096 busy for 202 us).
+// Rows of a run. Whole: enough workgroups to fill the device (about 1024 of them), at least 16 rows each, and one
+// launch for up to 128. By expert: 1024, so that an expert which gets most of the rows is still spread over many
+// workgroups and a workgroup's search of the numbers is worth its rows (16384 x 4096, 64 unlike experts, two for a
+// row: runs of 512 91, of 1024 65, of 2048 72, of 8192 202 us).
 int64_t run_rows(int64_t rows, int64_t cols, int64_t experts, bool by_expert) {
     const int64_t tiles = (cols + COLS - 1) / COLS * experts;
-    int64_t run = rows < IDS ? rows : IDS;
+    int64_t run = rows < RUN ? rows : RUN;
     if (!by_expert) {
         const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
         run = (rows + runs - 1) / runs;
         if (run < 16) run = 16;
-        if (rows <= 128) run = rows;                              // one launch
+        if (rows <= 128) run = rows;
     }
     while ((rows + run - 1) / run * tiles > (1 << 24)) run *= 2;
     return run;
@@ -230,7 +231,7 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     if (src_kind < SPA_SRC_BF16 || src_kind > SPA_SRC_F32) return fail(SPA_ERR_TYPE, "spa_add_squares: source kind %d", src_kind);
     if (rows < 0 || cols <= 0 || x_stride < cols || rows > INT32_MAX || cols > INT32_MAX)
         return fail(SPA_ERR_ARG, "spa_add_squares: bad shape %lld x %lld, stride %lld", (long long)rows, (long long)cols, (long long)x_stride);
-    if (which ? (experts < 1 || experts > 65535 || each < 1 || each > 65535) : experts != 0)
+    if (which ? (experts < 1 || experts > 65535 || each < 1 || each * rows > INT32_MAX) : experts != 0)
         return fail(SPA_ERR_ARG, "spa_add_squares: %lld experts, %lld for each row", (long long)experts, (long long)each);
     if (rows == 0) return SPA_OK;
     if (!x || !sums || !counts) return fail(SPA_ERR_ARG, "spa_add_squares: null pointer");
