@@ -160,17 +160,24 @@ __device__ __forceinline__ void product(const Gemm& g) {
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
             const bool last = part == PARTS - 1;
+            auto products = [&](int i0, int i1) {
+#pragma unroll
+                for (int i = i0; i < i1; ++i)
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) acc[i][j] = Op<HALF>::mul(fa[part & 1][i], fb[part & 1][j], acc[i][j]);
+            };
+            constexpr int AHEAD = FN / 4 > 0 ? FN / 4 : 1;        // (none: 2 % longer)
             if (last && N1) {
+                // some of the part's products are under way while the waves meet
+                products(0, AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             if (!last) read(buf, part + 1, (part + 1) & 1);
             else if (N1) read(buf ^ 1, 0, 0);
             if (part == 0 && N1) fetch(buf ^ 1, kt + 1, EARLY, LOADS);
             if (last && N2) fetch(buf, kt + 2, 0, EARLY);
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-#pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = Op<HALF>::mul(fa[part & 1][i], fb[part & 1][j], acc[i][j]);
+            products(last && N1 ? AHEAD : 0, FN);
 #pragma unroll
             for (int i = 0; i < FN * FM; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -208,7 +215,7 @@ __device__ __forceinline__ void product(const Gemm& g) {
             uint16_t* p = y + (int64_t)(mw + r) * ld + n;
             const u4 v = *reinterpret_cast<const u4*>(out + r * PITCH + c0 + c);
             if (wide16 && n + 8 <= most) {
-                *reinterpret_cast<u4*>(p) = v;
+                __builtin_nontemporal_store(v, reinterpret_cast<u4*>(p));
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
@@ -422,8 +429,10 @@ __device__ __forceinline__ void product(const Gemm& g) {
         if constexpr (OUT == OUT_GATED) {
             flush(g.y, g.ldy, 0, g.n);
         } else {
-            flush(g.grad, g.ldg, 0, (int)g.np);
-            flush(g.grad + g.np, g.ldg, RUN, (int)g.np);
+            for (int64_t at = 0; at <= (g.twice ? 2 * g.np : 0); at += 2 * g.np) {
+                flush(g.grad + at, g.ldg, 0, (int)g.np);
+                flush(g.grad + at + g.np, g.ldg, RUN, (int)g.np);
+            }
         }
     }
 }
@@ -488,6 +497,10 @@ __global__ __launch_bounds__(256) void k_join(const Gemm g) {
                     uint16_t* y = g.grad + (int64_t)m * g.ldg + ni;
                     y[0] = narrow(ni < g.n ? ldexpf(d * u * slope, e0 - ge) : 0.f, g.half);
                     y[g.np] = narrow(ni < g.n ? ldexpf(d * value, e1 - ge) : 0.f, g.half);
+                    if (g.twice) {
+                        y[2 * g.np] = y[0];
+                        y[3 * g.np] = y[g.np];
+                    }
                 }
             } else if (ni < g.n) {
                 if constexpr (OUT == OUT_GATED) a = act_value(a, g.act) * v[1][c];
@@ -497,30 +510,42 @@ __global__ __launch_bounds__(256) void k_join(const Gemm g) {
     }
 }
 
-// What a product takes: a tile of 256 x 256 is half again as fast as two of 128 x 128 on a compute unit,
-// but the device has 256 units and waits for its last round. Times of 64 k of a round, in units of 1/100 us on one
-// MI355X: 256 x 256 one to a unit 170; 128 x 128 two to a unit 126, alone on it 85. In pieces of k with too
-// few tiles: each adds 8 bytes of traffic an output and matrix (about 5 TB/s) and the joining launch.
+// What a product takes: the larger the tile, the less time for its work, but the device has 256 compute units and
+// waits for its last round. A round's time in units of 1/100 us on one MI355X, for each 64 k and for its beginning
+// and end: 256 x 256 162 and 1000; 128 x 128, two to a unit, 113 and 900, alone on it 83 and 600 (256 x 128 took 111,
+// no more for its work than 128 x 128). In pieces of k, where there are too few tiles: their sums leave as float32
+// (1500 or 700 a round), each adds 8 bytes of traffic an output and matrix (about 5 TB/s), and there is the joining
+// launch.
+enum Tile { SMALL, LARGE };
 struct Plan {
-    bool big;
+    int tile;
     int pieces;
     int64_t cost;
 };
+int64_t tile_time(int tile, int64_t n, int64_t m, int64_t times, int64_t steps, bool part) {
+    const int64_t t = tile == SMALL ? 128 : 256, tiles = (n + t - 1) / t * ((m + t - 1) / t) * times;
+    const int64_t out = part ? (tile == LARGE ? 1500 : 700) : 0;
+    if (tile == LARGE) return (tiles + 255) / 256 * (steps * 162 + 1000 + out);
+    return tiles <= 256 ? steps * 83 + 600 + out : (tiles + 511) / 512 * (steps * 113 + 900 + out);
+}
 Plan plan(const Gemm& g) {
-    const bool two = g.w1 != nullptr;
-    const int64_t steps = g.k / BK, m = g.m, n = g.n;
-    const int64_t nb = (n * (two ? 2 : 1) + 255) / 256 * ((m + 255) / 256), ns = (n * (two ? 2 : 1) + 127) / 128 * ((m + 127) / 128);
-    auto small = [](int64_t tiles, int64_t st) { return tiles <= 256 ? st * 85 : (tiles + 511) / 512 * st * 126; };
-    Plan best{true, 1, (nb + 255) / 256 * steps * 170};
-    if (small(ns, steps) < best.cost) best = Plan{false, 1, small(ns, steps)};
-    for (int p = 2; p <= g.most && p * 4 <= steps; ++p) {
-        const int64_t st = (steps + p - 1) / p, join = 600 + (int64_t)(m * n * (two ? 2 : 1) * 8 * p / 50000);
-        // in pieces the two matrices are products of their own
-        const int64_t b = (n + 255) / 256 * (two ? 2 : 1) * ((m + 255) / 256) * p, s = (n + 127) / 128 * (two ? 2 : 1) * ((m + 127) / 128) * p;
-        if ((b + 255) / 256 * st * 170 + join < best.cost) best = Plan{true, p, (b + 255) / 256 * st * 170 + join};
-        if (small(s, st) + join < best.cost) best = Plan{false, p, small(s, st) + join};
+    const int64_t steps = g.k / BK, m = g.m, n = g.n, matrices = g.w1 ? 2 : 1;
+    Plan best{LARGE, 1, INT64_MAX};
+    for (int tile = LARGE; tile >= SMALL; --tile) {
+        const int64_t whole = tile_time(tile, n * matrices, m, 1, steps, false);
+        if (whole < best.cost) best = Plan{tile, 1, whole};
+        for (int p = 2; p <= g.most && p * 4 <= steps; ++p) {
+            // in pieces the two matrices are products of their own
+            const int64_t c = tile_time(tile, n, m, matrices * p, (steps + p - 1) / p, true) + 600 + m * n * matrices * 8 * p / 50000;
+            if (c < best.cost) best = Plan{tile, p, c};
+        }
     }
     return best;
+}
+
+template <int HALF, int OUT>
+int launch_tile(int tile, const Gemm& g, hipStream_t st) {
+    return tile == LARGE ? launch<HALF, 256, 256, 2, 4, OUT>(g, st) : launch<HALF, 128, 128, 2, 2, OUT>(g, st);
 }
 
 template <int HALF, int OUT>
@@ -529,14 +554,14 @@ int pick(const Gemm& g, hipStream_t st) {
     if (p.pieces > 1) {
         Gemm q = g;
         q.pieces = p.pieces;
-        const int rc = p.big ? launch<HALF, 256, 256, 2, 4, OUT_PART>(q, st) : launch<HALF, 128, 128, 2, 2, OUT_PART>(q, st);
+        const int rc = launch_tile<HALF, OUT_PART>(p.tile, q, st);
         if (rc) return rc;
         const int64_t groups = ((int64_t)g.m * ((OUT == OUT_GRAD ? g.np : g.n) + 3) / 4 + 255) / 256;
         hipLaunchKernelGGL((k_join<OUT>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, st, q);
         SPA_HIP_TRY(hipGetLastError());
         return SPA_OK;
     }
-    return p.big ? launch<HALF, 256, 256, 2, 4, OUT>(g, st) : launch<HALF, 128, 128, 2, 2, OUT>(g, st);
+    return launch_tile<HALF, OUT>(p.tile, g, st);
 }
 
 template <int HALF>

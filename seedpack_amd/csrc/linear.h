@@ -6,7 +6,9 @@
 //   * many rows: both operands as binary16 with a power of two taken out of each row, so that the row's
 //     largest value lies below 2^15. A BF16 row keeps its values to 2^-39 of its largest (8 of 11 bits
 //     used, 2^-24 the least step); a decoded weight is rounded to 11 bits, an eighth of a BF16
-//     rounding. The powers are added back to the float32 sums as exponents;
+//     rounding. Beside F16 inputs, whose results have 11 bits too, the weights are taken to 22: what the
+//     rounding leaves over takes part as a second half of k. The powers are added back to the float32 sums as
+//     exponents;
 //   * few rows: each value as a sum of two BF16 numbers (16 bits, any exponent), whose products are
 //     summed by two or three BF16 instructions: the matrix unit idles there.
 #pragma once
@@ -140,6 +142,7 @@ struct Gemm {
     int64_t ldh;
     uint16_t* grad;           // OUT_GRAD: [m][2 np], the gate's gradient, then the up projection's; zeros beyond n
     int64_t np, ldg;          // its halves' width and its rows' distance
+    bool twice;               // OUT_GRAD: grad's columns again, 2 np further on
     const int32_t* ge;        // OUT_GRAD: power of two taken out of each row of grad (binary16), or null
     // pieces of k: the most that there may be (1: none), scratch of gemm_part() numbers for their sums
     // [matrix][piece][m][n], and how many there are
@@ -191,12 +194,13 @@ inline int64_t few_limit(int type) { return coded(type) && type != 14 ? 2 * FEW_
 // ---- rows (rows.hip)
 // rows of a 16-bit matrix copied into rows of kp (a multiple of 64), zeros beyond k
 int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, hipStream_t st);
-// the same into binary16, rows of ldd, with a power of two taken out of each row (e), and the row's 2-norm as it was (or null)
+// the same into binary16, rows of ldd, with a power of two taken out of each row (e), and the row's 2-norm as it was (or
+// null); twice: the row again kp further on
 int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e,
-              float* norm, hipStream_t st);
-// the same from a block type
+              float* norm, bool twice, hipStream_t st);
+// the same from a block type; rest: what the rounding leaves over kp further on
 int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e, float* norm,
-                hipStream_t st);
+                bool rest, hipStream_t st);
 // dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (rp and ldd multiples of 8)
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
                 hipStream_t st);

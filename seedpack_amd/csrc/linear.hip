@@ -58,19 +58,23 @@ struct Operands {
     const uint16_t *x = nullptr, *w0 = nullptr, *w1 = nullptr;
     int64_t ldx = 0, ldw = 0;
     int half = 0;
+    int64_t kp = 0, rest = 0;   // columns of the rows, and where the weights' second parts begin (0: none)
     int32_t *xe = nullptr, *we0 = nullptr, *we1 = nullptr;
     float *norm = nullptr, *n0 = nullptr, *n1 = nullptr;
 };
 
 // Inputs and weights brought into the form of the many-rows product. Where both are of one 16-bit type they
 // are used as they lie, or copied where rows are not whole 128-byte steps at 16-byte addresses; otherwise
-// both become binary16 rows. `run` false only lays out the workspace (for the widest case).
+// both become binary16 rows, beside F16 inputs the weights of block types in two parts. `run` false only lays out the workspace (for the widest case).
 int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64_t n, int64_t k, int kind, const void* x, int64_t m,
              int64_t ldx, bool bounds, Operands& o, hipStream_t st) {
     const int64_t kp = up64(k);
     const bool same = is16(type) && kind_of(type) == kind;
     o.half = same ? kind : SRC_F16;
-    const int64_t ldd = same ? kp : kp + PAD;
+    const bool both = !same && !is16(type) && kind == SRC_F16;
+    const int64_t ldd = same ? kp : (both ? 2 : 1) * kp + PAD;
+    o.kp = both ? 2 * kp : kp;
+    o.rest = both ? kp : 0;
     uint16_t* xp = wk.take<uint16_t>(m * ldd);
     int rc;
     if (same) {
@@ -103,7 +107,7 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
         o.n0 = wk.take<float>(n);
         o.n1 = wk.take<float>(n);
     }
-    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, ldd, o.xe, o.norm, st))) return rc;
+    if (run && (rc = half_rows((const uint16_t*)x, kind, ldx, m, k, xp, kp, ldd, o.xe, o.norm, both, st))) return rc;
     o.x = xp;
     o.ldx = o.ldw = ldd;
     for (int i = 0; i < (w1 ? 2 : 1); ++i) {
@@ -111,8 +115,8 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
         int32_t* e = wk.take<int32_t>(n);
         const void* w = i ? w1 : w0;
         if (run) {
-            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, ldd, e, i ? o.n1 : o.n0, st)
-                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, ldd, e, i ? o.n1 : o.n0, st);
+            rc = is16(type) ? half_rows((const uint16_t*)w, kind_of(type), k, n, k, p, kp, ldd, e, i ? o.n1 : o.n0, false, st)
+                            : half_blocks(type, (const uint8_t*)w, n, k, p, kp, ldd, e, i ? o.n1 : o.n0, both, st);
             if (rc) return rc;
         }
         (i ? o.w1 : o.w0) = p;
@@ -147,7 +151,7 @@ int few_operands(Work& wk, bool run, int type, const void* w0, const void* w1, i
     return SPA_OK;
 }
 
-Gemm gemm_of(const Operands& o, int64_t m, int64_t n, int64_t k) {
+Gemm gemm_of(const Operands& o, int64_t m, int64_t n) {
     Gemm g{};
     g.half = o.half;
     g.x = o.x;
@@ -157,7 +161,7 @@ Gemm gemm_of(const Operands& o, int64_t m, int64_t n, int64_t k) {
     g.ldw = o.ldw;
     g.m = (int)m;
     g.n = (int)n;
-    g.k = (int)up64(k);
+    g.k = (int)o.kp;
     g.xe = o.xe;
     g.we0 = o.we0;
     g.we1 = o.we1;
@@ -272,7 +276,7 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
     }
     Operands o;
     if ((rc = operands(wk, run, p.type, p.w, nullptr, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
-    Gemm g = gemm_of(o, p.m, p.n, p.k);
+    Gemm g = gemm_of(o, p.m, p.n);
     g.kind = p.kind;
     g.y = (uint16_t*)p.y;
     g.ldy = p.ldy;
@@ -321,7 +325,7 @@ int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
     }
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, up, p.n, p.k, p.kind, p.x, p.m, p.ldx, false, o, st))) return rc;
-    Gemm g = gemm_of(o, p.m, p.n, p.k);
+    Gemm g = gemm_of(o, p.m, p.n);
     g.kind = p.kind;
     g.y = (uint16_t*)p.h;
     g.ldy = p.ldh;
@@ -339,14 +343,14 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     const int64_t np = up64(p.n), mp = up64(p.m);
     Operands o;
     if ((rc = operands(wk, run, p.type, p.gate, run ? p.up : SOME, p.n, p.k, p.kind, p.x, p.m, p.ldx, true, o, st))) return rc;
-    const int64_t ldg = 2 * np + PAD, ldm = mp + PAD;
+    const int64_t wide = o.rest ? 4 * np : 2 * np, ldg = wide + PAD, ldm = mp + PAD;
     uint16_t* grad = wk.take<uint16_t>(p.m * ldg);
     int32_t* ge = o.norm ? wk.take<int32_t>(p.m) : nullptr;
     void* top = wk.take<uint8_t>(8);
     if (run && ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.n0, o.we0, o.n1, o.we1, top, ge, st)))
         return rc;
     {
-        Gemm g = gemm_of(o, p.m, p.n, p.k);
+        Gemm g = gemm_of(o, p.m, p.n);
         g.kind = p.kind;
         g.act = p.act;
         g.dh = (const uint16_t*)p.dh;
@@ -354,6 +358,7 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
         g.grad = grad;
         g.np = np;
         g.ldg = ldg;
+        g.twice = o.rest != 0;
         g.ge = ge;
         if ((rc = multiply(g, wk, run, st))) return rc;
     }
@@ -361,6 +366,8 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
         uint16_t* wt = wk.take<uint16_t>(p.k * ldg);
         if (run && (rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, ldg, np, st))) return rc;
         if (run && (rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, ldg, np, st))) return rc;
+        if (run && o.rest && (rc = transpose16(o.w0 + o.rest, o.ldw, p.n, p.k, wt + 2 * np, ldg, np, st))) return rc;
+        if (run && o.rest && (rc = transpose16(o.w1 + o.rest, o.ldw, p.n, p.k, wt + 3 * np, ldg, np, st))) return rc;
         Gemm g{};
         g.half = o.half;
         g.x = grad;
@@ -368,7 +375,7 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
         g.ldx = g.ldw = ldg;
         g.m = (int)p.m;
         g.n = (int)p.k;
-        g.k = (int)(2 * np);
+        g.k = (int)wide;
         g.xe = ge;
         g.kind = p.kind;
         g.y = (uint16_t*)p.dx;

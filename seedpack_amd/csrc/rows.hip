@@ -67,7 +67,7 @@ __device__ __forceinline__ int exponent_for(float top) {
 template <int KEEP, int LANES>
 __global__ __launch_bounds__(LANES) void k_half_rows(const uint16_t* __restrict__ src, int kind, int64_t ld, int64_t k,
                                                    uint16_t* __restrict__ dst, int64_t kp, int64_t ldd, int32_t* __restrict__ e_out,
-                                                   float* __restrict__ norm) {
+                                                   float* __restrict__ norm, bool twice) {
     __shared__ float lds[LANES / 64];
     const int64_t row = blockIdx.x;
     src += row * ld;
@@ -105,6 +105,7 @@ __global__ __launch_bounds__(LANES) void k_half_rows(const uint16_t* __restrict_
             h[i] = narrow2(a, b, SRC_F16);
         }
         *reinterpret_cast<u4*>(dst + c) = h;
+        if (twice) *reinterpret_cast<u4*>(dst + kp + c) = h;
     };
     if constexpr (KEEP != 0) {
 #pragma unroll
@@ -161,8 +162,8 @@ __device__ __forceinline__ float block_bound(const uint8_t* b) {
 // that its bytes are waited for once. Longer rows: the headers from memory first.
 template <int T, int QK, int BS, int TILE>
 __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__ src, int64_t k, uint16_t* __restrict__ dst,
-                                                     int64_t kp, int64_t ldd, int32_t* __restrict__ e_out, float* __restrict__ norm, DQ t,
-                                                     int align) {
+                                                     int64_t kp, int64_t ldd, int32_t* __restrict__ e_out, float* __restrict__ norm, bool rest,
+                                                     DQ t, int align) {
     constexpr int TB = TILE / QK, TBYTES = TB * BS;
     __shared__ __align__(16) uint8_t tile[TBYTES + 16];
     __shared__ int8_t kv[16];
@@ -214,10 +215,22 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
                 v[i] = ldexpf(v[i], -e);
                 sum = fmaf(size_of(v[i]), size_of(v[i]), sum);
             }
-            *reinterpret_cast<u2*>(dst + b0 * QK + o) = u2{narrow2(v[0], v[1], SRC_F16), narrow2(v[2], v[3], SRC_F16)};
+            const u2 h = u2{narrow2(v[0], v[1], SRC_F16), narrow2(v[2], v[3], SRC_F16)};
+            *reinterpret_cast<u2*>(dst + b0 * QK + o) = h;
+            if (rest) {                                           // what binary16 leaves over (nothing of infinities)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float w = wide((h[i >> 1] >> (16 * (i & 1))) & 0xffffu, SRC_F16);
+                    v[i] = size_of(w) == fabsf(w) ? v[i] - w : 0.f;
+                }
+                *reinterpret_cast<u2*>(dst + kp + b0 * QK + o) = u2{narrow2(v[0], v[1], SRC_F16), narrow2(v[2], v[3], SRC_F16)};
+            }
         }
     }
-    for (int64_t c = k + threadIdx.x; c < kp; c += 256) dst[c] = 0;
+    for (int64_t c = k + threadIdx.x; c < kp; c += 256) {
+        dst[c] = 0;
+        if (rest) dst[kp + c] = 0;
+    }
     if (threadIdx.x == 0) e_out[row] = e;
     if (norm) {
         sum = reduce<false>(sum, lds);
@@ -463,17 +476,17 @@ int pack_rows(const uint16_t* src, int64_t ld, int64_t rows, int64_t k, uint16_t
 }
 
 int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e,
-              float* norm, hipStream_t st) {
+              float* norm, bool twice, hipStream_t st) {
     const dim3 grid((unsigned)rows);
-    if (kp <= 4096) hipLaunchKernelGGL((k_half_rows<16, 256>), grid, dim3(256), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm);
-    else if (kp <= 16384) hipLaunchKernelGGL((k_half_rows<16, 1024>), grid, dim3(1024), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm);
-    else hipLaunchKernelGGL((k_half_rows<0, 1024>), grid, dim3(1024), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm);
+    if (kp <= 4096) hipLaunchKernelGGL((k_half_rows<16, 256>), grid, dim3(256), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm, twice);
+    else if (kp <= 16384) hipLaunchKernelGGL((k_half_rows<16, 1024>), grid, dim3(1024), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm, twice);
+    else hipLaunchKernelGGL((k_half_rows<0, 1024>), grid, dim3(1024), 0, st, src, kind, ld, k, dst, kp, ldd, e, norm, twice);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
 int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e, float* norm,
-                hipStream_t st) {
+                bool rest, hipStream_t st) {
     DQ t{nullptr};
     const int ti = iq_table_index(type);
     if (ti >= 0) {
@@ -487,8 +500,8 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
     switch (type) {
 #define SPA_BLOCKS(T, QK, BS)                                                                                           \
     case T:                                                                                                             \
-        if (k <= 4096) hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 4096>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, t, align); \
-        else hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 16384>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, t, align); \
+        if (k <= 4096) hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 4096>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, rest, t, align); \
+        else hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 16384>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, rest, t, align); \
         break;
         SPA_BLOCKS(2, 32, 18) SPA_BLOCKS(3, 32, 20) SPA_BLOCKS(6, 32, 22) SPA_BLOCKS(7, 32, 24) SPA_BLOCKS(8, 32, 34)
         SPA_BLOCKS(10, 256, 84) SPA_BLOCKS(11, 256, 110) SPA_BLOCKS(12, 256, 144) SPA_BLOCKS(13, 256, 176) SPA_BLOCKS(14, 256, 210)
