@@ -130,7 +130,6 @@ def project(x, w, adapters=None, which=None, out=None, x_stride=None, out_stride
     """x (rows, w.cols) -> (rows, w.rows): x W^T, plus for each row r the adapter which[r] (int32; numbers
     outside the pool: none)"""
     kind, m, _, ld = _rows("x", x, x_stride, w.cols)
-    out, ldo = _out("out", out, m, w.rows, x.dtype, out_stride)
     a = b = scale = ids = None
     pool = rank = 0
     if adapters is not None:
@@ -141,6 +140,7 @@ def project(x, w, adapters=None, which=None, out=None, x_stride=None, out_stride
                              f"and a {w.rows} x {w.cols} projection")
         _ids(which, m)
         a, b, scale, ids, pool, rank = adapters.a.ptr, adapters.b.ptr, adapters.scale.ptr, which.ptr, adapters.count, adapters.rank
+    out, ldo = _out("out", out, m, w.rows, x.dtype, out_stride)
     L = lib()
     keep, p, n = _scratch(L.spa_project_work_bytes(w.type, w.rows, w.cols, kind, m, pool, rank), work, stream)
     check(L.spa_project(w.type, w.data.ptr, w.rows, w.cols, kind, x.ptr, m, ld, out.ptr, ldo, a, b, scale, pool, rank, ids,
