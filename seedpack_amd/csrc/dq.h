@@ -27,6 +27,11 @@ struct Blk {
     }
     __device__ __forceinline__ float h(int k) const { return f16_to_f32(u16(k)); }
 };
+// The same with the hardware's conversion of a scale, which differs from the other in a NaN's payload only: for
+// callers whose results are not compared bit by bit.
+struct FastBlk : Blk {
+    __device__ __forceinline__ float h(int k) const { return (float)__builtin_bit_cast(_Float16, (uint16_t)u16(k)); }
+};
 // ksigns_iq2xs[i] (ggml-common.h:513): the 7 sign bits and an 8th that makes the count even
 __device__ __forceinline__ uint32_t ksigns(uint32_t i) { return i | ((uint32_t)(__popc(i) & 1) << 7); }
 // coordinates j0..j0+3 of point g of a lattice (the device tables hold 2l+1 per coordinate) as one word

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_few(const FewArgs a, DQ t) {
 #pragma unroll
             for (int h = 0; h <= TWO; ++h) {
                 const uint8_t* src = (h ? f.w1 : f.w0) + (int64_t)tmin(n0 + row, f.n - 1) * a.rowbytes + at;
-                const Blk b{mem, (row + 16 * h) * PITCH + (int)(reinterpret_cast<uintptr_t>(src) & 15) + blk * BS};
+                const FastBlk b{{mem, (row + 16 * h) * PITCH + (int)(reinterpret_cast<uintptr_t>(src) & 15) + blk * BS}};
                 float v[8], q[4];
                 dq4<T>(b, e - blk * QK, t, kv, q);
 #pragma unroll

@@ -159,8 +159,10 @@ __device__ __forceinline__ float block_bound(const uint8_t* b) {
 }
 
 // A row's blocks go to LDS, TILE weights at a time; a row of one tile is there before its headers are looked at, so
-// that its bytes are waited for once. Longer rows: the headers from memory first.
-template <int T, int QK, int BS, int TILE>
+// that its bytes are waited for once. Longer rows: the headers from memory first. FULL: with the norm or the rest.
+// Bound by the decoding's instructions (27 a weight for Q4_K, four weights a lane with the norm always summed: 44 us
+// for 4096 x 12288).
+template <int T, int QK, int BS, int TILE, bool FULL>
 __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__ src, int64_t k, uint16_t* __restrict__ dst,
                                                      int64_t kp, int64_t ldd, int32_t* __restrict__ e_out, float* __restrict__ norm, bool rest,
                                                      DQ t, int align) {
@@ -206,33 +208,45 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
             __syncthreads();
             stage(b0, n);
         }
-        for (int q = threadIdx.x; q < n * (QK / 4); q += 256) {
-            const int o = q * 4, blk = o / QK;
-            float v[4];
-            dq4<T>(Blk{tile, blk * BS}, o - blk * QK, t, kv, v);
+        // eight weights a lane: what a block's header says of them is worked out once
+        for (int q = threadIdx.x; q < n * (QK / 8); q += 256) {
+            const int o = q * 8, blk = o / QK;
+            const FastBlk in{{tile, blk * BS}};
+            float v[8], w[4];
+            dq4<T>(in, o - blk * QK, t, kv, w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = ldexpf(v[i], -e);
-                sum = fmaf(size_of(v[i]), size_of(v[i]), sum);
+            for (int i = 0; i < 4; ++i) v[i] = w[i];
+            dq4<T>(in, o - blk * QK + 4, t, kv, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 + i] = w[i];
+            u4 h;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], -e);
+            if (FULL && norm) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum = fmaf(size_of(v[i]), size_of(v[i]), sum);
             }
-            const u2 h = u2{narrow2(v[0], v[1], SRC_F16), narrow2(v[2], v[3], SRC_F16)};
-            *reinterpret_cast<u2*>(dst + b0 * QK + o) = h;
-            if (rest) {                                           // what binary16 leaves over (nothing of infinities)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = wide((h[i >> 1] >> (16 * (i & 1))) & 0xffffu, SRC_F16);
-                    v[i] = size_of(w) == fabsf(w) ? v[i] - w : 0.f;
+            for (int i = 0; i < 4; ++i) h[i] = narrow2(v[2 * i], v[2 * i + 1], SRC_F16);
+            *reinterpret_cast<u4*>(dst + b0 * QK + o) = h;
+            if (FULL && rest) {                                   // what binary16 leaves over (nothing of infinities)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float r = wide((h[i >> 1] >> (16 * (i & 1))) & 0xffffu, SRC_F16);
+                    v[i] = size_of(r) == fabsf(r) ? v[i] - r : 0.f;
                 }
-                *reinterpret_cast<u2*>(dst + kp + b0 * QK + o) = u2{narrow2(v[0], v[1], SRC_F16), narrow2(v[2], v[3], SRC_F16)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = narrow2(v[2 * i], v[2 * i + 1], SRC_F16);
+                *reinterpret_cast<u4*>(dst + kp + b0 * QK + o) = h;
             }
         }
     }
     for (int64_t c = k + threadIdx.x; c < kp; c += 256) {
         dst[c] = 0;
-        if (rest) dst[kp + c] = 0;
+        if (FULL && rest) dst[kp + c] = 0;
     }
     if (threadIdx.x == 0) e_out[row] = e;
-    if (norm) {
+    if (FULL && norm) {
         sum = reduce<false>(sum, lds);
         if (threadIdx.x == 0) norm[row] = fminf(ldexpf(sqrtf(sum), e), 3e38f);
     }
@@ -497,17 +511,27 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
     }
     const uintptr_t a = reinterpret_cast<uintptr_t>(src) | (uintptr_t)(k / type_qk(type) * type_bs(type));
     const int align = (a & 15) == 0 ? 16 : ((a & 3) == 0 ? 4 : ((a & 1) == 0 ? 2 : 1));
+#define SPA_BLOCKS_TILE(T, QK, BS, TILE, FULL)                                                                          \
+    hipLaunchKernelGGL((k_half_blocks<T, QK, BS, TILE, FULL>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, rest, t, align)
+#define SPA_BLOCKS_FORM(T, QK, BS)                                                                                      \
+    do {                                                                                                                \
+        if (k <= 4096 && (norm || rest)) SPA_BLOCKS_TILE(T, QK, BS, 4096, true);                                        \
+        else if (k <= 4096) SPA_BLOCKS_TILE(T, QK, BS, 4096, false);                                                    \
+        else if (norm || rest) SPA_BLOCKS_TILE(T, QK, BS, 16384, true);                                                 \
+        else SPA_BLOCKS_TILE(T, QK, BS, 16384, false);                                                                  \
+    } while (0)
     switch (type) {
 #define SPA_BLOCKS(T, QK, BS)                                                                                           \
     case T:                                                                                                             \
-        if (k <= 4096) hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 4096>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, rest, t, align); \
-        else hipLaunchKernelGGL((k_half_blocks<T, QK, BS, 16384>), dim3((unsigned)rows), dim3(256), 0, st, src, k, dst, kp, ldd, e, norm, rest, t, align); \
+        SPA_BLOCKS_FORM(T, QK, BS);                                                                                     \
         break;
         SPA_BLOCKS(2, 32, 18) SPA_BLOCKS(3, 32, 20) SPA_BLOCKS(6, 32, 22) SPA_BLOCKS(7, 32, 24) SPA_BLOCKS(8, 32, 34)
         SPA_BLOCKS(10, 256, 84) SPA_BLOCKS(11, 256, 110) SPA_BLOCKS(12, 256, 144) SPA_BLOCKS(13, 256, 176) SPA_BLOCKS(14, 256, 210)
         SPA_BLOCKS(16, 256, 66) SPA_BLOCKS(17, 256, 74) SPA_BLOCKS(18, 256, 98) SPA_BLOCKS(19, 256, 50) SPA_BLOCKS(20, 32, 18)
         SPA_BLOCKS(21, 256, 110) SPA_BLOCKS(22, 256, 82) SPA_BLOCKS(23, 256, 136) SPA_BLOCKS(29, 256, 56) SPA_BLOCKS(42, 64, 18)
 #undef SPA_BLOCKS
+#undef SPA_BLOCKS_FORM
+#undef SPA_BLOCKS_TILE
         default: return fail(SPA_ERR_TYPE, "weights of type %d are not supported", type);
     }
     SPA_HIP_TRY(hipGetLastError());
