@@ -325,7 +325,6 @@ __device__ __forceinline__ void product(const Gemm& g) {
             // float32 sums, 32 input rows at a time through the wave's staging place
             float* const stage = reinterpret_cast<float*>(mem) + wave * 32 * (COLS + 4);
             float* const part = g.part + ((int64_t)(side * g.pieces + piece) * g.m) * g.n;
-            const bool wide16 = (g.n & 3) == 0;
 #pragma unroll
             for (int j = 0; j < FM; ++j) {
 #pragma unroll
@@ -342,8 +341,8 @@ __device__ __forceinline__ void product(const Gemm& g) {
                     if (mi >= g.m || n >= g.n) continue;
                     const f4 v = *reinterpret_cast<const f4*>(stage + r * (COLS + 4) + c);
                     float* p = part + (int64_t)mi * g.n + n;
-                    if (wide16) {
-                        *reinterpret_cast<f4*>(p) = v;
+                    if (n + 4 <= g.n) {
+                        __builtin_memcpy(p, &v, 16);              // at any number's address
                     } else {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
@@ -453,13 +452,14 @@ int launch(const Gemm& g, hipStream_t st) {
     return SPA_OK;
 }
 
-// The pieces of k joined in their order, and what the one-launch forms do with the sums. Four columns a lane.
+// The pieces of k joined in their order, and what the one-launch forms do with the sums. Four columns a lane, AT
+// pieces' loads under way at once.
 template <int OUT>
 __global__ __launch_bounds__(256) void k_join(const Gemm g) {
     constexpr bool TWO = OUT == OUT_GATED || OUT == OUT_GRAD;
+    constexpr int AT = 4;
     const int width = OUT == OUT_GRAD ? (int)g.np : g.n, per = (width + 3) / 4;
     const int64_t total = (int64_t)g.m * per, size = (int64_t)g.m * g.n;
-    const bool wide16 = (g.n & 3) == 0;
     for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < total; at += gridDim.x * 256ll) {
         const int m = (int)(at / per), n = (int)(at - (int64_t)m * per) * 4;
         float v[1 + TWO][4];
@@ -468,26 +468,48 @@ __global__ __launch_bounds__(256) void k_join(const Gemm g) {
             const float* p = g.part + s * g.pieces * size + (int64_t)m * g.n + n;
 #pragma unroll
             for (int c = 0; c < 4; ++c) v[s][c] = 0.f;
-            for (int i = 0; i < g.pieces; ++i, p += size) {
-                if (wide16 && n < g.n) {
-                    const f4 a = *reinterpret_cast<const f4*>(p);
+            for (int i = 0; i < g.pieces; i += AT) {
+                f4 a[AT];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) v[s][c] += a[c];
-                } else {
+                for (int j = 0; j < AT; ++j) {                    // those beyond the last are dropped
+                    const float* q = p + tmin(i + j, g.pieces - 1) * size;
+                    if (n + 4 <= g.n) {
+                        __builtin_memcpy(&a[j], q, 16);           // at any number's address
+                    } else {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (n + c < g.n) v[s][c] += p[c];
+                        for (int c = 0; c < 4; ++c) a[j][c] = n + c < g.n ? q[c] : 0.f;
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < AT; ++j)
+                    if (i + j < g.pieces)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) v[s][c] += a[j][c];
             }
         }
+        if constexpr (OUT != OUT_GRAD) {
+            uint16_t h[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int ni = n + c;
-            float a = v[0][c];
-            if constexpr (OUT == OUT_GRAD) {
+            for (int c = 0; c < 4; ++c) {
+                float a = v[0][c];
+                if constexpr (TWO) a = act_value(a, g.act) * v[1][c];
+                h[c] = narrow(a, g.kind);
+            }
+            uint16_t* y = g.y + (int64_t)m * g.ldy + n;
+            if (n + 4 <= g.n) {
+                __builtin_memcpy(y, h, 8);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (n + c < g.n) y[c] = h[c];
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int ni = n + c;
                 float value = 0.f, slope = 0.f, d = 0.f;
                 if (ni < g.n) {
-                    act_both(a, g.act, value, slope);
+                    act_both(v[0][c], g.act, value, slope);
                     d = wide(g.dh[(int64_t)m * g.ldh + ni], g.kind);
                 }
                 const int ge = g.ge ? g.ge[m] : 0;
@@ -502,9 +524,6 @@ __global__ __launch_bounds__(256) void k_join(const Gemm g) {
                         y[3 * g.np] = y[g.np];
                     }
                 }
-            } else if (ni < g.n) {
-                if constexpr (OUT == OUT_GATED) a = act_value(a, g.act) * v[1][c];
-                g.y[(int64_t)m * g.ldy + ni] = narrow(a, g.kind);
             }
         }
     }

@@ -462,10 +462,12 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
     }
 }
 
-// the row's own adapter out of the products with all of them: part [piece][m][pool rank]
+// the row's own adapter out of the products with all of them: part [piece][m][pool rank], AT pieces' loads under way
+// at once
 __global__ __launch_bounds__(256) void k_low_pick(const float* __restrict__ part, int pieces, const float* __restrict__ scale,
                                                   const int32_t* __restrict__ which, int64_t m, int pool, int rank, float* __restrict__ low,
                                                   int rp) {
+    constexpr int AT = 8;
     const int64_t width = (int64_t)pool * rank, size = m * width;
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * rp; i += gridDim.x * 256ll) {
         const int64_t mi = i / rp;
@@ -473,7 +475,14 @@ __global__ __launch_bounds__(256) void k_low_pick(const float* __restrict__ part
         float v = 0.f;
         if (r < rank && a >= 0 && a < pool) {
             const float* p = part + mi * width + (int64_t)a * rank + r;
-            for (int j = 0; j < pieces; ++j) v += p[j * size];
+            for (int j = 0; j < pieces; j += AT) {
+                float t[AT];
+#pragma unroll
+                for (int c = 0; c < AT; ++c) t[c] = p[tmin(j + c, pieces - 1) * size];     // those beyond the last are dropped
+#pragma unroll
+                for (int c = 0; c < AT; ++c)
+                    if (j + c < pieces) v += t[c];
+            }
             v *= scale[a];
         }
         low[i] = v;
