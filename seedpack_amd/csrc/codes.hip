@@ -169,35 +169,6 @@ template <> struct Unit<2> {                                      // Q4_0: block
     }
 };
 
-// a block's bytes where they lie
-struct Bytes {
-    const uint8_t* p;
-    __device__ __forceinline__ uint32_t u8(int k) const { return p[k]; }
-    __device__ __forceinline__ uint32_t u16(int k) const { return u8(k) | (u8(k + 1) << 8); }
-    __device__ __forceinline__ uint32_t u32(int k) const { return u16(k) | (u16(k + 2) << 16); }
-    __device__ __forceinline__ float h(int k) const { return f16_to_f32(u16(k)); }
-};
-// an output's sum term by term: infinite inputs make code and offset sums that cancel to NaN, where the sum over
-// the weights may be infinite (or, with inputs near the largest number, finite)
-template <int T>
-struct Direct {
-    const FewArgs& a;
-    __device__ __forceinline__ float operator()(int s, int m, int n) const {
-        const Few& f = a.f;
-        const uint8_t* w = (s ? f.w1 : f.w0) + (int64_t)n * a.rowbytes;
-        const uint16_t* x = a.rows + (int64_t)m * f.ldx;
-        float sum = 0.f;
-        for (int k = 0; k < f.k; k += 4) {
-            float v[4];
-            const int b = k / Unit<T>::QK;
-            dq4<T>(Bytes{w + (int64_t)b * Unit<T>::BS}, k - b * Unit<T>::QK, DQ{nullptr}, nullptr, v);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum = fmaf(wide(x[k + i], f.kind), v[i], sum);
-        }
-        return sum;
-    }
-};
-
 typedef const __attribute__((address_space(1))) void* gptr;
 typedef __attribute__((address_space(3))) void* lptr;
 
@@ -314,7 +285,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_codes(const FewArgs a) {
             if ((s + 1) % AHEAD == 0) asm volatile("" ::: "memory");
         }
     }
-    finish<WAVES, MT, TWO, U::HALVES>(f, n0, reinterpret_cast<float*>(mem), acc, Direct<T>{a});
+    finish<WAVES, MT, TWO, U::HALVES>(f, n0, reinterpret_cast<float*>(mem), acc, Direct<T, U::QK, U::BS>{a, DQ{nullptr}, nullptr});
 }
 
 template <int T, int KIND, bool TWO, bool AL>

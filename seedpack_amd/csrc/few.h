@@ -26,6 +26,44 @@ __device__ __forceinline__ f4 mul16(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
 }
 
+// a block's bytes where they lie
+struct Bytes {
+    const uint8_t* p;
+    __device__ __forceinline__ uint32_t u8(int k) const { return p[k]; }
+    __device__ __forceinline__ uint32_t u16(int k) const { return u8(k) | (u8(k + 1) << 8); }
+    __device__ __forceinline__ uint32_t u32(int k) const { return u16(k) | (u16(k + 2) << 16); }
+    __device__ __forceinline__ float h(int k) const { return f16_to_f32(u16(k)); }
+};
+// An output's sum term by term. Sums of codes and of offsets, or of a value's two parts, are not numbers where an
+// infinity meets a code or a part of zero, or where they cancel; the sum over the weights may be infinite there (or,
+// with inputs near the largest number, finite).
+template <int T, int QK, int BS>
+struct Direct {
+    const FewArgs& a;
+    DQ t;
+    const int8_t* kv;
+    __device__ __forceinline__ float operator()(int s, int m, int n) const {
+        const Few& f = a.f;
+        const uint8_t* w = (s ? f.w1 : f.w0) + (int64_t)n * a.rowbytes;
+        const uint16_t* x = a.rows + (int64_t)m * f.ldx;
+        float sum = 0.f;
+        if constexpr (T == 1 || T == 30) {
+            const int cols = (int)(a.rowbytes / 2);
+            for (int k = 0; k < cols; ++k)
+                sum = fmaf(wide(x[k], f.kind), wide(reinterpret_cast<const uint16_t*>(w)[k], T == 1 ? SRC_F16 : SRC_BF16), sum);
+        } else {
+            for (int k = 0; k < f.k; k += 4) {
+                float v[4];
+                const int b = k / QK;
+                dq4<T>(Bytes{w + (int64_t)b * BS}, k - b * QK, t, kv, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum = fmaf(wide(x[k + i], f.kind), v[i], sum);
+            }
+        }
+        return sum;
+    }
+};
+
 // Joins the waves' sums and writes the outputs; red has WAVES (1 + TWO) MT 256 floats. With HALVES a tile is
 // 8 input rows, each as the sum of tile rows m and m + 8. again(matrix, m, n) gives a sum anew, term by
 // term, where the joined one is not a number.

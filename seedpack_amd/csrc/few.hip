@@ -54,7 +54,7 @@ __device__ __forceinline__ void step(const u4 (&x)[MT], const float (&v)[8], f4 
     }
 }
 
-struct Never {                                                   // sums that are not numbers stay so
+struct Never {                                                   // of exact products: sums that are not numbers stay so
     __device__ __forceinline__ float operator()(int, int, int) const { return __builtin_nanf(""); }
 };
 
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_few(const FewArgs a, DQ t) {
             }
         }
     }
-    finish<WAVES, MT, TWO, false>(f, n0, reinterpret_cast<float*>(mem), acc, Never());
+    finish<WAVES, MT, TWO, false>(f, n0, reinterpret_cast<float*>(mem), acc, Direct<T, QK, BS>{a, t, kv});
 }
 
 // 16-bit weights: fragments straight from memory, the loads of four steps under way at once. LINED: rows of whole
@@ -191,7 +191,8 @@ __global__ __launch_bounds__(W * 64) void k_few16(const FewArgs a) {
             }
         }
     }
-    finish<W, MT, TWO, false>(f, n0, red, acc, Never());
+    if constexpr (WKIND == KIND) finish<W, MT, TWO, false>(f, n0, red, acc, Never());
+    else finish<W, MT, TWO, false>(f, n0, red, acc, Direct<WKIND == SRC_F16 ? 1 : 30, 1, 2>{a, DQ{nullptr}, nullptr});
 }
 
 template <int T, int QK, int BS, int KIND, bool TWO>

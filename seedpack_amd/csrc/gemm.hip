@@ -206,16 +206,19 @@ __device__ __forceinline__ void product(const Gemm& g) {
     };
     // columns c0.. of the staged rows to or from columns n.. of a matrix, `most` columns wide, eight numbers a lane
     constexpr int RUN = TNE / WN;
-    auto flush = [&](uint16_t* y, int64_t ld, int c0, int most) {
+    auto flush = [&](uint16_t* y, int64_t ld, int c0, int most, bool again) {
         const bool wide16 = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         for (int u = lane; u < ROWS * (RUN / 8); u += 64) {
             const int r = u / (RUN / 8), c = u % (RUN / 8) * 8, n = n0 + wn * RUN + c;
             if (mw + r >= g.m || n >= most) continue;
             uint16_t* p = y + (int64_t)(mw + r) * ld + n;
-            const u4 v = *reinterpret_cast<const u4*>(out + r * PITCH + c0 + c);
+            u4 v = *reinterpret_cast<const u4*>(out + r * PITCH + c0 + c);
+            if (again) v = u4{finite2(v[0]), finite2(v[1]), finite2(v[2]), finite2(v[3])};
             if (wide16 && n + 8 <= most) {
                 __builtin_nontemporal_store(v, reinterpret_cast<u4*>(p));
+            } else if (n + 8 <= most) {
+                __builtin_memcpy(p, &v, 16);                      // at any number's address
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
@@ -238,7 +241,8 @@ __device__ __forceinline__ void product(const Gemm& g) {
         };
         if (OUT == OUT_LOW || (OUT == OUT_PART && g.ex.low)) {
             // the adapters' second product, one adapter of the tile's rows at a time: rows of another
-            // adapter take part with zeros. low is split into two BF16 parts, b into two where it is F16.
+            // adapter take part with zeros. low is split into two BF16 parts, b into two where it is F16. An infinity
+            // of low is in its second part alone, which meets b's first: b's second may be zero.
             const Expand& ex = g.ex;
 #pragma unroll
             for (int j = 0; j < FM; ++j)
@@ -297,10 +301,16 @@ __device__ __forceinline__ void product(const Gemm& g) {
                     bf8 zh[FM], zl[FM];
 #pragma unroll
                     for (int j = 0; j < FM; ++j) {
-                        float v[8];
+                        float v[8], w[8];
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) v[c] = mine[j] == a ? z[j][c >> 2][c & 3] : 0.f;
-                        split8(v, zh[j], zl[j]);
+                        for (int c = 0; c < 8; ++c) {
+                            v[c] = mine[j] == a ? z[j][c >> 2][c & 3] : 0.f;
+                            w[c] = __builtin_isinf(v[c]) ? 0.f : v[c];
+                        }
+                        split8(w, zh[j], zl[j]);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            if (__builtin_isinf(v[c])) zl[j][c] = (__bf16)v[c];
                     }
 #pragma unroll
                     for (int i = 0; i < FN; ++i) {
@@ -363,17 +373,16 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 for (int q = 0; q < 4; ++q)
                     place(j, i, q) = u2{narrow2(v[4 * q], v[4 * q + 1], g.kind), narrow2(v[4 * q + 2], v[4 * q + 3], g.kind)};
             }
-        flush(g.y, g.ldy, 0, g.n);
+        flush(g.y, g.ldy, 0, g.n, false);
     } else {
         if constexpr (OUT == OUT_GRAD) {                          // dh to where its gate's gradient will lie
-            const bool wide16 = (g.ldh & 7) == 0 && (reinterpret_cast<uintptr_t>(g.dh) & 15) == 0;
             for (int u = lane; u < ROWS * (RUN / 8); u += 64) {
                 const int r = u / (RUN / 8), c = u % (RUN / 8) * 8, n = n0 + wn * RUN + c;
                 u4 v = {0, 0, 0, 0};
                 if (mw + r < g.m && n < g.n) {
                     const uint16_t* p = g.dh + (int64_t)(mw + r) * g.ldh + n;
-                    if (wide16 && n + 8 <= g.n) {
-                        v = *reinterpret_cast<const u4*>(p);
+                    if (n + 8 <= g.n) {
+                        __builtin_memcpy(&v, p, 16);
                     } else {
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
@@ -426,11 +435,11 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 }
         }
         if constexpr (OUT == OUT_GATED) {
-            flush(g.y, g.ldy, 0, g.n);
+            flush(g.y, g.ldy, 0, g.n, false);
         } else {
             for (int64_t at = 0; at <= (g.twice ? 2 * g.np : 0); at += 2 * g.np) {
-                flush(g.grad + at, g.ldg, 0, (int)g.np);
-                flush(g.grad + at + g.np, g.ldg, RUN, (int)g.np);
+                flush(g.grad + at, g.ldg, 0, (int)g.np, at != 0);
+                flush(g.grad + at + g.np, g.ldg, RUN, (int)g.np, at != 0);
             }
         }
     }
@@ -520,8 +529,8 @@ __global__ __launch_bounds__(256) void k_join(const Gemm g) {
                     y[0] = narrow(ni < g.n ? ldexpf(d * u * slope, e0 - ge) : 0.f, g.half);
                     y[g.np] = narrow(ni < g.n ? ldexpf(d * value, e1 - ge) : 0.f, g.half);
                     if (g.twice) {
-                        y[2 * g.np] = y[0];
-                        y[3 * g.np] = y[g.np];
+                        y[2 * g.np] = (uint16_t)finite2(y[0]);
+                        y[3 * g.np] = (uint16_t)finite2(y[g.np]);
                     }
                 }
             }

@@ -37,6 +37,11 @@ __device__ __forceinline__ uint16_t narrow(float v, int kind) {
 __device__ __forceinline__ uint32_t narrow2(float a, float b, int kind) {
     return (uint32_t)narrow(a, kind) | ((uint32_t)narrow(b, kind) << 16);
 }
+// two binary16 numbers beside the second parts of weights: infinities as zeros. Beside the first parts they have
+// made the sum infinite, and a second part may be zero.
+__device__ __forceinline__ uint32_t finite2(uint32_t h) {
+    return h & (((h & 0x7fffu) == 0x7c00u ? 0u : 0xffffu) | ((h & 0x7fff0000u) == 0x7c000000u ? 0u : 0xffff0000u));
+}
 
 // v = hi + lo to 2^-17 of v: hi is v cut to BF16 (so that v - hi is exact), lo the rest rounded.
 // Infinities and NaN stay in hi alone.

@@ -27,9 +27,13 @@ struct Work {
 bool is16(int type) { return type == 1 || type == 30; }
 int kind_of(int type) { return type == 1 ? SRC_F16 : SRC_BF16; }
 
+// A tile's rows are fetched at 32-bit offsets from its first: 255 rows of four inner matrices' or twice the columns
+// and their last byte have to stay below 2^32.
+constexpr int64_t MOST_COLS = 4000000, MOST_INNER = 2000000;
+
 int check_weight(const char* who, int type, int64_t n, int64_t k) {
     if (!is16(type) && !type_qk(type)) return fail(SPA_ERR_TYPE, "%s: weights of type %d are not supported", who, type);
-    if (n < 0 || k <= 0 || n > INT32_MAX - 256 || k > (1 << 22))
+    if (n < 0 || k <= 0 || n > INT32_MAX - 256 || k > MOST_COLS)
         return fail(SPA_ERR_ARG, "%s: bad weight shape %lld x %lld", who, (long long)n, (long long)k);
     if (!is16(type) && k % type_qk(type))
         return fail(SPA_ERR_ARG, "%s: row of %lld not a multiple of %d (type %d)", who, (long long)k, type_qk(type), type);
@@ -80,7 +84,7 @@ int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64
     if (same) {
         o.x = (const uint16_t*)x;
         o.ldx = ldx;
-        if (run && (kp != k || !on(x, 16) || ldx % 8 || ldx > (1 << 22))) {
+        if (run && (kp != k || !on(x, 16) || ldx % 8 || ldx > MOST_COLS)) {
             if ((rc = pack_rows((const uint16_t*)x, ldx, m, k, xp, kp, st))) return rc;
             o.x = xp;
             o.ldx = kp;
@@ -235,7 +239,7 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
         ex.wide_b = p.rank % 8 == 0 && on(p.b, 16);
         const int64_t pieces = low_as_product(p);
         float* part = wk.take<float>(pieces * p.m * p.pool * p.rank);
-        if (run && pieces && on(p.x, 16) && on(p.a, 16) && p.ldx % 8 == 0 && p.ldx <= (1 << 22)) {
+        if (run && pieces && on(p.x, 16) && on(p.a, 16) && p.ldx % 8 == 0 && p.ldx <= MOST_COLS) {
             Gemm g{};
             g.half = p.kind;
             g.x = (const uint16_t*)p.x;
@@ -492,8 +496,10 @@ extern "C" int spa_gated_backward(int type, const void* gate, const void* up, in
     if (!dgate != !dup) return fail(SPA_ERR_ARG, "%s: the gradient of one of the two matrices only", who);
     if (dgate && !(is16(type) && kind_of(type) == x_kind))
         return fail(SPA_ERR_TYPE, "%s: gradients of weights of type %d beside inputs of kind %d", who, type, x_kind);
-    if (n > (1 << 21) || m > (1 << 22)) return fail(SPA_ERR_ARG, "%s: %lld rows, %lld weight rows are too many", who, (long long)m, (long long)n);
+    if (n > MOST_INNER || m > MOST_COLS) return fail(SPA_ERR_ARG, "%s: %lld rows, %lld weight rows are too many", who, (long long)m, (long long)n);
     if (!dx && !dgate) return SPA_OK;
+    if (!on(x, 2) || !on(dh, 2) || !on(dx, 2) || !on(dgate, 2) || !on(dup, 2))
+        return fail(SPA_ERR_ARG, "%s: a pointer is not aligned to its elements", who);
     hipStream_t st = (hipStream_t)stream;
     if (m == 0 || n == 0) {                                      // sums of nothing
         if (dx && m && (rc = zero_rows((uint16_t*)dx, dx_stride, m, k, st))) return rc;
@@ -501,8 +507,6 @@ extern "C" int spa_gated_backward(int type, const void* gate, const void* up, in
         return SPA_OK;
     }
     if (!gate || !up || !x || !dh) return fail(SPA_ERR_ARG, "%s: null pointer", who);
-    if (!on(x, 2) || !on(dh, 2) || !on(dx, 2) || !on(dgate, 2) || !on(dup, 2))
-        return fail(SPA_ERR_ARG, "%s: a pointer is not aligned to its elements", who);
     if ((rc = check_weight_at(who, type, gate)) || (rc = check_weight_at(who, type, up))) return rc;
     if ((rc = check_work(who, work, work_bytes, spa_gated_backward_work_bytes(type, n, k, x_kind, m, dx != nullptr, dgate != nullptr)))) return rc;
     Gated p{};

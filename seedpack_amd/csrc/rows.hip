@@ -105,7 +105,7 @@ __global__ __launch_bounds__(LANES) void k_half_rows(const uint16_t* __restrict_
             h[i] = narrow2(a, b, SRC_F16);
         }
         *reinterpret_cast<u4*>(dst + c) = h;
-        if (twice) *reinterpret_cast<u4*>(dst + kp + c) = h;
+        if (twice) *reinterpret_cast<u4*>(dst + kp + c) = u4{finite2(h[0]), finite2(h[1]), finite2(h[2]), finite2(h[3])};
     };
     if constexpr (KEEP != 0) {
 #pragma unroll

@@ -251,6 +251,56 @@ def test_project_infinite_and_nan_rows(m):
         assert np.array_equal(wide(got[1])[sure], np.where(w64[:, 5] > 0, np.inf, -np.inf)[sure])
 
 
+
+def same_class(got, want, sure, what):
+    """infinities and NaN where the definition has them"""
+    got = wide(got)
+    odd = sure & ~np.isfinite(want)
+    ok = np.where(np.isnan(want), np.isnan(got), got == want) | ~odd
+    assert odd.any() and ok.all(), (what, np.argwhere(~ok)[:4].tolist())
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("t", [linear.F16, linear.BF16] + sorted(QFUN))
+def test_project_infinities_of_every_type(t, kind):
+    """one infinity in a row, and two that cancel: what the weights in front of them make of it, whatever form they
+    take (weights below 2^-30 of their row's largest, which the many-rows form may take as zero, are left out)"""
+    g = rng(30, t, kind is F16)
+    n, k = 37, 256
+    w, w64 = weights(g, t, n, k)
+    fit = (np.abs(w64) >= 2.0 ** -30 * np.abs(w64).max(1, keepdims=True)) | (w64 == 0)
+    for m in (3, 40, 150):
+        x, x64 = inputs(g, m, k, kind)
+        x64[0, 7], x64[1, 100], x64[2, 31], x64[2, 200] = np.inf, -np.inf, np.inf, np.inf
+        with np.errstate(invalid="ignore"):
+            want = np.stack([np.where(np.isinf(x64[r]), x64[r] * w64, 0).sum(1) for r in range(3)])
+        sure = np.stack([fit[:, np.isinf(x64[r])].all(1) for r in range(3)])
+        got = linear.project(up(store(x64, kind)), w).to_host()
+        same_class(got[:3], want, sure, (t, m))
+        assert np.isfinite(wide(got[3:])).all()
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("m,k", [(3, 512), (40, 512), (150, 512), (300, 2048)])
+def test_adapters_infinite_inputs(m, k, kind):
+    """an infinite input's part by way of an adapter of rank one, beside the projection's own; other rows as without"""
+    g = rng(31, m, kind is F16)
+    n = 70
+    w, w64 = weights(g, linear.F16 if kind is F16 else linear.BF16, n, k)
+    pool, a64, b64, s = adapters(g, 3, 1, n, k, kind)
+    which = g.integers(0, 3, m).astype(np.int32)
+    x, x64 = inputs(g, m, k, kind)
+    clean = linear.project(up(x), w, pool, up(which)).to_host()
+    x64[1, 9] = -np.inf
+    i = which[1]
+    with np.errstate(invalid="ignore"):
+        want = -np.inf * w64[:, 9] + s[i] * b64[i][:, 0] * (-np.inf * a64[i][0, 9])
+    got = linear.project(up(store(x64, kind)), w, pool, up(which)).to_host()
+    same_class(got[1], want, np.ones(n, bool), (m, k))
+    keep = np.arange(m) != 1
+    assert np.array_equal(got[keep], clean[keep])
+
+
 def act64(g, act):
     t = g if act == "silu" else 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)
     dt = np.ones_like(g) if act == "silu" else 2 * np.sqrt(2 / np.pi) * (1 + 3 * 0.044715 * g ** 2)
@@ -415,6 +465,31 @@ def test_gated_backward_strides_and_nothing():
     assert not dgate.to_host().any() and not dup.to_host().any()
     assert linear.project(dev.DeviceArray((0, k), BF16), gate).shape == (0, n)
     assert linear.gated(dev.DeviceArray((0, k), BF16), gate, upw).shape == (0, n)
+
+
+
+@pytest.mark.parametrize("t,kind", [(linear.BF16, BF16), (linear.F16, F16), (8, BF16), (8, F16), (12, F16)])
+@pytest.mark.parametrize("m", [3, 300])
+def test_gated_backward_infinite_gradient(t, kind, m):
+    """an infinity in one row of dh: that row of dx is what the weights make of it, the others are as without it"""
+    g = rng(32, t, kind is F16, m)
+    n, k = 96, 256
+    (gate, wg), (up_, wu) = weights(g, t, n, k), weights(g, t, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    d64 = wide(store(g.normal(0, 1, (m, n)), kind))
+    clean = linear.gated_backward(up(x), gate, up_, up(store(d64, kind)))[0].to_host()
+    d64[1, 17] = np.inf
+    gv, uv = x64[1] @ wg[17], x64[1] @ wu[17]
+    value, slope = act64(gv, "silu")
+    with np.errstate(invalid="ignore"):
+        want = np.inf * (uv * slope) * wg[17] + np.inf * value * wu[17]
+    got = linear.gated_backward(up(x), gate, up_, up(store(d64, kind)))[0].to_host()
+    sure = np.ones(k, bool)
+    for w in (wg[17], wu[17]):
+        sure &= (np.abs(w) >= 2.0 ** -20 * np.abs(w).max()) | (w == 0)
+    same_class(got[1], want, sure, (t, m))
+    keep = np.arange(m) != 1
+    assert np.array_equal(got[keep], clean[keep])
 
 
 @pytest.mark.parametrize("kind", [BF16, F16, np.float32])
