@@ -556,9 +556,11 @@ int spa_rans_build_lut_pb(const uint32_t* cum, int ntab, int pb, uint8_t* lut, v
  * 20 block types, at any byte. Inputs and outputs are BF16 or F16 (SPA_SRC_BF16 / SPA_SRC_F16), m rows at a stride
  * given in elements; columns between a row's end and the stride are neither read nor written. Sums are float32 and
  * each output is rounded once; where inputs and weights differ in type, weights are taken to 11 bits or better of
- * their value (rows of any exponent) and inputs exactly. Outputs must not overlap inputs. `work` is device scratch
- * of at least the call's *_work_bytes, 256-byte aligned, free again when the call's work on the stream is done;
- * the sizes are those of the widest case, whatever the strides. Nothing is allocated, and calls may be captured. */
+ * their value (22 beside F16 inputs), and inputs and weights to 2^-39 of the largest of their row. Outputs must not
+ * overlap inputs. Up to 4,000,000 columns. `work` is device scratch of at least the call's *_work_bytes, 256-byte
+ * aligned, free again when the call's work on the stream is done; the sizes are those of the widest case, whatever
+ * the strides. Nothing is allocated and calls may be captured, but for the lattice types: their table is made at its
+ * first use on a device, and a call waits for its upload. */
 
 /* y[m][n] = sum_k x[m][k] W[n][k] + scale[a] sum_r (sum_k x[m][k] A[a][r][k]) B[a][n][r], a = which[m]: a shared
  * projection with the low-rank adapters of a batch's requests. a: [pool][rank][k], b: [pool][n][rank] of the inputs'
@@ -576,7 +578,8 @@ uint64_t spa_gated_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_
 
 /* The gradients of spa_gated from dh: of the inputs (dx, or NULL) and of both matrices (dgate and dup, [n][k], or
  * NULL; weights of the inputs' own type only). Both projections are computed again: nothing but x is kept from the
- * forward pass. The inner gradients are rounded to the inputs' type (frozen weights of another type: to 11 bits). */
+ * forward pass. The inner gradients are rounded to the inputs' type (frozen weights of another type: to 11 bits). Up
+ * to 4,000,000 rows and 2,000,000 outputs. */
 int spa_gated_backward(int type, const void* gate, const void* up, int64_t n, int64_t k, int x_kind, const void* x, int64_t m,
                        int64_t x_stride, int act, const void* dh, int64_t dh_stride, void* dx, int64_t dx_stride,
                        void* dgate, void* dup, void* work, uint64_t work_bytes, void* stream);

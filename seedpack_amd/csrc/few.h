@@ -104,7 +104,8 @@ __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f
 // The inputs as the matrix instruction takes them: for each step of 32 k and each tile a run of 64 lanes x 8
 // numbers, one contiguous load of a wave. Rows of 4096 numbers lie 8 KB apart, all in the same channel of the L2:
 // with two or more tiles of them fetched side by side Q8_0 12288 x 4096 took 55 us for 32 rows. One tile is
-// read as it lies (34.4 us for 151936 x 1024 with 3 rows, 36.8 by way of fragments). HALVES: see codes.hip.
+// read as it lies (34.4 us for 151936 x 1024 with 3 rows, 36.8 by way of fragments). HALVES: see codes.hip. 3.9 us
+// for 32 rows of 4096: a launch's latency.
 template <bool HALVES>
 __global__ __launch_bounds__(256) void k_fragments(const uint16_t* __restrict__ x, int64_t ldx, int m, int k, uint16_t* __restrict__ out,
                                                    int tiles) {

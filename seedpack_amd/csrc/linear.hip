@@ -69,7 +69,8 @@ struct Operands {
 
 // Inputs and weights brought into the form of the many-rows product. Where both are of one 16-bit type they
 // are used as they lie, or copied where rows are not whole 128-byte steps at 16-byte addresses; otherwise
-// both become binary16 rows, beside F16 inputs the weights of block types in two parts. `run` false only lays out the workspace (for the widest case).
+// both become binary16 rows, beside F16 inputs the weights of block types in two parts. `run` false only lays out
+// the workspace (for the widest case).
 int operands(Work& wk, bool run, int type, const void* w0, const void* w1, int64_t n, int64_t k, int kind, const void* x, int64_t m,
              int64_t ldx, bool bounds, Operands& o, hipStream_t st) {
     const int64_t kp = up64(k);
