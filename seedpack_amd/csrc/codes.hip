@@ -333,7 +333,7 @@ template <int T>
 int pick(const Few& f, uint16_t* frags, hipStream_t st) {
     FewArgs a{f, f.rowbytes, f.x};
     if (few_tiles(T, f.m) > 1) {
-        const int rc = fragments<Unit<T>::HALVES>(f, few_tiles(T, f.m), frags, st);
+        const int rc = fragments(f, Frags{frags, few_tiles(T, f.m), f.k, Unit<T>::HALVES}, st);
         if (rc) return rc;
         a.f.x = frags;
     }

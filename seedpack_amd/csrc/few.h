@@ -101,25 +101,18 @@ __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f
     }
 }
 
-// The inputs as the matrix instruction takes them: for each step of 32 k and each tile a run of 64 lanes x 8
-// numbers, one contiguous load of a wave. Rows of 4096 numbers lie 8 KB apart, all in the same channel of the L2:
-// with two or more tiles of them fetched side by side Q8_0 12288 x 4096 took 55 us for 32 rows. One tile is
-// read as it lies (34.4 us for 151936 x 1024 with 3 rows, 36.8 by way of fragments). HALVES: see codes.hip. 3.9 us
-// for 32 rows of 4096: a launch's latency.
-template <bool HALVES>
-__global__ __launch_bounds__(256) void k_fragments(const uint16_t* __restrict__ x, int64_t ldx, int m, int k, uint16_t* __restrict__ out,
-                                                   int tiles) {
-    const int i = blockIdx.x * 256 + threadIdx.x, lane = i & 63, tile = (i >> 6) % tiles, step = (i >> 6) / tiles;
-    if (step * 32 >= k) return;
-    const int row = lane & 15, g = lane >> 4, r = HALVES ? 8 * tile + (row & 7) : 16 * tile + row;
-    u4 v = {0, 0, 0, 0};
-    if (r < m && (!HALVES || (row < 8) == (g < 2))) v = *reinterpret_cast<const u4*>(x + (int64_t)r * ldx + step * 32 + 8 * g);
-    reinterpret_cast<u4*>(out)[i] = v;
+// Rows of 4096 numbers lie 8 KB apart, all in the same channel of the L2: with two or more tiles of them fetched side
+// by side Q8_0 12288 x 4096 took 55 us for 32 rows. So their fragments are laid out first, 3.9 us for 32 rows of 4096 (a
+// launch's latency), or by the launch of the adapters' first products. One tile is read as it lies (34.4 us for
+// 151936 x 1024 with 3 rows, 36.8 by way of fragments).
+__global__ __launch_bounds__(256) void k_fragments(const uint16_t* __restrict__ x, int64_t ldx, int m, Frags fr) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < fr.tiles * (fr.k / 32) * 64) fragment(fr, x, ldx, m, i);
 }
-template <bool HALVES>
-int fragments(const Few& f, int tiles, uint16_t* out, hipStream_t st) {
-    const int lanes = tiles * (f.k / 32) * 64;
-    hipLaunchKernelGGL((k_fragments<HALVES>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, f.x, f.ldx, f.m, f.k, out, tiles);
+int fragments(const Few& f, const Frags& fr, hipStream_t st) {
+    if (f.framed) return SPA_OK;
+    const int lanes = fr.tiles * (fr.k / 32) * 64;
+    hipLaunchKernelGGL(k_fragments, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, f.x, f.ldx, f.m, fr);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }

@@ -204,7 +204,7 @@ int launch(const FewArgs& given, DQ t, uint16_t* frags, hipStream_t st) {
         FewArgs a = given;
         const int tiles = few_tiles(T, a.f.m);
         if (tiles > 1) {
-            const int rc = fragments<false>(a.f, tiles, frags, st);
+            const int rc = fragments(a.f, Frags{frags, tiles, a.f.k, false}, st);
             if (rc) return rc;
             a.f.x = frags;
         }

@@ -130,6 +130,22 @@ __device__ __forceinline__ float expand(const Expand& ex, int m, int n, int coun
 enum GemmOut { OUT_PLAIN = 0, OUT_GATED = 1, OUT_GRAD = 2, OUT_LOW = 3, OUT_PART = 4 };
 constexpr int GEMM_PIECES = 16;
 
+// The inputs as the few-rows products' matrix instruction takes them: for each step of 32 k and each tile of 16 rows
+// a run of 64 lanes x 8 numbers, one contiguous load of a wave. halves: tiles of 8 rows, each there twice, with the
+// first 16 k of a step and with the second. k a multiple of 32, rows at 16-byte addresses.
+struct Frags {
+    uint16_t* out;            // null: none
+    int tiles, k;
+    bool halves;
+};
+__device__ __forceinline__ void fragment(const Frags& fr, const uint16_t* x, int64_t ldx, int64_t m, int i) {
+    const int lane = i & 63, tile = (i >> 6) % fr.tiles, step = (i >> 6) / fr.tiles;
+    const int row = lane & 15, g = lane >> 4, r = fr.halves ? 8 * tile + (row & 7) : 16 * tile + row;
+    u4 v = {0, 0, 0, 0};
+    if (r < m && (!fr.halves || (row < 8) == (g < 2))) v = *reinterpret_cast<const u4*>(x + (int64_t)r * ldx + step * 32 + 8 * g);
+    reinterpret_cast<u4*>(fr.out)[i] = v;
+}
+
 // sum_k x[m][k] w[n][k] over rows padded to a multiple of 64 (zeros), and what becomes of it
 struct Gemm {
     int half;                 // SRC_BF16 / SRC_F16: the type of both operands
@@ -176,6 +192,7 @@ struct Few {
     int64_t ldy;
     Expand ex;
     int act;
+    bool framed;              // frags holds the inputs' fragments already
 };
 constexpr int FEW_ROWS = 64;
 // frags: scratch of few_fragments numbers
@@ -214,9 +231,9 @@ int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uin
 int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const float* n0,
                    const int32_t* e0, const float* n1, const int32_t* e1, void* top, int32_t* e, hipStream_t st);
 int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st);
-// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]
+// low[m][rp] = scale[a] x[m] A_a^T, a = which[m]; with fr.out the same launch writes the rows' fragments
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
-             const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st);
+             const int32_t* which, int pool, int rank, float* low, int rp, const Frags& fr, hipStream_t st);
 
 // the same from the pieces of x [A_0; A_1; ..]^T (gemm_pieces)
 int low_pick(const float* part, int pieces, const float* scale, const int32_t* which, int64_t m, int pool, int rank, float* low, int rp,

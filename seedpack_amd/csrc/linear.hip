@@ -228,6 +228,7 @@ int64_t tail_rows(const Gemm& g, int type) {
 int project(const Project& p, Work& wk, bool run, hipStream_t st) {
     Expand ex{};
     int rc;
+    uint16_t* framed = nullptr;                                  // the fragments of a few-rows form, made beside low
     if (p.pool) {
         ex.rank = (int)p.rank;
         ex.rp = (int)((p.rank + 15) / 16 * 16);
@@ -254,9 +255,13 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
             g.pieces = (int)pieces;
             if ((rc = gemm_pieces(g, st))) return rc;
             if ((rc = low_pick(part, (int)pieces, p.scale, p.which, p.m, (int)p.pool, (int)p.rank, low, ex.rp, st))) return rc;
-        } else if (run && (rc = low_rows((const uint16_t*)p.x, p.ldx, p.kind, p.m, p.k, (const uint16_t*)p.a, p.scale, p.which,
-                                         (int)p.pool, (int)p.rank, low, ex.rp, st))) {
-            return rc;
+        } else {
+            const int64_t frags = p.m <= FEW_ROWS && p.k % 32 == 0 ? few_fragments(p.type, p.m, p.k) : 0;
+            uint16_t* to = wk.take<uint16_t>(frags);
+            if (run && frags && on(p.x, 16) && p.ldx % 8 == 0) framed = to;
+            if (run && (rc = low_rows((const uint16_t*)p.x, p.ldx, p.kind, p.m, p.k, (const uint16_t*)p.a, p.scale, p.which, (int)p.pool,
+                                      (int)p.rank, low, ex.rp, Frags{framed, few_tiles(p.type, p.m), (int)p.k, p.type == 14}, st)))
+                return rc;
         }
     }
     auto few_rows = [&](int64_t from, int64_t m) {
@@ -272,7 +277,8 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
             f.ex.low += from * ex.rp;
             f.ex.which += from;
         }
-        return few(f, frags, st);
+        f.framed = framed != nullptr;
+        return few(f, framed ? framed : frags, st);
     };
     if (p.m <= few_limit(p.type)) {
         for (int64_t at = 0; at < p.m; at += FEW_ROWS)

@@ -349,7 +349,7 @@ __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * k; i += gridDim.x * 256ll) p[i / k * ld + i % k] = 0;
 }
 
-// low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 MT rows a workgroup and one adapter: gridDim.y workgroups take
+// low[m][r] = s_a sum_k x[m][k] A_a[r][k] for 16 MT rows a workgroup and one adapter: `most` workgroups take
 // the adapters among the rows in turn, in rising order, most of them finding none. The whole tile is
 // multiplied by the adapter's matrix and its own rows are kept. The 16 waves take 64 k (a line of each row)
 // in turn, the loads of 128 or 256 k under way at once; up to 64 ranks at a time, so that x is read once for the
@@ -360,7 +360,12 @@ template <int KIND, int MT, int TILES>
 __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restrict__ x, int64_t ldx, int64_t m, int64_t k,
                                                         const uint16_t* __restrict__ a_all, const float* __restrict__ scale,
                                                         const int32_t* __restrict__ which, int pool, int rank,
-                                                        float* __restrict__ low, int rp) {
+                                                        float* __restrict__ low, int rp, int most, const Frags fr) {
+    if (blockIdx.y >= (unsigned)most) {                           // the other job of the launch
+        const int count = fr.tiles * (fr.k / 32) * 64, step = (gridDim.y - most) * gridDim.x * (LOW_WAVES * 64);
+        for (int i = ((blockIdx.y - most) * gridDim.x + blockIdx.x) * (LOW_WAVES * 64) + threadIdx.x; i < count; i += step) fragment(fr, x, ldx, m, i);
+        return;
+    }
     __shared__ float part[LOW_WAVES][TILES][256];
     __shared__ int ids[16 * MT];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -574,11 +579,15 @@ int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st) 
 }
 
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
-             const int32_t* which, int pool, int rank, float* low, int rp, hipStream_t st) {
-    const int64_t rows = m > 256 ? 32 : 16;
-    const dim3 grid((unsigned)((m + rows - 1) / rows), (unsigned)(pool < rows ? pool : rows)), block(LOW_WAVES * 64);
+             const int32_t* which, int pool, int rank, float* low, int rp, const Frags& fr, hipStream_t st) {
+    const int64_t rows = m > 256 ? 32 : 16, tiles = (m + rows - 1) / rows;
+    const int most = pool < rows ? pool : (int)rows;
+    int64_t more = 0;                                             // two fragments a lane
+    if (fr.out) more = ((int64_t)fr.tiles * (fr.k / 32) * 64 + tiles * LOW_WAVES * 128 - 1) / (tiles * LOW_WAVES * 128);
+    if (more > 256) more = 256;
+    const dim3 grid((unsigned)tiles, (unsigned)(most + more)), block(LOW_WAVES * 64);
 #define SPA_LOW(KIND, MT, TILES) \
-    hipLaunchKernelGGL((k_low<KIND, MT, TILES>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp)
+    hipLaunchKernelGGL((k_low<KIND, MT, TILES>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, most, fr)
 #define SPA_LOW_ROWS(KIND)                                  \
     do {                                                    \
         if (rows == 32) SPA_LOW(KIND, 2, 4);                \
