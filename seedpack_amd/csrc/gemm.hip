@@ -94,6 +94,17 @@ __device__ __forceinline__ void product(const Gemm& g) {
     const int height = tmin(GROUP, mt - band * GROUP);
     const int m0 = (band * GROUP + in % height) * TM, n0 = in / height * TNE;
 
+    if (OUT == OUT_PART && g.which) {                             // a tile that serves none of its rows
+        const int a0 = n0 / g.rank, a1 = (tmin(n0 + TNE, g.n) - 1) / g.rank;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < TM / 64; ++i) {
+            const int a = g.which[tmin(m0 + 64 * i + lane, g.m - 1)];
+            any = any || (a >= a0 && a <= a1);
+        }
+        if (!__ballot(any)) return;                               // the same in every wave
+    }
+
     // where this lane fetches from: row lane / 8 of an 8-row load, the chunk that belongs at its place. Buffer
     // loads, whose addresses are a wave's base and a lane's 32-bit offset (and whose LDS writes, unlike those of
     // global loads, do not make the compiler wait for every LDS read at once).

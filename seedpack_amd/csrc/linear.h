@@ -170,6 +170,8 @@ struct Gemm {
     int most;
     float* part;
     int pieces;
+    const int32_t* which;     // gemm_pieces: weight row n serves the rows m with which[m] = n / rank only, or null
+    int rank;
 };
 int64_t gemm_part(const Gemm& g);
 // what a product is expected to take, in hundredths of a microsecond

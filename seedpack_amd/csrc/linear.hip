@@ -198,11 +198,12 @@ struct Project {
 
 // Many rows' first products as one product with every adapter of the pool, where it is small enough that
 // the rows' other adapters cost less than reading x a few lanes at a time (2053 rows of 12288, 4 adapters of rank
-// 64: 55 us row by row): 128 x 128 tiles in pieces of k that fill the device.
+// 64: 55 us row by row): 128 x 128 tiles in pieces of k that fill the device, two to a compute unit. Tiles of
+// adapters that none of their rows have are left out.
 int64_t low_as_product(const Project& p) {
     const int64_t width = p.pool * p.rank;
     if (p.m <= 256 || width > 1024 || p.k % 64 || p.k < 2048) return 0;
-    const int64_t tiles = (p.m + 127) / 128 * ((width + 127) / 128), pieces = tiles < 256 ? 256 / tiles : 1;
+    const int64_t tiles = (p.m + 127) / 128 * ((width + 127) / 128), pieces = tiles < 512 ? 512 / tiles : 1;
     return pieces < p.k / 256 ? pieces : p.k / 256;
 }
 
@@ -253,6 +254,8 @@ int project(const Project& p, Work& wk, bool run, hipStream_t st) {
             g.k = (int)p.k;
             g.part = part;
             g.pieces = (int)pieces;
+            g.which = p.which;
+            g.rank = (int)p.rank;
             if ((rc = gemm_pieces(g, st))) return rc;
             if ((rc = low_pick(part, (int)pieces, p.scale, p.which, p.m, (int)p.pool, (int)p.rank, low, ex.rp, st))) return rc;
         } else {
