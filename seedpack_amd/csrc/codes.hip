@@ -177,7 +177,7 @@ typedef __attribute__((address_space(3))) void* lptr;
 // MT = 1: the inputs are read as they lie, and MR of a lane's four sums count. More tiles: as fragments. AL: every
 // unit of a row begins at a 16-byte address.
 template <int T, int KIND, int MT, int MR, bool TWO, bool AL, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void k_codes(const FewArgs a) {
+__global__ __launch_bounds__(WAVES * 64, WAVES < 8 ? 2 : WAVES / 4) void k_codes(const FewArgs a) {
     typedef Unit<T> U;
     constexpr int STEPS = UNIT / 32, AHEAD = MT == 1 ? 8 : (MT == 2 ? 4 : (MT == 4 ? 2 : 1));
     // 16-byte words of a row's unit, wherever in the first of them it begins
