@@ -71,9 +71,13 @@ __device__ __forceinline__ void product(const Gemm& g) {
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Tiles are dealt so that each of the 8 XCDs, which take workgroups in turn, has a run of neighbours
-    // (its L2 then serves their shared rows), and a run covers 8 tiles of input rows per tile of weights.
+    // (its L2 then serves their shared rows) of one piece of k, and a run covers 8 tiles of input rows per tile of weights.
     const int nt = (g.n + TNE - 1) / TNE, mt = (g.m + TM - 1) / TM, total = nt * mt;
-    int id = blockIdx.x, piece = 0, side = 0;
+    int id, piece = 0, side = 0;
+    {
+        const int all = gridDim.x, q = all / 8, r = all % 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+        id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
+    }
     const uint16_t* w0 = g.w0;
     int k0 = 0, steps = g.k / BK;
     if (OUT == OUT_PART) {                                        // a piece of k of one matrix
@@ -84,10 +88,6 @@ __device__ __forceinline__ void product(const Gemm& g) {
         if (side) w0 = g.w1;
         k0 = steps * piece / g.pieces;
         steps = steps * (piece + 1) / g.pieces - k0;
-    }
-    {
-        const int q = total / 8, r = total % 8, xcd = id & 7, at = id >> 3;
-        id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
     }
     constexpr int GROUP = 8;
     const int band = id / (GROUP * nt), in = id - band * GROUP * nt;
