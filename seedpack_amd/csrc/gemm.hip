@@ -14,8 +14,9 @@
 // that one lane holds both values of an output.
 //
 // Bound by the matrix unit, whose clock the card's power limit lowers with the data: 4096 x 12288 x 4096 gated in
-// BF16 (two products) 658 us, 1250 TFLOP/s, matrix instructions in 73 % of the cycles; zeros in place of the numbers
-// run a quarter faster. A library's product of one such matrix took 328 us of the same data, here 340.
+// BF16 (two products) 658 us, 1250 TFLOP/s, on one card, 695 on another, matrix instructions in 70 to 76 % of the
+// cycles; zeros in place of the numbers run a quarter faster. A library's product of one such matrix took 328 us of
+// the same data, here 340.
 #include "../../include/seedpack_amd.h"
 #include "launch.h"
 #include "linear.h"

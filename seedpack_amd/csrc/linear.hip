@@ -198,7 +198,7 @@ struct Project {
 
 // Many rows' first products as one product with every adapter of the pool, where it is small enough that
 // the rows' other adapters cost less than reading x a few lanes at a time (2053 rows of 12288, 4 adapters of rank
-// 64: 55 us row by row): 128 x 128 tiles in pieces of k that fill the device, two to a compute unit. Tiles of
+// 64: 55 us row by row, 27 and 5 of picking): 128 x 128 tiles in pieces of k that fill the device, two to a compute unit. Tiles of
 // adapters that none of their rows have are left out.
 int64_t low_as_product(const Project& p) {
     const int64_t width = p.pool * p.rank;
