@@ -427,7 +427,9 @@ using namespace spa;
 using namespace spa::lin;
 
 extern "C" uint64_t spa_project_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_t m, int64_t pool, int64_t rank) {
-    if (check_weight("", type, n, k) || check_rows("", x_kind, m, k, k) || pool < 0 || (pool && rank < 1) || m == 0 || n == 0) return 0;
+    if (check_weight("", type, n, k) || check_rows("", x_kind, m, k, k) || pool < 0 || pool > INT32_MAX || (pool && (rank < 1 || rank > 256)) ||
+        m == 0 || n == 0)
+        return 0;
     Project p{};
     p.type = type, p.n = n, p.k = k, p.kind = x_kind, p.m = m, p.ldx = k, p.pool = pool, p.rank = rank;
     Work wk{nullptr};

@@ -190,8 +190,9 @@ __global__ __launch_bounds__(256) void k_squares_join(const Sq q) {
     }
 }
 
-// Rows of a run. Whole: enough workgroups to fill the device (about 1024 of them), at least 16 rows each, and one
-// launch for up to 128. By expert: 1024, so that an expert which gets most of the rows is still spread over many
+// Rows of a run. Whole: enough workgroups to fill the device (about 1024 of them), 16 to 1024 rows each (a lane's sum
+// over thousands of rows would lose its last bits: 1200000 x 4096 by 9375 rows were 3.9e-6 off), and one launch for up
+// to 128. By expert: 1024, so that an expert which gets most of the rows is still spread over many
 // workgroups and a workgroup's search of the numbers is worth its rows (16384 x 4096, 64 unlike experts, two for a
 // row: runs of 512 91, of 1024 65, of 2048 72, of 8192 202 us).
 int64_t run_rows(int64_t rows, int64_t cols, int64_t experts, bool by_expert) {
@@ -201,9 +202,10 @@ int64_t run_rows(int64_t rows, int64_t cols, int64_t experts, bool by_expert) {
         const int64_t runs = tiles < 1024 ? 1024 / tiles : 1;
         run = (rows + runs - 1) / runs;
         if (run < 16) run = 16;
+        if (run > RUN) run = RUN;
         if (rows <= 128) run = rows;
     }
-    while ((rows + run - 1) / run * tiles > (1 << 24)) run *= 2;
+    while (run < rows && (rows + run - 1) / run * tiles > (1 << 24)) run *= 2;
     return run;
 }
 uint64_t part_bytes(int64_t runs, int64_t cols, int64_t experts) {
@@ -218,7 +220,7 @@ using namespace spa;
 using namespace spa::lin;
 
 extern "C" uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts) {
-    if (rows <= 0 || cols <= 0 || experts < 0) return 0;
+    if (rows <= 0 || cols <= 0 || experts < 0 || rows > INT32_MAX || cols > INT32_MAX || experts > 65535) return 0;
     const bool by_expert = experts != 0;
     if (!by_expert) experts = 1;
     const int64_t run = run_rows(rows, cols, experts, by_expert), runs = (rows + run - 1) / run;

@@ -140,3 +140,13 @@ def test_python_refusals():
         with pytest.raises((ValueError, TypeError)):
             f()
             pytest.fail(f"refusal {i} was taken")
+
+
+def test_sizes_beyond_the_limits():
+    """sizes are answered at once, whatever is asked"""
+    L = lib()
+    assert L.spa_add_squares_work_bytes(1000, 200000, 65535) == 0                  # one run: nothing to join
+    assert L.spa_add_squares_work_bytes(5000, 200000, 65535) == 0
+    assert L.spa_add_squares_work_bytes(1000, 4096, 1 << 20) == 0
+    assert L.spa_project_work_bytes(12, 64, 256, 0, 300, 1 << 40, 1 << 40) == 0
+    assert squares(which=P, rows=1000, cols=1 << 30, xs=1 << 30, experts=65535, each=1) == ARG
