@@ -127,10 +127,12 @@ __global__ __launch_bounds__(WAVES * 64) void k_few(const FewArgs a, DQ t) {
 }
 
 // 16-bit weights: fragments straight from memory, the loads of four steps under way at once. LINED: rows of whole
-// steps at 16-byte addresses. Other rows begin at any number: their 16-byte loads cross words, and the step that
+// steps at 16-byte addresses. WORDS: rows that begin at words. ANYWHERE: at any number (three rows of 14221 x 8471: 95 us
+// with 16-byte loads from there, 59 by whole words; 3649 x 10174, whose rows begin at words, 20 and 22). The step that
 // reaches past a row's end is read number by number, with zeros (the inputs hold zeros there too, but the next
 // row's weights may be infinite).
-template <int WKIND, int KIND, int MT, bool TWO, bool LINED, int W>
+enum Lie { ANYWHERE, WORDS, LINED };
+template <int WKIND, int KIND, int MT, bool TWO, Lie LIE, int W>
 __global__ __launch_bounds__(W * 64) void k_few16(const FewArgs a) {
     const Few& f = a.f;
     __shared__ float red[W * (1 + TWO) * MT * 256];
@@ -158,10 +160,11 @@ __global__ __launch_bounds__(W * 64) void k_few16(const FewArgs a) {
 #pragma unroll
             for (int h = 0; h <= TWO; ++h) {
                 const uint8_t* p = (h ? f.w1 : f.w0) + wrow + 2 * (k + kl);
-                if (LINED) {
+                if (LIE == LINED) {
                     w[u][h] = *reinterpret_cast<const u4*>(p);
                 } else if (k + 32 <= cols) {
-                    __builtin_memcpy(&w[u][h], p, 16);
+                    if (LIE == WORDS) __builtin_memcpy(&w[u][h], p, 16);
+                    else w[u][h] = load8_words(reinterpret_cast<const uint16_t*>(p));
                 } else {
                     const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
@@ -209,12 +212,14 @@ int launch(const FewArgs& given, DQ t, uint16_t* frags, hipStream_t st) {
             a.f.x = frags;
         }
         const bool lined = a.rowbytes == 2 * (int64_t)a.f.k && ((reinterpret_cast<uintptr_t>(a.f.w0) | reinterpret_cast<uintptr_t>(a.f.w1)) & 15) == 0;
+        const bool words = a.rowbytes % 4 == 0;                   // 16-bit matrices begin at 16-byte addresses
         // few weight rows fill the device with waves only if more of them share a row's k (one row of 4060 x 5795
         // with 8 waves: 80 us)
 #define SPA_FEW16(MT, W)                                                                                    \
     do {                                                                                                    \
-        if (lined) hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, true, W>), grid, dim3(W * 64), 0, st, a); \
-        else hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, false, W>), grid, dim3(W * 64), 0, st, a);      \
+        if (lined) hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, LINED, W>), grid, dim3(W * 64), 0, st, a);         \
+        else if (words) hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, WORDS, W>), grid, dim3(W * 64), 0, st, a);    \
+        else hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, ANYWHERE, W>), grid, dim3(W * 64), 0, st, a);            \
     } while (0)
         if (a.f.m <= 16) {
             if (a.f.n < 8192) SPA_FEW16(1, 16);

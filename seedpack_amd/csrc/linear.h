@@ -37,6 +37,20 @@ __device__ __forceinline__ uint16_t narrow(float v, int kind) {
 __device__ __forceinline__ uint32_t narrow2(float a, float b, int kind) {
     return (uint32_t)narrow(a, kind) | ((uint32_t)narrow(b, kind) << 16);
 }
+// Eight 16-bit numbers from any number's address, by whole aligned words (each holds at least one of them): 16-byte
+// loads that begin between words take several times as long as others.
+__device__ __forceinline__ u4 load8_words(const uint16_t* p) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+    const uint32_t odd = (uint32_t)at & 2;
+    u4 v;
+    __builtin_memcpy(&v, w, 16);
+    const uint32_t t = w[odd ? 4 : 3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_alignbyte(i < 3 ? v[i + 1] : t, v[i], odd);
+    return v;
+}
+
 // two binary16 numbers beside the second parts of weights: infinities as zeros. Beside the first parts they have
 // made the sum infinite, and a second part may be zero.
 __device__ __forceinline__ uint32_t finite2(uint32_t h) {

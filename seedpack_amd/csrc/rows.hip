@@ -11,9 +11,12 @@ namespace lin {
 namespace {
 
 // eight elements from k on, zeros from n on. The address may be any element's: gfx950 loads 16 bytes from any byte.
+// WORDS false: see load8_words
+template <bool WORDS = true>
 __device__ __forceinline__ void load8(const uint16_t* row, int64_t k, int64_t n, u4& v) {
     if (k + 8 <= n) {
-        __builtin_memcpy(&v, row + k, 16);
+        if (WORDS) __builtin_memcpy(&v, row + k, 16);
+        else v = load8_words(row + k);
         return;
     }
 #pragma unroll
@@ -356,7 +359,7 @@ __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
 // usual ranks. Bound by the latency of its few workgroups' loads: 7 us for a row of 4096 at rank 16, 12 us for 32 rows
 // with 16 adapters.
 constexpr int LOW_WAVES = 16;
-template <int KIND, int MT, int TILES>
+template <int KIND, int MT, int TILES, bool WORDS>
 __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restrict__ x, int64_t ldx, int64_t m, int64_t k,
                                                         const uint16_t* __restrict__ a_all, const float* __restrict__ scale,
                                                         const int32_t* __restrict__ which, int pool, int rank,
@@ -415,7 +418,7 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t][j] = f4{0, 0, 0, 0};
         }
-        constexpr int U = TILES == 1 ? 8 : (MT == 1 ? 4 : 2);                        // steps of 32 k at once
+        constexpr int U = (TILES == 1 ? 8 : 4) / MT;              // steps of 32 k at once
         for (int64_t l = wave; l < lines; l += LOW_WAVES * (U / 2)) {
             u4 xv[U][MT], av[U][TILES];
 #pragma unroll
@@ -427,12 +430,12 @@ __global__ __launch_bounds__(LOW_WAVES * 64) void k_low(const uint16_t* __restri
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     xv[u][t] = u4{0, 0, 0, 0};
-                    if (in) load8(xr[t], k0, k, xv[u][t]);
+                    if (in) load8<WORDS>(xr[t], k0, k, xv[u][t]);
                 }
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) {
                     av[u][j] = u4{0, 0, 0, 0};
-                    if (in && j < tiles) load8(ar[j], k0, k, av[u][j]);
+                    if (in && j < tiles) load8<WORDS>(ar[j], k0, k, av[u][j]);
                 }
             }
 #pragma unroll
@@ -580,19 +583,26 @@ int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st) 
 
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,
              const int32_t* which, int pool, int rank, float* low, int rp, const Frags& fr, hipStream_t st) {
-    const int64_t rows = m > 256 ? 32 : 16, tiles = (m + rows - 1) / rows;
+    const bool words = k % 2 == 0 && ldx % 2 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a)) & 3) == 0;
+    // two tiles of four, whose loads begin anywhere, do not fit in the registers
+    const int64_t rows = m > 256 && (words || rp <= 16) ? 32 : 16, tiles = (m + rows - 1) / rows;
     const int most = pool < rows ? pool : (int)rows;
     int64_t more = 0;                                             // two fragments a lane
     if (fr.out) more = ((int64_t)fr.tiles * (fr.k / 32) * 64 + tiles * LOW_WAVES * 128 - 1) / (tiles * LOW_WAVES * 128);
     if (more > 256) more = 256;
     const dim3 grid((unsigned)tiles, (unsigned)(most + more)), block(LOW_WAVES * 64);
-#define SPA_LOW(KIND, MT, TILES) \
-    hipLaunchKernelGGL((k_low<KIND, MT, TILES>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, rp, most, fr)
-#define SPA_LOW_ROWS(KIND)                                  \
-    do {                                                    \
-        if (rows == 32) SPA_LOW(KIND, 2, 4);                \
-        else if (rp <= 16) SPA_LOW(KIND, 1, 1);             \
-        else SPA_LOW(KIND, 1, 4);                           \
+#define SPA_LOW(KIND, MT, TILES, WORDS)                                                                                       \
+    hipLaunchKernelGGL((k_low<KIND, MT, TILES, WORDS>), grid, block, 0, st, x, ldx, m, k, a, scale, which, pool, rank, low, \
+                       rp, most, fr)
+#define SPA_LOW_ROWS(KIND)                                           \
+    do {                                                             \
+        if (rows == 32 && rp > 16) SPA_LOW(KIND, 2, 4, true);        \
+        else if (rows == 32 && words) SPA_LOW(KIND, 2, 1, true);     \
+        else if (rows == 32) SPA_LOW(KIND, 2, 1, false);             \
+        else if (rp <= 16 && words) SPA_LOW(KIND, 1, 1, true);       \
+        else if (rp <= 16) SPA_LOW(KIND, 1, 1, false);               \
+        else if (words) SPA_LOW(KIND, 1, 4, true);                   \
+        else SPA_LOW(KIND, 1, 4, false);                             \
     } while (0)
     if (kind == SRC_BF16) SPA_LOW_ROWS(SRC_BF16);
     else SPA_LOW_ROWS(SRC_F16);
