@@ -255,11 +255,16 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 v[c] = ldexpf(v[c], xe + (we ? we[ni] : 0));
             }
         };
+        const Expand& ex = g.ex;
+        // pieces of k share the ranks, 16 at a time
+        const int first = OUT == OUT_PART ? piece * 16 : 0, stride = OUT == OUT_PART ? g.pieces * 16 : 16;
+        bool odd = false;                                         // some number of b was not finite
         if (OUT == OUT_LOW || (OUT == OUT_PART && g.ex.low)) {
             // the adapters' second product, one adapter of the tile's rows at a time: rows of another
             // adapter take part with zeros. low is split into two BF16 parts, b into two where it is F16. An infinity
-            // of low is in its second part alone, which meets b's first: b's second may be zero.
-            const Expand& ex = g.ex;
+            // of low is in its second part alone, which meets b's first: b's second may be zero. Infinities and NaN of
+            // b, which zeros would make NaN in other adapters' rows, are the largest number here; their rows
+            // get them below.
 #pragma unroll
             for (int j = 0; j < FM; ++j)
 #pragma unroll
@@ -274,9 +279,7 @@ __device__ __forceinline__ void product(const Gemm& g) {
             }
 #pragma unroll
             for (int i = 0; i < FN; ++i) brow0[i] = tmin(n0 + arow[i], g.n - 1);
-            // pieces of k share the ranks, 16 at a time. Rows and columns beyond the last are read as the last: they
-            // are not kept.
-            const int first = OUT == OUT_PART ? piece * 16 : 0, stride = OUT == OUT_PART ? g.pieces * 16 : 16;
+            // rows and columns beyond the last are read as the last: they are not kept
             int ids[TM / 64];                                     // those outside the pool as -1
 #pragma unroll
             for (int i = 0; i < TM / 64; ++i) {
@@ -313,6 +316,11 @@ __device__ __forceinline__ void product(const Gemm& g) {
                         for (int c = 0; c < 4; ++c) {
                             const int left = ex.rank - r - 2 * c;
                             h[i][c] &= left >= 2 ? 0xffffffffu : (left == 1 ? 0xffffu : 0u);
+                            const uint32_t top = ex.kind == SRC_BF16 ? 0x7f80u : 0x7c00u, most = ex.kind == SRC_BF16 ? 0x7f7fu : 0x7bffu;
+                            const bool lo = (h[i][c] & top) == top, hi = (h[i][c] >> 16 & top) == top;
+                            odd = odd || lo || hi;
+                            if (lo) h[i][c] = (h[i][c] & 0xffff8000u) | most;
+                            if (hi) h[i][c] = (h[i][c] & 0x8000ffffu) | most << 16;
                         }
                     bf8 zh[FM], zl[FM];
 #pragma unroll
@@ -347,6 +355,20 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 }
             }
         }
+        odd = __ballot(odd) != 0;
+        // what the numbers of b that are not finite give output (mi, ni): infinities, NaN, or nothing
+        auto lost = [&](int mi, int ni) {
+            float t = 0.f;
+            const int a = ex.which[mi];
+            if (a < 0 || a >= ex.pool) return t;
+            const uint16_t* p = ex.b + ((int64_t)a * g.n + ni) * ex.rank;
+            for (int r0 = first; r0 < ex.rank; r0 += stride)
+                for (int r = r0; r < tmin(r0 + 16, ex.rank); ++r) {
+                    const float b = wide(p[r], ex.kind);
+                    if (!(fabsf(b) <= 3.4028235e38f)) t = fmaf(ex.low[(int64_t)mi * ex.rp + r], b, t);
+                }
+            return t;
+        };
         if constexpr (OUT == OUT_PART) {
             // float32 sums, 32 input rows at a time through the wave's staging place
             float* const stage = reinterpret_cast<float*>(mem) + wave * 32 * (COLS + 4);
@@ -365,7 +387,10 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 for (int u = lane; u < 32 * (COLS / 4); u += 64) {
                     const int r = u / (COLS / 4), c = u % (COLS / 4) * 4, n = n0 + wn * COLS + c, mi = mw + 32 * j + r;
                     if (mi >= g.m || n >= g.n) continue;
-                    const f4 v = *reinterpret_cast<const f4*>(stage + r * (COLS + 4) + c);
+                    f4 v = *reinterpret_cast<const f4*>(stage + r * (COLS + 4) + c);
+                    if (odd)
+                        for (int k = 0; k < 4; ++k)
+                            if (n + k < g.n) v[k] += lost(mi, n + k);
                     float* p = part + (int64_t)mi * g.n + n;
                     if (n + 4 <= g.n) {
                         __builtin_memcpy(p, &v, 16);              // at any number's address
@@ -389,6 +414,16 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 for (int q = 0; q < 4; ++q)
                     place(j, i, q) = u2{narrow2(v[4 * q], v[4 * q + 1], g.kind), narrow2(v[4 * q + 2], v[4 * q + 3], g.kind)};
             }
+        if (odd) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int u = lane; u < ROWS * COLS; u += 64) {
+                const int r = u / COLS, c = u % COLS, n = n0 + wn * COLS + c;
+                if (mw + r >= g.m || n >= g.n) continue;
+                const float t = lost(mw + r, n);
+                uint16_t& at = out[r * PITCH + c];
+                if (t != 0.f) at = narrow(wide(at, g.kind) + t, g.kind);
+            }
+        }
         flush(g.y, g.ldy, 0, g.n, false);
     } else {
         if constexpr (OUT == OUT_GRAD) {                          // dh to where its gate's gradient will lie

@@ -1,0 +1,41 @@
+"""The products with packed weights at the ends of their ranges, against float64 restatements: numbers that are not
+finite and whom they may reach, the largest and the least inputs, and what the forms keep of weights of many bits.
+
+Tolerances are those of test_linear_gpu (an output's rounding, K 2^-24 T for float32 sums of K terms, T the sum over
+absolute values, and what a form's operands lose), with the operands' part named by each test."""
+import numpy as np
+import pytest
+
+from seedpack_amd import linear
+from seedpack_amd.gpuquant import GPUQuant
+from seedpack_amd.requant import QFUN
+from tests.test_linear_gpu import (BF16, F16, _named, adapters, close, gated_backward64, inputs, project64, random_blocks,  # noqa: F401
+                                   rng, slack, store, up, weights, wide)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("m,k,rank", [(40, 512, 5), (150, 512, 5), (300, 512, 16), (300, 2048, 20)])
+def test_adapter_that_is_not_finite(m, k, rank, bad, kind):
+    """one number of one adapter's second matrix: its own rows have what the definition says in that column; rows of
+    other adapters and of none, in the same tile, are bit for bit as without it"""
+    g = rng(40, m, k, kind is F16)
+    n, pool = 140, 3
+    w, w64 = weights(g, linear.F16 if kind is F16 else linear.BF16, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    ad, a, b, s = adapters(g, pool, rank, n, k, kind)
+    which = g.integers(-1, pool, m).astype(np.int32)
+    clean = linear.project(up(x), w, ad, up(which)).to_host()
+    worse = b.copy()
+    worse[1, 9, 2] = bad
+    got = linear.project(up(x), w, linear.Adapters(ad.a, up(store(worse, kind)), ad.scale), up(which)).to_host()
+    mine = which == 1
+    assert mine.any() and not mine.all()
+    assert np.array_equal(got[~mine], clean[~mine])
+    rest = np.arange(n) != 9
+    y, total = project64(x64[mine], w64, a, b, s, which[mine])
+    close(np.ascontiguousarray(got[mine][:, rest]), y[:, rest], slack(total[:, rest], k + rank), kind)
+    want = bad * np.sign(x64[mine] @ a[1][2])
+    assert np.array_equal(wide(got[mine][:, 9]), want, equal_nan=True)
