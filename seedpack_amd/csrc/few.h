@@ -35,10 +35,12 @@ struct Bytes {
     __device__ __forceinline__ float h(int k) const { return f16_to_f32(u16(k)); }
 };
 // An output's sum term by term. Sums of codes and of offsets, or of a value's two parts, are not numbers where an
-// infinity meets a code or a part of zero, or where they cancel; the sum over the weights may be infinite there (or,
-// with inputs near the largest number, finite).
+// infinity meets a code or a part of zero, or where they cancel; the sum over the weights may be infinite there. And
+// with inputs near the largest number (BF16 from about 1e36) a code's base, 128 times its input, passes float32: the
+// sum of codes is infinite or not a number where the sum over the weights is finite.
 template <int T, int QK, int BS>
 struct Direct {
+    static constexpr bool ANEW = true;
     const FewArgs& a;
     DQ t;
     const int8_t* kv;
@@ -66,7 +68,7 @@ struct Direct {
 
 // Joins the waves' sums and writes the outputs; red has WAVES (1 + TWO) MT 256 floats. With HALVES a tile is
 // 8 input rows, each as the sum of tile rows m and m + 8. again(matrix, m, n) gives a sum anew, term by
-// term, where the joined one is not a number.
+// term, where the joined one is infinite or not a number.
 template <int WAVES, int MT, bool TWO, bool HALVES, class Again>
 __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f4 (&acc)[1 + TWO][MT], Again again) {
     constexpr int HIGH = HALVES ? 8 : 16, S = (1 + TWO) * MT * 256;
@@ -92,7 +94,8 @@ __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f
                 const float* p = red + w * S + s * MT * 256 + at;
                 v[s] += HALVES ? p[0] + p[128] : p[0];
             }
-            if (v[s] != v[s]) v[s] = again(s, m, n);
+            if constexpr (Again::ANEW)
+                if (!(fabsf(v[s]) <= 3.4028235e38f)) v[s] = again(s, m, n);
         }
         float y;
         if constexpr (TWO) y = act_value(v[0], f.act) * v[1];

@@ -55,8 +55,8 @@ __device__ __forceinline__ void step(const u4 (&x)[MT], const float (&v)[8], f4 
     }
 }
 
-struct Never {                                                   // of exact products: sums that are not numbers stay so
-    __device__ __forceinline__ float operator()(int, int, int) const { return __builtin_nanf(""); }
+struct Never {                                                   // of exact products: sums stay as they are
+    static constexpr bool ANEW = false;
 };
 
 // Block types: a chunk of 1024 k of the 16 rows is copied to LDS as it lies (whole 16-byte words around each

@@ -39,3 +39,32 @@ def test_adapter_that_is_not_finite(m, k, rank, bad, kind):
     close(np.ascontiguousarray(got[mine][:, rest]), y[:, rest], slack(total[:, rest], k + rank), kind)
     want = bad * np.sign(x64[mine] @ a[1][2])
     assert np.array_equal(wide(got[mine][:, 9]), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 64, 100, 150])
+@pytest.mark.parametrize("t", [linear.F16, linear.BF16, 2, 8, 12, 13, 14, 3, 16, 20, 23])
+def test_project_largest_inputs(t, m):
+    """BF16 inputs so large that the sums come near the largest float32 and codes times inputs pass it: finite as
+    the definition is"""
+    g = rng(41, t, m)
+    n, k = 37, 512
+    w, w64 = weights(g, t, n, k)
+    x = g.normal(0, 1, (m, k))
+    x *= 2.0 ** np.floor(np.log2(2.0 ** 127 / (np.abs(x) @ np.abs(w64.T)).max(1, keepdims=True)))
+    x = store(np.clip(x, -3e38, 3e38), BF16)
+    y, total = project64(wide(x), w64)
+    assert total.max() < 3.4e38 and np.isfinite(wide(x)).all()
+    close(linear.project(up(x), w).to_host(), y, slack(total, k), BF16)
+
+
+@pytest.mark.parametrize("m", [1, 20, 64])
+@pytest.mark.parametrize("t", [2, 8, 12, 13, 14])
+def test_gated_largest_inputs(t, m):
+    """the same gate beside an up projection of zeros: zeros, not an infinity times zero"""
+    g = rng(42, t, m)
+    n, k = 37, 512
+    gate, w64 = weights(g, t, n, k)
+    zero = linear.Weight(t, up(np.zeros(gate.data.nbytes, np.uint8)), n, k)
+    x = g.normal(0, 1, (m, k))
+    x *= 2.0 ** np.floor(np.log2(2.0 ** 127 / (np.abs(x) @ np.abs(w64.T)).max(1, keepdims=True)))
+    assert (wide(linear.gated(up(store(np.clip(x, -3e38, 3e38), BF16)), gate, zero).to_host()) == 0).all()
