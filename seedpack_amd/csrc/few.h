@@ -34,27 +34,43 @@ struct Bytes {
     __device__ __forceinline__ uint32_t u32(int k) const { return u16(k) | (u16(k + 2) << 16); }
     __device__ __forceinline__ float h(int k) const { return f16_to_f32(u16(k)); }
 };
-// An output's sum term by term. Sums of codes and of offsets, or of a value's two parts, are not numbers where an
-// infinity meets a code or a part of zero, or where they cancel; the sum over the weights may be infinite there. And
-// with inputs near the largest number (BF16 from about 1e36) a code's base, 128 times its input, passes float32: the
-// sum of codes is infinite or not a number where the sum over the weights is finite.
+// An output's sum term by term, by a wave. Sums of codes and of offsets, or of a value's two parts, are not numbers
+// where an infinity meets a code or a part of zero, or where they cancel; the sum over the weights may be infinite
+// there. And with inputs near the largest number (BF16 from about 1e36) a code's base, 128 times its input, passes
+// float32: the sum of codes is infinite or not a number where the sum over the weights is finite.
+// A row that holds a NaN is looked through first: its sums are NaN whatever the weights are. (One lane for an output,
+// weight by weight, with no such look: one row of 4096 through 12288 x 4096 Q4_K 620 us instead of 9.)
 template <int T, int QK, int BS>
 struct Direct {
     static constexpr bool ANEW = true;
     const FewArgs& a;
     DQ t;
     const int8_t* kv;
+    __device__ __forceinline__ bool nan_in(int m) const {
+        const Few& f = a.f;
+        const int lane = threadIdx.x & 63;
+        const uint16_t* x = a.rows + (int64_t)m * f.ldx;
+        bool nan = false;
+        for (int k = 8 * lane; k < f.k; k += 512) {               // rows of whole steps of 32 at 16-byte addresses
+            const u4 h = *reinterpret_cast<const u4*>(x + k);
+            const uint32_t top = f.kind == SRC_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan = nan || (h[i] & 0x7fffu) > top || (h[i] >> 16 & 0x7fffu) > top;
+        }
+        return __ballot(nan) != 0;
+    }
     __device__ __forceinline__ float operator()(int s, int m, int n) const {
         const Few& f = a.f;
+        const int lane = threadIdx.x & 63;
         const uint8_t* w = (s ? f.w1 : f.w0) + (int64_t)n * a.rowbytes;
         const uint16_t* x = a.rows + (int64_t)m * f.ldx;
         float sum = 0.f;
         if constexpr (T == 1 || T == 30) {
             const int cols = (int)(a.rowbytes / 2);
-            for (int k = 0; k < cols; ++k)
+            for (int k = lane; k < cols; k += 64)
                 sum = fmaf(wide(x[k], f.kind), wide(reinterpret_cast<const uint16_t*>(w)[k], T == 1 ? SRC_F16 : SRC_BF16), sum);
         } else {
-            for (int k = 0; k < f.k; k += 4) {
+            for (int k = 4 * lane; k < f.k; k += 256) {
                 float v[4];
                 const int b = k / QK;
                 dq4<T>(Bytes{w + (int64_t)b * BS}, k - b * QK, t, kv, v);
@@ -62,13 +78,15 @@ struct Direct {
                 for (int i = 0; i < 4; ++i) sum = fmaf(wide(x[k + i], f.kind), v[i], sum);
             }
         }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
         return sum;
     }
 };
 
 // Joins the waves' sums and writes the outputs; red has WAVES (1 + TWO) MT 256 floats. With HALVES a tile is
-// 8 input rows, each as the sum of tile rows m and m + 8. again(matrix, m, n) gives a sum anew, term by
-// term, where the joined one is infinite or not a number.
+// 8 input rows, each as the sum of tile rows m and m + 8. again(matrix, m, n), called by whole waves, gives a
+// sum anew, term by term, where the joined one is infinite or not a number and again.nan_in(m) does not say why.
 template <int WAVES, int MT, bool TWO, bool HALVES, class Again>
 __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f4 (&acc)[1 + TWO][MT], Again again) {
     constexpr int HIGH = HALVES ? 8 : 16, S = (1 + TWO) * MT * 256;
@@ -84,19 +102,32 @@ __device__ __forceinline__ void finish(const Few& f, int n0, float* red, const f
     __syncthreads();
     for (int i = threadIdx.x; i < MT * HIGH * 16; i += WAVES * 64) {
         const int m = i >> 4, n = n0 + (i & 15), at = HALVES ? (m >> 3) * 256 + (m & 7) * 16 + (i & 15) : i;
-        if (m >= f.m || n >= f.n) continue;
+        const bool in = m < f.m && n < f.n;
         float v[1 + TWO];
 #pragma unroll
         for (int s = 0; s <= TWO; ++s) {
             v[s] = 0.f;
+            if (!in) continue;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 const float* p = red + w * S + s * MT * 256 + at;
                 v[s] += HALVES ? p[0] + p[128] : p[0];
             }
-            if constexpr (Again::ANEW)
-                if (!(fabsf(v[s]) <= 3.4028235e38f)) v[s] = again(s, m, n);
         }
+        if constexpr (Again::ANEW) {
+            int looked = -1;
+            bool nan = false;
+#pragma unroll
+            for (int s = 0; s <= TWO; ++s)
+                for (uint64_t left = __ballot(!(fabsf(v[s]) <= 3.4028235e38f)); left; left &= left - 1) {
+                    const int from = __builtin_ctzll(left), row = __builtin_amdgcn_readlane(m, from);
+                    if (row != looked) nan = again.nan_in(row);
+                    looked = row;
+                    const float sum = nan ? __builtin_nanf("") : again(s, row, __builtin_amdgcn_readlane(n, from));
+                    if (lane == from) v[s] = sum;
+                }
+        }
+        if (!in) continue;
         float y;
         if constexpr (TWO) y = act_value(v[0], f.act) * v[1];
         else y = f.ex.low ? v[0] + expand(f.ex, m, n, f.n) : v[0];

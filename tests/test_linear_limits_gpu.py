@@ -68,3 +68,27 @@ def test_gated_largest_inputs(t, m):
     x = g.normal(0, 1, (m, k))
     x *= 2.0 ** np.floor(np.log2(2.0 ** 127 / (np.abs(x) @ np.abs(w64.T)).max(1, keepdims=True)))
     assert (wide(linear.gated(up(store(np.clip(x, -3e38, 3e38), BF16)), gate, zero).to_host()) == 0).all()
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 64])
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("t", [linear.F16, linear.BF16, 8, 12, 14, 10, 19])
+def test_few_rows_with_numbers_that_are_not_finite(t, kind, m):
+    """all of a row infinite or NaN, or one number in its first or last places: every output of the row as defined"""
+    g = rng(43, t, m, kind is F16)
+    n, k = 70, 1280
+    w, w64 = weights(g, t, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    clean = linear.project(up(x), w).to_host()
+    for at, v in ((0, np.nan), (k - 1, np.nan), (slice(0, None), np.nan), (0, np.inf), (k - 1, -np.inf), (777, np.inf)):
+        bad = x64.copy()
+        bad[m // 2, at] = v
+        got = linear.project(up(store(bad, kind)), w).to_host()
+        keep = np.arange(m) != m // 2
+        assert np.array_equal(got[keep], clean[keep])
+        row = wide(got[m // 2])
+        if np.isnan(v):
+            assert np.isnan(row).all()
+        else:
+            with np.errstate(invalid="ignore"):
+                assert np.array_equal(row, v * w64[:, at], equal_nan=True)
