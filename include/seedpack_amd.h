@@ -578,8 +578,10 @@ uint64_t spa_gated_work_bytes(int type, int64_t n, int64_t k, int x_kind, int64_
 
 /* The gradients of spa_gated from dh: of the inputs (dx, or NULL) and of both matrices (dgate and dup, [n][k], or
  * NULL; weights of the inputs' own type only). Both projections are computed again: nothing but x is kept from the
- * forward pass. The inner gradients are rounded to the inputs' type (frozen weights of another type: to 11 bits). Up
- * to 4,000,000 rows and 2,000,000 outputs. */
+ * forward pass. The inner gradients dh up(x) act' and dh act are rounded once, to 8 bits beside BF16 weights and inputs,
+ * else to 11 bits and to 2^-34 of what their row (for the weights' gradients: their column too) can hold at most,
+ * 1.13 max|dh| |x| max|w|: they neither overflow nor vanish where the results do not. Up to 4,000,000 rows and 2,000,000
+ * outputs. */
 int spa_gated_backward(int type, const void* gate, const void* up, int64_t n, int64_t k, int x_kind, const void* x, int64_t m,
                        int64_t x_stride, int act, const void* dh, int64_t dh_stride, void* dx, int64_t dx_stride,
                        void* dgate, void* dup, void* work, uint64_t work_bytes, void* stream);

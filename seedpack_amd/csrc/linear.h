@@ -239,13 +239,22 @@ int half_rows(const uint16_t* src, int kind, int64_t ld, int64_t rows, int64_t k
 // the same from a block type; rest: what the rounding leaves over kp further on
 int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t* dst, int64_t kp, int64_t ldd, int32_t* e, float* norm,
                 bool rest, hipStream_t st);
-// dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (rp and ldd multiples of 8)
+// dst[c][r] = src[r][c], rows of ldd, r padded with zeros to rp (rp and ldd multiples of 8); with re and ce F16 values
+// times 2^(re[r] - ce[c])
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
-                hipStream_t st);
+                const int32_t* re, const int32_t* ce, hipStream_t st);
 // the power of two to take out of each row of the gated block's inner gradients, by the 2-norms of the inputs'
 // rows and of both matrices' rows; top: 8 bytes of scratch
 int grad_exponents(const uint16_t* dh, int kind, int64_t ld, int64_t rows, int64_t n, const float* xnorm, const float* n0,
                    const int32_t* e0, const float* n1, const int32_t* e1, void* top, int32_t* e, hipStream_t st);
+// the 2-norms of the rows of x and of both matrices (F16)
+int norms16(const uint16_t* x, int64_t ldx, int64_t m, const uint16_t* w0, const uint16_t* w1, int64_t n, int64_t k, float* xn, float* n0,
+            float* n1, hipStream_t st);
+// and the powers of two to take out of each row of the inner gradients, ge, and of each column, ce [gate np][up np], np
+// the next multiple of 64; part: scratch of tops_part(m, n) numbers
+int64_t tops_part(int64_t m, int64_t n);
+int tops16(const uint16_t* dh, int64_t ld, int64_t m, int64_t n, const float* xn, const float* n0, const float* n1, float* part, int32_t* ge,
+           int32_t* ce, hipStream_t st);
 int zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k, hipStream_t st);
 // low[m][rp] = scale[a] x[m] A_a^T, a = which[m]; with fr.out the same launch writes the rows' fragments
 int low_rows(const uint16_t* x, int64_t ldx, int kind, int64_t m, int64_t k, const uint16_t* a, const float* scale,

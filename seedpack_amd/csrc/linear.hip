@@ -351,7 +351,10 @@ int gated(const Gated& p, Work& wk, bool run, hipStream_t st) {
 }
 
 // grad = [dG | dU] in one matrix of 2 np columns; dx = grad [Wg; Wu] is then one product over 2 np, with the
-// weights transposed side by side, and the weights' gradients are products over the rows.
+// weights transposed side by side, and the weights' gradients are products over the rows. grad is rounded once to the
+// operands' type, as a program that keeps it would store it: in float32 parts the products that follow would be twice
+// or three times as many. BF16 holds any size; beside binary16 operands a power of two is taken out of each row, and for
+// the weights' gradients (F16 weights) of each column in its place.
 int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w, hipStream_t st) {
     int rc;
     const int64_t np = up64(p.n), mp = up64(p.m);
@@ -359,10 +362,19 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     if ((rc = operands(wk, run, p.type, p.gate, run ? p.up : SOME, p.n, p.k, p.kind, p.x, p.m, p.ldx, true, o, st))) return rc;
     const int64_t wide = o.rest ? 4 * np : 2 * np, ldg = wide + PAD, ldm = mp + PAD;
     uint16_t* grad = wk.take<uint16_t>(p.m * ldg);
-    int32_t* ge = o.norm ? wk.take<int32_t>(p.m) : nullptr;
-    void* top = wk.take<uint8_t>(8);
-    if (run && ge && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.n0, o.we0, o.n1, o.we1, top, ge, st)))
-        return rc;
+    int32_t *ge = nullptr, *ce = nullptr;                        // taken out of grad's rows; out of its columns
+    if (o.norm) {
+        ge = wk.take<int32_t>(p.m);
+        void* top = wk.take<uint8_t>(8);
+        if (run && (rc = grad_exponents((const uint16_t*)p.dh, p.kind, p.ldh, p.m, p.n, o.norm, o.n0, o.we0, o.n1, o.we1, top, ge, st)))
+            return rc;
+    } else if (o.half == SRC_F16) {
+        ge = wk.take<int32_t>(p.m);
+        ce = wk.take<int32_t>(2 * np);
+        float *xn = wk.take<float>(p.m), *n0 = wk.take<float>(p.n), *n1 = wk.take<float>(p.n), *part = wk.take<float>(tops_part(p.m, p.n));
+        if (run && (rc = norms16((const uint16_t*)p.x, p.ldx, p.m, (const uint16_t*)p.gate, (const uint16_t*)p.up, p.n, p.k, xn, n0, n1, st))) return rc;
+        if (run && (rc = tops16((const uint16_t*)p.dh, p.ldh, p.m, p.n, xn, n0, n1, part, ge, ce, st))) return rc;
+    }
     {
         Gemm g = gemm_of(o, p.m, p.n);
         g.kind = p.kind;
@@ -378,10 +390,10 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     }
     if (want_x) {
         uint16_t* wt = wk.take<uint16_t>(p.k * ldg);
-        if (run && (rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, ldg, np, st))) return rc;
-        if (run && (rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, ldg, np, st))) return rc;
-        if (run && o.rest && (rc = transpose16(o.w0 + o.rest, o.ldw, p.n, p.k, wt + 2 * np, ldg, np, st))) return rc;
-        if (run && o.rest && (rc = transpose16(o.w1 + o.rest, o.ldw, p.n, p.k, wt + 3 * np, ldg, np, st))) return rc;
+        if (run && (rc = transpose16(o.w0, o.ldw, p.n, p.k, wt, ldg, np, nullptr, nullptr, st))) return rc;
+        if (run && (rc = transpose16(o.w1, o.ldw, p.n, p.k, wt + np, ldg, np, nullptr, nullptr, st))) return rc;
+        if (run && o.rest && (rc = transpose16(o.w0 + o.rest, o.ldw, p.n, p.k, wt + 2 * np, ldg, np, nullptr, nullptr, st))) return rc;
+        if (run && o.rest && (rc = transpose16(o.w1 + o.rest, o.ldw, p.n, p.k, wt + 3 * np, ldg, np, nullptr, nullptr, st))) return rc;
         Gemm g{};
         g.half = o.half;
         g.x = grad;
@@ -399,8 +411,8 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
     if (want_w) {
         uint16_t* gt = wk.take<uint16_t>(2 * np * ldm);
         uint16_t* xt = wk.take<uint16_t>(p.k * ldm);
-        if (run && (rc = transpose16(grad, ldg, p.m, 2 * np, gt, ldm, mp, st))) return rc;
-        if (run && (rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, ldm, mp, st))) return rc;
+        if (run && (rc = transpose16(grad, ldg, p.m, 2 * np, gt, ldm, mp, ge, ce, st))) return rc;
+        if (run && (rc = transpose16((const uint16_t*)p.x, p.ldx, p.m, p.k, xt, ldm, mp, nullptr, nullptr, st))) return rc;
         for (int i = 0; i < 2; ++i) {
             Gemm g{};
             g.half = o.half;
@@ -410,6 +422,7 @@ int gated_backward(const Gated& p, Work& wk, bool run, bool want_x, bool want_w,
             g.m = (int)p.n;
             g.n = (int)p.k;
             g.k = (int)mp;
+            g.xe = ce ? ce + i * np : nullptr;
             g.kind = p.kind;
             g.y = (uint16_t*)(i ? p.dup : p.dgate);
             g.ldy = p.k;

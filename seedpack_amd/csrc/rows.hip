@@ -255,18 +255,66 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     }
 }
 
+// 2-norms of the rows of three F16 matrices of k columns, a workgroup a row: x's, then those of both
+// weights. 4096 and 2 x 12288 rows of 4096: 47 us, 5.0 TB/s.
+struct Norms {
+    const uint16_t *x, *w0, *w1;
+    int64_t ldx, m, n, k;
+    float *xn, *n0, *n1;
+};
+__global__ __launch_bounds__(256) void k_norms(const Norms q) {
+    __shared__ float lds[4];
+    const int64_t row = blockIdx.x, at = row < q.m ? row : (row - q.m) % q.n;
+    const bool first = row - q.m < q.n;
+    const uint16_t* src = row < q.m ? q.x + at * q.ldx : (first ? q.w0 : q.w1) + at * q.k;
+    float sum = 0.f;
+    for (int64_t c = threadIdx.x * 8; c < q.k; c += 2048) {
+        u4 h;
+        load8(src, c, q.k, h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = size_of(wide(h[i] & 0xffffu, SRC_F16)), b = size_of(wide(h[i] >> 16, SRC_F16));
+            sum = fmaf(a, a, fmaf(b, b, sum));
+        }
+    }
+    sum = reduce<false>(sum, lds);
+    if (threadIdx.x == 0) (row < q.m ? q.xn : (first ? q.n0 : q.n1))[at] = sqrtf(sum);
+}
+
 // 64 x 64 tiles through LDS: read along a row's columns, written along a column's rows, eight numbers a lane both
-// ways. 12288 x 4096: 35 us, 5.7 TB/s read and written.
+// ways. 12288 x 4096: 35 us, 5.7 TB/s read and written. SCALED: F16 rows of src have 2^re taken out, rows of dst
+// get 2^ce taken out in its place (4096 x 24576: 60 us without, 87 with).
+template <bool SCALED>
 __global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
-                                                   uint16_t* __restrict__ dst, int64_t ldd, int64_t rp, int64_t tiles_c) {
+                                                   uint16_t* __restrict__ dst, int64_t ldd, int64_t rp, int64_t tiles_c,
+                                                   const int32_t* __restrict__ re, const int32_t* __restrict__ ce) {
     __shared__ uint16_t t[64][66];                                // 33 words a row: a column's reads meet few banks twice
     const int64_t r0 = blockIdx.x / tiles_c * 64, c0 = blockIdx.x % tiles_c * 64;
+    int out[8];                                                   // of the lane's eight columns, which both its loads are of
+    if constexpr (SCALED) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t C = c0 + (threadIdx.x & 7) * 8 + k;
+            out[k] = ce[C < cols ? C : cols - 1];
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int u = i * 256 + threadIdx.x, r = u >> 3, c = (u & 7) * 8;
         const int64_t R = r0 + r, C = c0 + c;
         u4 v = {0, 0, 0, 0};
-        if (R < rows && C < cols) load8(src + R * ld, C, cols, v);
+        if (R < rows && C < cols) {
+            load8(src + R * ld, C, cols, v);
+            if constexpr (SCALED) {
+                const int e = re[R];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint16_t h = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+                    const uint32_t s = narrow(ldexpf(wide(h, SRC_F16), e - out[k]), SRC_F16);
+                    v[k >> 1] = k & 1 ? (v[k >> 1] & 0xffffu) | s << 16 : (v[k >> 1] & 0xffff0000u) | s;
+                }
+            }
+        }
         uint32_t* p = reinterpret_cast<uint32_t*>(&t[r][c]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) p[k] = v[k];
@@ -346,6 +394,85 @@ __global__ __launch_bounds__(256) void k_grad_exponents(const uint16_t* __restri
     frexpf(a, &ea);
     frexpf(b, &eb);
     e[row] = em + ea + eb + 1 + top->e - 15;
+}
+
+// The same bounds for F16 weights beside F16 inputs, of each row of the inner gradients (for dx) and of each column
+// (for the weights' gradients, sums over rows): the largest |dh| |w_n| of a row, the largest |dh| |x_m| of a column. One
+// pass over dh, 512 columns and a run of rows a workgroup, its waves every fourth row: 47 us for 4096 x 12288 (2.1 TB/s),
+// 5.6 of joining; 517 x 2053, whose rows begin at any number, 7.6 and 4.4.
+constexpr int TOP_COLS = 512, TOP_RUN = 16, TOP_PIECES = 64;
+struct Tops {
+    const uint16_t* dh;
+    int64_t ld, m, n, np, run;
+    const float *xn, *n0, *n1;
+    float *rows, *cols;       // [column tile][m], [run][np]
+    int pieces, tiles;
+    int32_t *ge, *ce;
+};
+template <bool WORDS>
+__global__ __launch_bounds__(256) void k_tops(const Tops q) {
+    __shared__ float lds[3][TOP_COLS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * TOP_COLS + 8 * lane, r0 = blockIdx.y * q.run, r1 = r0 + q.run < q.m ? r0 + q.run : q.m;
+    float top[8] = {0, 0, 0, 0, 0, 0, 0, 0}, w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = c + i < q.n ? fmaxf(q.n0[c + i], q.n1[c + i]) : 0.f;
+    for (int64_t at = r0 + wave; at < r1; at += 16) {             // four rows' loads under way at once
+        u4 h[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            h[u] = u4{0, 0, 0, 0};
+            if (at + 4 * u < r1 && c < q.n) load8<WORDS>(q.dh + (at + 4 * u) * q.ld, c, q.n, h[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t r = at + 4 * u;
+            const float a = q.xn[r < r1 ? r : r1 - 1];
+            float row = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = size_of(wide((h[u][i >> 1] >> (16 * (i & 1))) & 0xffffu, SRC_F16));
+                top[i] = fmaxf(top[i], a * d);
+                row = fmaxf(row, w[i] * d);
+            }
+#pragma unroll
+            for (int s = 32; s; s >>= 1) row = fmaxf(row, __shfl_xor(row, s));
+            if (lane == 0 && r < r1) q.rows[blockIdx.x * q.m + r] = row;
+        }
+    }
+    if (wave) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lds[wave - 1][i * 64 + lane] = top[i];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = fmaxf(fmaxf(top[i], lds[0][i * 64 + lane]), fmaxf(lds[1][i * 64 + lane], lds[2][i * 64 + lane]));
+        if (c + i < q.np) q.cols[blockIdx.y * q.np + c + i] = v;
+    }
+}
+__device__ __forceinline__ int bound_exponent(float a, float b) {
+    int ea = 0, eb = 0;
+    frexpf(a, &ea);
+    frexpf(b, &eb);
+    return a > 0.f && b > 0.f ? ea + eb + 1 - 15 : 0;
+}
+// dG' of column n goes with the up projection's norm, dU' with the gate's
+__global__ __launch_bounds__(256) void k_exponents(const Tops q) {
+    const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+    float v = 0.f;
+    if (i < q.m) {
+#pragma unroll 8
+        for (int p = 0; p < q.tiles; ++p) v = fmaxf(v, q.rows[p * q.m + i]);
+        q.ge[i] = bound_exponent(v, q.xn[i]);
+    } else if (i < q.m + q.np) {
+        const int64_t n = i - q.m;
+#pragma unroll 8
+        for (int p = 0; p < q.pieces; ++p) v = fmaxf(v, q.cols[p * q.np + n]);
+        q.ce[n] = bound_exponent(v, n < q.n ? q.n1[n] : 0.f);
+        q.ce[q.np + n] = bound_exponent(v, n < q.n ? q.n0[n] : 0.f);
+    }
 }
 
 __global__ void k_zero_rows(uint16_t* p, int64_t ld, int64_t rows, int64_t k) {
@@ -558,9 +685,53 @@ int half_blocks(int type, const uint8_t* src, int64_t rows, int64_t k, uint16_t*
 }
 
 int transpose16(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd, int64_t rp,
-                hipStream_t st) {
+                const int32_t* re, const int32_t* ce, hipStream_t st) {
     const int64_t tr = (rp + 63) / 64, tc = (cols + 63) / 64;
-    hipLaunchKernelGGL(k_transpose, dim3((unsigned)(tr * tc)), dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc);
+    const dim3 grid((unsigned)(tr * tc));
+    if (re) hipLaunchKernelGGL((k_transpose<true>), grid, dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc, re, ce);
+    else hipLaunchKernelGGL((k_transpose<false>), grid, dim3(256), 0, st, src, ld, rows, cols, dst, ldd, rp, tc, re, ce);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+int norms16(const uint16_t* x, int64_t ldx, int64_t m, const uint16_t* w0, const uint16_t* w1, int64_t n, int64_t k, float* xn, float* n0,
+            float* n1, hipStream_t st) {
+    hipLaunchKernelGGL(k_norms, dim3((unsigned)(m + 2 * n)), dim3(256), 0, st, Norms{x, w0, w1, ldx, m, n, k, xn, n0, n1});
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+int64_t top_run(int64_t m) {
+    const int64_t r = (m + TOP_PIECES - 1) / TOP_PIECES;
+    return r < TOP_RUN ? TOP_RUN : r;
+}
+int64_t tops_part(int64_t m, int64_t n) {
+    const int64_t np = (n + 63) / 64 * 64;
+    return (n + TOP_COLS - 1) / TOP_COLS * m + (m + top_run(m) - 1) / top_run(m) * np;
+}
+int tops16(const uint16_t* dh, int64_t ld, int64_t m, int64_t n, const float* xn, const float* n0, const float* n1, float* part, int32_t* ge,
+           int32_t* ce, hipStream_t st) {
+    Tops q{};
+    q.dh = dh;
+    q.ld = ld;
+    q.m = m;
+    q.n = n;
+    q.np = (n + 63) / 64 * 64;
+    q.run = top_run(m);
+    q.xn = xn;
+    q.n0 = n0;
+    q.n1 = n1;
+    q.tiles = (int)((n + TOP_COLS - 1) / TOP_COLS);
+    q.pieces = (int)((m + q.run - 1) / q.run);
+    q.rows = part;
+    q.cols = part + q.tiles * m;
+    q.ge = ge;
+    q.ce = ce;
+    const dim3 grid((unsigned)q.tiles, (unsigned)q.pieces);
+    if (ld % 2 == 0 && (reinterpret_cast<uintptr_t>(dh) & 3) == 0) hipLaunchKernelGGL((k_tops<true>), grid, dim3(256), 0, st, q);
+    else hipLaunchKernelGGL((k_tops<false>), grid, dim3(256), 0, st, q);
+    SPA_HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(k_exponents, dim3((unsigned)((m + q.np + 255) / 256)), dim3(256), 0, st, q);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }

@@ -92,3 +92,56 @@ def test_few_rows_with_numbers_that_are_not_finite(t, kind, m):
         else:
             with np.errstate(invalid="ignore"):
                 assert np.array_equal(row, v * w64[:, at], equal_nan=True)
+
+
+def backward_f16(g, m, n, k, sx, sw, sd):
+    """F16 operands of the given sizes (powers of two), the columns of dh of unlike size -> what gated_backward takes, in float64 too"""
+    pair = lambda shape, s: (lambda h: (h, wide(h)))(store(np.clip(g.normal(0, 1, shape) * s, -6e4, 6e4), F16))
+    (x, x64), (wg, g64), (wu, u64) = pair((m, k), sx), pair((n, k), sw), pair((n, k), sw)
+    dh, d64 = pair((m, n), sd * np.exp2(-g.integers(0, 9, n).astype(float)))
+    return (x, wg, wu, dh), (x64, g64, u64, d64)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,n,k", [(5, 64, 64), (150, 96, 70), (600, 300, 200)])
+@pytest.mark.parametrize("sx,sw,sd,which", [(2.0 ** 5, 2.0 ** -8, 2.0 ** 14, ("dx",)), (2.0 ** -10, 2.0 ** 5, 2.0 ** 14, ("dgate", "dup")),
+                                            (2.0 ** -16, 2.0 ** 8, 2.0 ** -16, ("dx",)), (2.0 ** 6, 2.0 ** -16, 2.0 ** -14, ("dgate", "dup"))])
+def test_gated_backward_range(sx, sw, sd, which, m, n, k, act):
+    """F16: inner gradients that pass the largest F16 number or fall below the least, and outputs that do not. Inner
+    gradients are taken to 11 bits, and to 2^-34 of what their row (for dx; their column for the weights' gradients)
+    can hold at most, 1.13 max |dh| |x| |w| (the powers of two put the bound between 2^11 and 2^15; half a step of F16 is 2^-25)"""
+    g = rng(44, m, int(np.log2(sx)) + 50, len(act))
+    (x, wg, wu, dh), (x64, g64, u64, d64) = backward_f16(g, m, n, k, sx, sw, sd)
+    gate, upw = (linear.Weight(linear.F16, up(v), n, k) for v in (wg, wu))
+    arrays = {"dx": np.zeros((m, k), F16), "dgate": np.zeros((n, k), F16), "dup": np.zeros((n, k), F16)}
+    arrays = {name: up(a) for name, a in arrays.items()}
+    linear.gated_backward(up(x), gate, upw, up(dh), act, **arrays)
+    want = gated_backward64(x64, g64, u64, d64, act, k, 2.0 ** -11)
+    xn, wn = np.linalg.norm(x64, axis=1), np.maximum(np.linalg.norm(g64, axis=1), np.linalg.norm(u64, axis=1))
+    ad = np.abs(d64)
+    # rows are held to their own bound before columns are to theirs: both parts for the weights' gradients
+    rows = 2.0 ** -34 * 1.13 * ad.max(1) * xn * wn.max()
+    cols = 2.0 ** -34 * 1.13 * (ad * xn[:, None]).max(0) * wn
+    extra = {"dx": rows[:, None] * (np.abs(g64).sum(0) + np.abs(u64).sum(0))[None],
+             "dgate": (rows @ np.abs(x64))[None] + cols[:, None] * np.abs(x64).sum(0)[None]}
+    extra["dup"] = extra["dgate"]
+    for name in which:
+        y, off = want[name]
+        assert 2.0 ** -14 < np.abs(y).max() < 60000, (name, np.abs(y).max())
+        close(arrays[name].to_host(), y, off + extra[name], F16, name)
+
+
+def test_gated_backward_rows_of_unlike_size():
+    """F16 rows of dh and of x from far apart: each row of dx to its own size, the sums over rows to their largest"""
+    g = rng(45)
+    m, n, k = 200, 128, 96
+    (x, wg, wu, dh), _ = backward_f16(g, m, n, k, 0.25, 0.05, 1.0)
+    size = np.exp2(g.integers(-12, 12, (m, 1)).astype(float))
+    dh = store(wide(dh) * size, F16)
+    x64, g64, u64, d64 = wide(x), wide(wg), wide(wu), wide(dh)
+    gate, upw = (linear.Weight(linear.F16, up(v), n, k) for v in (wg, wu))
+    arrays = {"dx": up(np.zeros((m, k), F16)), "dgate": up(np.zeros((n, k), F16)), "dup": up(np.zeros((n, k), F16))}
+    linear.gated_backward(up(x), gate, upw, up(dh), **arrays)
+    want = gated_backward64(x64, g64, u64, d64, "silu", k, 2.0 ** -11)
+    for name, a in arrays.items():
+        close(a.to_host(), *want[name], F16, name)
