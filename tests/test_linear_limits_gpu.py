@@ -145,3 +145,55 @@ def test_gated_backward_rows_of_unlike_size():
     want = gated_backward64(x64, g64, u64, d64, "silu", k, 2.0 ** -11)
     for name, a in arrays.items():
         close(a.to_host(), *want[name], F16, name)
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("m", [150])
+@pytest.mark.parametrize("t", [8, 12, 14])
+def test_blocks_of_large_scales_and_no_weights(t, m, kind):
+    """a block whose scale is the largest and whose codes (or their scales) are zero, beside blocks of tiny weights:
+    the tiny ones count in full"""
+    g = rng(46, t, m, kind is F16)
+    n, k = 50, 512
+    _, qk, bs = QFUN[t]
+    b, _ = random_blocks(g, t, n, k)
+    b = b.reshape(n, k // qk, bs)
+    at = {8: [0], 12: [0, 2], 14: [208]}[t]
+    for o in at:
+        b[:, :, o:o + 2] = np.frombuffer(np.float16(2.0 ** -20).tobytes(), np.uint8)
+    codes = slice(2, 34) if t == 8 else (slice(4, 16) if t == 12 else slice(192, 208))
+    if t == 12:
+        b[:, :, 4:16] = 0x11 * g.integers(0, 2, b[:, :, 4:16].shape, dtype=np.uint8)      # scales and offsets 0, 1, 16, 17
+    elif t == 14:
+        b[:, :, codes] = 1
+    else:
+        b[:, :, codes] = g.integers(0, 3, b[:, :, codes].shape, dtype=np.uint8)
+    b[:, 0, at[0]:at[0] + 2] = np.frombuffer(np.float16(65504).tobytes(), np.uint8)
+    b[:, 0, codes] = 0
+    w64 = GPUQuant().dequantize(t, b.reshape(-1), k).to_host().reshape(n, k).astype(np.float64)
+    assert (w64[:, :qk] <= 0).all() and np.abs(w64).max() < 1e-2
+    w64[:, :qk] += 0.0
+    x, x64 = inputs(g, m, k, kind)
+    y, total = project64(x64, w64)
+    scale = 1.0 if kind is BF16 else 2.0 ** 10       # F16 outputs: away from its least numbers
+    if kind is F16:
+        x, x64 = store(x64 * scale, kind), x64 * scale
+        y, total = project64(wide(x), w64)
+    close(linear.project(up(x), linear.Weight(t, up(b.reshape(-1)), n, k)).to_host(), y,
+          slack(total, k, 2.0 ** -11 if kind is BF16 else 2.0 ** -21), kind)
+
+
+@pytest.mark.parametrize("t", [2, 8, 12, 14, 23])
+def test_long_rows_of_blocks(t):
+    """rows of more weights than the conversion to binary16 holds at once, their largest weight in the last part"""
+    g = rng(52, t)
+    n, k, m = 9, 16384 + 512, 140
+    b, _ = random_blocks(g, t, n, k)
+    _, qk, bs = QFUN[t]
+    b = b.reshape(n, k // qk, bs)
+    at = {14: 208}.get(t, 0)
+    b[:, -1, at:at + 2] = np.frombuffer(np.float16(0.25).tobytes(), np.uint8)
+    w64 = GPUQuant().dequantize(t, b.reshape(-1), k).to_host().reshape(n, k).astype(np.float64)
+    x, x64 = inputs(g, m, k, BF16)
+    y, total = project64(x64, w64)
+    close(linear.project(up(x), linear.Weight(t, up(b.reshape(-1)), n, k)).to_host(), y, slack(total, k), BF16)
