@@ -3,10 +3,14 @@
 //     sum_k x[k] w[k] = s sum_k x[k] c[k] - o sum_k x[k]:
 // the codes, not the weights, are the matrix instruction's operand. A code of up to 7 bits becomes a BF16
 // number by putting its bits under the exponent of 128 (0x4300 | c = 128 + c, exact), two codes by one byte
-// permutation; 128 s then goes into o. For F16 the same under 1024 (0x6400 | c). Q8_0's 8 bits are exact as
-// BF16 too, by way of float32. So no weight is rounded, unpacking costs about one instruction a weight
+// permutation; 128 s then goes into o. For F16 the same under 1024 (0x6400 | c). Q8_0's codes have no offset: they are
+// signed numbers, exact in BF16 by way of float32 and in F16 by a subtraction of 1152. So no weight is rounded, unpacking costs about one instruction a weight
 // instead of the six to eight of decoding to float32 and splitting, and the sums of x alone come from a
 // second instruction with an operand of ones, in the registers where they are needed.
+//
+// The base costs bits: sums over base + code and less base times the inputs' sum are rounded at 128 (beside F16 1024)
+// scales' size, so with codes of half their range a sum's error is that of 3 to 17 (24 to 130) times as many float32
+// roundings; a block of a large scale whose codes are all near zero adds errors of its scale, not of its weights.
 //
 // A lane holds 8 codes of weight row lane & 15 for a step of 32 k. A wave works alone on units of 256 k: the
 // unit's bytes of its 16 rows go to LDS of its own by 16-byte loads that bypass the registers, each byte
@@ -59,6 +63,8 @@ struct Row {
 };
 __device__ __forceinline__ float half_of(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
 
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
 // codes of up to 7 bits, four bytes -> four numbers BASE + code
 template <int KIND> constexpr float BASE = KIND == SRC_BF16 ? 128.f : 1024.f;
 template <int KIND>
@@ -90,7 +96,7 @@ struct K4 {                                                       // Q4_K / Q5_K
 };
 template <> struct Unit<12> {                                     // Q4_K: 4 x 32 bytes of two nibbles
     static constexpr int QK = 256, BS = 144;
-    static constexpr bool HALVES = false;
+    static constexpr bool HALVES = false, OFFSET = true;
     K4 k;
     template <class R> __device__ __forceinline__ void open(const R& r) { k.set(u4{r.word(0), r.word(4), r.word(8), r.word(12)}); }
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
@@ -102,7 +108,7 @@ template <> struct Unit<12> {                                     // Q4_K: 4 x 3
 };
 template <> struct Unit<13> {                                     // Q5_K: the same, and bit f of 32 bytes
     static constexpr int QK = 256, BS = 176;
-    static constexpr bool HALVES = false;
+    static constexpr bool HALVES = false, OFFSET = true;
     K4 k;
     template <class R> __device__ __forceinline__ void open(const R& r) { k.set(u4{r.word(0), r.word(4), r.word(8), r.word(12)}); }
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
@@ -117,7 +123,7 @@ template <> struct Unit<13> {                                     // Q5_K: the s
 };
 template <> struct Unit<14> {                                     // Q6_K: per half of 128, 4 quarters of 32
     static constexpr int QK = 256, BS = 210;
-    static constexpr bool HALVES = true;
+    static constexpr bool HALVES = true, OFFSET = true;
     u4 sc;
     float d;
     template <class R> __device__ __forceinline__ void open(const R& r) {
@@ -139,28 +145,32 @@ template <> struct Unit<14> {                                     // Q6_K: per h
 };
 template <> struct Unit<8> {                                      // Q8_0: blocks of 32 codes of 8 bits
     static constexpr int QK = 32, BS = 34;
-    static constexpr bool HALVES = false;
+    static constexpr bool HALVES = false, OFFSET = false;
     template <class R> __device__ __forceinline__ void open(const R&) {}
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
         const u2 q = r.pair(34 * f + 2 + 8 * g);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t c = q[i] ^ 0x80808080u;                // code + 128, 0..255
             if (KIND == SRC_F16) {
-                put4<KIND>(c, w, 2 * i);
+                put4<KIND>(q[i] ^ 0x80808080u, w, 2 * i);         // 1024 + 128 + code
+#pragma unroll
+                for (int c = 2 * i; c < 2 * i + 2; ++c) {
+                    const uint32_t pair = w[c];                   // (a bit cast of a vector's element itself takes its first)
+                    w[c] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair) - h2{1152, 1152});
+                }
             } else {
-                const float a = (float)(c & 0xffu), b = (float)((c >> 8) & 0xffu), e = (float)((c >> 16) & 0xffu), h = (float)(c >> 24);
+                const float a = (float)(int8_t)q[i], b = (float)(int8_t)(q[i] >> 8), e = (float)(int8_t)(q[i] >> 16), h = (float)((int32_t)q[i] >> 24);
                 w[2 * i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
                 w[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(h), __float_as_uint(e), 0x07060302u);
             }
         }
         s = half_of(r.half(34 * f));
-        o = (KIND == SRC_F16 ? 1152.f : 128.f) * s;
+        o = 0.f;
     }
 };
 template <> struct Unit<2> {                                      // Q4_0: blocks of 16 low nibbles, then 16 high ones
     static constexpr int QK = 32, BS = 18;
-    static constexpr bool HALVES = false;
+    static constexpr bool HALVES = false, OFFSET = true;
     template <class R> __device__ __forceinline__ void open(const R&) {}
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
         const u2 q = r.pair(18 * f + 2 + 8 * (g & 1));
@@ -270,7 +280,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES < 8 ? 2 : WAVES / 4) void k_codes
             for (int j = 0; j < MT; ++j) {
                 if constexpr (MT == 1) x[j] = x0[s];
                 else x[j] = reinterpret_cast<const u4*>(f.x)[((u * STEPS + s) * MT + j) * 64 + lane];
-                sx[j] = mul16<KIND>(x[j], ones, zero);
+                if constexpr (U::OFFSET) sx[j] = mul16<KIND>(x[j], ones, zero);
             }
 #pragma unroll
             for (int h = 0; h <= TWO; ++h) {
@@ -281,7 +291,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES < 8 ? 2 : WAVES / 4) void k_codes
                 for (int j = 0; j < MT; ++j) {
                     const f4 p = mul16<KIND>(x[j], w, zero);
 #pragma unroll
-                    for (int c = 0; c < MR; ++c) acc[h][j][c] = fmaf(sc, p[c], fmaf(-off, sx[j][c], acc[h][j][c]));
+                    for (int c = 0; c < MR; ++c) acc[h][j][c] = fmaf(sc, p[c], U::OFFSET ? fmaf(-off, sx[j][c], acc[h][j][c]) : acc[h][j][c]);
                 }
             }
             // no more of x ahead of its use than the registers hold

@@ -148,7 +148,7 @@ def test_gated_backward_rows_of_unlike_size():
 
 
 @pytest.mark.parametrize("kind", [BF16, F16])
-@pytest.mark.parametrize("m", [150])
+@pytest.mark.parametrize("m", [20, 150])
 @pytest.mark.parametrize("t", [8, 12, 14])
 def test_blocks_of_large_scales_and_no_weights(t, m, kind):
     """a block whose scale is the largest and whose codes (or their scales) are zero, beside blocks of tiny weights:
