@@ -3,14 +3,16 @@
 //     sum_k x[k] w[k] = s sum_k x[k] c[k] - o sum_k x[k]:
 // the codes, not the weights, are the matrix instruction's operand. A code of up to 7 bits becomes a BF16
 // number by putting its bits under the exponent of 128 (0x4300 | c = 128 + c, exact), two codes by one byte
-// permutation; 128 s then goes into o. For F16 the same under 1024 (0x6400 | c). Q8_0's codes have no offset: they are
-// signed numbers, exact in BF16 by way of float32 and in F16 by a subtraction of 1152. So no weight is rounded, unpacking costs about one instruction a weight
-// instead of the six to eight of decoding to float32 and splitting, and the sums of x alone come from a
-// second instruction with an operand of ones, in the registers where they are needed.
+// permutation; 128 s then goes into o. For F16 the same under 1024 (0x6400 | c) and 1024 less, exact too, with what is
+// taken from a code of Q4_0, Q6_K or Q8_0: those have no offset then. Nor have Q8_0's beside BF16, signed numbers by
+// way of float32. So no weight is rounded, unpacking costs one to one and a half instructions a weight instead of the
+// six to eight of decoding to float32 and splitting, and the sums of x alone come from a second instruction with an
+// operand of ones, in the registers where they are needed.
 //
-// The base costs bits: sums over base + code and less base times the inputs' sum are rounded at 128 (beside F16 1024)
-// scales' size, so with codes of half their range a sum's error is that of 3 to 17 (24 to 130) times as many float32
-// roundings; a block of a large scale whose codes are all near zero adds errors of its scale, not of its weights.
+// The base of 128 costs bits: sums over base + code and less base times the inputs' sum are rounded at 128 scales'
+// size, so with codes of half their range a sum's error is that of 5 (Q6_K) to 33 (Q4_0) times as many float32
+// roundings, far below a BF16 result's; but a block of a large scale whose codes are all near zero adds errors of its
+// scale, not of its weights.
 //
 // A lane holds 8 codes of weight row lane & 15 for a step of 32 k. A wave works alone on units of 256 k: the
 // unit's bytes of its 16 rows go to LDS of its own by 16-byte loads that bypass the registers, each byte
@@ -65,13 +67,15 @@ __device__ __forceinline__ float half_of(uint32_t h) { return (float)__builtin_b
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-// codes of up to 7 bits, four bytes -> four numbers BASE + code
-template <int KIND> constexpr float BASE = KIND == SRC_BF16 ? 128.f : 1024.f;
-template <int KIND>
+// codes of up to 8 bits, four bytes -> four numbers: BF16 BASE + code (up to 7 bits), F16 code - LESS
+template <int KIND> constexpr float BASE = KIND == SRC_BF16 ? 128.f : 0.f;
+template <int KIND, int LESS = 0>
 __device__ __forceinline__ void put4(uint32_t c, u4& w, int at) {
     constexpr uint32_t E = KIND == SRC_BF16 ? 0x43434343u : 0x64646464u;
-    w[at] = __builtin_amdgcn_perm(E, c, 0x04010400u);
-    w[at + 1] = __builtin_amdgcn_perm(E, c, 0x04030402u);
+    const uint32_t a = __builtin_amdgcn_perm(E, c, 0x04010400u), b = __builtin_amdgcn_perm(E, c, 0x04030402u);
+    constexpr _Float16 TAKEN = 1024 + LESS;
+    w[at] = KIND == SRC_BF16 ? a : __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, a) - h2{TAKEN, TAKEN});
+    w[at + 1] = KIND == SRC_BF16 ? b : __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, b) - h2{TAKEN, TAKEN});
 }
 
 // a unit of 256 weights of one row as lane group g (0..3) reads it; step f: codes 32 f + 8 g .. of it
@@ -96,7 +100,8 @@ struct K4 {                                                       // Q4_K / Q5_K
 };
 template <> struct Unit<12> {                                     // Q4_K: 4 x 32 bytes of two nibbles
     static constexpr int QK = 256, BS = 144;
-    static constexpr bool HALVES = false, OFFSET = true;
+    static constexpr bool HALVES = false;
+    template <int KIND> static constexpr bool OFFSET = true;
     K4 k;
     template <class R> __device__ __forceinline__ void open(const R& r) { k.set(u4{r.word(0), r.word(4), r.word(8), r.word(12)}); }
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
@@ -108,7 +113,8 @@ template <> struct Unit<12> {                                     // Q4_K: 4 x 3
 };
 template <> struct Unit<13> {                                     // Q5_K: the same, and bit f of 32 bytes
     static constexpr int QK = 256, BS = 176;
-    static constexpr bool HALVES = false, OFFSET = true;
+    static constexpr bool HALVES = false;
+    template <int KIND> static constexpr bool OFFSET = true;
     K4 k;
     template <class R> __device__ __forceinline__ void open(const R& r) { k.set(u4{r.word(0), r.word(4), r.word(8), r.word(12)}); }
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
@@ -123,7 +129,8 @@ template <> struct Unit<13> {                                     // Q5_K: the s
 };
 template <> struct Unit<14> {                                     // Q6_K: per half of 128, 4 quarters of 32
     static constexpr int QK = 256, BS = 210;
-    static constexpr bool HALVES = true, OFFSET = true;
+    static constexpr bool HALVES = true;
+    template <int KIND> static constexpr bool OFFSET = KIND == SRC_BF16;
     u4 sc;
     float d;
     template <class R> __device__ __forceinline__ void open(const R& r) {
@@ -136,28 +143,24 @@ template <> struct Unit<14> {                                     // Q6_K: per h
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t c = (qd < 2 ? l[i] : l[i] >> 4) & 0x0f0f0f0fu, b = (hi[i] >> (2 * qd)) & 0x03030303u;
-            put4<KIND>(c | (b << 4), w, 2 * i);
+            put4<KIND, 32>(c | (b << 4), w, 2 * i);
         }
         const int byte = (int)(sc[2 * h + (qd >> 1)] << (24 - 16 * (qd & 1) - 8 * (g >> 1))) >> 24;   // scale 8 h + 2 qd + g / 2
         s = d * (float)byte;
-        o = (BASE<KIND> + 32.f) * s;
+        o = OFFSET<KIND> ? (BASE<KIND> + 32.f) * s : 0.f;
     }
 };
 template <> struct Unit<8> {                                      // Q8_0: blocks of 32 codes of 8 bits
     static constexpr int QK = 32, BS = 34;
-    static constexpr bool HALVES = false, OFFSET = false;
+    static constexpr bool HALVES = false;
+    template <int KIND> static constexpr bool OFFSET = false;
     template <class R> __device__ __forceinline__ void open(const R&) {}
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
         const u2 q = r.pair(34 * f + 2 + 8 * g);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (KIND == SRC_F16) {
-                put4<KIND>(q[i] ^ 0x80808080u, w, 2 * i);         // 1024 + 128 + code
-#pragma unroll
-                for (int c = 2 * i; c < 2 * i + 2; ++c) {
-                    const uint32_t pair = w[c];                   // (a bit cast of a vector's element itself takes its first)
-                    w[c] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair) - h2{1152, 1152});
-                }
+                put4<KIND, 128>(q[i] ^ 0x80808080u, w, 2 * i);
             } else {
                 const float a = (float)(int8_t)q[i], b = (float)(int8_t)(q[i] >> 8), e = (float)(int8_t)(q[i] >> 16), h = (float)((int32_t)q[i] >> 24);
                 w[2 * i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
@@ -170,14 +173,15 @@ template <> struct Unit<8> {                                      // Q8_0: block
 };
 template <> struct Unit<2> {                                      // Q4_0: blocks of 16 low nibbles, then 16 high ones
     static constexpr int QK = 32, BS = 18;
-    static constexpr bool HALVES = false, OFFSET = true;
+    static constexpr bool HALVES = false;
+    template <int KIND> static constexpr bool OFFSET = KIND == SRC_BF16;
     template <class R> __device__ __forceinline__ void open(const R&) {}
     template <int KIND, class R> __device__ __forceinline__ void step(const R& r, int f, int g, u4& w, float& s, float& o) const {
         const u2 q = r.pair(18 * f + 2 + 8 * (g & 1));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) put4<KIND>((q[i] >> (g & 2 ? 4 : 0)) & 0x0f0f0f0fu, w, 2 * i);
+        for (int i = 0; i < 2; ++i) put4<KIND, 8>((q[i] >> (g & 2 ? 4 : 0)) & 0x0f0f0f0fu, w, 2 * i);
         s = half_of(r.half(18 * f));
-        o = (BASE<KIND> + 8.f) * s;
+        o = OFFSET<KIND> ? (BASE<KIND> + 8.f) * s : 0.f;
     }
 };
 
@@ -280,7 +284,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES < 8 ? 2 : WAVES / 4) void k_codes
             for (int j = 0; j < MT; ++j) {
                 if constexpr (MT == 1) x[j] = x0[s];
                 else x[j] = reinterpret_cast<const u4*>(f.x)[((u * STEPS + s) * MT + j) * 64 + lane];
-                if constexpr (U::OFFSET) sx[j] = mul16<KIND>(x[j], ones, zero);
+                if constexpr (U::template OFFSET<KIND>) sx[j] = mul16<KIND>(x[j], ones, zero);
             }
 #pragma unroll
             for (int h = 0; h <= TWO; ++h) {
@@ -291,7 +295,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES < 8 ? 2 : WAVES / 4) void k_codes
                 for (int j = 0; j < MT; ++j) {
                     const f4 p = mul16<KIND>(x[j], w, zero);
 #pragma unroll
-                    for (int c = 0; c < MR; ++c) acc[h][j][c] = fmaf(sc, p[c], U::OFFSET ? fmaf(-off, sx[j][c], acc[h][j][c]) : acc[h][j][c]);
+                    for (int c = 0; c < MR; ++c) acc[h][j][c] = fmaf(sc, p[c], U::template OFFSET<KIND> ? fmaf(-off, sx[j][c], acc[h][j][c]) : acc[h][j][c]);
                 }
             }
             // no more of x ahead of its use than the registers hold

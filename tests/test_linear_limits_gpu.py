@@ -197,3 +197,144 @@ def test_long_rows_of_blocks(t):
     x, x64 = inputs(g, m, k, BF16)
     y, total = project64(x64, w64)
     close(linear.project(up(x), linear.Weight(t, up(b.reshape(-1)), n, k)).to_host(), y, slack(total, k), BF16)
+
+
+def near_pairs(g, values, count):
+    """pairs of (index, index) of values that round to the same 11 bits and differ by 2^-11.5 of themselves or more, the first the larger"""
+    v = np.asarray(values, np.float64)
+    e = np.exp2(np.floor(np.log2(v)))
+    held = np.round(v / e * 1024) / 1024 * e              # to 11 bits
+    out = []
+    for i in g.permutation(len(v)):
+        j = np.flatnonzero((held == held[i]) & (v < v[i] * (1 - 2.0 ** -11.5)))
+        if len(j):
+            out.append((i, int(g.choice(j))))
+            if len(out) == count:
+                return out
+    raise AssertionError("too few pairs")
+
+
+def fine_blocks(g, t, n, k):
+    """n rows whose runs of 32 weights are +v1 and -v2 in turn, v1 and v2 the same 11-bit number but not the same -> bytes, weights"""
+    _, qk, bs = QFUN[t]
+    b = np.zeros((n, k // qk, bs), np.uint8)
+    put = lambda r, j, o, h: b[r, j].__setitem__(slice(o, o + 2), np.frombuffer(np.float16(h).tobytes(), np.uint8))
+    d = (1024 + np.arange(1024)) * 2.0 ** -19             # all F16 numbers of one binary order
+    if t in (6, 8):
+        # Q8_0: codes 64..127 and their negatives; Q5_0: 8..15 (its codes are held over 16)
+        q = np.arange(64, 128) if t == 8 else np.arange(8, 16)
+        pairs = near_pairs(g, (d[:, None] * q).reshape(-1), n * k // 64)
+        for i, (a, c) in enumerate(pairs):
+            r, j = divmod(i, k // 64)
+            for s, p in ((0, a), (1, c)):
+                put(r, 2 * j + s, 0, d[p // len(q)])
+                code = int(q[p % len(q)]) * (1 - 2 * s)
+                if t == 8:
+                    b[r, 2 * j + s, 2:] = code & 0xff
+                else:
+                    b[r, 2 * j + s, 2:6] = 0xff if code + 16 >= 16 else 0
+                    b[r, 2 * j + s, 6:] = ((code + 16) & 15) * 0x11
+    else:                                                 # Q4_K: d sc 15 and -dm mn, 32 weights each
+        for r in range(n):
+            while True:
+                a, c = int(g.integers(1024)), int(g.integers(1024))
+                sc, mn = np.meshgrid(np.arange(32, 64), np.arange(32, 64), indexing="ij")
+                v1, v2 = d[a] * sc * 15, 16 * d[c] * mn
+                e = np.exp2(np.floor(np.log2(v1)))
+                ok = np.argwhere((np.round(v1 / e * 1024) == np.round(v2 / e * 1024)) & (v1 * (1 - 2.0 ** -11.5) > v2))
+                if len(ok):
+                    i, j = ok[g.integers(len(ok))]
+                    break
+            s, o = np.zeros(8, int), np.zeros(8, int)
+            s[::2], o[1::2] = 32 + i, 32 + j
+            for blk in range(k // qk):
+                put(r, blk, 0, d[a])
+                put(r, blk, 2, 16 * d[c])
+                b[r, blk, 4:8] = s[:4] | (s[4:] >> 4 << 6)
+                b[r, blk, 8:12] = o[:4] | (o[4:] >> 4 << 6)
+                b[r, blk, 12:16] = (s[4:] & 15) | ((o[4:] & 15) << 4)
+                b[r, blk, 16:] = 0x0f                     # the even runs' codes 15, the odd runs' 0
+    w = GPUQuant().dequantize(t, b.reshape(-1), k).to_host().reshape(n, k).astype(np.float64)
+    assert (w.reshape(n, -1, 2, 32)[:, :, 0] > 0).all() and (w.reshape(n, -1, 2, 32)[:, :, 1] < 0).all()
+    return b.reshape(-1), w
+
+
+@pytest.mark.parametrize("t,kind,m,extra", [(8, F16, 3, 0), (8, F16, 40, 0), (12, F16, 3, 0), (12, F16, 40, 0), (8, BF16, 3, 0), (8, BF16, 40, 0), (12, BF16, 3, 0), (12, BF16, 40, 0),
+                                            (6, F16, 3, 2.0 ** -16), (6, F16, 40, 2.0 ** -16), (6, BF16, 3, 2.0 ** -16), (6, BF16, 40, 2.0 ** -16),
+                                            (8, F16, 150, 2.0 ** -21), (6, F16, 150, 2.0 ** -21), (12, F16, 150, 2.0 ** -21), (12, F16, 700, 2.0 ** -21)])
+def test_weights_beyond_eleven_bits(t, kind, m, extra):
+    """weights whose first 11 bits cancel: what is left are the bits beyond. Few rows of Q8_0 and Q4_K go by codes (Q4_K's
+    beside BF16 as 128 + code), whose sums of 32 are added one after another: (32 + k / 32) roundings, of sums so many
+    times T (an offset of Q4_K is that of 15 codes in each of 32 terms, and no more than T)"""
+    g = rng(47, t, m, kind is F16)
+    n, k = 60, 256 if t == 12 else 64
+    b, w64 = fine_blocks(g, t, n, k)
+    x = g.random((m, k // 64, 1, 32)) + 0.5
+    x = store(np.broadcast_to(x, (m, k // 64, 2, 32)).reshape(m, k), kind)
+    y, total = project64(wide(x), w64)
+    per = {(8, F16): 1, (8, BF16): 1, (12, F16): 2, (12, BF16): 2 * 143 / 15}.get((t, kind)) if m <= 128 else None
+    allowed = total * ((per * (32 + k / 32) if per else k) * 2.0 ** -24 + extra)
+    assert (np.abs(y) > 2.0 ** -12.6 * total).all() and (allowed < 0.4 * np.abs(y)).all()
+    close(linear.project(up(x), linear.Weight(t, up(b), n, k)).to_host(), y, allowed, kind)
+
+
+@pytest.mark.parametrize("t", [8, 12])
+@pytest.mark.parametrize("m", [20, 300])
+def test_gradient_through_weights_beyond_eleven_bits(t, m):
+    """the same for the inputs' gradient: rows of the gate in pairs of +v1 and -v2, gates of zero (silu' = 1/2, silu = 0), up
+    projections of one power of two"""
+    g = rng(48, t, m)
+    n, k = 64, 256
+    _, qk, bs = QFUN[t]
+    fine, _ = fine_blocks(g, t, n, 64 if t == 8 else 256)
+    rows = fine.reshape(n, -1, bs)
+    gate = np.zeros((n, k // qk, bs), np.uint8)
+    if t == 8:                                            # run 0 of a fine row into all of row 2 i, run 1 into 2 i + 1
+        for i in range(n // 2):
+            gate[2 * i], gate[2 * i + 1] = rows[i, 0], rows[i, 1]
+        upw = np.zeros((n, k // qk, bs), np.uint8)
+        upw[:, :, :2] = np.frombuffer(np.float16(2.0 ** -12).tobytes(), np.uint8)
+        upw[:, ::2, 2:], upw[:, 1::2, 2:] = 64, 0xc0
+    else:                                                 # all runs d sc 15, or all -dm mn
+        gate[:n] = rows[:n]
+        for i in range(n // 2):
+            gate[2 * i] = gate[2 * i + 1] = rows[i, 0]
+            sc, mn = int(rows[i, 0, 4] & 63), int(rows[i, 0, 9] & 63)
+            for r, s, o in ((2 * i, sc, 0), (2 * i + 1, 0, mn)):
+                gate[r, :, 4:8], gate[r, :, 8:12] = s | (s >> 4 << 6), o | (o >> 4 << 6)
+                gate[r, :, 12:16] = (s & 15) | ((o & 15) << 4)
+                gate[r, :, 16:] = 0xff if s else 0
+        upw = np.zeros((n, k // qk, bs), np.uint8)
+        for o in (0, 2):
+            upw[:, :, o:o + 2] = np.frombuffer(np.float16(2.0 ** -8).tobytes(), np.uint8)
+        s, o = np.zeros(8, int), np.zeros(8, int)
+        s[::2], o[1::2] = 1, 8
+        upw[:, :, 4:8], upw[:, :, 8:12] = s[:4], o[:4]
+        upw[:, :, 12:16] = (s[4:] & 15) | ((o[4:] & 15) << 4)
+        upw[:, :, 16:] = 0x08                             # 8 in the even runs, 0 in the odd
+    of = lambda b: GPUQuant().dequantize(t, b.reshape(-1), k).to_host().reshape(n, k).astype(np.float64)
+    g64, u64 = of(gate), of(upw)
+    x64 = np.broadcast_to(np.where(np.arange(k) // 32 % 2, -1.0, 1.0), (m, k))
+    assert not (x64 @ g64.T).any() and len(np.unique(np.abs(u64))) == 1 and (g64[::2] > 0).all() and (g64[1::2] < 0).all()
+    u = x64 @ u64.T
+    assert (u == u[0, 0]).all() and u[0, 0] > 0
+    d64 = np.repeat(np.exp2(g.integers(-4, 3, (m, n // 2)).astype(float)), 2, axis=1)
+    dg = 0.5 * d64 * u
+    y, total = dg @ g64, np.abs(dg) @ np.abs(g64)
+    allowed = total * (2 * n * 2.0 ** -24 + 2.0 ** -21)
+    assert (y > 0.4 * 2.0 ** -13 * total).all() and (allowed < 0.2 * y).all()
+    wt = lambda b: linear.Weight(t, up(b.reshape(-1)), n, k)
+    dx = linear.gated_backward(up(store(x64, F16)), wt(gate), wt(upw), up(store(d64, F16)))[0]
+    close(dx.to_host(), y, allowed, F16)
+
+
+@pytest.mark.parametrize("t,kind", [(linear.BF16, BF16), (linear.F16, F16)])
+@pytest.mark.parametrize("m", [1, 20, 150, 1100])
+def test_products_of_one_type_are_exact(t, kind, m):
+    """operands of one 16-bit type: nothing but the float32 sums and the output's rounding"""
+    g = rng(49, m, t)
+    n, k = 133, 192
+    w, w64 = weights(g, t, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    y, total = project64(x64, w64)
+    close(linear.project(up(x), w).to_host(), y, slack(total, k, 0), kind)
