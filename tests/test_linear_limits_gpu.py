@@ -338,3 +338,18 @@ def test_products_of_one_type_are_exact(t, kind, m):
     x, x64 = inputs(g, m, k, kind)
     y, total = project64(x64, w64)
     close(linear.project(up(x), w).to_host(), y, slack(total, k, 0), kind)
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("m,pool,rank", [(1, 40, 256), (20, 40, 3), (64, 100, 17), (100, 40, 16), (150, 3, 256), (300, 33, 200)])
+def test_adapters_of_large_pools_and_ranks(m, pool, rank, kind):
+    """more adapters than a tile has rows, ranks up to the largest"""
+    g = rng(51, m, rank, kind is F16)
+    n, k = 70, 256
+    w, w64 = weights(g, 12, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    ad, a, b, s = adapters(g, pool, rank, n, k, kind)
+    which = g.integers(-1, pool + 1, m).astype(np.int32)
+    which[0] = pool - 1
+    y, total = project64(x64, w64, a, b, s, which)
+    close(linear.project(up(x), w, ad, up(which)).to_host(), y, slack(total, k + rank), kind)
