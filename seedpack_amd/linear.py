@@ -91,6 +91,21 @@ def _ids(which, rows):
 _kept = threading.local()
 
 
+class _Block:
+    """a workspace's memory, apart from the arrays' cache: a block there may still be in use by the work of another
+    stream. Freeing it waits for the device."""
+    __slots__ = ("ptr", "nbytes")
+
+    def __init__(self, n):
+        self.ptr, self.nbytes = dev.CACHE.alloc(n), n
+
+    def __del__(self):
+        try:
+            lib().spa_free(self.ptr)
+        except Exception:
+            pass
+
+
 def _scratch(n, work, stream):
     """the call's workspace: the one given, or this thread's own for the device and stream, kept for its next calls
     there. One that has to grow waits for the stream once, so that work still queued on the old block is done.
@@ -103,12 +118,13 @@ def _scratch(n, work, stream):
         if work is None or work.nbytes < n:
             if work is not None:
                 check(lib().spa_stream_synchronize(stream))
-            work = blocks[key] = dev.DeviceArray(max(n, 1 << 20), np.uint8)
+                del blocks[key], work
+            work = blocks[key] = _Block(max(n, 1 << 20))
     return work, work.ptr, work.nbytes
 
 
 def release():
-    """gives this thread's workspaces back to the cache of device blocks, after waiting for their work"""
+    """frees this thread's workspaces, after waiting for their work"""
     for _, stream in list(_kept.__dict__):
         check(lib().spa_stream_synchronize(stream))
     _kept.__dict__.clear()
