@@ -273,6 +273,8 @@ def mem_info():
 
 
 class Stream:
+    ends = []                                             # called with the handle of a stream that is about to be destroyed
+
     def __init__(self):
         p = ctypes.c_void_p()
         check(lib().spa_stream_create(ctypes.byref(p)))
@@ -288,6 +290,8 @@ class Stream:
     def __del__(self):
         if getattr(self, "handle", None):
             try:
+                for f in Stream.ends:
+                    f(self.handle)
                 lib().spa_stream_destroy(self.handle)
             except Exception:
                 pass

@@ -9,7 +9,7 @@ Weights are BF16 or F16 matrices or any of the 20 GGUF block types, as they lie 
 Inputs and outputs are two-dimensional DeviceArrays of BF16 bits (uint16) or float16, row-major; with a
 `*_stride` (in elements) an array's rows may lie further apart than their columns. Every call only queues
 work on `stream` and returns; results are float32 sums rounded once. A call's scratch is the calling thread's
-own for that device and stream, kept between calls (`release` gives it back), or is given as `work`. Arrays
+own for that device and stream, kept between calls (until the stream ends or `release`), or is given as `work`. Arrays
 that a call makes for its results come from the thread's cache of device blocks, whose work is on one stream
 (device._Cache): a thread that uses several gives its own.
 
@@ -17,6 +17,7 @@ The reference has no counterpart: it makes and packs weights (seedpack/gpuquant.
 their use to llama.cpp.
 """
 import threading
+import weakref
 
 import numpy as np
 
@@ -88,7 +89,32 @@ def _ids(which, rows):
         raise ValueError(f"{which.shape[0]} row numbers for {rows} rows")
 
 
-_kept = threading.local()
+class _Kept(threading.local):
+    """a thread's workspaces by (device, stream)"""
+
+    def __init__(self):
+        self.blocks = _Blocks()
+        with _threads_lock:
+            _threads.add(self.blocks)
+
+
+class _Blocks(dict):
+    __hash__ = object.__hash__                            # one of its thread, whatever it holds
+
+
+_threads, _threads_lock = weakref.WeakSet(), threading.RLock()
+_kept = _Kept()
+
+
+def _stream_ends(stream):
+    """a stream that ends takes every thread's workspace for it along: the next stream may get its handle"""
+    with _threads_lock:
+        for blocks in list(_threads):
+            for key in [k for k in list(blocks) if k[1] == stream]:
+                blocks.pop(key, None)
+
+
+dev.Stream.ends.append(_stream_ends)
 
 
 class _Block:
@@ -113,7 +139,7 @@ def _scratch(n, work, stream):
     if not n:
         return None, None, 0
     if work is None:
-        blocks, key = _kept.__dict__, (dev.current_device(), stream)
+        blocks, key = _kept.blocks, (dev.current_device(), stream)
         work = blocks.get(key)
         if work is None or work.nbytes < n:
             if work is not None:
@@ -124,10 +150,16 @@ def _scratch(n, work, stream):
 
 
 def release():
-    """frees this thread's workspaces, after waiting for their work"""
-    for _, stream in list(_kept.__dict__):
-        check(lib().spa_stream_synchronize(stream))
-    _kept.__dict__.clear()
+    """frees this thread's workspaces, after waiting for the work of their devices (not for their streams, which may
+    have ended). To be called before a stream that is not a device.Stream ends, if calls were made on it."""
+    blocks, here = _kept.blocks, dev.current_device()
+    try:
+        for d in sorted({d for d, _ in list(blocks)}):
+            dev.set_device(d)
+            check(lib().spa_device_synchronize())
+    finally:
+        dev.set_device(here)
+        blocks.clear()
 
 
 def _out(name, out, m, n, dtype, stride):

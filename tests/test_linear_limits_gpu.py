@@ -6,6 +6,7 @@ absolute values, and what a form's operands lose), with the operands' part named
 import numpy as np
 import pytest
 
+from seedpack_amd import device as dev
 from seedpack_amd import linear
 from seedpack_amd.gpuquant import GPUQuant
 from seedpack_amd.requant import QFUN
@@ -353,3 +354,20 @@ def test_adapters_of_large_pools_and_ranks(m, pool, rank, kind):
     which[0] = pool - 1
     y, total = project64(x64, w64, a, b, s, which)
     close(linear.project(up(x), w, ad, up(which)).to_host(), y, slack(total, k + rank), kind)
+
+
+def test_streams_that_end():
+    """workspaces of streams that come and go: right results, and release() afterwards"""
+    g = rng(53)
+    n, k, m = 300, 1024, 140
+    w, w64 = weights(g, 12, n, k)
+    x, x64 = inputs(g, m, k, BF16)
+    y, total = project64(x64, w64)
+    xd = up(x)
+    for _ in range(6):
+        st = dev.Stream()
+        out = linear.project(xd, w, stream=st.handle)
+        close(out.to_host(stream=st.handle), y, slack(total, k), BF16)
+        del out, st
+    linear.release()
+    close(linear.project(xd, w).to_host(), y, slack(total, k), BF16)

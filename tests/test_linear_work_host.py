@@ -109,3 +109,50 @@ def test_threads_have_workspaces_of_their_own(library):
     t.join()
     a, b = library.work()
     assert a != b and not library.freed(a)
+
+
+def test_release_waits_for_devices_and_reaches_every_workspace(library):
+    """streams that are gone by now, workspaces of several devices: no handle is called, all memory is back"""
+    for d in (0, 1):
+        library.device = d
+        for s in (None, 7, 8):
+            call(s)
+    library.dead = {7, 8}
+    library.log, calls = [], library.work()
+    linear.release()
+    assert library.device == 1 and all(library.freed(p) for p in calls)
+    assert [c for c in library.log if c[0] == "stream_synchronize"] == []
+    first = [c[0] for c in library.log].index("free")
+    assert {c[1] for c in library.log[:first] if c[0] == "device_synchronize"} == {0, 1}
+    call(8)
+    assert library.work()[0] not in calls
+
+
+def test_a_stream_takes_its_workspaces_with_it(library, monkeypatch):
+    """a new stream may get the number of one that has been destroyed: it does not get that one's workspace"""
+    monkeypatch.setattr(library, "spa_stream_create", lambda p: setattr(p._obj, "value", 99) or 0, raising=False)
+    s = dev.Stream()
+    call(s.handle)
+    other = threading.Event(), threading.Event()
+
+    def elsewhere():
+        call(s.handle)
+        other[0].set()
+        other[1].wait(10)
+
+    t = threading.Thread(target=elsewhere)
+    t.start()
+    other[0].wait(10)
+    a, b = library.work()
+    call(7)
+    kept = library.work()[-1]
+    del s
+    names = [c[0] for c in library.log]
+    assert library.freed(a) and library.freed(b) and not library.freed(kept)
+    # before the handle can be given again
+    assert library.log[-1] == ("stream_destroy", 99) and names.count("free") == 2
+    t2 = dev.Stream()
+    call(t2.handle)
+    assert library.work()[-1] not in (a, b)
+    other[1].set()
+    t.join()
