@@ -59,6 +59,7 @@ int spa_memset(void* ptr, int value, size_t nbytes, void* stream);
 int spa_stream_create(void** stream);
 int spa_stream_destroy(void* stream);
 int spa_stream_synchronize(void* stream);
+int spa_stream_is_capturing(void* stream, int* yes);   /* whether a graph is being captured from it */
 int spa_device_synchronize(void);
 int spa_event_create(void** event);
 int spa_event_destroy(void* event);

@@ -35,6 +35,7 @@ SIGNATURES = {
     "spa_stream_create": (c_int, [ctypes.POINTER(c_void_p)]),
     "spa_stream_destroy": (c_int, [c_void_p]),
     "spa_stream_synchronize": (c_int, [c_void_p]),
+    "spa_stream_is_capturing": (c_int, [c_void_p, ctypes.POINTER(c_int)]),
     "spa_device_synchronize": (c_int, []),
     "spa_event_create": (c_int, [ctypes.POINTER(c_void_p)]),
     "spa_event_destroy": (c_int, [c_void_p]),

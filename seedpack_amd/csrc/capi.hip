@@ -130,6 +130,13 @@ int spa_memset(void* p, int v, size_t n, void* s) { SPA_HIP_TRY(hipMemsetAsync(p
 int spa_stream_create(void** s) { SPA_HIP_TRY(hipStreamCreateWithFlags((hipStream_t*)s, hipStreamNonBlocking)); return SPA_OK; }
 int spa_stream_destroy(void* s) { SPA_HIP_TRY(hipStreamDestroy((hipStream_t)s)); return SPA_OK; }
 int spa_stream_synchronize(void* s) { SPA_HIP_TRY(wait_stream((hipStream_t)s)); return SPA_OK; }
+int spa_stream_is_capturing(void* s, int* yes) {
+    if (!yes) return fail(SPA_ERR_ARG, "spa_stream_is_capturing: null out pointer");
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (s) SPA_HIP_TRY(hipStreamIsCapturing((hipStream_t)s, &st));   // nothing is captured from the default stream
+    *yes = st != hipStreamCaptureStatusNone;
+    return SPA_OK;
+}
 int spa_device_synchronize(void) { SPA_HIP_TRY(hipDeviceSynchronize()); return SPA_OK; }
 int spa_event_create(void** e) { SPA_HIP_TRY(hipEventCreate((hipEvent_t*)e)); return SPA_OK; }
 int spa_event_destroy(void* e) { SPA_HIP_TRY(hipEventDestroy((hipEvent_t)e)); return SPA_OK; }

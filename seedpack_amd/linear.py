@@ -11,11 +11,13 @@ Inputs and outputs are two-dimensional DeviceArrays of BF16 bits (uint16) or flo
 work on `stream` and returns; results are float32 sums rounded once. A call's scratch is the calling thread's
 own for that device and stream, kept between calls (until the stream ends or `release`), or is given as `work`. Arrays
 that a call makes for its results come from the thread's cache of device blocks, whose work is on one stream
-(device._Cache): a thread that uses several gives its own.
+(device._Cache): a thread that uses several gives its own. A call that is captured into a graph is given both, with
+workspaces of the C entries' `*_work_bytes`.
 
 The reference has no counterpart: it makes and packs weights (seedpack/gpuquant.py:284-456) and leaves
 their use to llama.cpp.
 """
+import ctypes
 import threading
 import weakref
 
@@ -132,13 +134,23 @@ class _Block:
             pass
 
 
+def _not_captured(stream, what):
+    """a graph keeps the addresses of its capture, so what it uses has to be the caller's"""
+    if stream is not None:
+        yes = ctypes.c_int()
+        check(lib().spa_stream_is_capturing(stream, ctypes.byref(yes)))
+        if yes.value:
+            raise ValueError(f"a call that is captured needs its {what} given")
+
+
 def _scratch(n, work, stream):
     """the call's workspace: the one given, or this thread's own for the device and stream, kept for its next calls
-    there. One that has to grow waits for the stream once, so that work still queued on the old block is done.
+    there (a captured call's is given: the graph keeps its address). One that has to grow waits for the stream once, so that work still queued on the old block is done.
     -> (what keeps it alive, pointer, bytes)"""
     if not n:
         return None, None, 0
     if work is None:
+        _not_captured(stream, "workspace (work)")
         blocks, key = _kept.blocks, (dev.current_device(), stream)
         work = blocks.get(key)
         if work is None or work.nbytes < n:
@@ -162,10 +174,11 @@ def release():
         blocks.clear()
 
 
-def _out(name, out, m, n, dtype, stride):
+def _out(name, out, m, n, dtype, stride, stream):
     if out is None:
         if stride is not None:
             raise ValueError(f"a stride of {name} needs its array")
+        _not_captured(stream, f"result ({name})")
         return dev.DeviceArray((m, n), dtype), n
     if out.dtype != dtype or out.shape != (m, n):
         raise ValueError(f"{name} is {out.shape} {out.dtype}, ({m}, {n}) {dtype} is needed")
@@ -188,7 +201,7 @@ def project(x, w, adapters=None, which=None, out=None, x_stride=None, out_stride
                              f"and a {w.rows} x {w.cols} projection")
         _ids(which, m)
         a, b, scale, ids, pool, rank = adapters.a.ptr, adapters.b.ptr, adapters.scale.ptr, which.ptr, adapters.count, adapters.rank
-    out, ldo = _out("out", out, m, w.rows, x.dtype, out_stride)
+    out, ldo = _out("out", out, m, w.rows, x.dtype, out_stride, stream)
     L = lib()
     keep, p, n = _scratch(L.spa_project_work_bytes(w.type, w.rows, w.cols, kind, m, pool, rank), work, stream)
     check(L.spa_project(w.type, w.data.ptr, w.rows, w.cols, kind, x.ptr, m, ld, out.ptr, ldo, a, b, scale, pool, rank, ids,
@@ -208,7 +221,7 @@ def gated(x, gate, up, act="silu", out=None, x_stride=None, out_stride=None, wor
     """x (rows, cols) -> act(x gate^T) * (x up^T), (rows, gate.rows); act "silu" or "gelu" (tanh form)"""
     act = _pair(gate, up, act)
     kind, m, _, ld = _rows("x", x, x_stride, gate.cols)
-    out, ldo = _out("out", out, m, gate.rows, x.dtype, out_stride)
+    out, ldo = _out("out", out, m, gate.rows, x.dtype, out_stride, stream)
     L = lib()
     keep, p, n = _scratch(L.spa_gated_work_bytes(gate.type, gate.rows, gate.cols, kind, m), work, stream)
     check(L.spa_gated(gate.type, gate.data.ptr, up.data.ptr, gate.rows, gate.cols, kind, x.ptr, m, ld, act, out.ptr, ldo, p, n,
@@ -230,10 +243,10 @@ def gated_backward(x, gate, up, dh, act="silu", dx=None, dgate=None, dup=None, x
         raise ValueError("both matrices' gradients or neither")
     ldx = k
     if dx is not None or dgate is None:
-        dx, ldx = _out("dx", dx, m, k, x.dtype, dx_stride)
+        dx, ldx = _out("dx", dx, m, k, x.dtype, dx_stride, stream)
     if dgate is not None:
-        dgate, _ = _out("dgate", dgate, gate.rows, k, x.dtype, None)
-        dup, _ = _out("dup", dup, gate.rows, k, x.dtype, None)
+        dgate, _ = _out("dgate", dgate, gate.rows, k, x.dtype, None, stream)
+        dup, _ = _out("dup", dup, gate.rows, k, x.dtype, None, stream)
     L = lib()
     keep, p, n = _scratch(L.spa_gated_backward_work_bytes(gate.type, gate.rows, k, kind, m, dx is not None, dgate is not None), work, stream)
     check(L.spa_gated_backward(gate.type, gate.data.ptr, up.data.ptr, gate.rows, k, kind, x.ptr, m, ld, act, dh.ptr, ldh,

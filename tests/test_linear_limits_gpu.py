@@ -3,11 +3,14 @@ finite and whom they may reach, the largest and the least inputs, and what the f
 
 Tolerances are those of test_linear_gpu (an output's rounding, K 2^-24 T for float32 sums of K terms, T the sum over
 absolute values, and what a form's operands lose), with the operands' part named by each test."""
+import ctypes
+
 import numpy as np
 import pytest
 
 from seedpack_amd import device as dev
 from seedpack_amd import linear
+from seedpack_amd._lib import LIB_PATH, check, lib
 from seedpack_amd.gpuquant import GPUQuant
 from seedpack_amd.requant import QFUN
 from tests.test_linear_gpu import (BF16, F16, _named, adapters, close, gated_backward64, inputs, project64, random_blocks,  # noqa: F401
@@ -371,3 +374,81 @@ def test_streams_that_end():
         del out, st
     linear.release()
     close(linear.project(xd, w).to_host(), y, slack(total, k), BF16)
+
+
+class Graph:
+    """what a stream's calls left in a capture, by the HIP runtime that the library is linked with"""
+
+    def __init__(self, stream, calls):
+        self.hip = ctypes.CDLL(LIB_PATH)
+        graph, self.made = ctypes.c_void_p(), ctypes.c_void_p()
+        self.ok(self.hip.hipStreamBeginCapture(ctypes.c_void_p(stream), 0))
+        try:
+            calls()
+        finally:
+            self.ok(self.hip.hipStreamEndCapture(ctypes.c_void_p(stream), ctypes.byref(graph)))
+        self.ok(self.hip.hipGraphInstantiate(ctypes.byref(self.made), graph, None, None, ctypes.c_size_t(0)))
+        self.ok(self.hip.hipGraphDestroy(graph))
+
+    def ok(self, code):
+        assert code == 0, code
+
+    def replay(self, stream):
+        self.ok(self.hip.hipGraphLaunch(self.made, ctypes.c_void_p(stream)))
+
+    def close(self):
+        self.ok(self.hip.hipGraphExecDestroy(self.made))
+
+
+@pytest.mark.parametrize("t", [linear.BF16, 8, 10])
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_captured_calls(t, m):
+    """all four calls in one graph, replayed on new numbers between eager calls: the same bits; a captured call without
+    its own memory is refused, and the graph's memory is not what eager calls use"""
+    g = rng(54, t, m)
+    n, k = 512, 2048
+    (gate, _), (upw, _) = weights(g, t, n, k), weights(g, t, n, k)
+    pool = adapters(g, 3, 16, n, k, BF16)[0]
+    ids = up(g.integers(-1, 4, m).astype(np.int32))
+    x, dh, work = (dev.DeviceArray(s, d) for s, d in (((m, k), BF16), ((m, n), BF16), (1 << 26, np.uint8)))
+    outs = {"y": ((m, n), BF16), "h": ((m, n), BF16), "dx": ((m, k), BF16), "sums": ((1, k), np.float32), "counts": (1, np.int64)}
+    if t == linear.BF16:
+        outs |= {"dgate": ((n, k), BF16), "dup": ((n, k), BF16)}
+    outs = {name: dev.DeviceArray(*of) for name, of in outs.items()}
+    st = dev.Stream()
+
+    def calls(**memory):
+        linear.project(x, gate, pool, ids, out=outs["y"], stream=st.handle, **memory)
+        linear.gated(x, gate, upw, out=outs["h"], stream=st.handle, **memory)
+        linear.gated_backward(x, gate, upw, dh, stream=st.handle, **{d: outs[d] for d in ("dx", "dgate", "dup") if d in outs}, **memory)
+        linear.add_squares(x, outs["sums"], outs["counts"], stream=st.handle, **memory)
+
+    def captured():
+        calls(work=work)
+        with pytest.raises(ValueError):
+            linear.gated(x, gate, upw, stream=st.handle, work=work)
+        with pytest.raises(ValueError):
+            linear.gated_backward(x, gate, upw, dh, dx=outs["dx"], stream=st.handle)
+
+    def clear():
+        outs["sums"].zero(st.handle)
+        outs["counts"].zero(st.handle)
+
+    def result():
+        st.synchronize()
+        return {name: a.to_host(stream=st.handle).tobytes() for name, a in outs.items()}
+
+    calls(work=work)
+    st.synchronize()
+    graph = Graph(st.handle, captured)
+    for _ in range(4):
+        for a in (x, dh):
+            h = store(g.normal(0, 0.3, a.shape), BF16)
+            check(lib().spa_memcpy_h2d(a.ptr, h.ctypes.data, h.nbytes, st.handle))
+        clear()
+        graph.replay(st.handle)
+        got = result()
+        clear()
+        calls()
+        assert got == result()
+    graph.close()

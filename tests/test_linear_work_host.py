@@ -47,6 +47,10 @@ class Library:
         self.log.append(("stream_synchronize", self.device, s))
         return -3 if s in self.dead else 0
 
+    def spa_stream_is_capturing(self, s, yes):
+        yes._obj.value = int(s in self.capturing)
+        return 0
+
     def spa_device_synchronize(self):
         self.log.append(("device_synchronize", self.device))
         return 0
@@ -156,3 +160,24 @@ def test_a_stream_takes_its_workspaces_with_it(library, monkeypatch):
     assert library.work()[-1] not in (a, b)
     other[1].set()
     t.join()
+
+
+def test_a_captured_call_brings_its_own_memory(library):
+    """a graph keeps the addresses of its capture: neither the kept workspace nor an array made for the result"""
+    call(7)
+    library.capturing = {7}
+    own = dev.DeviceArray(NEED, np.uint8, ptr=1 << 20, owner=dev)
+    with pytest.raises(ValueError, match="work"):
+        call(7)
+    with pytest.raises(ValueError, match="out"):
+        call(7, out=None, work=own)
+    with pytest.raises(ValueError, match="work"):
+        linear.add_squares(dev.DeviceArray((4, 8), np.uint16, ptr=4096, owner=dev), dev.DeviceArray((1, 8), np.float32, ptr=4096, owner=dev),
+                           dev.DeviceArray(1, np.int64, ptr=4096, owner=dev), stream=7)
+    n = len(library.work())
+    call(7, work=own)
+    call(8)
+    call(None)
+    library.need = 0                                       # needs none
+    call(7)
+    assert len(library.work()) == n + 4 and library.work()[n] == 1 << 20
