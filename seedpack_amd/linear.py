@@ -7,12 +7,13 @@
 
 Weights are BF16 or F16 matrices or any of the 20 GGUF block types, as they lie in a file (`Weight`).
 Inputs and outputs are two-dimensional DeviceArrays of BF16 bits (uint16) or float16, row-major; with a
-`*_stride` (in elements) an array's rows may lie further apart than their columns. Every call only queues
-work on `stream` and returns; results are float32 sums rounded once. A call's scratch is the calling thread's
-own for that device and stream, kept between calls (until the stream ends or `release`), or is given as `work`. Arrays
-that a call makes for its results come from the thread's cache of device blocks, whose work is on one stream
-(device._Cache): a thread that uses several gives its own. A call that is captured into a graph is given both, with
-workspaces of the C entries' `*_work_bytes`.
+`*_stride` (in elements) an array's rows may lie further apart than their columns: the array is then a part of
+another one (`DeviceArray(shape, dtype, ptr=.., owner=other)`), which its last row has to end in. Every call only
+queues work on `stream` and returns; results are float32 sums rounded once. A call's scratch is the calling
+thread's own for that device and stream, kept between calls (until the stream ends or `release`), or is given as
+`work`. Arrays that a call makes for its results come from the thread's cache of device blocks, whose work is on
+one stream (device._Cache): a thread that uses several gives its own. A call that is captured into a graph is
+given both, with workspaces of the C entries' `*_work_bytes`.
 
 The reference has no counterpart: it makes and packs weights (seedpack/gpuquant.py:284-456) and leaves
 their use to llama.cpp.
@@ -69,6 +70,17 @@ class Adapters:
         self.a, self.b, self.scale = a, b, scale
 
 
+def _within(name, a, m, n, stride):
+    """rows further apart than an array's columns lie inside the array that it is a part of; memory that is not a
+    DeviceArray's own (a framework's tensor behind it) is the caller's word"""
+    if m and stride != n:
+        last, of = a.ptr + ((m - 1) * stride + n) * a.dtype.itemsize, a
+        while isinstance(of._owner, dev.DeviceArray) and of._owner is not of:
+            of = of._owner
+        if (of is not a or of._owner is None) and last > of.ptr + of.nbytes:
+            raise ValueError(f"{name}: {m} rows of {n} at a stride of {stride} reach {last - of.ptr - of.nbytes} bytes past its memory")
+
+
 def _rows(name, a, stride, cols=None):
     """a 2-D array -> (kind, rows, columns, stride)"""
     kind = _KIND.get(a.dtype)
@@ -81,6 +93,7 @@ def _rows(name, a, stride, cols=None):
         return kind, m, k, k
     if stride < k:
         raise ValueError(f"{name}: rows of {k} at a stride of {stride}")
+    _within(name, a, m, k, stride)
     return kind, m, k, stride
 
 
@@ -184,6 +197,8 @@ def _out(name, out, m, n, dtype, stride, stream):
         raise ValueError(f"{name} is {out.shape} {out.dtype}, ({m}, {n}) {dtype} is needed")
     if stride is not None and stride < n:
         raise ValueError(f"{name}: rows of {n} at a stride of {stride}")
+    if stride is not None:
+        _within(name, out, m, n, stride)
     return out, n if stride is None else stride
 
 
