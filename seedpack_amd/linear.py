@@ -215,6 +215,8 @@ def project(x, w, adapters=None, which=None, out=None, x_stride=None, out_stride
             raise ValueError(f"adapters of {adapters.a.dtype} {adapters.a.shape}, {adapters.b.shape} beside {x.dtype} inputs "
                              f"and a {w.rows} x {w.cols} projection")
         _ids(which, m)
+        if which.size != m:
+            raise ValueError(f"adapters' numbers of shape {which.shape}: one for each of the {m} rows")
         a, b, scale, ids, pool, rank = adapters.a.ptr, adapters.b.ptr, adapters.scale.ptr, which.ptr, adapters.count, adapters.rank
     out, ldo = _out("out", out, m, w.rows, x.dtype, out_stride, stream)
     L = lib()

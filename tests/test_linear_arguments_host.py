@@ -58,3 +58,13 @@ def test_strides_that_fit():
     assert linear._rows("x", memory((4, 256), np.uint16), 300, 256) == (0, 4, 256, 300)      # a framework's tensor behind it
     with pytest.raises(ValueError):
         linear._rows("x", part(of, (4, 256), np.uint16, 2), 300, 256)
+
+
+def test_one_adapter_a_row():
+    """numbers of adapters are one a row, not rows of them"""
+    of = memory(1 << 16)
+    x, out = part(of, (4, 256), np.uint16), part(of, (4, 8), np.uint16)
+    pool = linear.Adapters(memory((2, 8, 256), np.uint16), memory((2, 8, 8), np.uint16), memory(2, np.float32))
+    for shape in ((4, 2), (4, 4), (4, 1, 3)):
+        with pytest.raises(ValueError):
+            linear.project(x, weight(), pool, memory(shape, np.int32), out=out)
