@@ -234,7 +234,7 @@ extern "C" int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_
     if (src_kind < SPA_SRC_BF16 || src_kind > SPA_SRC_F32) return fail(SPA_ERR_TYPE, "spa_add_squares: source kind %d", src_kind);
     if (rows < 0 || cols <= 0 || x_stride < cols || rows > INT32_MAX || cols > INT32_MAX)
         return fail(SPA_ERR_ARG, "spa_add_squares: bad shape %lld x %lld, stride %lld", (long long)rows, (long long)cols, (long long)x_stride);
-    if (which ? (experts < 1 || experts > 65535 || each < 1 || each * rows > INT32_MAX) : experts != 0)
+    if (which ? (experts < 1 || experts > 65535 || each < 1 || (rows && each > INT32_MAX / rows)) : experts != 0)
         return fail(SPA_ERR_ARG, "spa_add_squares: %lld experts, %lld for each row", (long long)experts, (long long)each);
     if (rows == 0) return SPA_OK;
     if (!x || !sums || !counts) return fail(SPA_ERR_ARG, "spa_add_squares: null pointer");

@@ -68,3 +68,9 @@ def test_one_adapter_a_row():
     for shape in ((4, 2), (4, 4), (4, 1, 3)):
         with pytest.raises(ValueError):
             linear.project(x, weight(), pool, memory(shape, np.int32), out=out)
+
+
+@pytest.mark.parametrize("each", [1 << 62, (1 << 62) + 1, (1 << 61) + 2, (1 << 63) - 1, 1 << 40])
+def test_experts_of_a_row_beyond_counting(each):
+    """numbers of experts whose product with the rows passes 64 bits"""
+    assert lib().spa_add_squares(P, 0, 8, 64, 64, P, each, 3, P, P, P, 1 << 40, None) == ARG
