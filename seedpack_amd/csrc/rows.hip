@@ -130,6 +130,8 @@ __global__ __launch_bounds__(LANES) void k_half_rows(const uint16_t* __restrict_
     }
 }
 
+typedef uint16_t h2u __attribute__((ext_vector_type(2)));
+
 // what a block's weights are at most in size, by its header: scale (and offset) times the largest code
 template <int T>
 __device__ __forceinline__ float block_bound(const uint8_t* b) {
@@ -164,9 +166,9 @@ __device__ __forceinline__ float block_bound(const uint8_t* b) {
 // that its bytes are waited for once. Longer rows: the headers from memory first. FULL: with the norm or the rest.
 // A quantizer's largest weight of a row lies within 2^1.4 of its headers' bound (19 types, normal weights), but where
 // codes are small or zero the bound may be any power of two above: a row whose largest weight turns out 2^5 or more below
-// is converted once more by that weight, so that weights are there to 2^-34 of their row's largest. The look costs
-// about 1 us for 4096 x 8192. (Decoded once into registers and converted by the true largest: 300 rows beside Q6_K
-// 4096 x 8192 in all 78 us, 71 this way.)
+// is converted once more by that weight, so that weights are there to 2^-34 of their row's largest. The look at the
+// halves as they leave costs 1.2 us of 16 for Q4_K 4096 x 4096. (Decoded once into registers and converted by the true
+// largest: 300 rows beside Q6_K 4096 x 8192 in all 78 us, 68 this way.)
 // Bound by the decoding's instructions: 33 us for Q4_K 4096 x 12288 (27 instructions a weight with four weights a
 // lane and the norm always summed: 44 us), 3.9 TB/s read and written.
 template <int T, int QK, int BS, int TILE, bool FULL>
@@ -177,6 +179,8 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     __shared__ __align__(16) uint8_t tile[TBYTES + 16];
     __shared__ int8_t kv[16];
     __shared__ float lds[4];
+    __shared__ int near;
+    if (threadIdx.x == 0) near = 0;
     if (T == 20 || T == 23) {
         if (threadIdx.x < 16) kv[threadIdx.x] = KV_IQ4NL[threadIdx.x];
     }
@@ -207,17 +211,14 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
     if (one) stage(0, (int)nb);
     float most = 0.f;
     for (int64_t b = threadIdx.x; b < nb; b += 256) most = fmaxf(most, block_bound<T>((one ? tile : src) + b * BS));
-    int e = exponent_for(reduce<true>(most, lds));
-    float sum;
-    for (bool first = true;; first = false) {
-        sum = most = 0.f;
+    // f(the first of eight weights, all eight): what a block's header says of them is worked out once
+    auto each = [&](auto f) {
         for (int64_t b0 = 0; b0 < nb; b0 += TB) {
             const int n = (int)(nb - b0 < TB ? nb - b0 : TB);
             if (!one) {
                 __syncthreads();
                 stage(b0, n);
             }
-            // eight weights a lane: what a block's header says of them is worked out once
             for (int q = threadIdx.x; q < n * (QK / 8); q += 256) {
                 const int o = q * 8, blk = o / QK;
                 const FastBlk in{{tile, blk * BS}};
@@ -228,39 +229,57 @@ __global__ __launch_bounds__(256) void k_half_blocks(const uint8_t* __restrict__
                 dq4<T>(in, o - blk * QK + 4, t, kv, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[4 + i] = w[i];
-                u4 h;
+                f(b0 * QK + o, v);
+            }
+        }
+    };
+    const float bound = reduce<true>(most, lds);
+    int e = exponent_for(bound);
+    float sum;
+    for (bool first = true;; first = false) {
+        h2u top = {0, 0};                                         // the largest halves, without their signs
+        sum = 0.f;
+        each([&](int64_t at, float (&v)[8]) {
+            u4 h;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], -e);
-                float top = 0.f;
+            for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], -e);
+            if (FULL && norm) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-                if (size_of(top) != top) {                        // an infinity among them: the largest of the others
-                    top = 0.f;
+                for (int i = 0; i < 8; ++i) sum = fmaf(size_of(v[i]), size_of(v[i]), sum);
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, size_of(v[i]));
-                }
-                most = fmaxf(most, top);
-                if (FULL && norm) {
+            for (int i = 0; i < 4; ++i) {
+                h[i] = narrow2(v[2 * i], v[2 * i + 1], SRC_F16);
+                const uint32_t size = h[i] & 0x7fff7fffu;
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(h2u, size));
+            }
+            *reinterpret_cast<u4*>(dst + at) = h;
+            if (FULL && rest) {                                   // what binary16 leaves over (nothing of infinities)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum = fmaf(size_of(v[i]), size_of(v[i]), sum);
+                for (int i = 0; i < 8; ++i) {
+                    const float r = wide((h[i >> 1] >> (16 * (i & 1))) & 0xffffu, SRC_F16);
+                    v[i] = size_of(r) == fabsf(r) ? v[i] - r : 0.f;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[i] = narrow2(v[2 * i], v[2 * i + 1], SRC_F16);
-                *reinterpret_cast<u4*>(dst + b0 * QK + o) = h;
-                if (FULL && rest) {                               // what binary16 leaves over (nothing of infinities)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float r = wide((h[i >> 1] >> (16 * (i & 1))) & 0xffffu, SRC_F16);
-                        v[i] = size_of(r) == fabsf(r) ? v[i] - r : 0.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) h[i] = narrow2(v[2 * i], v[2 * i + 1], SRC_F16);
-                    *reinterpret_cast<u4*>(dst + kp + b0 * QK + o) = h;
-                }
+                *reinterpret_cast<u4*>(dst + kp + at) = h;
             }
-        }
+        });
         if (!first) break;
-        most = reduce<true>(most, lds);
+        const uint32_t mine = tmax(top[0], top[1]);
+        if (__ballot(mine >= 0x6400u && mine < 0x7c00u)) near = 1;   // 2^10 and above: the same from every writer
+        __syncthreads();
+        if (near || !(bound > 0.f)) break;
+        const uint32_t bits = (uint32_t)reduce<true>((float)mine, lds);
+        most = wide(bits, SRC_F16);
+        if (bits == 0 || bits >= 0x7c00u) {                       // nothing left, or infinities: by the numbers themselves
+            most = 0.f;
+            each([&](int64_t, float (&v)[8]) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, ldexpf(size_of(v[i]), -e));
+            });
+            most = reduce<true>(most, lds);
+        }
         const int over = most > 0.f ? -exponent_for(most) : 0;
         if (over < 5) break;
         e -= over;
