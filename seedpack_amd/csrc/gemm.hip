@@ -44,6 +44,7 @@ __device__ __forceinline__ f16v mul_bf(bf8 a, bf8 b, f16v c) { return __builtin_
 
 typedef __amdgpu_buffer_rsrc_t rsrc;
 typedef __attribute__((address_space(3))) void* lptr;
+typedef uint16_t h2u __attribute__((ext_vector_type(2)));
 
 // the least adapter number above `after` among the tile's rows (held by the wave's lanes), or INT32_MAX
 template <int N>
@@ -310,18 +311,27 @@ __device__ __forceinline__ void product(const Gemm& g) {
                         }
                     }
                     // ranks beyond the last: low holds zeros there, b's numbers are cleared (they may be infinite)
+                    h2u largest = {0, 0};
 #pragma unroll
                     for (int i = 0; i < FN; ++i)
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             const int left = ex.rank - r - 2 * c;
                             h[i][c] &= left >= 2 ? 0xffffffffu : (left == 1 ? 0xffffu : 0u);
-                            const uint32_t top = ex.kind == SRC_BF16 ? 0x7f80u : 0x7c00u, most = ex.kind == SRC_BF16 ? 0x7f7fu : 0x7bffu;
-                            const bool lo = (h[i][c] & top) == top, hi = (h[i][c] >> 16 & top) == top;
-                            odd = odd || lo || hi;
-                            if (lo) h[i][c] = (h[i][c] & 0xffff8000u) | most;
-                            if (hi) h[i][c] = (h[i][c] & 0x8000ffffu) | most << 16;
+                            const uint32_t size = h[i][c] & 0x7fff7fffu;
+                            largest = __builtin_elementwise_max(largest, __builtin_bit_cast(h2u, size));
                         }
+                    const uint32_t top = ex.kind == SRC_BF16 ? 0x7f80u : 0x7c00u;
+                    if (__ballot(largest[0] >= top || largest[1] >= top)) {
+                        odd = true;
+#pragma unroll
+                        for (int i = 0; i < FN; ++i)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                if ((h[i][c] & top) == top) h[i][c] = (h[i][c] & 0xffff8000u) | (top - 1);
+                                if ((h[i][c] >> 16 & top) == top) h[i][c] = (h[i][c] & 0x8000ffffu) | (top - 1) << 16;
+                            }
+                    }
                     bf8 zh[FM], zl[FM];
 #pragma unroll
                     for (int j = 0; j < FM; ++j) {
@@ -355,7 +365,6 @@ __device__ __forceinline__ void product(const Gemm& g) {
                 }
             }
         }
-        odd = __ballot(odd) != 0;
         // what the numbers of b that are not finite give output (mi, ni): infinities, NaN, or nothing
         auto lost = [&](int mi, int ni) {
             float t = 0.f;
