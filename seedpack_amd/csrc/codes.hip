@@ -310,9 +310,11 @@ int launch(const FewArgs& a, hipStream_t st) {
     constexpr int HIGH = Unit<T>::HALVES ? 8 : 16;
     const dim3 grid((unsigned)((a.f.n + 15) / 16));
     const int tiles = few_tiles(T, a.f.m);
-    // A wave has at least one unit of k to itself (151936 x 1024 with 3 rows: 8 waves, half of them idle, 54 us, 4 waves 34);
-    // few weight rows fill the device with waves only if more of them
-    // share a row's k.
+    // A wave has at least one unit of k to itself (one row of k = 1024, Q4_K with 4, 8 and 16 waves: n = 4096 7.0, 7.1 and
+    // 7.1 us, 12288 6.9, 7.0 and 7.9, 32768 8.4, 10.1 and 17.5, 151936 25, 35 and 71; Q6_K 34, 52 and 85). Few weight rows
+    // fill the device with waves only if more of them share a row's k (k = 4096, 8 and 16 waves: n = 4096 Q4_K 6.2 and
+    // 6.0, Q8_0 8.1 and 7.5, Q6_K 10.3 and 7.9; 8192 9.0 and 9.7, 11.5 and 12.9, 12.0 and 12.4; 32768 24 and 30, 31 and
+    // 42, 32 and 37).
     const int units = (a.f.k + UNIT - 1) / UNIT;
     const bool many = TWO || a.f.n >= 8192, low = units <= 4 && a.f.n >= 4096;
     constexpr int MOST = TWO ? 8 : 16;

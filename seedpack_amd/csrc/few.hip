@@ -213,8 +213,13 @@ int launch(const FewArgs& given, DQ t, uint16_t* frags, hipStream_t st) {
         }
         const bool lined = a.rowbytes == 2 * (int64_t)a.f.k && ((reinterpret_cast<uintptr_t>(a.f.w0) | reinterpret_cast<uintptr_t>(a.f.w1)) & 15) == 0;
         const bool words = a.rowbytes % 4 == 0;                   // 16-bit matrices begin at 16-byte addresses
-        // few weight rows fill the device with waves only if more of them share a row's k (one row of 4060 x 5795
-        // with 8 waves: 80 us)
+        // Few weight rows fill the device with waves only if more of them share a row's k (one row of 4060 x 5795
+        // with 8 waves: 80 us), and a long k keeps 16 busy whatever the rows: one row with 8 and with 16 waves, us:
+        //     k      n = 4096       8192      12288       32768
+        //  1024     6.1  6.1     6.1  6.1    7.3  8.2   13.4 16.9
+        //  2048     7.4  6.7    11.2  9.0   14.9 12.0   31.0 25.1
+        //  4096     9.9  9.6    17.1 15.3   23.3 21.0   52.9 49.0
+        //  8192    19.0 18.7    32.3 30.8   45.2 43.1  108.3 99.1
 #define SPA_FEW16(MT, W)                                                                                    \
     do {                                                                                                    \
         if (lined) hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, LINED, W>), grid, dim3(W * 64), 0, st, a);         \
@@ -222,7 +227,7 @@ int launch(const FewArgs& given, DQ t, uint16_t* frags, hipStream_t st) {
         else hipLaunchKernelGGL((k_few16<WK, KIND, MT, TWO, ANYWHERE, W>), grid, dim3(W * 64), 0, st, a);            \
     } while (0)
         if (a.f.m <= 16) {
-            if (a.f.n < 8192) SPA_FEW16(1, 16);
+            if (a.f.n < 8192 || a.f.k >= 2048) SPA_FEW16(1, 16);
             else SPA_FEW16(1, 8);
         } else if (a.f.m <= 32) {
             SPA_FEW16(2, 8);

@@ -199,10 +199,19 @@ struct Project {
 // Many rows' first products as one product with every adapter of the pool, where it is small enough that
 // the rows' other adapters cost less than reading x a few lanes at a time (2053 rows of 12288, 4 adapters of rank
 // 64: 55 us row by row, 27 and 5 of picking): 128 x 128 tiles in pieces of k that fill the device, two to a compute unit. Tiles of
-// adapters that none of their rows have are left out.
+// adapters that none of their rows have are left out. Whole calls row by row and this way, BF16 with 1024 outputs, us:
+//     k   rows    4 x 16     4 x 64    16 x 64    32 x 64 (width 2048)
+//  1024    512    20  24     33  33     54  54     73  73
+//  2048    128    24  28     31  30     51  49     74  73
+//  2048    512    26  27     36  31     42  37     49  44
+//  4096     65    28  29     40  30     57  47     83  73
+//  4096   4096    61  62     81  71     82  83     96 106
+// 12288     65    48  37     81  38     99  59    118  80
+// 12288   4096   143 130    179 140    182 183    201 276
+// (200 rows beside Q4_K 4096 x 4096, 16 of rank 16 in any order: 75 and 80)
 int64_t low_as_product(const Project& p) {
     const int64_t width = p.pool * p.rank;
-    if (p.m <= 256 || width > 1024 || p.k % 64 || p.k < 2048) return 0;
+    if (p.m <= (p.k < 4096 || p.rank <= 16 ? 256 : FEW_ROWS) || width > 1024 || p.k % 64 || p.k < 2048) return 0;
     const int64_t tiles = (p.m + 127) / 128 * ((width + 127) / 128), pieces = tiles < 512 ? 512 / tiles : 1;
     return pieces < p.k / 256 ? pieces : p.k / 256;
 }

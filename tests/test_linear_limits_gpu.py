@@ -359,6 +359,21 @@ def test_adapters_of_large_pools_and_ranks(m, pool, rank, kind):
     close(linear.project(up(x), w, ad, up(which)).to_host(), y, slack(total, k + rank), kind)
 
 
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("t", [8, 12, linear.F16])
+@pytest.mark.parametrize("m", [64, 65, 100, 128, 129])
+def test_adapters_first_product_over_a_long_k(t, m, kind):
+    """rows around the number from which all adapters' first products are one product; their order is any"""
+    g = rng(55, t, m, kind is F16)
+    n, k, pool, rank = 70, 4096, 5, 20
+    w, w64 = weights(g, t, n, k)
+    x, x64 = inputs(g, m, k, kind)
+    ad, a, b, s = adapters(g, pool, rank, n, k, kind)
+    which = g.integers(-1, pool + 1, m).astype(np.int32)
+    y, total = project64(x64, w64, a, b, s, which)
+    close(linear.project(up(x), w, ad, up(which)).to_host(), y, slack(total, k + rank), kind)
+
+
 def test_streams_that_end():
     """workspaces of streams that come and go: right results, and release() afterwards"""
     g = rng(53)
