@@ -556,12 +556,18 @@ int spa_rans_build_lut_pb(const uint32_t* cum, int ntab, int pb, uint8_t* lut, v
  * Weights W are row-major matrices of n rows of k: ggml type 1 (F16) or 30 (BF16), 16-byte aligned, or any of the
  * 20 block types, at any byte. Inputs and outputs are BF16 or F16 (SPA_SRC_BF16 / SPA_SRC_F16), m rows at a stride
  * given in elements; columns between a row's end and the stride are neither read nor written. Sums are float32 and
- * each output is rounded once; where inputs and weights differ in type, weights are taken to 11 bits or better of
- * their value (22 beside F16 inputs), and inputs and weights to 2^-39 of the largest of their row. Outputs must not
- * overlap inputs. Up to 4,000,000 columns. `work` is device scratch of at least the call's *_work_bytes, 256-byte
- * aligned, free again when the call's work on the stream is done; the sizes are those of the widest case, whatever
- * the strides. Nothing is allocated and calls may be captured, but for the lattice types: their table is made at its
- * first use on a device, and a call waits for its upload. */
+ * each output is rounded once. Inputs and weights of one 16-bit type are multiplied as they are. Where they differ:
+ *   many rows (over 64; over 128 for Q4_0, Q8_0, Q4_K and Q5_K): inputs and 16-bit weights to 2^-39 of the largest of
+ *   their row; weights of blocks to 11 bits, beside F16 inputs to 22, and to 2^-34 of the largest of their row;
+ *   few rows, and last rows past whole tiles: whole codes of Q4_0, Q8_0, Q4_K, Q5_K and Q6_K (beside BF16 inputs all
+ *   but Q8_0's over a base of 128, whose float32 rounding stays: 2^-24 of 128 scales times the inputs' sizes); weights
+ *   of other types to 16 bits.
+ * Infinities and NaN give what the definition gives them, in the rows that hold them only (an infinity beside a
+ * weight so small that a form holds it as zero: NaN). Outputs must not overlap inputs. Up to 4,000,000 columns.
+ * `work` is device scratch of at least the call's *_work_bytes, 256-byte aligned, free again when the call's work on
+ * the stream is done; the sizes are those of the widest case, whatever the strides. Nothing is allocated and calls may
+ * be captured, but for the lattice types: their table is made at its first use on a device, and a call waits for its
+ * upload. */
 
 /* y[m][n] = sum_k x[m][k] W[n][k] + scale[a] sum_r (sum_k x[m][k] A[a][r][k]) B[a][n][r], a = which[m]: a shared
  * projection with the low-rank adapters of a batch's requests. a: [pool][rank][k], b: [pool][n][rank] of the inputs'

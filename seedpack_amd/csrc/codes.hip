@@ -20,7 +20,7 @@
 // again: Q8_0 12288 x 4096 took 63 us, Q6_K 151936 x 1024 149 us), and no barrier is needed before the join. The
 // loads of many waves of a compute unit keep the memory busy while others compute.
 // Bound by memory latency and, from a few rows on, by the unpacking: one row through two Q4_K matrices 12288 x 4096
-// 14.4 us (3.9 TB/s), three through Q6_K 151936 x 1024 31 us (4.1), 32 through Q8_0 12288 x 4096 20 us (2.7).
+// 14.4 us (3.9 TB/s), three through Q6_K 151936 x 1024 31 us (4.1), 32 through Q8_0 12288 x 4096 18.4 us (2.9).
 // Q6_K's scales cover 16 k, half a step: its tiles take 8 input rows twice, rows 0-7 with the first 16 k and
 // rows 8-15 with the second (zeros elsewhere), so that a lane's sums belong to one scale.
 #include "../../include/seedpack_amd.h"

@@ -4,13 +4,14 @@
 // their products are exact in float32 and go through that type's matrix instruction. Where they do not
 // (block types, BF16 beside F16) there are two forms:
 //   * many rows: both operands as binary16 with a power of two taken out of each row, so that the row's
-//     largest value lies below 2^15. A BF16 row keeps its values to 2^-39 of its largest (8 of 11 bits
-//     used, 2^-24 the least step); a decoded weight is rounded to 11 bits, an eighth of a BF16
-//     rounding. Beside F16 inputs, whose results have 11 bits too, the weights are taken to 22: what the
-//     rounding leaves over takes part as a second half of k. The powers are added back to the float32 sums as
-//     exponents;
-//   * few rows: each value as a sum of two BF16 numbers (16 bits, any exponent), whose products are
-//     summed by two or three BF16 instructions: the matrix unit idles there.
+//     largest value lies below 2^15. A row of 16-bit numbers keeps its values to 2^-39 of its largest (2^-24 is the
+//     least step), one of blocks to 2^-34; a decoded weight is rounded to 11 bits, an eighth of a BF16
+//     rounding: an output's own rounding is eight times that, and 22 bits would take the product twice as long. Beside
+//     F16 inputs, whose results have 11 bits too, the weights are taken to 22: what the rounding leaves over
+//     takes part as a second half of k. The powers are added back to the float32 sums as exponents;
+//   * few rows: whole codes of five block types as they are (codes.hip), each value of the others as a sum of two
+//     BF16 numbers (16 bits, any exponent), whose products are summed by two or three BF16 instructions: the
+//     matrix unit idles there.
 #pragma once
 
 #include "common.h"

@@ -208,7 +208,7 @@ struct Project {
 //  4096   4096    61  62     81  71     82  83     96 106
 // 12288     65    48  37     81  38     99  59    118  80
 // 12288   4096   143 130    179 140    182 183    201 276
-// (200 rows beside Q4_K 4096 x 4096, 16 of rank 16 in any order: 75 and 80)
+// (adapters of rank 16, whose rows form has one tile of them, gain nothing below 257 rows but from k = 12288)
 int64_t low_as_product(const Project& p) {
     const int64_t width = p.pool * p.rank;
     if (p.m <= (p.k < 4096 || p.rank <= 16 ? 256 : FEW_ROWS) || width > 1024 || p.k % 64 || p.k < 2048) return 0;

@@ -275,7 +275,8 @@ def gated_backward(x, gate, up, dh, act="silu", dx=None, dgate=None, dup=None, x
 def add_squares(x, sums, counts, which=None, x_stride=None, work=None, stream=None):
     """x (rows, cols), float32 too: adds the rows' squares to sums (experts, cols) float32 and their numbers to
     counts (experts,) int64. which (rows, each) int32 holds the experts of each row; without it there is one sum
-    over all rows. An importance matrix is sums / counts (imatrix.load of its "in_sum2" and "counts")."""
+    over all rows. An importance matrix is sums / counts, and 1 for an expert without rows, as
+    imatrix.load reads "in_sum2" and "counts"; imatrix.write_dat makes a file of it."""
     kind, m, k, ld = _rows("x", x, x_stride)
     experts = each = 0
     if which is not None:

@@ -4,6 +4,7 @@ finite and whom they may reach, the largest and the least inputs, and what the f
 Tolerances are those of test_linear_gpu (an output's rounding, K 2^-24 T for float32 sums of K terms, T the sum over
 absolute values, and what a form's operands lose), with the operands' part named by each test."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -389,6 +390,31 @@ def test_streams_that_end():
         del out, st
     linear.release()
     close(linear.project(xd, w).to_host(), y, slack(total, k), BF16)
+
+
+def test_threads_at_once():
+    """two threads, each with a stream of its own, many and few rows in turn: every result as alone"""
+    g = rng(56)
+    n, k = 300, 1024
+    w, _ = weights(g, 12, n, k)
+    x = {m: inputs(g, m, k, BF16)[0] for m in (3, 140, 300)}
+    want = {m: linear.project(up(a), w).to_host() for m, a in x.items()}
+    wrong = []
+
+    def work():
+        st = dev.Stream()
+        arrays = {m: dev.DeviceArray.from_host(a, st.handle) for m, a in x.items()}
+        for _ in range(8):
+            got = {m: linear.project(a, w, stream=st.handle) for m, a in arrays.items()}
+            wrong.extend(m for m, a in got.items() if not np.array_equal(a.to_host(stream=st.handle), want[m]))
+        linear.release()
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 class Graph:
