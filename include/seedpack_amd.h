@@ -602,6 +602,80 @@ int spa_add_squares(const void* x, int src_kind, int64_t rows, int64_t cols, int
                     int64_t each, int64_t experts, float* sums, int64_t* counts, void* work, uint64_t work_bytes, void* stream);
 uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts);
 
+/* ---- experts (no reference counterpart) ----
+ * Routing sends each row to `each` of `experts` experts: slot p = row * each + j is row's place j. Logits, rows of results and
+ * their gradients are BF16, F16 or F32 (SPA_SRC_*), numbers and weights of slots int32 and float32, dense. Nothing
+ * is allocated, and calls may be captured. `work` as with the products. Up to 1024 experts, 32 a row. */
+
+/* Each row's experts, the best first, and their weights. score 0: softmax over the row, 1: 1 / (1 + e^-l). The chosen
+ * have the largest keys: the logits, or, with a bias ([experts], or NULL) or more than one group, score + bias in 64 bits (keys
+ * whose first 42 bits agree count as equal). Of equal keys the lowest number wins, NaN is above all. With `groups`
+ * equal runs of experts only the `keep` best take part; a group is worth the sum of its `best` (1 or 2) highest keys. A
+ * logit of -infinity, or a key of it, is never chosen: where fewer than `each` are left, which is -1 and the weight 0.
+ * Weights are scale * score, with renorm divided by the row's chosen scores' sum. order and starts (both or neither)
+ * as spa_by_expert gives them. */
+int spa_route(const void* logits, int kind, int64_t rows, int64_t experts, int64_t stride, int score, const float* bias,
+              int64_t groups, int64_t keep, int64_t best, int64_t each, int renorm, float scale, int32_t* which,
+              float* weights, int32_t* order, int32_t* starts, void* work, uint64_t work_bytes, void* stream);
+uint64_t spa_route_work_bytes(int64_t rows, int64_t experts, int64_t each, int sorted);
+
+/* The logits' gradient (their type; every number is written) from the weights': through scores and, with renorm, their
+ * sum; the choice and the bias have none. which: as spa_route gave it (numbers outside 0..experts-1 are passed over). */
+int spa_route_backward(const void* logits, int kind, int64_t rows, int64_t experts, int64_t stride, int score, int64_t each,
+                       int renorm, float scale, const int32_t* which, const float* dweights, void* dlogits, int64_t dstride,
+                       void* stream);
+
+/* order: the slots in the order of their experts, those of one expert in their own; slots whose number lies outside
+ * 0..experts-1 come last. starts[e]: where e's begin, starts[experts]: their end ([experts + 1]). */
+int spa_by_expert(const int32_t* which, int64_t slots, int64_t experts, int32_t* order, int32_t* starts, void* work,
+                  uint64_t work_bytes, void* stream);
+uint64_t spa_by_expert_work_bytes(int64_t slots, int64_t experts);
+
+/* out[r] = sum_j weights[r][j] y[r * each + j], rows of n, float32 sums in j's order rounded once. which ([rows][each], or
+ * NULL): slots whose number lies outside 0..experts-1 are passed over, whatever y and weights hold there. */
+int spa_join(const void* y, int kind, int64_t rows, int64_t each, int64_t n, int64_t y_stride, const float* weights,
+             const int32_t* which, int64_t experts, void* out, int64_t out_stride, void* stream);
+
+/* Its gradients: dy[p] = weights[p] dout[row], dweights[p] = sum dout[row] y[p]; zeros for slots that are passed over. */
+int spa_join_backward(const void* y, int kind, int64_t rows, int64_t each, int64_t n, int64_t y_stride, const float* weights,
+                      const int32_t* which, int64_t experts, const void* dout, int64_t dout_stride, void* dy,
+                      int64_t dy_stride, float* dweights, void* stream);
+
+/* ---- 4-bit floating point in microscaled blocks (no reference counterpart) ----
+ * A matrix of rows of `cols` numbers is codes ([rows][pitch][16 bytes], 16-byte aligned) and scales ([rows][pitch], 8-byte
+ * aligned), pitch = spa_mx4_pitch(cols) blocks of 32: cols / 256 rounded up, times 8. Block b of a row holds its
+ * numbers 32 b to 32 b + 31: j in the low half of byte j, j + 16 in the high half (as GGUF's MXFP4 does). A code is a sign
+ * and 0 .5 1 1.5 2 3 4 6, a scale s stands for 2^(s - 127), 255 for a block of NaN. Blocks behind a row's last number are
+ * zeros, codes and scales. Up to 4,000,000 columns. Nothing is allocated, and calls may be captured. */
+int64_t spa_mx4_pitch(int64_t cols);
+
+/* x (BF16, F16 or F32) to blocks along its rows, or, across, along its columns: the matrix of x^T, cols rows of `rows`.
+ * A block's scale is 2^(floor(log2 max|x|) - 2), not below 2^-127; numbers are rounded to nearest, ties to even codes,
+ * and held at 6. A block with an infinity or a NaN is a block of NaN. */
+int spa_mx4_quantize(const void* x, int kind, int64_t rows, int64_t cols, int64_t stride, int across, uint8_t* codes,
+                     uint8_t* scales, void* stream);
+/* The values, rounded once to BF16, F16 or F32. */
+int spa_mx4_values(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y, int kind, int64_t stride,
+                   void* stream);
+/* A matrix from GGUF's MXFP4 blocks (17 bytes, the scale first; cols a multiple of 32), at any byte. */
+int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales, void* stream);
+
+/* y = x w^T of two 4-bit matrices, x of x_rows rows and w of n, both of k: products are exact, sums float32, an
+ * output is rounded once to BF16, F16 or F32. experts = 0: one w for all rows (order and starts are not read,
+ * slots is x_rows). Else w is `experts` matrices one behind another, order and starts are spa_by_expert's for `slots` slots,
+ * a multiple of x_rows: slot p is row p of y, from row p / (slots / x_rows) of x. Rows of slots without an expert are left as
+ * they are. Numbers of order or starts out of range read or write nothing outside the arrays. */
+int spa_mx4_project(const uint8_t* x_codes, const uint8_t* x_scales, int64_t x_rows, int64_t k, const uint8_t* w_codes,
+                    const uint8_t* w_scales, int64_t n, int64_t experts, const int32_t* order, const int32_t* starts, int64_t slots,
+                    void* y, int y_kind, int64_t y_stride, void* work, uint64_t work_bytes, void* stream);
+/* h = act(x gate^T) * (x up^T), act 0: silu, 1: gelu (tanh form). */
+int spa_mx4_gated(const uint8_t* x_codes, const uint8_t* x_scales, int64_t x_rows, int64_t k, const uint8_t* gate_codes,
+                  const uint8_t* gate_scales, const uint8_t* up_codes, const uint8_t* up_scales, int64_t n, int act, int64_t experts,
+                  const int32_t* order, const int32_t* starts, int64_t slots, void* h, int h_kind, int64_t h_stride, void* work,
+                  uint64_t work_bytes, void* stream);
+/* Scratch of both (gated: 1 for two matrices): device memory, 256-byte aligned, as with the products above. */
+uint64_t spa_mx4_product_work_bytes(int64_t x_rows, int64_t k, int64_t n, int64_t experts, int64_t slots, int gated);
+
 #ifdef __cplusplus
 }
 #endif

@@ -179,6 +179,26 @@ SIGNATURES = {
     "spa_add_squares": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                 c_void_p, c_void_p, c_uint64, c_void_p]),
     "spa_add_squares_work_bytes": (c_uint64, [c_int64, c_int64, c_int64]),
+    "spa_route": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,
+                          c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint64, c_void_p]),
+    "spa_route_work_bytes": (c_uint64, [c_int64, c_int64, c_int64, c_int]),
+    "spa_route_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_void_p,
+                                   c_void_p, c_int64, c_void_p]),
+    "spa_by_expert": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_uint64, c_void_p]),
+    "spa_by_expert_work_bytes": (c_uint64, [c_int64, c_int64]),
+    "spa_join": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                         c_void_p]),
+    "spa_join_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                  c_void_p, c_int64, c_void_p, c_void_p]),
+    "spa_mx4_pitch": (c_int64, [c_int64]),
+    "spa_mx4_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "spa_mx4_values": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p]),
+    "spa_mx4_from_blocks": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "spa_mx4_project": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                c_int64, c_void_p, c_int, c_int64, c_void_p, c_uint64, c_void_p]),
+    "spa_mx4_gated": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64,
+                              c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p, c_uint64, c_void_p]),
+    "spa_mx4_product_work_bytes": (c_uint64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
 }
 
 

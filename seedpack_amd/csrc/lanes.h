@@ -1,0 +1,57 @@
+// Reductions over 16 or 64 neighbouring lanes whose result every lane holds, by moves between lanes that need no LDS.
+#pragma once
+
+#include "common.h"
+
+namespace spa {
+
+template <int CTRL> __device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL, typename T> __device__ __forceinline__ T lane_move(T v) {
+    if constexpr (sizeof(T) == 8) {
+        uint64_t b;
+        __builtin_memcpy(&b, &v, 8);
+        b = (uint64_t)moved<CTRL>((uint32_t)(b >> 32)) << 32 | moved<CTRL>((uint32_t)b);
+        __builtin_memcpy(&v, &b, 8);
+    } else {
+        uint32_t b;
+        __builtin_memcpy(&b, &v, 4);
+        b = moved<CTRL>(b);
+        __builtin_memcpy(&v, &b, 4);
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ T lane_xor(T v, int mask) {
+    if constexpr (sizeof(T) == 8) {
+        uint64_t b;
+        __builtin_memcpy(&b, &v, 8);
+        b = (uint64_t)(uint32_t)__shfl_xor((int)(b >> 32), mask) << 32 | (uint32_t)__shfl_xor((int)b, mask);
+        __builtin_memcpy(&v, &b, 8);
+        return v;
+    } else {
+        return __shfl_xor(v, mask);
+    }
+}
+
+// op over the L = 16 or 64 lanes of a row, in an order of its own that is the same for every lane: neighbours, pairs,
+// and, the pairs being alike, mirrored fours and eights.
+template <int L, typename T, typename F> __device__ __forceinline__ T over_row(T v, F op) {
+    v = op(v, lane_move<0xb1>(v));                               // lanes 1 0 3 2
+    v = op(v, lane_move<0x4e>(v));                               // lanes 2 3 0 1
+    v = op(v, lane_move<0x141>(v));                              // eight lanes mirrored
+    v = op(v, lane_move<0x140>(v));                              // sixteen lanes mirrored
+    if constexpr (L == 64) {
+        v = op(v, lane_xor(v, 16));
+        v = op(v, lane_xor(v, 32));
+    }
+    return v;
+}
+template <int L, typename T> __device__ __forceinline__ T row_sum(T v) {
+    return over_row<L>(v, [](T a, T b) { return a + b; });
+}
+template <int L, typename T> __device__ __forceinline__ T row_max(T v) {
+    return over_row<L>(v, [](T a, T b) { return a > b ? a : b; });
+}
+
+}  // namespace spa

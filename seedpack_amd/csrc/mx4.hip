@@ -1,0 +1,359 @@
+// Numbers to 4-bit floating point in microscaled blocks, and back.
+//
+// A block's scale is 2^e, e = floor(log2(its largest magnitude)) - 2 and not below -127, so that the largest lies
+// in [4, 8) units; each number is rounded to the nearest of the grid, ties to the even code, and held at 6 units (the
+// microscaling formats' published rule). The hardware's conversions do exactly that for every float and every scale.
+// e comes from the float's exponent field: the scale's byte is that field less 2.
+//
+// Bound by memory: four lanes share a block, eight numbers each (16 bytes of 16-bit numbers a lane), and change
+// their codes between pairs of lanes, so that loads and stores both are whole lines.
+#include "../../include/seedpack_amd.h"
+#include "lanes.h"
+#include "launch.h"
+#include "mx4.h"
+
+namespace spa {
+namespace mx {
+namespace {
+
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+template <int KIND> __device__ __forceinline__ float wide_at(const void* p, int64_t i) {
+    if constexpr (KIND == SRC_F32) return static_cast<const float*>(p)[i];
+    else return lin::wide(static_cast<const uint16_t*>(p)[i], KIND);
+}
+template <int KIND> __device__ __forceinline__ void put(void* p, int64_t i, float v) {
+    if constexpr (KIND == SRC_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = lin::narrow(v, KIND);
+}
+
+// the scale's byte of a block whose largest magnitude is `top`
+__device__ __forceinline__ uint32_t scale_byte(float top) {
+    const int field = (int)(__float_as_uint(top) >> 23);
+    return field == 255 ? 255u : (uint32_t)tmax(field - 2, 0);
+}
+// the largest magnitude; infinities and NaN stay above all
+__device__ __forceinline__ float larger(float a, float b) {
+    return __uint_as_float(tmax(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+}
+// eight numbers' codes, the first lowest; a block of NaN has codes 0
+__device__ __forceinline__ uint32_t codes8(const float (&x)[8], uint32_t byte) {
+    const float scale = __uint_as_float(byte << 23);
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], scale, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], scale, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
+    return byte == 255 ? 0u : c;
+}
+// four codes in the low halves of four bytes
+__device__ __forceinline__ uint32_t spread(uint32_t v) {
+    v = (v | v << 8) & 0x00ff00ffu;
+    return (v | v << 4) & 0x0f0f0f0fu;
+}
+
+// eight numbers of a row at column c, zeros behind its last
+template <int KIND> __device__ __forceinline__ void load8(const void* x, int64_t at, int64_t left, bool wide, float (&v)[8]) {
+    if (wide && left >= 8) {
+        if constexpr (KIND == SRC_F32) {
+            const u4v* p = reinterpret_cast<const u4v*>(static_cast<const float*>(x) + at);
+            const u4v a = p[0], b = p[1];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) { v[c] = __uint_as_float(a[c]); v[4 + c] = __uint_as_float(b[c]); }
+        } else {
+            const u4v a = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(x) + at);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = lin::wide((a[c >> 1] >> (16 * (c & 1))) & 0xffffu, KIND);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = c < left ? wide_at<KIND>(x, at + c) : 0.f;
+    }
+}
+
+struct Rows {
+    const void* x;
+    int64_t rows, cols, stride;
+    int pitch;
+    bool wide;
+    uint8_t *codes, *scales;
+};
+
+template <int KIND>
+__global__ __launch_bounds__(256) void k_quantize(const Rows a) {
+    const int64_t per = (int64_t)a.pitch * 4, id = blockIdx.x * 256ll + threadIdx.x;
+    const int64_t row = id / per;
+    if (row >= a.rows) return;                                    // whole blocks of lanes: per is a multiple of 4
+    const int64_t quarter = id - row * per, c = quarter * 8;
+    float v[8];
+    load8<KIND>(a.x, row * a.stride + c, a.cols - c, a.wide, v);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = larger(top, v[i]);
+    top = larger(top, lane_move<0xb1>(top));
+    top = larger(top, lane_move<0x4e>(top));
+    const uint32_t byte = scale_byte(top), mine = codes8(v, byte), other = moved<0x4e>(mine);
+    // lanes 0 and 2 hold numbers 0-7 and 16-23 of the block: bytes 0-7; lanes 1 and 3 the rest
+    const int q = threadIdx.x & 3;
+    const bool upper = q >= 2;
+    const uint32_t lo = upper ? other >> 16 : mine & 0xffffu, hi = upper ? mine >> 16 : other & 0xffffu;
+    const int64_t block = id >> 2;
+    reinterpret_cast<uint32_t*>(a.codes)[block * 4 + (q & 1) * 2 + (q >> 1)] = spread(lo) | spread(hi) << 4;
+    if (q == 0) a.scales[block] = (uint8_t)byte;
+}
+
+// Blocks along columns: the matrix of x^T. A workgroup takes 64 columns of 256 rows, a lane a column of 32 of them; the
+// codes leave by way of LDS, 128 bytes of a column at a time.
+template <int KIND>
+__global__ __launch_bounds__(512) void k_quantize_across(const Rows a) {
+    __shared__ __align__(16) uint32_t codes[64][33];
+    __shared__ uint8_t scales[64][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c0 = (int64_t)blockIdx.y * 64, c = c0 + lane, r0 = (int64_t)blockIdx.x * 256 + wave * 32;
+    const bool in = c < a.cols;
+    float v[32], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = in && r0 + i < a.rows ? wide_at<KIND>(a.x, (r0 + i) * a.stride + c) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = larger(top, v[i]);
+    const uint32_t byte = scale_byte(top);
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float part[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[j] = v[8 * i + j];
+        q[i] = codes8(part, byte);
+    }
+    codes[lane][wave * 4 + 0] = spread(q[0] & 0xffffu) | spread(q[2] & 0xffffu) << 4;
+    codes[lane][wave * 4 + 1] = spread(q[0] >> 16) | spread(q[2] >> 16) << 4;
+    codes[lane][wave * 4 + 2] = spread(q[1] & 0xffffu) | spread(q[3] & 0xffffu) << 4;
+    codes[lane][wave * 4 + 3] = spread(q[1] >> 16) | spread(q[3] >> 16) << 4;
+    scales[lane][wave] = (uint8_t)byte;
+    __syncthreads();
+    for (int u = threadIdx.x; u < 64 * 32; u += 512) {
+        const int64_t to = c0 + u / 32;
+        if (to < a.cols) reinterpret_cast<uint32_t*>(a.codes)[(to * a.pitch + blockIdx.x * 8) * 4 + u % 32] = codes[u / 32][u % 32];
+    }
+    for (int u = threadIdx.x; u < 64 * 8; u += 512) {
+        const int64_t to = c0 + u / 8;
+        if (to < a.cols) a.scales[to * a.pitch + blockIdx.x * 8 + u % 8] = scales[u / 8][u % 8];
+    }
+}
+
+struct Values {
+    const uint8_t *codes, *scales;
+    int64_t rows, cols, stride;
+    int pitch;
+    bool wide;
+    void* y;
+};
+
+// A lane takes 4 bytes of a block: numbers 4 q .. 4 q + 3 and those 16 behind
+template <int KIND>
+__global__ __launch_bounds__(256) void k_values(const Values a) {
+    const int64_t per = (a.cols + 31) / 32 * 4, id = blockIdx.x * 256ll + threadIdx.x;
+    const int64_t row = id / per;
+    if (row >= a.rows) return;
+    const int64_t quarter = id - row * per, block = row * a.pitch + (quarter >> 2);
+    const int q = (int)(quarter & 3);
+    const uint32_t v = reinterpret_cast<const uint32_t*>(a.codes)[block * 4 + q];
+    const float scale = __uint_as_float((uint32_t)a.scales[block] << 23);
+    const f2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 1),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 3)};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t c = (quarter >> 2) * 32 + 16 * h + 4 * q, at = row * a.stride + c;
+        if (a.wide && c + 4 <= a.cols) {
+            if constexpr (KIND == SRC_F32) {
+                *reinterpret_cast<lin::f4*>(static_cast<float*>(a.y) + at) = lin::f4{p[0][h], p[1][h], p[2][h], p[3][h]};
+            } else {
+                *reinterpret_cast<lin::u2*>(static_cast<uint16_t*>(a.y) + at) = lin::u2{lin::narrow2(p[0][h], p[1][h], KIND), lin::narrow2(p[2][h], p[3][h], KIND)};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < a.cols) put<KIND>(a.y, at + i, p[i][h]);
+        }
+    }
+}
+
+// GGUF blocks, a scale's byte before 16 bytes of codes, taken apart: a lane 4 bytes of a block
+__global__ __launch_bounds__(256) void k_from_blocks(const uint8_t* b, int64_t rows, int64_t blocks, int pitch, uint8_t* codes, uint8_t* scales) {
+    const int64_t per = (int64_t)pitch * 4, id = blockIdx.x * 256ll + threadIdx.x, row = id / per;
+    if (row >= rows) return;
+    const int64_t block = (id - row * per) >> 2;
+    const int q = threadIdx.x & 3;
+    uint32_t v = 0;
+    uint8_t s = 0;
+    if (block < blocks) {
+        const uint8_t* p = b + (row * blocks + block) * 17;
+        __builtin_memcpy(&v, p + 1 + 4 * q, 4);
+        s = p[0];
+    }
+    reinterpret_cast<uint32_t*>(codes)[id] = v;
+    if (q == 0) scales[id >> 2] = s;
+}
+
+bool on(const void* p, uintptr_t unit) { return (reinterpret_cast<uintptr_t>(p) & (unit - 1)) == 0; }
+constexpr int64_t MOST_COLS = 4000000;
+
+int check_kind(const char* who, int kind) {
+    if (kind != SPA_SRC_BF16 && kind != SPA_SRC_F16 && kind != SPA_SRC_F32) return fail(SPA_ERR_TYPE, "%s: numbers of kind %d (BF16, F16 and F32 are taken)", who, kind);
+    return SPA_OK;
+}
+// a matrix of `rows` rows of `cols`; its codes and scales where given
+int check_matrix(const char* who, int64_t rows, int64_t cols, const void* codes, const void* scales) {
+    if (rows < 0 || cols < 1 || cols > MOST_COLS || rows > INT32_MAX - 1024 || rows * pitch_of(cols) * 4 / 256 >= INT32_MAX) return fail(SPA_ERR_ARG, "%s: bad shape %lld x %lld", who, (long long)rows, (long long)cols);
+    if (rows && (!codes || !scales)) return fail(SPA_ERR_ARG, "%s: a pointer is NULL", who);
+    if (!on(codes, 16) || !on(scales, 8)) return fail(SPA_ERR_ARG, "%s: codes have to be 16-byte aligned, scales 8-byte aligned", who);
+    return SPA_OK;
+}
+
+}  // namespace
+}  // namespace mx
+}  // namespace spa
+
+using namespace spa;
+using namespace spa::mx;
+
+extern "C" {
+
+int64_t spa_mx4_pitch(int64_t cols) { return cols < 1 || cols > MOST_COLS ? 0 : pitch_of(cols); }
+
+int spa_mx4_quantize(const void* x, int kind, int64_t rows, int64_t cols, int64_t stride, int across, uint8_t* codes,
+                     uint8_t* scales, void* stream) {
+    if (int rc = check_kind("mx4_quantize", kind)) return rc;
+    if (across && rows < 1) return fail(SPA_ERR_ARG, "mx4_quantize: columns of %lld numbers", (long long)rows);
+    if (int rc = check_matrix("mx4_quantize", across ? cols : rows, across ? rows : cols, codes, scales)) return rc;
+    if (cols < 1 || stride < cols) return fail(SPA_ERR_ARG, "mx4_quantize: rows of %lld at a stride of %lld", (long long)cols, (long long)stride);
+    if (!rows) return SPA_OK;
+    if (!x) return fail(SPA_ERR_ARG, "mx4_quantize: a pointer is NULL");
+    Rows a{x, rows, cols, stride, (int)pitch_of(across ? rows : cols), on(x, 16) && stride % (kind == SPA_SRC_F32 ? 4 : 8) == 0, codes, scales};
+    hipStream_t st = (hipStream_t)stream;
+    if (across) {
+        const int64_t strips = (cols + 63) / 64;
+        for (int64_t y0 = 0; y0 < strips; y0 += 65535) {          // a launch's second dimension is limited
+            Rows b = a;
+            const int64_t skip = y0 * 64;
+            b.x = static_cast<const char*>(x) + skip * (kind == SPA_SRC_F32 ? 4 : 2);
+            b.cols = cols - skip;
+            b.codes = codes + skip * a.pitch * 16;
+            b.scales = scales + skip * a.pitch;
+            const dim3 grid((unsigned)(a.pitch / 8), (unsigned)(strips - y0 < 65535 ? strips - y0 : 65535));
+            if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_quantize_across<SRC_BF16>, grid, dim3(512), 0, st, b);
+            else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_quantize_across<SRC_F16>, grid, dim3(512), 0, st, b);
+            else hipLaunchKernelGGL(k_quantize_across<SRC_F32>, grid, dim3(512), 0, st, b);
+            SPA_HIP_TRY(hipGetLastError());
+        }
+        return SPA_OK;
+    }
+    const dim3 grid((unsigned)((rows * a.pitch * 4 + 255) / 256));
+    if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_quantize<SRC_BF16>, grid, dim3(256), 0, st, a);
+    else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_quantize<SRC_F16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_quantize<SRC_F32>, grid, dim3(256), 0, st, a);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+int spa_mx4_values(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y, int kind, int64_t stride,
+                   void* stream) {
+    if (int rc = check_kind("mx4_values", kind)) return rc;
+    if (int rc = check_matrix("mx4_values", rows, cols, codes, scales)) return rc;
+    if (stride < cols) return fail(SPA_ERR_ARG, "mx4_values: rows of %lld at a stride of %lld", (long long)cols, (long long)stride);
+    if (!rows) return SPA_OK;
+    if (!y) return fail(SPA_ERR_ARG, "mx4_values: a pointer is NULL");
+    Values a{codes, scales, rows, cols, stride, (int)pitch_of(cols), on(y, kind == SPA_SRC_F32 ? 16 : 8) && stride % 4 == 0, y};
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)((rows * ((cols + 31) / 32) * 4 + 255) / 256));
+    if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_values<SRC_BF16>, grid, dim3(256), 0, st, a);
+    else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_values<SRC_F16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_values<SRC_F32>, grid, dim3(256), 0, st, a);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales, void* stream) {
+    if (int rc = check_matrix("mx4_from_blocks", rows, cols, codes, scales)) return rc;
+    if (cols % 32) return fail(SPA_ERR_ARG, "mx4_from_blocks: rows of %lld are not whole blocks of 32", (long long)cols);
+    if (!rows) return SPA_OK;
+    if (!blocks) return fail(SPA_ERR_ARG, "mx4_from_blocks: a pointer is NULL");
+    const int64_t pitch = pitch_of(cols);
+    hipLaunchKernelGGL(k_from_blocks, dim3((unsigned)((rows * pitch * 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                       (const uint8_t*)blocks, rows, cols / 32, (int)pitch, codes, scales);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
+}
+
+namespace {
+
+// one of the products: checked, then launched
+int product(const char* who, Product p, int64_t x_rows, int64_t k, int64_t n, int64_t experts, const int32_t* order, const int32_t* starts,
+            int64_t slots, int64_t y_stride, void* work, uint64_t work_bytes, hipStream_t st) {
+    if (int rc = check_kind(who, p.kind)) return rc;
+    if (int rc = check_matrix(who, x_rows, k, p.xc, p.xs)) return rc;
+    if (experts < 0 || experts > 1024 || n < 0 || n > INT32_MAX - 1024) return fail(SPA_ERR_ARG, "%s: %lld experts of %lld outputs (up to 1024 experts)", who, (long long)experts, (long long)n);
+    if (int rc = check_matrix(who, n, k, p.w0c, p.w0s)) return rc;
+    if ((p.w1c || p.w1s) && check_matrix(who, n, k, p.w1c, p.w1s)) return SPA_ERR_ARG;
+    const int64_t m = experts ? slots : x_rows;
+    if (m < 0 || m > INT32_MAX - 1024 || y_stride < n) return fail(SPA_ERR_ARG, "%s: bad shape %lld x %lld, stride %lld", who, (long long)m, (long long)n, (long long)y_stride);
+    if (m == 0 || n == 0) return SPA_OK;
+    if (!p.y) return fail(SPA_ERR_ARG, "%s: a pointer is NULL", who);
+    p.pitch = (int)pitch_of(k);
+    p.m = (int)m;
+    p.n = (int)n;
+    p.ldy = y_stride;
+    p.each = 1;
+    if (experts) {
+        if (!order || !starts) return fail(SPA_ERR_ARG, "%s: order and starts are needed beside experts", who);
+        if (x_rows == 0 || slots % x_rows) return fail(SPA_ERR_ARG, "%s: %lld slots of %lld rows", who, (long long)slots, (long long)x_rows);
+        // rows are read at 32-bit offsets from the matrix's first
+        if (x_rows * p.pitch * 16 >= (1ll << 32)) return fail(SPA_ERR_ARG, "%s: %lld rows of %lld by expert are more than 4 GiB of codes", who, (long long)x_rows, (long long)k);
+        p.each = (int)(slots / x_rows);
+        p.experts = (int)experts;
+        p.order = order;
+        p.starts = starts;
+    }
+    return product_few(p, st);
+}
+
+}  // namespace
+
+uint64_t spa_mx4_product_work_bytes(int64_t x_rows, int64_t k, int64_t n, int64_t experts, int64_t slots, int gated) {
+    return 0;
+}
+
+int spa_mx4_project(const uint8_t* x_codes, const uint8_t* x_scales, int64_t x_rows, int64_t k, const uint8_t* w_codes,
+                    const uint8_t* w_scales, int64_t n, int64_t experts, const int32_t* order, const int32_t* starts, int64_t slots,
+                    void* y, int y_kind, int64_t y_stride, void* work, uint64_t work_bytes, void* stream) {
+    Product p{};
+    p.xc = x_codes;
+    p.xs = x_scales;
+    p.w0c = w_codes;
+    p.w0s = w_scales;
+    p.y = y;
+    p.kind = y_kind;
+    return product("mx4_project", p, x_rows, k, n, experts, order, starts, slots, y_stride, work, work_bytes, (hipStream_t)stream);
+}
+
+int spa_mx4_gated(const uint8_t* x_codes, const uint8_t* x_scales, int64_t x_rows, int64_t k, const uint8_t* gate_codes,
+                  const uint8_t* gate_scales, const uint8_t* up_codes, const uint8_t* up_scales, int64_t n, int act, int64_t experts,
+                  const int32_t* order, const int32_t* starts, int64_t slots, void* h, int h_kind, int64_t h_stride, void* work,
+                  uint64_t work_bytes, void* stream) {
+    if (act != 0 && act != 1) return fail(SPA_ERR_ARG, "mx4_gated: unknown activation %d", act);
+    if (n && (!up_codes || !up_scales)) return fail(SPA_ERR_ARG, "mx4_gated: a pointer is NULL");
+    Product p{};
+    p.xc = x_codes;
+    p.xs = x_scales;
+    p.w0c = gate_codes;
+    p.w0s = gate_scales;
+    p.w1c = up_codes;
+    p.w1s = up_scales;
+    p.act = act;
+    p.y = h;
+    p.kind = h_kind;
+    return product("mx4_gated", p, x_rows, k, n, experts, order, starts, slots, h_stride, work, work_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"
