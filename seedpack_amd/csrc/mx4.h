@@ -26,9 +26,12 @@ struct Product {
     void* y;
     int64_t ldy;
     int kind, act;
+    int pieces;                          // of k, whose float32 sums are joined by a second launch; 1: none
+    float* part;                         // [pieces, of the gate's and of the up projection][m][n]
 };
 
-int product_few(const Product& p, hipStream_t st);
+int product_few(const Product& p, bool wide, hipStream_t st);
+int product_many(const Product& p, bool large, hipStream_t st);
 
 }  // namespace mx
 }  // namespace spa

@@ -12,6 +12,8 @@
 #include "launch.h"
 #include "mx4.h"
 
+#include <math.h>
+
 namespace spa {
 namespace mx {
 namespace {
@@ -288,6 +290,52 @@ int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t*
 
 namespace {
 
+// What a product takes, by the forms' times on one MI355X, in us:
+//   FEW16, FEW32  16 x 16 and 32 x 32 outputs a wave: 3.3 and 6.0 for a launch, then 6.6 and 6.9 for 26.7 MB of weights, which
+//                 each tile of 16 or 32 rows reads again
+//   SMALL         128 x 128 tiles: 4.5 and 0.74 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
+//                 in pieces of k, where there are too few tiles: 2.5 for the joining launch and 5 TB/s for its sums
+//   LARGE         256 x 256 tiles, one to a compute unit: 7 and 1.95 a step (1.5 with most units idle)
+// k = 4096 of 12288 outputs, us:  rows  16: 9.8 11.4 14.7 20.3   32: 16.5 13.2 15.3 21.3   64: 29.3 18.3 16.4 23.1
+//   128: 55 32 17.9 24.5   256: 107 62 18.4 30.5   4096: - - 136 112;   k = 12288 of 4096, SMALL whole and in 4 pieces:
+//   64: 37.5 17.1   256: 41.9 23.3   512: 42.3 31.7.
+// By expert the rows' spread is not known on the host: half of the experts that have any are taken to end in a tile of their
+// own.
+enum Form { FEW16, FEW32, SMALL, LARGE };
+struct Plan {
+    int form, pieces;
+};
+Plan plan(int64_t m, int64_t n, int64_t pitch, int64_t experts, bool gated) {
+    const double steps = (double)pitch / 8, sides = gated ? 2 : 1, mb = (double)n * pitch * 17 * sides * 1e-6 / 26.7;
+    const int64_t used = experts && experts < m ? experts : experts ? m : 0;
+    auto rows = [&](int64_t t) { return experts ? (double)(m / t) + (used + 1) / 2 : (double)((m + t - 1) / t); };
+    auto small = [&](double tiles, double k) { return tiles <= 256 ? 4.5 + 0.74 * k : ceil(tiles / 512) * (5 + 1.19 * k); };
+    Plan best{FEW16, 1};
+    double least = 3.3 + 6.6 * rows(16) * mb;
+    auto take = [&](int form, int pieces, double us) {
+        if (us < least) {
+            best = Plan{form, pieces};
+            least = us;
+        }
+    };
+    take(FEW32, 1, 6.0 + 6.9 * rows(32) * mb);
+    const double wide = ceil(n * sides / 128.0), tiles = wide * rows(128);
+    take(SMALL, 1, small(tiles, steps));
+    for (int p = 2; p <= 8 && 2 * p <= steps; ++p)
+        take(SMALL, p, small(tiles * p, ceil(steps / p)) + 2.5 + (double)m * n * 8 * p * sides / 5e6);
+    const double large = ceil(n * sides / 256.0) * rows(256);
+    take(LARGE, 1, ceil(large / 256) * (7 + (large <= 64 ? 1.5 : 1.95) * steps));
+    return best;
+}
+uint64_t part_bytes(const Plan& c, int64_t m, int64_t n, bool gated) {
+    return c.pieces > 1 ? ((uint64_t)c.pieces * (gated ? 2 : 1) * m * n * 4 + 255) / 256 * 256 : 0;
+}
+int check_work(const char* who, const void* work, uint64_t have, uint64_t need) {
+    if (need && (!work || !on(work, 256) || have < need))
+        return fail(SPA_ERR_ARG, "%s: needs a 256-byte aligned workspace of %llu bytes, got %llu", who, (unsigned long long)need, (unsigned long long)(work ? have : 0));
+    return SPA_OK;
+}
+
 // one of the products: checked, then launched
 int product(const char* who, Product p, int64_t x_rows, int64_t k, int64_t n, int64_t experts, const int32_t* order, const int32_t* starts,
             int64_t slots, int64_t y_stride, void* work, uint64_t work_bytes, hipStream_t st) {
@@ -315,13 +363,19 @@ int product(const char* who, Product p, int64_t x_rows, int64_t k, int64_t n, in
         p.order = order;
         p.starts = starts;
     }
-    return product_few(p, st);
+    const Plan c = plan(p.m, p.n, p.pitch, p.experts, p.w1c != nullptr);
+    if (int rc = check_work(who, work, work_bytes, part_bytes(c, p.m, p.n, p.w1c != nullptr))) return rc;
+    p.pieces = c.pieces;
+    p.part = (float*)work;
+    return c.form <= FEW32 ? product_few(p, c.form == FEW32, st) : product_many(p, c.form == LARGE, st);
 }
 
 }  // namespace
 
 uint64_t spa_mx4_product_work_bytes(int64_t x_rows, int64_t k, int64_t n, int64_t experts, int64_t slots, int gated) {
-    return 0;
+    const int64_t m = experts > 0 ? slots : x_rows;
+    if (m <= 0 || m > INT32_MAX - 1024 || n <= 0 || n > INT32_MAX - 1024 || k < 1 || k > MOST_COLS || experts > 1024) return 0;
+    return part_bytes(plan(m, n, pitch_of(k), experts > 0 ? experts : 0, gated), m, n, gated);
 }
 
 int spa_mx4_project(const uint8_t* x_codes, const uint8_t* x_scales, int64_t x_rows, int64_t k, const uint8_t* w_codes,

@@ -1,9 +1,11 @@
 // Products of few 4-bit rows with 4-bit weights: the weights are read once, straight into the matrix instruction.
 //
-// A workgroup's waves share 16 weight rows and take 512 of k in turn; a lane reads 64 bytes of its row's codes and the four
-// scales of them as one word, whose bytes the instruction picks. Which 32 of k an instruction's quarter of lanes
+// A wave takes 16 NT weight rows and 16 MT input rows, 512 of k at a time: a lane reads 64 bytes of its row's codes and the
+// four scales of them as one word, whose bytes the instruction picks. Which 32 of k an instruction's quarter of lanes
 // holds does not matter as long as inputs and weights agree: quarter g of the lanes holds blocks 4 g + u, in
-// instruction u. The waves' sums are added in LDS.
+// instruction u. (Whole lines in each load, a block a lane, need two words of scales and shifts: 8.4 us for one row of
+// 12288 x 4096, not 7.4.) Of a workgroup's eight waves `split` share their rows and take the pieces of k in turn, so that a
+// short row's loads are all under way at once; their sums are added in LDS.
 #include "../../include/seedpack_amd.h"
 #include "launch.h"
 #include "mx4.h"
@@ -19,22 +21,16 @@ using lin::u4;
 
 __device__ __forceinline__ v8i operand(u4 v) { return v8i{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
 
-// a row's 512 of k: 64 bytes of a lane's codes, and their scales; blocks behind the row's last are zeros
+// 512 of a row's k: 64 bytes of a lane's codes, and their scales
 struct Part {
     u4 codes[4];
     uint32_t scales;
 };
-__device__ __forceinline__ Part load_part(const uint8_t* codes, const uint8_t* scales, int block, int pitch) {
+__device__ __forceinline__ Part load_part(const uint8_t* codes, const uint8_t* scales, int block) {
     Part p;
-    if (block < pitch) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) p.codes[u] = *reinterpret_cast<const u4*>(codes + (block + u) * 16);
-        p.scales = *reinterpret_cast<const uint32_t*>(scales + block);
-    } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) p.codes[u] = u4{0, 0, 0, 0};
-        p.scales = 0;
-    }
+    for (int u = 0; u < 4; ++u) p.codes[u] = *reinterpret_cast<const u4*>(codes + (block + u) * 16);
+    p.scales = *reinterpret_cast<const uint32_t*>(scales + block);
     return p;
 }
 __device__ __forceinline__ f4 multiply(const Part& w, const Part& x, f4 acc) {
@@ -46,54 +42,143 @@ __device__ __forceinline__ f4 multiply(const Part& w, const Part& x, f4 acc) {
 
 constexpr int W = 8;                                             // waves
 
-template <bool TWO>
-__global__ __launch_bounds__(W * 64) void k_few(const Product p) {
-    __shared__ f4 sums[W][1 + TWO][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int nt = (p.n + 15) / 16, n0 = blockIdx.x % nt * 16;
-    const Tile t = tile_at(p, blockIdx.x / nt, 16);
+template <int MT, int NT, bool TWO>
+__device__ __forceinline__ void few(const Product& p, int split) {
+    constexpr int SUMS = MT * NT * (1 + TWO);
+    __shared__ f4 sums[W][SUMS][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int width = W / split * 16 * NT, nt = (p.n + width - 1) / width;
+    const int part = wave % split, n0 = blockIdx.x % nt * width + wave / split * 16 * NT;
+    const Tile t = tile_at(p, blockIdx.x / nt, 16 * MT);
     if (t.rows == 0) return;
-    const int64_t wrow = (int64_t)t.expert * p.n + tmin(n0 + r, p.n - 1);
-    const int64_t xrow = input_row(p, t.first + tmin(r, t.rows - 1));
-    const uint8_t *wc = p.w0c + wrow * p.pitch * 16, *ws = p.w0s + wrow * p.pitch, *xc = p.xc + xrow * p.pitch * 16, *xs = p.xs + xrow * p.pitch;
-    const uint8_t *vc = TWO ? p.w1c + wrow * p.pitch * 16 : nullptr, *vs = TWO ? p.w1s + wrow * p.pitch : nullptr;
-    f4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-    for (int k = wave * 16; k < p.pitch; k += W * 16) {
-        const Part w = load_part(wc, ws, k + 4 * g, p.pitch), x = load_part(xc, xs, k + 4 * g, p.pitch);
-        a = multiply(w, x, a);
-        if (TWO) b = multiply(load_part(vc, vs, k + 4 * g, p.pitch), x, b);
-    }
-    sums[wave][0][lane] = a;
-    if (TWO) sums[wave][TWO][lane] = b;
-    __syncthreads();
-    if (wave) return;
-    for (int i = 1; i < W; ++i) {
-        a += sums[i][0][lane];
-        if (TWO) b += sums[i][TWO][lane];
-    }
-    // lane: input row r, weight rows 4 g + i
-    const int64_t row = r < t.rows ? output_row(p, t.first + r) : -1;
-    if (row < 0) return;
-    const int64_t to = row * p.ldy + n0 + 4 * g;
+    const int64_t row16 = (int64_t)p.pitch * 16;
+    const uint8_t *wc[NT][1 + TWO], *ws[NT][1 + TWO], *xc[MT], *xs[MT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (n0 + 4 * g + i >= p.n) continue;
-        const float v = TWO ? lin::act_value(a[i], p.act) * b[i] : a[i];
-        if (p.kind == SRC_F32) static_cast<float*>(p.y)[to + i] = v;
-        else static_cast<uint16_t*>(p.y)[to + i] = lin::narrow(v, p.kind);
+    for (int i = 0; i < NT; ++i) {
+        const int64_t row = (int64_t)t.expert * p.n + tmin(n0 + 16 * i + r, p.n - 1);
+        wc[i][0] = p.w0c + row * row16;
+        ws[i][0] = p.w0s + row * p.pitch;
+        if (TWO) {
+            wc[i][TWO] = p.w1c + row * row16;
+            ws[i][TWO] = p.w1s + row * p.pitch;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int64_t row = input_row(p, t.first + tmin(16 * j + r, t.rows - 1));
+        xc[j] = p.xc + row * row16;
+        xs[j] = p.xs + row * p.pitch;
+    }
+    f4 acc[1 + TWO][NT][MT];
+#pragma unroll
+    for (int s = 0; s <= TWO; ++s)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[s][i][j] = f4{0, 0, 0, 0};
+    for (int k = part * 16; k < p.pitch; k += split * 16) {
+        // blocks behind a row's last (half of a last piece): others in their place, inputs as zeros, no scale NaN
+        const int mine = k + 4 * g, block = tmin(mine, p.pitch - 4);
+        const uint32_t in = mine < p.pitch ? ~0u : 0u;
+        Part w[NT][1 + TWO], x[MT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int s = 0; s <= TWO; ++s) w[i][s] = load_part(wc[i][s], ws[i][s], block);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) x[j] = load_part(xc[j], xs[j], block);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int s = 0; s <= TWO; ++s) w[i][s].scales &= in;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            x[j].scales &= in;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[j].codes[u] &= in;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int s = 0; s <= TWO; ++s) acc[s][i][j] = multiply(w[i][s], x[j], acc[s][i][j]);
+        }
+    }
+    if (split > 1) {
+#pragma unroll
+        for (int s = 0; s <= TWO; ++s)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) sums[wave][(s * NT + i) * MT + j][lane] = acc[s][i][j];
+        __syncthreads();
+    }
+    // the waves of the same rows share their fragments among them
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            if ((i * MT + j) % split != part) continue;
+            f4 v[1 + TWO];
+#pragma unroll
+            for (int s = 0; s <= TWO; ++s) {
+                v[s] = acc[s][i][j];
+                if (split > 1) {
+                    v[s] = f4{0, 0, 0, 0};
+                    for (int o = 0; o < split; ++o) v[s] += sums[wave - part + o][(s * NT + i) * MT + j][lane];
+                }
+            }
+            // lane: input row r, weight rows 4 g + c
+            const int64_t row = 16 * j + r < t.rows ? output_row(p, t.first + 16 * j + r) : -1;
+            const int n = n0 + 16 * i + 4 * g;
+            if (row < 0 || n >= p.n) continue;
+            const int64_t to = row * p.ldy + n;
+            if (TWO) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[0][c] = lin::act_value(v[0][c], p.act) * v[TWO][c];
+            }
+            if (p.kind == SRC_F32) {
+                float* const y = static_cast<float*>(p.y) + to;
+                if (n + 4 <= p.n) {
+                    __builtin_memcpy(y, &v[0], 16);               // at any number's address
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (n + c < p.n) y[c] = v[0][c];
+                }
+            } else {
+                uint16_t* const y = static_cast<uint16_t*>(p.y) + to;
+                const lin::u2 h = {lin::narrow2(v[0][0], v[0][1], p.kind), lin::narrow2(v[0][2], v[0][3], p.kind)};
+                if (n + 4 <= p.n) {
+                    __builtin_memcpy(y, &h, 8);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (n + c < p.n) y[c] = (uint16_t)(h[c >> 1] >> (16 * (c & 1)));
+                }
+            }
+        }
+}
+
+template <int MT, int NT, bool TWO>
+__global__ __launch_bounds__(W * 64) void k_few(const Product p, int split) {
+    few<MT, NT, TWO>(p, split);
+}
+
+template <int MT, int NT> int launch(const Product& p, hipStream_t st) {
+    const int pieces = (p.pitch + 15) / 16;
+    int split = 1;
+    while (split < W && 2 * split <= pieces) split *= 2;
+    const int width = W / split * 16 * NT;
+    const int64_t groups = (int64_t)((p.n + width - 1) / width) * most_tiles(p, 16 * MT);
+    if (groups > INT32_MAX) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
+    if (p.w1c) hipLaunchKernelGGL((k_few<MT, NT, true>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
+    else hipLaunchKernelGGL((k_few<MT, NT, false>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
 }
 
 }  // namespace
 
-int product_few(const Product& p, hipStream_t st) {
-    const int64_t groups = (int64_t)((p.n + 15) / 16) * most_tiles(p, 16);
-    if (groups > INT32_MAX) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
-    if (p.w1c) hipLaunchKernelGGL(k_few<true>, dim3((unsigned)groups), dim3(W * 64), 0, st, p);
-    else hipLaunchKernelGGL(k_few<false>, dim3((unsigned)groups), dim3(W * 64), 0, st, p);
-    SPA_HIP_TRY(hipGetLastError());
-    return SPA_OK;
-}
+int product_few(const Product& p, bool wide, hipStream_t st) { return wide ? launch<2, 2>(p, st) : launch<1, 1>(p, st); }
 
 }  // namespace mx
 }  // namespace spa

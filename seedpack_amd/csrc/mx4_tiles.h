@@ -16,6 +16,26 @@ inline int64_t most_tiles(const Product& p, int height) {
     return p.m / height + (p.m < p.experts ? p.m : p.experts);
 }
 
+// a lane's expert e: its first slot and the end, which lie in 0..m whatever the numbers are
+struct Span { int begin, end; };
+__device__ __forceinline__ Span span_of(const Product& p, int e) {
+    if (e >= p.experts) return Span{0, 0};
+    const int begin = tmin(tmax(p.starts[e], 0), p.m);
+    return Span{begin, tmin(tmax(p.starts[e + 1], begin), p.m)};
+}
+
+// the tiles that there are
+__device__ __forceinline__ int tiles_of(const Product& p, int height) {
+    int sum = 0;
+    for (int e = threadIdx.x & 63; e < p.experts; e += 64) {
+        const Span s = span_of(p, e);
+        sum += (s.end - s.begin + height - 1) / height;
+    }
+#pragma unroll
+    for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
+    return __builtin_amdgcn_readfirstlane(sum);
+}
+
 // Tile `id` of `height` rows; no rows behind the last. An expert's tiles follow those of the experts before it: each
 // lane counts the tiles of its own, 64 experts at a time.
 __device__ __forceinline__ Tile tile_at(const Product& p, int id, int height) {
@@ -26,9 +46,7 @@ __device__ __forceinline__ Tile tile_at(const Product& p, int id, int height) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 64) {
-        const int e = e0 + lane;
-        // whatever the numbers are, a tile's slots lie in 0..m-1
-        const int begin = e < p.experts ? tmin(tmax(p.starts[e], 0), p.m) : 0, end = e < p.experts ? tmin(tmax(p.starts[e + 1], begin), p.m) : 0;
+        const auto [begin, end] = span_of(p, e0 + lane);
         const int own = (end - begin + height - 1) / height;
         int sum = own;
 #pragma unroll
