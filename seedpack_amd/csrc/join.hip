@@ -4,6 +4,7 @@
 #include "../../include/seedpack_amd.h"
 #include "lanes.h"
 #include "launch.h"
+#include "linear.h"
 
 namespace spa {
 namespace {
@@ -29,7 +30,7 @@ template <int KIND> __device__ __forceinline__ void put_number(void* p, int64_t 
     if constexpr (KIND == SRC_F32) static_cast<float*>(p)[i] = v;
     else static_cast<uint16_t*>(p)[i] = KIND == SRC_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (_Float16)v);
 }
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+using u4v = lin::u4;
 // 16 bytes of numbers as floats, and back
 template <int KIND, int V> __device__ __forceinline__ void widen(u4v v, float (&x)[V]) {
 #pragma unroll
@@ -56,18 +57,23 @@ __device__ __forceinline__ bool has_expert(const Join& a, int64_t slot) {
     return e >= 0 && e < a.experts;
 }
 
-// a row's part of up to V numbers at column c
+// a row's part of up to V numbers; wide: rows begin at whole 16 bytes
 template <int KIND, int V> __device__ __forceinline__ void load_part(const void* p, int64_t at, int left, bool wide, float (&x)[V]) {
-    if (wide && left >= V) {
-        widen<KIND>(*reinterpret_cast<const u4v*>(static_cast<const char*>(p) + at * (KIND == SRC_F32 ? 4 : 2)), x);
+    if (left >= V) {
+        u4v v;
+        if constexpr (KIND == SRC_F32) __builtin_memcpy(&v, static_cast<const float*>(p) + at, 16);
+        else if (wide) v = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(p) + at);
+        else v = lin::load8_words(static_cast<const uint16_t*>(p) + at);
+        widen<KIND>(v, x);
     } else {
 #pragma unroll
         for (int c = 0; c < V; ++c) x[c] = c < left ? number_at<KIND>(p, at + c) : 0.f;
     }
 }
-template <int KIND, int V> __device__ __forceinline__ void store_part(void* p, int64_t at, int left, bool wide, const float (&x)[V]) {
-    if (wide && left >= V) {
-        *reinterpret_cast<u4v*>(static_cast<char*>(p) + at * (KIND == SRC_F32 ? 4 : 2)) = shorten<KIND>(x);
+template <int KIND, int V> __device__ __forceinline__ void store_part(void* p, int64_t at, int left, const float (&x)[V]) {
+    if (left >= V) {
+        const u4v v = shorten<KIND>(x);
+        __builtin_memcpy(static_cast<char*>(p) + at * (KIND == SRC_F32 ? 4 : 2), &v, 16);    // at any number's address
     } else {
 #pragma unroll
         for (int c = 0; c < V; ++c)
@@ -94,7 +100,7 @@ __global__ __launch_bounds__(256) void k_join(const Join a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[i] = fmaf(w, x[i], sum[i]);
     }
-    store_part<KIND>(a.out, row * a.ldo + c, left, a.wide, sum);
+    store_part<KIND>(a.out, row * a.ldo + c, left, sum);
 }
 
 // one workgroup a slot
@@ -121,7 +127,7 @@ __global__ __launch_bounds__(256) void k_join_back(const Join a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) d[i] = 0.f;
         }
-        store_part<KIND>(a.dy, slot * a.ldo + c, left, a.wide, d);
+        store_part<KIND>(a.dy, slot * a.ldo + c, left, d);
     }
     dot = row_sum<64>(dot);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
@@ -164,7 +170,7 @@ int spa_join(const void* y, int kind, int64_t rows, int64_t each, int64_t n, int
     a.weights = weights;
     a.which = which;
     a.out = out;
-    a.wide = on16(y) && on16(out) && y_stride % v == 0 && out_stride % v == 0;
+    a.wide = on16(y) && y_stride % v == 0;
     const dim3 grid((unsigned)((rows * ((n + v - 1) / v) + 255) / 256));
     if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_join<SRC_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_join<SRC_F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -195,7 +201,7 @@ int spa_join_backward(const void* y, int kind, int64_t rows, int64_t each, int64
     a.which = which;
     a.dy = dy;
     a.dweights = dweights;
-    a.wide = on16(y) && on16(dout) && on16(dy) && y_stride % v == 0 && dout_stride % v == 0 && dy_stride % v == 0;
+    a.wide = on16(y) && on16(dout) && y_stride % v == 0 && dout_stride % v == 0;
     const dim3 grid((unsigned)(rows * each));
     if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_join_back<SRC_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_join_back<SRC_F16>, grid, dim3(256), 0, (hipStream_t)stream, a);

@@ -34,16 +34,35 @@ template <typename T> __device__ __forceinline__ T lane_xor(T v, int mask) {
     }
 }
 
+// A number's two copies after rows of 16 (or 32) lanes changed places between them: the even rows' numbers everywhere, and the
+// odd ones'.
+template <int ROW, typename T> __device__ __forceinline__ void across_rows(T v, T& even, T& odd) {
+    constexpr int N = sizeof(T) / 4;
+    uint32_t b[N], c[N];
+    __builtin_memcpy(b, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const auto r = ROW == 16 ? __builtin_amdgcn_permlane16_swap(b[i], b[i], false, false) : __builtin_amdgcn_permlane32_swap(b[i], b[i], false, false);
+        b[i] = r[0];
+        c[i] = r[1];
+    }
+    __builtin_memcpy(&even, b, sizeof(T));
+    __builtin_memcpy(&odd, c, sizeof(T));
+}
+
 // op over the L = 16 or 64 lanes of a row, in an order of its own that is the same for every lane: neighbours, pairs,
-// and, the pairs being alike, mirrored fours and eights.
+// and, the pairs being alike, mirrored fours and eights, then rows of 16.
 template <int L, typename T, typename F> __device__ __forceinline__ T over_row(T v, F op) {
     v = op(v, lane_move<0xb1>(v));                               // lanes 1 0 3 2
     v = op(v, lane_move<0x4e>(v));                               // lanes 2 3 0 1
     v = op(v, lane_move<0x141>(v));                              // eight lanes mirrored
     v = op(v, lane_move<0x140>(v));                              // sixteen lanes mirrored
     if constexpr (L == 64) {
-        v = op(v, lane_xor(v, 16));
-        v = op(v, lane_xor(v, 32));
+        T even, odd;
+        across_rows<16>(v, even, odd);
+        v = op(even, odd);
+        across_rows<32>(v, even, odd);
+        v = op(even, odd);
     }
     return v;
 }

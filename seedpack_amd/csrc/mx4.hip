@@ -57,14 +57,12 @@ __device__ __forceinline__ uint32_t spread(uint32_t v) {
 
 // eight numbers of a row at column c, zeros behind its last
 template <int KIND> __device__ __forceinline__ void load8(const void* x, int64_t at, int64_t left, bool wide, float (&v)[8]) {
-    if (wide && left >= 8) {
+    if (left >= 8) {
         if constexpr (KIND == SRC_F32) {
-            const u4v* p = reinterpret_cast<const u4v*>(static_cast<const float*>(x) + at);
-            const u4v a = p[0], b = p[1];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) { v[c] = __uint_as_float(a[c]); v[4 + c] = __uint_as_float(b[c]); }
+            __builtin_memcpy(v, static_cast<const float*>(x) + at, 32);   // at any number's address
         } else {
-            const u4v a = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(x) + at);
+            const uint16_t* const p = static_cast<const uint16_t*>(x) + at;
+            const u4v a = wide ? *reinterpret_cast<const u4v*>(p) : lin::load8_words(p);
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = lin::wide((a[c >> 1] >> (16 * (c & 1))) & 0xffffu, KIND);
         }
@@ -148,36 +146,43 @@ struct Values {
     const uint8_t *codes, *scales;
     int64_t rows, cols, stride;
     int pitch;
-    bool wide;
     void* y;
 };
 
-// A lane takes 4 bytes of a block: numbers 4 q .. 4 q + 3 and those 16 behind
+// A lane takes eight neighbours of a block: the low or the high halves of eight bytes, brought together two to a byte
 template <int KIND>
 __global__ __launch_bounds__(256) void k_values(const Values a) {
     const int64_t per = (a.cols + 31) / 32 * 4, id = blockIdx.x * 256ll + threadIdx.x;
     const int64_t row = id / per;
     if (row >= a.rows) return;
-    const int64_t quarter = id - row * per, block = row * a.pitch + (quarter >> 2);
-    const int q = (int)(quarter & 3);
-    const uint32_t v = reinterpret_cast<const uint32_t*>(a.codes)[block * 4 + q];
+    const int64_t eighth = id - row * per, block = row * a.pitch + (eighth >> 2), c = eighth * 8, left = a.cols - c;
+    if (left <= 0) return;
+    const int q = (int)(eighth & 3);
+    const lin::u2 v = reinterpret_cast<const lin::u2*>(a.codes)[block * 2 + (q & 1)];
     const float scale = __uint_as_float((uint32_t)a.scales[block] << 23);
-    const f2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 1),
-                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v, scale, 3)};
+    float x[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int64_t c = (quarter >> 2) * 32 + 16 * h + 4 * q, at = row * a.stride + c;
-        if (a.wide && c + 4 <= a.cols) {
-            if constexpr (KIND == SRC_F32) {
-                *reinterpret_cast<lin::f4*>(static_cast<float*>(a.y) + at) = lin::f4{p[0][h], p[1][h], p[2][h], p[3][h]};
-            } else {
-                *reinterpret_cast<lin::u2*>(static_cast<uint16_t*>(a.y) + at) = lin::u2{lin::narrow2(p[0][h], p[1][h], KIND), lin::narrow2(p[2][h], p[3][h], KIND)};
-            }
+        const uint32_t m = (v[h] >> (4 * (q >> 1))) & 0x0f0f0f0fu, both = m | m >> 4;
+        const f2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(both, scale, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(both, scale, 2);
+        x[4 * h] = lo[0];
+        x[4 * h + 1] = lo[1];
+        x[4 * h + 2] = hi[0];
+        x[4 * h + 3] = hi[1];
+    }
+    const int64_t at = row * a.stride + c;
+    if (left >= 8) {
+        // at any number's address
+        if constexpr (KIND == SRC_F32) {
+            __builtin_memcpy(static_cast<float*>(a.y) + at, x, 32);
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < a.cols) put<KIND>(a.y, at + i, p[i][h]);
+            const u4v w = {lin::narrow2(x[0], x[1], KIND), lin::narrow2(x[2], x[3], KIND), lin::narrow2(x[4], x[5], KIND), lin::narrow2(x[6], x[7], KIND)};
+            __builtin_memcpy(static_cast<uint16_t*>(a.y) + at, &w, 16);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) put<KIND>(a.y, at + i, x[i]);
     }
 }
 
@@ -266,7 +271,7 @@ int spa_mx4_values(const uint8_t* codes, const uint8_t* scales, int64_t rows, in
     if (stride < cols) return fail(SPA_ERR_ARG, "mx4_values: rows of %lld at a stride of %lld", (long long)cols, (long long)stride);
     if (!rows) return SPA_OK;
     if (!y) return fail(SPA_ERR_ARG, "mx4_values: a pointer is NULL");
-    Values a{codes, scales, rows, cols, stride, (int)pitch_of(cols), on(y, kind == SPA_SRC_F32 ? 16 : 8) && stride % 4 == 0, y};
+    Values a{codes, scales, rows, cols, stride, (int)pitch_of(cols), y};
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)((rows * ((cols + 31) / 32) * 4 + 255) / 256));
     if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_values<SRC_BF16>, grid, dim3(256), 0, st, a);

@@ -5,10 +5,9 @@
 // themselves (both scores rise with them), or, with a bias or groups, s + b in 64 bits, for keys are compared with each
 // other: in 32 bits one row in some thousands would have two of its experts' keys rounded across each other.
 //
-// 16 lanes hold a row of up to 256 experts (64 lanes above), so that a wave takes four rows at once and what the lanes
-// tell each other stays within 16 of them. A key carries its expert's number in its low bits (reversed: of equal
+// A row's lanes, 16 or 64, hold its experts. A key carries its expert's number in its low bits (reversed: of equal
 // keys the lowest number wins), which makes all keys of a row different: each lane sorts its own few, and the
-// row's next expert is the largest of 16 heads, whose lane moves its list up.
+// row's next expert is the largest of the lanes' heads, whose lane moves its list up.
 #include "../../include/seedpack_amd.h"
 #include "lanes.h"
 #include "launch.h"
@@ -57,7 +56,7 @@ __device__ __forceinline__ void load_row(const void* logits, int64_t at, int exp
         const int i = place<L, V>(j, lane);
         if (wide && i + V <= experts) {
             if constexpr (KIND == SRC_F32) {
-                typedef float fv __attribute__((ext_vector_type(4)));
+                typedef float fv __attribute__((ext_vector_type(V)));
                 const fv v = *reinterpret_cast<const fv*>(static_cast<const float*>(logits) + at + i);
 #pragma unroll
                 for (int c = 0; c < V; ++c) x[j + c] = v[c];
@@ -114,24 +113,85 @@ template <int N, typename K> __device__ __forceinline__ void sort_down(K (&k)[N]
                 }
 }
 
-// the logarithm of a score, up to a number that all of a row's scores share
-__device__ __forceinline__ double log_score(float l, int score) {
-    if (score == SOFTMAX) return l;
-    return l < 0 ? l - log1p(exp((double)l)) : -log1p(exp(-(double)l));
+// e^x for x <= 0 (NaN stays): x = n ln 2 + r with ln 2 in two parts, and the series to r^13 / 13!, |r| <= 0.347: 4e-18.
+// (The library's exp and a division of full rounding, whose arguments may be anything, made 8191 rows of 256 experts
+// in groups 19 us.)
+__device__ __forceinline__ double exp_down(double x) {
+    const double c = fmax(x, -800.), n = rint(c * 1.4426950408889634);
+    const double r = fma(n, -0x1.abc9e3b39803fp-56, fma(n, -0x1.62e42fefa39efp-1, c));
+    double p = 1. / 6227020800.;
+    p = fma(p, r, 1. / 479001600.);
+    p = fma(p, r, 1. / 39916800.);
+    p = fma(p, r, 1. / 3628800.);
+    p = fma(p, r, 1. / 362880.);
+    p = fma(p, r, 1. / 40320.);
+    p = fma(p, r, 1. / 5040.);
+    p = fma(p, r, 1. / 720.);
+    p = fma(p, r, 1. / 120.);
+    p = fma(p, r, 1. / 24.);
+    p = fma(p, r, 1. / 6.);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.);
+    p = fma(p, r, 1.);
+    p = ldexp(p, (int)n);
+    return x == x ? p : x;
+}
+// 1 / y of 1 <= y <= 2: the hardware's estimate and two steps of Newton's
+__device__ __forceinline__ double reciprocal(double y) {
+    double r = __builtin_amdgcn_rcp(y);
+    r = fma(r, fma(-y, r, 1.), r);
+    return fma(r, fma(-y, r, 1.), r);
 }
 __device__ __forceinline__ double logistic(double l) {
-    const double e = exp(-fabs(l)), q = 1 / (1 + e);
+    const double e = exp_down(-fabs(l)), q = reciprocal(1 + e);
     return l < 0 ? e * q : q;
 }
 
-template <int KIND, int L, int PER, bool DEEP>
-__global__ __launch_bounds__(256) void k_route(const Route a) {
-    constexpr int ROWS = 256 / L, V = run_of<KIND, PER>(), HELD = MOST_EACH / L > 1 ? MOST_EACH / L : 1;
+// The chosen scores up to a factor that a row's have in common, and their sum. Logistic scores that all but vanish are taken
+// by their logarithms: their ratios do not.
+template <int L, int HELD>
+__device__ __forceinline__ double chosen(const float (&l)[HELD], const int (&mine)[HELD], int score, double (&v)[HELD]) {
+    double sum = 0;
+    if (score == SIGMOID) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            v[h] = mine[h] < 0 ? 0 : logistic(l[h]);
+            sum += v[h];
+        }
+        sum = row_sum<L>(sum);
+        if (!(sum < 1e-280)) return sum;
+    }
+    // below -600 the logarithm of the logistic is the logit itself
+    float most = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) most = mine[h] >= 0 ? fmaxf(most, l[h]) : most;
+    most = row_max<L>(most);
+    sum = 0;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        v[h] = mine[h] < 0 ? 0 : exp_down((double)l[h] - most);
+        sum += v[h];
+    }
+    return row_sum<L>(sum);
+}
+
+// what is written to LDS by this wave may be read by it
+__device__ __forceinline__ void own_lds() {
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// numbers of LDS of a row's keys in groups: a group's and a row's begin a bank further than the last one's, for the lanes read
+// those of different groups and rows at a time
+__host__ __device__ __forceinline__ int group_keys(int experts, int groups) { return (experts + 2 * groups) | 1; }
+
+// One row by its L lanes; keys: LDS for group_keys numbers of its own (DEEP, groups). Lane j of them gives the expert of place
+// j + h L in mine[h].
+template <int KIND, int L, int PER, bool DEEP, int HELD>
+__device__ __forceinline__ void route_row(const Route& a, int64_t row, bool in, int lane, double* keys, int (&mine)[HELD]) {
+    constexpr int V = run_of<KIND, PER>();
     typedef typename std::conditional<DEEP || KIND == SRC_F32, uint64_t, uint32_t>::type K;
-    extern __shared__ double shared[];
-    const int lane = threadIdx.x % L, slot = threadIdx.x / L;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + slot;
-    const bool in = row < a.rows;
     const int64_t at = (in ? row : 0) * a.stride;
 
     float x[PER];
@@ -149,7 +209,7 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
         double s[PER], sum = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            s[j] = a.score == SOFTMAX ? (x[j] == -INFINITY ? 0 : exp((double)x[j] - top)) : logistic(x[j]);
+            s[j] = a.score == SOFTMAX ? (x[j] == -INFINITY ? 0 : exp_down((double)x[j] - top)) : logistic(x[j]);
             sum += s[j];
         }
         if (a.score == SOFTMAX) {
@@ -165,16 +225,16 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
         }
         uint64_t kept = ~0ull;
         const int per = a.experts / a.groups;
+        const uint32_t inverse = ((1u << 20) + per - 1) / per;     // i / per for i < 1024
         if (a.groups > 1) {
             // each group by as many lanes as there are for it, its two best keys
-            double* const keys = shared + slot * (a.experts + MOST_GROUPS);
-            double* const score = keys + a.experts;
+            double* const score = keys + a.experts + a.groups;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int i = place<L, V>(j, lane);
-                if (i < a.experts) keys[i] = s[j] == s[j] ? s[j] : INFINITY;
+                if (i < a.experts) keys[i + ((i * inverse) >> 20)] = s[j] == s[j] ? s[j] : INFINITY;
             }
-            __syncthreads();
+            own_lds();
             int lanes = L;
             while (lanes > 1 && lanes * a.groups > L) lanes >>= 1;
             for (int g0 = 0; g0 < a.groups; g0 += L / lanes) {
@@ -182,7 +242,7 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
                 double one = -INFINITY, two = -INFINITY;
                 if (g < a.groups)
                     for (int i = lane % lanes; i < per; i += lanes) {
-                        const double v = keys[g * per + i];
+                        const double v = keys[g * (per + 1) + i];
                         two = fmax(two, fmin(one, v));
                         one = fmax(one, v);
                     }
@@ -193,7 +253,7 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
                 }
                 if (g < a.groups && lane % lanes == 0) score[g] = a.best == 2 && per > 1 ? one + two : one;
             }
-            __syncthreads();
+            own_lds();
             kept = 0;
             for (int g = lane; g < a.groups; g += L) {
                 const double mine = score[g];
@@ -203,7 +263,6 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
             }
             kept = over_row<L>(kept, [](uint64_t p, uint64_t q) { return p | q; });
         }
-        const uint32_t inverse = ((1u << 20) + per - 1) / per;     // i / per for i < 1024
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = place<L, V>(j, lane);
@@ -213,7 +272,6 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
     }
     sort_down(k);
 
-    int mine[HELD];
 #pragma unroll
     for (int h = 0; h < HELD; ++h) mine[h] = -1;
     for (int j = 0; j < a.each; ++j) {
@@ -228,35 +286,21 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
             if (j == h * L + lane && best) mine[h] = expert_of(best);
     }
 
-    // weights: the chosen scores' ratios from their logarithms, so that none of them vanishes together
-    double v[HELD], most = -INFINITY;
+    float l[HELD];
+    double v[HELD], total = 1;
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        const float l = mine[h] < 0 ? -INFINITY : logit_at<KIND>(a.logits, at + mine[h]);
-        if (a.renorm) {
-            v[h] = mine[h] < 0 ? -INFINITY : log_score(l, a.score);
-            most = v[h] > most || v[h] != v[h] ? v[h] : most;
-        } else if (a.score == SIGMOID) {
-            v[h] = mine[h] < 0 ? 0 : logistic(l);
-        } else {
-            v[h] = mine[h] < 0 ? 0 : exp((double)l - top);
-        }
-    }
-    double total = 1;
+    for (int h = 0; h < HELD; ++h) l[h] = mine[h] < 0 ? -INFINITY : logit_at<KIND>(a.logits, at + mine[h]);
     if (a.renorm) {
-        most = row_max<L>(most);
-        double sum = 0;
+        total = chosen<L>(l, mine, a.score, v);
+    } else {
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            v[h] = mine[h] < 0 ? 0 : exp(v[h] - most);
-            sum += v[h];
+        for (int h = 0; h < HELD; ++h) v[h] = mine[h] < 0 ? 0 : a.score == SIGMOID ? logistic(l[h]) : exp_down((double)l[h] - top);
+        if (a.score == SOFTMAX) {
+            float sum = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) sum += x[j] == -INFINITY ? 0.f : expf(x[j] - top);
+            total = row_sum<L>(sum);
         }
-        total = row_sum<L>(sum);
-    } else if (a.score == SOFTMAX) {
-        float sum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) sum += x[j] == -INFINITY ? 0.f : expf(x[j] - top);
-        total = row_sum<L>(sum);
     }
     if (!in) return;
 #pragma unroll
@@ -268,38 +312,26 @@ __global__ __launch_bounds__(256) void k_route(const Route a) {
     }
 }
 
-template <int KIND, bool DEEP> int route_kind(const Route& a, hipStream_t st) {
-    auto go = [&](auto kernel, int rows) {
-        const int64_t groups = (a.rows + rows - 1) / rows;
-        const size_t bytes = DEEP && a.groups > 1 ? (size_t)rows * (a.experts + MOST_GROUPS) * 8 : 0;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), bytes, st, a);
-        SPA_HIP_TRY(hipGetLastError());
-        return SPA_OK;
-    };
-    if (a.experts <= 64) return go(k_route<KIND, 16, 4, DEEP>, 16);
-    if (a.experts <= 128) return go(k_route<KIND, 16, 8, DEEP>, 16);
-    if (a.experts <= 256) return go(k_route<KIND, 16, 16, DEEP>, 16);
-    if (a.experts <= 512) return go(k_route<KIND, 64, 8, DEEP>, 4);
-    return go(k_route<KIND, 64, 16, DEEP>, 4);
-}
-template <int KIND> int route_deep(const Route& a, hipStream_t st) {
-    return a.bias || a.groups > 1 ? route_kind<KIND, true>(a, st) : route_kind<KIND, false>(a, st);
-}
-
 // ---- slots in the order of their experts ----
 //
-// A counting sort that keeps the order of equal ones: 64 slots are a wave's, whose lanes of the same expert find each
-// other by one ballot for each bit of the number; the first of them counts all. A slot's place is the
-// number of slots of lower experts, of its expert in earlier runs, and in its own run below it. Numbers outside
+// A counting sort that keeps the order of equal ones. 64 slots are a wave's, whose lanes of the same expert find each
+// other by one ballot for each bit of the number; the first of them counts all. A slot's place is the number of slots of
+// lower experts, of its expert in earlier tiles, in earlier runs of 64 of its tile, and in its own run below it. Numbers outside
 // 0..experts-1 count as `experts`: behind all others.
-constexpr int RUN = 512, WAVES = RUN / 64;
+//
+// The routing kernel counts its own rows' experts, a launch adds the counts up, one workgroup an expert, and the last places
+// some of the counted tiles at a time; a few rows are routed and ordered by one workgroup, in one launch. (Placing
+// workgroups that add up all counts themselves, for one launch less, took 13.5 us for 256 tiles of 128 experts, not 3 and 4.4.)
+constexpr int TILE = 512;                // slots that a workgroup places at most
+constexpr int FEW = 2048;                // slots that one workgroup routes and orders
 
 struct Order {
     const int32_t* which;
     int slots, experts, bits;
     int32_t *order, *starts;
-    uint32_t* counts;        // [tile][experts + 1]: a tile's slots of each expert, then their places
-    int tiles;
+    uint16_t* counts;        // [tiles][experts + 1]: a tile's slots of each expert
+    uint32_t* sums;          // [tiles + 1][experts + 1]: those of the tiles before, and all
+    int tile, tiles, group;  // slots of a tile, tiles, and the tiles that a workgroup places
 };
 
 // the lanes that hold `key`, of `bits` bits, among those of the wave with `has`
@@ -312,188 +344,284 @@ __device__ __forceinline__ uint64_t alike(int key, bool has, int bits) {
     }
     return m;
 }
-__device__ __forceinline__ int key_at(const Order& o, int i) {
-    const int e = o.which[i];
-    return e >= 0 && e < o.experts ? e : o.experts;
-}
+__device__ __forceinline__ int key_of_slot(const Order& o, int e) { return e >= 0 && e < o.experts ? e : o.experts; }
 
-// everything in one workgroup: counts[run][expert] in LDS
-__global__ __launch_bounds__(1024) void k_order_one(const Order o) {
-    extern __shared__ uint32_t count[];
-    __shared__ uint32_t wave_sum[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, keys = o.experts + 1;
-    const int runs = (o.slots + 63) / 64;
-    for (int i = threadIdx.x; i < runs * keys; i += 1024) count[i] = 0;
-    __syncthreads();
-    for (int r = wave; r < runs; r += 16) {
-        const int i = r * 64 + lane;
-        const bool has = i < o.slots;
-        const int key = has ? key_at(o, i) : 0;
-        const uint64_t m = alike(key, has, o.bits);
-        if (has && (m & ((1ull << lane) - 1)) == 0) count[r * keys + key] = (uint32_t)__popcll(m);
-    }
-    __syncthreads();
-    // each expert's places, thread by thread: up to two experts each (keys <= 1025)
-    uint32_t total[2] = {0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int e = threadIdx.x * 2 + h;
-        if (e < keys)
-            for (int r = 0; r < runs; ++r) {
-                const uint32_t c = count[r * keys + e];
-                count[r * keys + e] = total[h];
-                total[h] += c;
-            }
-    }
-    uint32_t before = total[0] + total[1];
-    const uint32_t own = before;
+// inclusive sums over the workgroup's threads; scratch: one number a wave
+__device__ __forceinline__ uint32_t running(uint32_t v, uint32_t* scratch) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-        const uint32_t t = __shfl_up(before, s);
-        if (lane >= s) before += t;
+        const uint32_t t = __shfl_up(v, s);
+        if (lane >= s) v += t;
     }
-    if (lane == 63) wave_sum[wave] = before;
+    if (lane == 63) scratch[wave] = v;
     __syncthreads();
-    uint32_t base = before - own;
-    for (int w = 0; w < wave; ++w) base += wave_sum[w];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int e = threadIdx.x * 2 + h;
-        if (e < keys) {
-            o.starts[e] = (int32_t)base;
-            for (int r = 0; r < runs; ++r) count[r * keys + e] += base;
+    for (int w = 0; w < wave; ++w) v += scratch[w];
+    return v;
+}
+
+size_t order_lds(int64_t slots, int64_t experts) { return (size_t)((slots + 63) / 64 * 2 + 8) * (experts + 1); }
+
+// Places the slots first .. first + n - 1 of `which` (in LDS or memory, from `first` on) by a workgroup of T threads; tile: its
+// number. LDS: order_lds(n, experts) bytes, 16-byte aligned.
+template <int T>
+__device__ __forceinline__ void place_tile(const Order& o, int tile, int first, int n, const int32_t* which, uint8_t* lds) {
+    __shared__ uint32_t scratch[T / 64];
+    constexpr int PER = (MOST_EXPERTS + T) / T;                  // experts of a thread
+    const int keys = o.experts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, runs = (n + 63) / 64;
+    uint32_t *const before = reinterpret_cast<uint32_t*>(lds), *const total = before + keys;
+    uint16_t* const count = reinterpret_cast<uint16_t*>(total + keys);
+    for (int i = threadIdx.x; i < runs * keys; i += T) count[i] = 0;
+    for (int i = threadIdx.x; i < 2 * keys; i += T) before[i] = 0;
+    __syncthreads();
+    if (o.tiles > 1) {
+        for (int e = threadIdx.x; e < keys; e += T) {
+            before[e] = o.sums[(int64_t)tile * keys + e];
+            total[e] = o.sums[(int64_t)o.tiles * keys + e];
         }
-        base += total[h];
+    }
+    for (int r = wave; r < runs; r += T / 64) {
+        const int i = r * 64 + lane;
+        const bool has = i < n;
+        const int key = has ? key_of_slot(o, which[i]) : 0;
+        const uint64_t m = alike(key, has, o.bits);
+        if (has && (m & ((1ull << lane) - 1)) == 0) count[r * keys + key] = (uint16_t)__popcll(m);
     }
     __syncthreads();
-    for (int r = wave; r < runs; r += 16) {
-        const int i = r * 64 + lane;
-        const bool has = i < o.slots;
-        const int key = has ? key_at(o, i) : 0;
-        const uint64_t m = alike(key, has, o.bits);
-        if (has) o.order[count[r * keys + key] + __popcll(m & ((1ull << lane) - 1))] = i;
+    // each expert's runs; then the experts
+    uint32_t sum = 0;
+#pragma unroll
+    for (int h = 0; h < PER; ++h) {
+        const int e = threadIdx.x * PER + h;
+        if (e < keys) {
+            uint32_t c = 0;
+            for (int r = 0; r < runs; ++r) {
+                const uint32_t v = count[r * keys + e];
+                count[r * keys + e] = (uint16_t)c;
+                c += v;
+            }
+            if (o.tiles == 1) total[e] = c;
+            sum += total[e];
+        }
     }
+    uint32_t at = running(sum, scratch) - sum;
+#pragma unroll
+    for (int h = 0; h < PER; ++h) {
+        const int e = threadIdx.x * PER + h;
+        if (e < keys) {
+            if (tile == 0) o.starts[e] = (int32_t)at;
+            before[e] += at;
+            at += total[e];
+        }
+    }
+    __syncthreads();
+    for (int r = wave; r < runs; r += T / 64) {
+        const int i = r * 64 + lane;
+        const bool has = i < n;
+        const int key = has ? key_of_slot(o, which[i]) : 0;
+        const uint64_t m = alike(key, has, o.bits);
+        if (has) o.order[before[key] + count[r * keys + key] + __popcll(m & ((1ull << lane) - 1))] = first + i;
+    }
+}
+
+__global__ __launch_bounds__(512) void k_place(const Order o) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tile = blockIdx.x * o.group, first = tile * o.tile;
+    place_tile<512>(o, tile, first, tmin(o.tile * o.group, o.slots - first), o.which + first, lds);
 }
 
 // a tile's slots of each expert
-__global__ __launch_bounds__(RUN) void k_order_count(const Order o) {
-    extern __shared__ uint32_t count[];
+__global__ __launch_bounds__(1024) void k_count(const Order o) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t* const count = reinterpret_cast<uint32_t*>(lds);
     const int keys = o.experts + 1, lane = threadIdx.x & 63;
-    for (int e = threadIdx.x; e < keys; e += RUN) count[e] = 0;
+    for (int e = threadIdx.x; e < keys; e += 1024) count[e] = 0;
     __syncthreads();
-    const int i = blockIdx.x * RUN + threadIdx.x;
-    const bool has = i < o.slots;
-    const int key = has ? key_at(o, i) : 0;
-    const uint64_t m = alike(key, has, o.bits);
-    if (has && (m & ((1ull << lane) - 1)) == 0) atomicAdd(&count[key], (uint32_t)__popcll(m));
+    const int first = blockIdx.x * o.tile, n = tmin(o.tile, o.slots - first);
+    for (int i0 = 0; i0 < n; i0 += 1024) {
+        const int i = i0 + threadIdx.x;
+        const bool has = i < n;
+        const int key = has ? key_of_slot(o, o.which[first + i]) : 0;
+        const uint64_t m = alike(key, has, o.bits);
+        if (has && (m & ((1ull << lane) - 1)) == 0) atomicAdd(&count[key], (uint32_t)__popcll(m));
+    }
     __syncthreads();
-    for (int e = threadIdx.x; e < keys; e += RUN) o.counts[(int64_t)blockIdx.x * keys + e] = count[e];
+    for (int e = threadIdx.x; e < keys; e += 1024) o.counts[(int64_t)blockIdx.x * keys + e] = (uint16_t)count[e];
 }
 
-// each expert's counts as sums of the tiles before, and its total: one workgroup an expert
-__global__ __launch_bounds__(256) void k_order_scan(const Order o) {
-    __shared__ uint32_t wave_sum[4];
-    const int keys = o.experts + 1, e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// each expert's counts added up over the tiles: one workgroup an expert
+__global__ __launch_bounds__(256) void k_sums(const Order o) {
+    __shared__ uint32_t scratch[4], all;
+    const int keys = o.experts + 1, e = blockIdx.x;
     uint32_t carry = 0;
     for (int t0 = 0; t0 < o.tiles; t0 += 256) {
         const int t = t0 + threadIdx.x;
         const uint32_t own = t < o.tiles ? o.counts[(int64_t)t * keys + e] : 0;
-        uint32_t sum = own;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint32_t v = __shfl_up(sum, s);
-            if (lane >= s) sum += v;
-        }
+        const uint32_t sum = running(own, scratch);
+        if (threadIdx.x == 255) all = sum;
+        if (t < o.tiles) o.sums[(int64_t)t * keys + e] = carry + sum - own;
         __syncthreads();
-        if (lane == 63) wave_sum[wave] = sum;
+        carry += all;
         __syncthreads();
-        uint32_t base = carry;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) base += wave_sum[w];
-            carry += wave_sum[w];
-        }
-        if (t < o.tiles) o.counts[(int64_t)t * keys + e] = base + sum - own;
     }
-    if (threadIdx.x == 0) o.counts[(int64_t)o.tiles * keys + e] = carry;
+    if (threadIdx.x == 0) o.sums[(int64_t)o.tiles * keys + e] = carry;
 }
 
-__global__ __launch_bounds__(RUN) void k_order_place(const Order o) {
-    extern __shared__ uint32_t count[];                          // [WAVES][keys], then [keys]
-    __shared__ uint32_t wave_sum[WAVES];
-    const int keys = o.experts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t* const base = count + WAVES * keys;
-    for (int e = threadIdx.x; e < WAVES * keys; e += RUN) count[e] = 0;
-    // where each expert's slots begin: the totals' sums, up to three experts a thread
-    constexpr int PER = (MOST_EXPERTS + 1 + RUN - 1) / RUN;
-    uint32_t total[PER], sum = 0;
-#pragma unroll
-    for (int h = 0; h < PER; ++h) {
-        const int e = threadIdx.x * PER + h;
-        total[h] = e < keys ? o.counts[(int64_t)o.tiles * keys + e] : 0;
-        sum += total[h];
-    }
-    const uint32_t own = sum;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const uint32_t v = __shfl_up(sum, s);
-        if (lane >= s) sum += v;
-    }
-    if (lane == 63) wave_sum[wave] = sum;
-    __syncthreads();
-    uint32_t at = sum - own;
-    for (int w = 0; w < wave; ++w) at += wave_sum[w];
-#pragma unroll
-    for (int h = 0; h < PER; ++h) {
-        const int e = threadIdx.x * PER + h;
-        if (e < keys) {
-            base[e] = at + o.counts[(int64_t)blockIdx.x * keys + e];
-            if (blockIdx.x == 0) o.starts[e] = (int32_t)at;
-        }
-        at += total[h];
-    }
-    const int i = blockIdx.x * RUN + threadIdx.x;
-    const bool has = i < o.slots;
-    const int key = has ? key_at(o, i) : 0;
-    const uint64_t m = alike(key, has, o.bits);
-    const int below = __popcll(m & ((1ull << lane) - 1));
-    if (has && below == 0) count[wave * keys + key] = (uint32_t)__popcll(m);
-    __syncthreads();
-    if (has) {
-        uint32_t p = base[key] + below;
-        for (int w = 0; w < wave; ++w) p += count[w * keys + key];
-        o.order[p] = i;
-    }
+// the slots that a workgroup places, its counts in LDS that needs no leave
+int64_t most_placed(int64_t experts) {
+    int64_t n = TILE;
+    while (order_lds(n, experts) > 60 * 1024) n /= 2;
+    return n;
 }
-
-// one workgroup while its counts fit into a part of LDS that needs no leave
-bool one_block(int64_t slots, int64_t experts) { return (slots + 63) / 64 * (experts + 1) * 4 <= 60 * 1024 && slots <= 4096; }
-uint64_t order_bytes(int64_t slots, int64_t experts) {
-    return one_block(slots, experts) ? 0 : (uint64_t)((slots + RUN - 1) / RUN + 1) * (experts + 1) * 4;
+// the tiles of an order, and its workspace
+void lay_out(Order& o, int64_t slots, int64_t experts, int64_t tile, void* work) {
+    o.slots = (int)slots;
+    o.experts = (int)experts;
+    while (experts >> o.bits) ++o.bits;
+    o.tile = (int)tile;
+    o.tiles = (int)((slots + tile - 1) / tile);
+    o.group = (int)(most_placed(experts) / tile);
+    if (!o.group) o.group = 1;
+    o.counts = static_cast<uint16_t*>(work);
+    o.sums = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(work) + ((int64_t)o.tiles * (experts + 1) * 2 + 255) / 256 * 256);
+}
+uint64_t order_bytes(int64_t slots, int64_t experts, int64_t tile) {
+    const int64_t tiles = (slots + tile - 1) / tile, counts = tiles * (experts + 1);
+    return tiles > 1 ? (uint64_t)((counts * 2 + 255) / 256 * 256 + (counts + experts + 1) * 4) : 0;
+}
+// after the counts
+int place(const Order& o, hipStream_t st) {
+    if (o.tiles > 1) {
+        hipLaunchKernelGGL(k_sums, dim3((unsigned)o.experts + 1), dim3(256), 0, st, o);
+        SPA_HIP_TRY(hipGetLastError());
+    }
+    const int64_t most = (int64_t)o.tile * o.group, groups = o.tiles ? ((int64_t)o.tiles + o.group - 1) / o.group : 1;
+    hipLaunchKernelGGL(k_place, dim3((unsigned)groups), dim3(512), order_lds(o.slots < most ? o.slots : most, o.experts), st, o);
+    SPA_HIP_TRY(hipGetLastError());
+    return SPA_OK;
 }
 
 int by_expert(const int32_t* which, int64_t slots, int64_t experts, int32_t* order, int32_t* starts, void* work, hipStream_t st) {
     Order o{};
     o.which = which;
-    o.slots = (int)slots;
-    o.experts = (int)experts;
-    while (experts >> o.bits) ++o.bits;
     o.order = order;
     o.starts = starts;
-    o.counts = (uint32_t*)work;
-    o.tiles = (int)((slots + RUN - 1) / RUN);
-    const size_t keys = (size_t)experts + 1;
-    if (one_block(slots, experts)) {
-        hipLaunchKernelGGL(k_order_one, dim3(1), dim3(1024), (size_t)((slots + 63) / 64) * keys * 4, st, o);
+    lay_out(o, slots, experts, most_placed(experts), work);
+    if (o.tiles > 1) {
+        hipLaunchKernelGGL(k_count, dim3((unsigned)o.tiles), dim3(1024), (size_t)(experts + 1) * 4, st, o);
+        SPA_HIP_TRY(hipGetLastError());
+    }
+    return place(o, st);
+}
+
+// ---- the routing's kernels ----
+
+// Rows by workgroups of 512 (1024 where their registers allow it), `reps` times as many as they hold at once; with counts, the
+// slots of each expert among them
+template <int KIND, int L, int PER, bool DEEP, int T>
+__global__ __launch_bounds__(T) void k_route(const Route a, const Order o, int reps) {
+    constexpr int ROWS = T / L, HELD = MOST_EACH / L > 1 ? MOST_EACH / L : 1;
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t* const count = reinterpret_cast<uint32_t*>(lds);
+    const int lane = threadIdx.x % L, slot = threadIdx.x / L, keys = o.experts + 1;
+    double* const mine_lds = reinterpret_cast<double*>(lds + (o.counts ? (keys * 4 + 15) / 16 * 16 : 0)) + slot * group_keys(a.experts, a.groups);
+    if (o.counts) {
+        for (int e = threadIdx.x; e < keys; e += T) count[e] = 0;
+        __syncthreads();
+    }
+    for (int q = 0; q < reps; ++q) {
+        const int64_t row = ((int64_t)blockIdx.x * reps + q) * ROWS + slot;
+        const bool in = row < a.rows;
+        int mine[HELD];
+        route_row<KIND, L, PER, DEEP, HELD>(a, row, in, lane, mine_lds, mine);
+        if (in && o.counts) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+                if (h * L + lane < a.each) atomicAdd(&count[mine[h] < 0 ? a.experts : mine[h]], 1u);
+        }
+    }
+    if (o.counts) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < keys; e += T) o.counts[(int64_t)blockIdx.x * keys + e] = (uint16_t)count[e];
+    }
+}
+
+// a few rows, a wave each at a time, routed and ordered
+template <int KIND, int PER, bool DEEP>
+__global__ __launch_bounds__(1024) void k_route_few(const Route a, const Order o) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ int32_t which[FEW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int row = wave; row < a.rows; row += 16) {
+        int mine[1];
+        route_row<KIND, 64, PER, DEEP, 1>(a, row, true, lane, reinterpret_cast<double*>(lds) + wave * group_keys(a.experts, a.groups), mine);
+        if (lane < a.each) which[row * a.each + lane] = mine[0];
+    }
+    __syncthreads();
+    place_tile<1024>(o, 0, 0, o.slots, which, lds);
+}
+
+// How a routing is launched: 64 lanes a row where 16 would leave a long chain of work to few waves (4 rows of 256 experts in
+// groups: 13.8 us by 16 lanes), or hold more than 16 numbers each; four times the rows a workgroup of those where there are
+// enough, for fewer tiles to add up.
+struct Shape {
+    bool few, slim;          // one workgroup does all; 16 lanes a row
+    int threads, rows, reps; // rows of a workgroup at once, and how often
+};
+size_t group_lds(const Route& a, int rows) { return a.groups > 1 ? (size_t)rows * group_keys(a.experts, a.groups) * 8 : 0; }
+Shape shape_of(const Route& a, bool deep, bool sorted) {
+    Shape s{};
+    const int64_t slots = a.rows * a.each;
+    s.few = sorted && a.rows <= 64 && slots <= FEW && order_lds(slots, a.experts) <= 50 * 1024 && group_lds(a, 16) <= 50 * 1024;
+    s.slim = a.experts <= (deep ? 256 : 128) && a.rows > 4096;
+    s.threads = s.slim && !deep ? 1024 : 512;
+    s.rows = s.threads / (s.slim ? 16 : 64);
+    s.reps = s.slim || a.rows <= 4096 ? 1 : 4;
+    return s;
+}
+
+template <int KIND, bool DEEP> int route_kind(const Route& a, Order& o, bool sorted, void* work, hipStream_t st) {
+    const Shape s = shape_of(a, DEEP, sorted);
+    if (s.few) {
+        lay_out(o, a.rows * a.each, a.experts, FEW, nullptr);
+        size_t bytes = order_lds(o.slots, a.experts);
+        if (DEEP && group_lds(a, 16) > bytes) bytes = group_lds(a, 16);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), bytes, st, a, o);
+            SPA_HIP_TRY(hipGetLastError());
+            return SPA_OK;
+        };
+        if (a.experts <= 64) return go(k_route_few<KIND, 1, DEEP>);
+        if (a.experts <= 128) return go(k_route_few<KIND, 2, DEEP>);
+        if (a.experts <= 256) return go(k_route_few<KIND, 4, DEEP>);
+        if (a.experts <= 512) return go(k_route_few<KIND, 8, DEEP>);
+        return go(k_route_few<KIND, 16, DEEP>);
+    }
+    const int64_t rows = (int64_t)s.rows * s.reps;
+    if (sorted) lay_out(o, a.rows * a.each, a.experts, rows * a.each, work);
+    const size_t bytes = (sorted ? (size_t)(a.experts + 1 + 3) / 4 * 16 : 0) + (DEEP ? group_lds(a, s.rows) : 0);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3((unsigned)s.threads), bytes, st, a, o, s.reps);
         SPA_HIP_TRY(hipGetLastError());
         return SPA_OK;
+    };
+    int rc = SPA_OK;
+    if (s.slim) {
+        constexpr int T = DEEP ? 512 : 1024;
+        if (a.experts <= 64) rc = go(k_route<KIND, 16, 4, DEEP, T>);
+        else if (a.experts <= 128) rc = go(k_route<KIND, 16, 8, DEEP, T>);
+        else if constexpr (DEEP) rc = go(k_route<KIND, 16, 16, DEEP, T>);
+    } else {
+        if (a.experts <= 64) rc = go(k_route<KIND, 64, 1, DEEP, 512>);
+        else if (a.experts <= 128) rc = go(k_route<KIND, 64, 2, DEEP, 512>);
+        else if (a.experts <= 256) rc = go(k_route<KIND, 64, 4, DEEP, 512>);
+        else if (a.experts <= 512) rc = go(k_route<KIND, 64, 8, DEEP, 512>);
+        else rc = go(k_route<KIND, 64, 16, DEEP, 512>);
     }
-    hipLaunchKernelGGL(k_order_count, dim3((unsigned)o.tiles), dim3(RUN), keys * 4, st, o);
-    SPA_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(k_order_scan, dim3((unsigned)keys), dim3(256), 0, st, o);
-    SPA_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(k_order_place, dim3((unsigned)o.tiles), dim3(RUN), (WAVES + 1) * keys * 4, st, o);
-    SPA_HIP_TRY(hipGetLastError());
-    return SPA_OK;
+    return rc || !sorted ? rc : place(o, st);
+}
+template <int KIND> int route_deep(const Route& a, Order& o, bool sorted, void* work, hipStream_t st) {
+    return a.bias || a.groups > 1 ? route_kind<KIND, true>(a, o, sorted, work, st) : route_kind<KIND, false>(a, o, sorted, work, st);
 }
 
 // ---- the logits' gradient ----
@@ -538,7 +666,8 @@ __global__ __launch_bounds__(256) void k_route_back(const Back a) {
         total = row_sum<L>(total);
     }
     int mine[HELD];
-    double v[HELD], l[HELD], d[HELD], most = -INFINITY;
+    float l[HELD];
+    double v[HELD], d[HELD];
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
         const int j = h * L + lane;
@@ -546,31 +675,21 @@ __global__ __launch_bounds__(256) void k_route_back(const Back a) {
         if (mine[h] >= a.experts) mine[h] = -1;
         l[h] = mine[h] < 0 ? -INFINITY : logit_at<KIND>(a.logits, at + mine[h]);
         d[h] = mine[h] < 0 ? 0 : a.dweights[r * a.each + j];
-        if (a.renorm) {
-            v[h] = mine[h] < 0 ? -INFINITY : log_score((float)l[h], a.score);
-            most = v[h] > most || v[h] != v[h] ? v[h] : most;
-        } else if (a.score == SIGMOID) {
-            v[h] = mine[h] < 0 ? 0 : logistic(l[h]);
-        } else {
-            v[h] = mine[h] < 0 ? 0 : exp(l[h] - top) / total;
-        }
     }
     if (a.renorm) {
-        most = row_max<L>(most);
-        double sum = 0, dot = 0;
+        const double sum = chosen<L>(l, mine, a.score, v);
+        double dot = 0;
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            v[h] = mine[h] < 0 ? 0 : exp(v[h] - most);
-            sum += v[h];
+            v[h] = mine[h] < 0 ? 0 : v[h] / sum;
             dot += v[h] * d[h];
         }
-        sum = row_sum<L>(sum);
         dot = row_sum<L>(dot);
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            d[h] -= dot / sum;
-            v[h] = mine[h] < 0 ? 0 : v[h] / sum;
-        }
+        for (int h = 0; h < HELD; ++h) d[h] -= dot;
+    } else {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) v[h] = mine[h] < 0 ? 0 : a.score == SIGMOID ? logistic(l[h]) : exp_down((double)l[h] - top) / total;
     }
     float g[HELD];
     double sum = 0;
@@ -676,7 +795,7 @@ extern "C" {
 
 uint64_t spa_by_expert_work_bytes(int64_t slots, int64_t experts) {
     if (slots <= 0 || experts < 1 || experts > MOST_EXPERTS) return 0;
-    return order_bytes(slots, experts);
+    return order_bytes(slots, experts, most_placed(experts));
 }
 
 int spa_by_expert(const int32_t* which, int64_t slots, int64_t experts, int32_t* order, int32_t* starts, void* work,
@@ -689,7 +808,8 @@ int spa_by_expert(const int32_t* which, int64_t slots, int64_t experts, int32_t*
 }
 
 uint64_t spa_route_work_bytes(int64_t rows, int64_t experts, int64_t each, int sorted) {
-    return sorted && rows > 0 && each > 0 ? spa_by_expert_work_bytes(rows * each, experts) : 0;
+    if (!sorted || rows <= 0 || each <= 0 || each > MOST_EACH || experts < 1 || experts > MOST_EXPERTS) return 0;
+    return order_bytes(rows * each, experts, 8 * each);          // the smallest tiles that any form takes
 }
 
 int spa_route(const void* logits, int kind, int64_t rows, int64_t experts, int64_t stride, int score, const float* bias,
@@ -703,12 +823,15 @@ int spa_route(const void* logits, int kind, int64_t rows, int64_t experts, int64
     if (rows && (!logits || !which || !weights)) return fail(SPA_ERR_ARG, "route: a pointer is NULL");
     if (int rc = check_work("route", work, work_bytes, spa_route_work_bytes(rows, experts, each, order != nullptr))) return rc;
     hipStream_t st = (hipStream_t)stream;
-    if (rows) {
-        Route a{logits, rows, stride, (int)experts, score, (int)groups, (int)keep, (int)best, (int)each, renorm, bias, scale, wide_rows(logits, kind, stride), which, weights};
-        const int rc = kind == SPA_SRC_BF16 ? route_deep<SRC_BF16>(a, st) : kind == SPA_SRC_F16 ? route_deep<SRC_F16>(a, st) : route_deep<SRC_F32>(a, st);
-        if (rc) return rc;
-    }
-    return order ? by_expert(which, rows * each, experts, order, starts, work, st) : SPA_OK;
+    if (!rows) return order ? by_expert(which, 0, experts, order, starts, work, st) : SPA_OK;
+    Route a{logits, rows, stride, (int)experts, score, (int)groups, (int)keep, (int)best, (int)each, renorm, bias, scale, wide_rows(logits, kind, stride), which, weights};
+    Order o{};
+    o.which = which;
+    o.order = order;
+    o.starts = starts;
+    return kind == SPA_SRC_BF16 ? route_deep<SRC_BF16>(a, o, order != nullptr, work, st)
+         : kind == SPA_SRC_F16 ? route_deep<SRC_F16>(a, o, order != nullptr, work, st)
+                               : route_deep<SRC_F32>(a, o, order != nullptr, work, st);
 }
 
 int spa_route_backward(const void* logits, int kind, int64_t rows, int64_t experts, int64_t stride, int score, int64_t each,
