@@ -48,8 +48,7 @@ __device__ __forceinline__ void product(const Product& p) {
     constexpr int FN = TN / WN / 32, FM = TM / WM / 32;      // 32 x 32 fragments of a wave
     constexpr int ROWS = TN + TM;
     constexpr int LOADS = ROWS / 8 / NW;                     // 8 rows by one load of a wave
-    constexpr int SLOADS = ROWS / 8 / NW / 4;                // scales: 8 rows of 32 bytes, in one of four steps
-    static_assert(TNE % (8 * NW) == 0 && SLOADS * NW * 32 == ROWS && (!TWO || FN % 2 == 0) && NW % 4 == 0, "tile shape");
+    static_assert(TNE % (8 * NW) == 0 && 32 * NW == TN && TM == TN && TNE % 32 == 0 && (!TWO || FN % 2 == 0), "tile shape");
     constexpr int COLS = TNE / WN;                           // a wave's columns on their way out
     constexpr int STAGES = 2 * ROWS * 128, SCALES = 2 * ROWS * 32, OUTS = NW * 32 * (COLS + 4) * 4;
     __shared__ __align__(16) uint8_t mem[STAGES + SCALES > OUTS ? STAGES + SCALES : OUTS];
@@ -97,23 +96,21 @@ __device__ __forceinline__ void product(const Product& p) {
         const int m = tmin(r - TN, t.rows - 1);
         return p.experts ? (uint32_t)input_row(p, t.first + m) : (uint32_t)m;
     };
-    uint32_t off[LOADS], soff[SLOADS * 4];
+    uint32_t off[LOADS], soff[2];
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((lr >> 1) + 4 * (wave & 1));
-    // A load of scales takes 8 words of 8 rows and leaves them word by word, the words of the four runs of a
-    // fragment's 32 rows in places of their own: its rows' same word then lies in different banks.
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-        const uint32_t row = tile_row((j * NW + wave) * 8 + lr);
-        off[j] = row * row16 + 16 * chunk;
-        soff[j] = (uint32_t)__shfl((int)row, 8 * (lane & 7)) * (uint32_t)p.pitch;
-    }
-    const int sword = 4 * ((lane >> 3) ^ (2 * (wave & 3)));
+    for (int j = 0; j < LOADS; ++j) off[j] = tile_row((j * NW + wave) * 8 + lr) * row16 + 16 * chunk;
+    // A wave's scales: 32 of the weights' rows by one load, 32 of the inputs' by another, two pieces of 16 bytes a row; the
+    // pieces of every other run of 8 rows lie exchanged, for a fragment's reads.
+#pragma unroll
+    for (int h = 0; h < 2; ++h) soff[h] = tile_row(h * TN + wave * 32 + (lane >> 1)) * (uint32_t)p.pitch;
+    const int spiece = 16 * ((lane & 1) ^ (lane >> 4 & 1));
     constexpr int RAW = 0x00027000;                               // a plain buffer of bytes
     auto buffer = [&](const uint8_t* b, int64_t first, int64_t row) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(b + first * row), 0, -1, RAW); };
     const uint8_t *const wc = second ? p.w1c : p.w0c, *const ws = second ? p.w1s : p.w0s;
     const rsrc rw0 = buffer(wc + from * 128, wfirst, row16), rw1 = TWO ? buffer(p.w1c, wfirst, row16) : rw0, rx = buffer(p.xc + from * 128, xfirst, row16);
-    const uint64_t sw0 = (uint64_t)(ws + from * 8 + wfirst * p.pitch), sw1 = TWO ? (uint64_t)(p.w1s + wfirst * p.pitch) : sw0, sx = (uint64_t)(p.xs + from * 8 + xfirst * p.pitch);
-    const int last_word = p.pitch - 8 * from - 4;
+    const rsrc sw = buffer((TWO && wave * 32 >= TNE ? p.w1s : ws) + from * 8, wfirst, p.pitch), sx = buffer(p.xs + from * 8, xfirst, p.pitch);
+    const int left = p.pitch - 8 * from;                     // scales of a row from here on
     auto fetch = [&](int buf, int kt, int j0, int j1) {
 #pragma unroll
         for (int j = j0; j < j1; ++j) {
@@ -121,22 +118,26 @@ __device__ __forceinline__ void product(const Product& p) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)(mem + buf * ROWS * 128 + (j * NW + wave) * 8 * 128), 16, off[j], kt * 128, 0, 0);
         }
     };
-    // a quarter of the scales of steps 4 g .. 4 g + 3; words behind a row's last are its last. Choices by masks: conditional
-    // ones become loads from an array in scratch memory.
-    auto fetch_scales = [&](int g, int quarter) {
+    // half of the scales of steps 4 g .. 4 g + 3, the weights' or the inputs'. A piece that would end 8 bytes behind its row
+    // is taken 8 bytes early (odd_end); those behind the row's last are others. A row that has only 8: word by word.
+    auto fetch_scales = [&](int g, auto half) {
+        constexpr int H = decltype(half)::value;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(H ? sx : sw, (lptr)(smem + (g & 1) * ROWS * 32 + (H * TN + wave * 32) * 32), 16,
+                                                 soff[H] + (uint32_t)tmin(32 * g + spiece, left - 16), 0, 0, 0);
+    };
+    auto fetch_words = [&](auto half) {
+        constexpr int H = decltype(half)::value;
 #pragma unroll
-        for (int s = 0; s < SLOADS; ++s) {
-            const int j = quarter * SLOADS + s;
-            uint32_t o = 0;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) o |= soff[q * SLOADS + s] & (uint32_t)-(int)(quarter == q);
-            const int row = j * NW * 8;
-            const uint64_t isx = -(uint64_t)(row >= TN), is1 = -(uint64_t)(TWO && row >= TNE && row < TN);
-            const uint64_t base = (sx & isx) | (sw1 & is1) | (sw0 & ~(isx | is1));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer((const uint8_t*)base, 0, 0), (lptr)(smem + (g & 1) * ROWS * 32 + (j * NW + wave) * 8 * 32), 4,
-                                                     o + (uint32_t)tmin(32 * g + sword, last_word), 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t row = (uint32_t)__shfl((int)soff[H], 16 * i + 2 * (lane >> 3));
+            const int piece = (lane >> 2 & 1) ^ (i & 1);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(H ? sx : sw, (lptr)(smem + (H * TN + wave * 32 + 8 * i) * 32), 4,
+                                                     row + (uint32_t)tmin(16 * piece + 4 * (lane & 3), left - 4), 0, 0, 0);
         }
     };
+    const std::integral_constant<int, 0> H0;
+    const std::integral_constant<int, 1> H1;
+    auto odd_end = [&](int kt) { return 16 * (kt >> 1) > left - 16 && left > 8 ? 8 : 0; };
 
     const int wn = wave % WN, wm = wave / WN;
     const int fr = lane & 31, fk = lane >> 5;                // a fragment's row and its half of 64 k
@@ -167,9 +168,8 @@ __device__ __forceinline__ void product(const Product& p) {
         for (int i = 0; i < FM; ++i) fb[to][i] = *reinterpret_cast<const u4*>(b + brow[i] * 128 + ((4 * fk + part) ^ ((brow[i] >> 1) & 7)) * 16);
     };
     auto read_scales = [&](int kt) {
-        const uint8_t* const b = smem + (kt >> 2 & 1) * ROWS * 32;
-        const int word = 2 * (kt & 3) + fk;
-        auto at = [&](int row) { return *reinterpret_cast<const uint32_t*>(b + (row >> 3) * 256 + (word ^ (2 * (row >> 3 & 3))) * 32 + (row & 7) * 4); };
+        const uint8_t* const b = smem + (kt >> 2 & 1) * ROWS * 32 + (kt & 1) * 8 + odd_end(kt) + 4 * fk;
+        auto at = [&](int row) { return *reinterpret_cast<const uint32_t*>(b + row * 32 + ((kt >> 1 & 1) ^ (row >> 3 & 1)) * 16); };
 #pragma unroll
         for (int i = 0; i < FN; ++i) na[i] = at(arow[i]);
 #pragma unroll
@@ -215,7 +215,8 @@ __device__ __forceinline__ void product(const Product& p) {
             if (U == 0 && N1) fetch(buf ^ 1, kt + 1, EARLY, LOADS);
             if (last && N2) {
                 fetch(buf, kt + 2, 0, EARLY);
-                fetch_scales((kt + 1) / 4 + 1, (kt + 1) & 3);
+                if (((kt + 1) & 3) == 0) fetch_scales((kt + 1) / 4 + 1, H0);
+                if (((kt + 1) & 3) == 1) fetch_scales((kt + 1) / 4 + 1, H1);
             }
             if (ACTIVE) {
                 products(last && N1 ? AHEAD : 0, FN);
@@ -242,15 +243,18 @@ __device__ __forceinline__ void product(const Product& p) {
         if (steps > 1) tile_step(steps - 2, std::true_type(), std::false_type(), act);
         tile_step(steps - 1, std::false_type(), std::false_type(), act);
     };
-    fetch_scales(0, 0);
-    fetch_scales(0, 1);
-    fetch_scales(0, 2);
-    fetch_scales(0, 3);
+    if (left > 8) {
+        fetch_scales(0, H0);
+        fetch_scales(0, H1);
+    } else {
+        fetch_words(H0);
+        fetch_words(H1);
+    }
     fetch(0, 0, 0, LOADS);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (steps > 1) {
         fetch(1, 1, 0, EARLY);
-        fetch_scales(1, 0);
+        fetch_scales(1, H0);
     }
     const bool active = wm * (TM / WM) < t.rows;
     if (active) sums(std::true_type());
