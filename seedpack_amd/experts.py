@@ -13,13 +13,21 @@ both.
 
 The reference has no counterpart: it packs a mixture's tensors like any others and leaves their use to llama.cpp.
 """
+import functools
+
 import numpy as np
 
+from . import device as dev
 from ._lib import check, lib
 from .linear import _ids, _not_captured, _out, _rows, _scratch
-from . import device as dev
 
 SCORE = {"softmax": 0, "sigmoid": 1}
+_I32, _F32 = np.dtype(np.int32), np.dtype(np.float32)
+
+
+@functools.lru_cache(256)
+def _route_work_bytes(rows, experts, each):
+    return lib().spa_route_work_bytes(rows, experts, each, 1)
 
 
 class Routing:
@@ -38,6 +46,13 @@ class Routing:
             raise ValueError(f"weights {weights.shape} {weights.dtype} beside which {which.shape}")
         self.which, self.order, self.starts, self.weights = which, order, starts, weights
 
+    @classmethod
+    def _of(cls, which, order, starts, weights):
+        """of arrays that a call here has looked at"""
+        r = cls.__new__(cls)
+        r.which, r.order, r.starts, r.weights = which, order, starts, weights
+        return r
+
     @property
     def experts(self):
         return self.starts.size - 1
@@ -47,8 +62,8 @@ def _made(name, a, shape, dtype, stream):
     if a is None:
         _not_captured(stream, f"result ({name})")
         return dev.DeviceArray(shape, dtype)
-    if a.dtype != dtype or a.shape != shape:
-        raise ValueError(f"{name} is {a.shape} {a.dtype}, {shape} {np.dtype(dtype)} is needed")
+    if a.dtype is not dtype and a.dtype != dtype or a.shape != shape:
+        raise ValueError(f"{name} is {a.shape} {a.dtype}, {shape} {dtype} is needed")
     return a
 
 
@@ -70,19 +85,19 @@ def route(logits, each, score="softmax", bias=None, groups=1, keep=1, best=2, re
     score = _score(score)
     if bias is not None and (bias.dtype != np.float32 or bias.size != e):
         raise ValueError(f"bias {bias.shape} {bias.dtype} for {e} experts (float32)")
-    which = _made("which", which, (m, each), np.int32, stream)
-    weights = _made("weights", weights, (m, each), np.float32, stream)
+    which = _made("which", which, (m, each), _I32, stream)
+    weights = _made("weights", weights, (m, each), _F32, stream)
     L = lib()
     p, n = None, 0
     if sort:
-        order = _made("order", order, (m * each,), np.int32, stream)
-        starts = _made("starts", starts, (e + 1,), np.int32, stream)
-        held, p, n = _scratch(L.spa_route_work_bytes(m, e, each, 1), work, stream)
+        order = _made("order", order, (m * each,), _I32, stream)
+        starts = _made("starts", starts, (e + 1,), _I32, stream)
+        held, p, n = _scratch(_route_work_bytes(m, e, each), work, stream)
     elif order is not None or starts is not None:
         raise ValueError("order and starts are written with sort only")
     check(L.spa_route(logits.ptr, kind, m, e, ld, score, None if bias is None else bias.ptr, groups, keep, best, each, bool(renorm),
                       scale, which.ptr, weights.ptr, order.ptr if sort else None, starts.ptr if sort else None, p, n, stream))
-    return Routing(which, order, starts, weights)
+    return Routing._of(which, order, starts, weights)
 
 
 def route_backward(logits, which, dweights, score="softmax", renorm=True, scale=1.0, dlogits=None, logits_stride=None,
@@ -105,12 +120,12 @@ def by_expert(which, experts, order=None, starts=None, work=None, stream=None):
     without an expert last) and where each expert's begin"""
     if which.dtype != np.int32 or len(which.shape) != 2:
         raise ValueError(f"which is {which.shape} {which.dtype}: (rows, each) int32 is taken")
-    order = _made("order", order, (which.size,), np.int32, stream)
-    starts = _made("starts", starts, (experts + 1,), np.int32, stream)
+    order = _made("order", order, (which.size,), _I32, stream)
+    starts = _made("starts", starts, (experts + 1,), _I32, stream)
     L = lib()
     keep, p, n = _scratch(L.spa_by_expert_work_bytes(which.size, experts), work, stream)
     check(L.spa_by_expert(which.ptr, which.size, experts, order.ptr, starts.ptr, p, n, stream))
-    return Routing(which, order, starts)
+    return Routing._of(which, order, starts, None)
 
 
 def _slots(y, weights, which, experts, y_stride):
@@ -143,7 +158,7 @@ def join_backward(y, weights, dout, which=None, experts=None, dy=None, dweights=
     if mo != m or dout.dtype != y.dtype:
         raise ValueError(f"dout is {dout.shape} {dout.dtype} for {m} rows of {y.dtype}")
     dy, ldy = _out("dy", dy, m * each, n, y.dtype, dy_stride, stream)
-    dweights = _made("dweights", dweights, (m, each), np.float32, stream)
+    dweights = _made("dweights", dweights, (m, each), _F32, stream)
     check(lib().spa_join_backward(y.ptr, kind, m, each, n, ld, weights.ptr, None if which is None else which.ptr, experts or 0, dout.ptr,
                                   ldd, dy.ptr, ldy, dweights.ptr, stream))
     return dy, dweights

@@ -13,6 +13,8 @@ rounded once. Arrays, streams, strides, workspaces and capture as in linear.
 
 The reference has no counterpart: it codes the bytes of such tensors, and leaves their use to llama.cpp.
 """
+import functools
+
 import numpy as np
 
 from . import device as dev
@@ -23,6 +25,11 @@ from .linear import ACT, _KIND, _not_captured, _out, _rows, _scratch
 def pitch(cols):
     """the blocks that a row of `cols` numbers takes: whole runs of eight"""
     return -(-cols // 256) * 8
+
+
+@functools.lru_cache(256)
+def _work_bytes(x_rows, cols, n, experts, slots, gated):
+    return lib().spa_mx4_product_work_bytes(x_rows, cols, n, experts, slots, gated)
 
 
 class Matrix:
@@ -113,9 +120,8 @@ def project(x, w, routing=None, out=None, dtype=np.uint16, out_stride=None, work
     matrix, from row p of x, or from row p // each where x has a row for each of the routing's; rows of slots without an
     expert are left as they are. Of out's type or dtype (bf16 bits as uint16)."""
     out, ld, kind, experts, order, starts, slots = _product(x, w, routing, out, dtype, out_stride, stream)
-    L = lib()
-    keep, p, n = _scratch(L.spa_mx4_product_work_bytes(x.rows, x.cols, w.rows, experts, slots, 0), work, stream)
-    check(L.spa_mx4_project(x.codes.ptr, x.scales.ptr, x.rows, x.cols, w.codes.ptr, w.scales.ptr, w.rows, experts, order, starts, slots,
+    keep, p, n = _scratch(_work_bytes(x.rows, x.cols, w.rows, experts, slots, 0), work, stream)
+    check(lib().spa_mx4_project(x.codes.ptr, x.scales.ptr, x.rows, x.cols, w.codes.ptr, w.scales.ptr, w.rows, experts, order, starts, slots,
                             out.ptr, kind, ld, p, n, stream))
     return out
 
@@ -127,8 +133,7 @@ def gated(x, gate, up, act="silu", routing=None, out=None, dtype=np.uint16, out_
     if act not in ACT:
         raise ValueError(f"unknown activation {act!r}: {sorted(ACT)}")
     out, ld, kind, experts, order, starts, slots = _product(x, gate, routing, out, dtype, out_stride, stream)
-    L = lib()
-    keep, p, n = _scratch(L.spa_mx4_product_work_bytes(x.rows, x.cols, gate.rows, experts, slots, 1), work, stream)
-    check(L.spa_mx4_gated(x.codes.ptr, x.scales.ptr, x.rows, x.cols, gate.codes.ptr, gate.scales.ptr, up.codes.ptr, up.scales.ptr,
+    keep, p, n = _scratch(_work_bytes(x.rows, x.cols, gate.rows, experts, slots, 1), work, stream)
+    check(lib().spa_mx4_gated(x.codes.ptr, x.scales.ptr, x.rows, x.cols, gate.codes.ptr, gate.scales.ptr, up.codes.ptr, up.scales.ptr,
                           gate.rows, ACT[act], experts, order, starts, slots, out.ptr, kind, ld, p, n, stream))
     return out
