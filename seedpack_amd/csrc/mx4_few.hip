@@ -53,6 +53,7 @@ __device__ __forceinline__ void few(const Product& p, int split) {
     if (t.rows == 0) return;
     const int64_t row16 = (int64_t)p.pitch * 16;
     const uint8_t *wc[NT][1 + TWO], *ws[NT][1 + TWO], *xc[MT], *xs[MT];
+    int out[MT];                                             // a lane's rows of the output
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const int64_t row = (int64_t)t.expert * p.n + tmin(n0 + 16 * i + r, p.n - 1);
@@ -65,7 +66,8 @@ __device__ __forceinline__ void few(const Product& p, int split) {
     }
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-        const int64_t row = input_row(p, t.first + tmin(16 * j + r, t.rows - 1));
+        out[j] = output_row(p, t.first + tmin(16 * j + r, t.rows - 1));
+        const int64_t row = input_row(p, out[j]);
         xc[j] = p.xc + row * row16;
         xs[j] = p.xs + row * p.pitch;
     }
@@ -127,7 +129,7 @@ __device__ __forceinline__ void few(const Product& p, int split) {
                 }
             }
             // lane: input row r, weight rows 4 g + c
-            const int64_t row = 16 * j + r < t.rows ? output_row(p, t.first + 16 * j + r) : -1;
+            const int64_t row = 16 * j + r < t.rows ? out[j] : -1;
             const int n = n0 + 16 * i + 4 * g;
             if (row < 0 || n >= p.n) continue;
             const int64_t to = row * p.ldy + n;

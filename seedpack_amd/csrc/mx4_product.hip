@@ -36,8 +36,8 @@ enum Out { OUT_PLAIN, OUT_GATED, OUT_PART };                  // PART: float32 s
 // An activation's value by the hardware's 2^x and 1 / x, both good to an ulp: the logit's rounding in units of log2 costs
 // |logit| 2^-24 of the result. (With a logit of two parts, as the products of 16 bits have it, the outputs of 128 x 256 take
 // 5 us, not 3.)
-__device__ __forceinline__ float act_short(float g, int act) {
-    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * lin::act_logit(g, act)));
+template <int ACT> __device__ __forceinline__ float act_short(float g) {
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * lin::act_logit(g, ACT)));
 }
 
 template <int TN, int TM, int WN, int WM, int OUT>
@@ -94,7 +94,7 @@ __device__ __forceinline__ void product(const Product& p) {
     auto tile_row = [&](int r) -> uint32_t {
         if (r < TN) return (uint32_t)tmin(r - (TWO && r >= TNE ? TNE : 0), p.n - 1 - n0);
         const int m = tmin(r - TN, t.rows - 1);
-        return p.experts ? (uint32_t)input_row(p, t.first + m) : (uint32_t)m;
+        return p.experts ? (uint32_t)input_row(p, output_row(p, t.first + m)) : (uint32_t)m;
     };
     uint32_t off[LOADS], soff[2];
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((lr >> 1) + 4 * (wave & 1));
@@ -140,6 +140,9 @@ __device__ __forceinline__ void product(const Product& p) {
     auto odd_end = [&](int kt) { return 16 * (kt >> 1) > left - 16 && left > 8 ? 8 : 0; };
 
     const int wn = wave % WN, wm = wave / WN;
+    // the output's rows of the wave, one a lane: looked up as the outputs leave, each run of them would wait for memory
+    static_assert(TM / WM == 64, "tile shape");
+    const int out_rows = OUT == OUT_PART || wm * 64 + lane >= t.rows ? -1 : output_row(p, t.first + wm * 64 + lane);
     const int fr = lane & 31, fk = lane >> 5;                // a fragment's row and its half of 64 k
     int arow[FN], brow[FM];
 #pragma unroll
@@ -266,69 +269,70 @@ __device__ __forceinline__ void product(const Product& p) {
     if (!active) return;
     constexpr int PITCH = COLS + 4;
     float* const stage = reinterpret_cast<float*>(mem) + wave * 32 * PITCH;
-    const int size = p.kind == SRC_F32 ? 4 : 2;
-    const bool wide16 = (p.ldy * size & 15) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+    // (a body for each activation and type: with both activations worked out for every output, or choices among types, the
+    // outputs of 256 x 128 gated take 6 us)
+    auto leave = [&](auto kind, auto act) {
+        constexpr int KIND = decltype(kind)::value, ACT = decltype(act)::value;
+        const bool wide16 = (p.ldy * (KIND == SRC_F32 ? 4 : 2) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
+        for (int j = 0; j < FM; ++j) {
 #pragma unroll
-        for (int i = 0; i < (TWO ? FN / 2 : FN); ++i)
+            for (int i = 0; i < (TWO ? FN / 2 : FN); ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f4 v;
+                for (int q = 0; q < 4; ++q) {
+                    f4 v;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    v[c] = acc[i][j][4 * q + c];
-                    if (TWO) v[c] = act_short(v[c], p.act) * acc[i + (TWO ? FN / 2 : 0)][j][4 * q + c];
+                    for (int c = 0; c < 4; ++c) {
+                        v[c] = acc[i][j][4 * q + c];
+                        if (TWO) v[c] = act_short<ACT>(v[c]) * acc[i + (TWO ? FN / 2 : 0)][j][4 * q + c];
+                    }
+                    *reinterpret_cast<f4*>(stage + fr * PITCH + 32 * i + 8 * q + 4 * fk) = v;
                 }
-                *reinterpret_cast<f4*>(stage + fr * PITCH + 32 * i + 8 * q + 4 * fk) = v;
-            }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int m0 = wm * (TM / WM) + 32 * j;
-        for (int u = lane; u < 32 * (COLS / 8); u += 64) {
-            const int r = u / (COLS / 8), c = u % (COLS / 8) * 8, n = n0 + wn * COLS + c;
-            if (m0 + r >= t.rows || n >= p.n) continue;
-            const f4 a = *reinterpret_cast<const f4*>(stage + r * PITCH + c), b = *reinterpret_cast<const f4*>(stage + r * PITCH + c + 4);
-            const bool whole = n + 8 <= p.n;
-            if (OUT == OUT_PART) {
-                float* const y = p.part + ((int64_t)piece * p.m + t.first + m0 + r) * p.n + n;
-                if (whole) {
-                    __builtin_memcpy(y, &a, 16);                  // at any number's address
-                    __builtin_memcpy(y + 4, &b, 16);
-                } else {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int m0 = wm * (TM / WM) + 32 * j;
+            for (int u = lane; u < 32 * (COLS / 8); u += 64) {
+                const int r = u / (COLS / 8), c = u % (COLS / 8) * 8, n = n0 + wn * COLS + c;
+                const int64_t row = OUT == OUT_PART ? 0 : __shfl(out_rows, 32 * j + r);
+                if (m0 + r >= t.rows || n >= p.n || row < 0) continue;
+                const f4 a = *reinterpret_cast<const f4*>(stage + r * PITCH + c), b = *reinterpret_cast<const f4*>(stage + r * PITCH + c + 4);
+                const bool whole = n + 8 <= p.n;
+                if constexpr (KIND == SRC_F32) {
+                    float* const y = OUT == OUT_PART ? p.part + ((int64_t)piece * p.m + t.first + m0 + r) * p.n + n : static_cast<float*>(p.y) + row * p.ldy + n;
+                    if (whole && wide16 && OUT != OUT_PART) {
+                        __builtin_nontemporal_store(a, reinterpret_cast<f4*>(y));
+                        __builtin_nontemporal_store(b, reinterpret_cast<f4*>(y) + 1);
+                    } else if (whole) {
+                        __builtin_memcpy(y, &a, 16);              // at any number's address
+                        __builtin_memcpy(y + 4, &b, 16);
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (n + k < p.n) y[k] = k < 4 ? a[k & 3] : b[k & 3];
-                }
-                continue;
-            }
-            const int64_t row = output_row(p, t.first + m0 + r);
-            if (row < 0) continue;
-            if (p.kind == SRC_F32) {
-                float* const y = static_cast<float*>(p.y) + row * p.ldy + n;
-                if (whole && wide16) {
-                    __builtin_nontemporal_store(a, reinterpret_cast<f4*>(y));
-                    __builtin_nontemporal_store(b, reinterpret_cast<f4*>(y) + 1);
+                        for (int k = 0; k < 8; ++k)
+                            if (n + k < p.n) y[k] = k < 4 ? a[k & 3] : b[k & 3];
+                    }
                 } else {
+                    uint16_t* const y = static_cast<uint16_t*>(p.y) + row * p.ldy + n;
+                    const u4 v = {lin::narrow2(a[0], a[1], KIND), lin::narrow2(a[2], a[3], KIND), lin::narrow2(b[0], b[1], KIND), lin::narrow2(b[2], b[3], KIND)};
+                    if (whole && wide16) {
+                        __builtin_nontemporal_store(v, reinterpret_cast<u4*>(y));
+                    } else if (whole) {
+                        __builtin_memcpy(y, &v, 16);
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (n + k < p.n) y[k] = k < 4 ? a[k & 3] : b[k & 3];
-                }
-            } else {
-                uint16_t* const y = static_cast<uint16_t*>(p.y) + row * p.ldy + n;
-                const u4 v = {lin::narrow2(a[0], a[1], p.kind), lin::narrow2(a[2], a[3], p.kind), lin::narrow2(b[0], b[1], p.kind), lin::narrow2(b[2], b[3], p.kind)};
-                if (whole && wide16) {
-                    __builtin_nontemporal_store(v, reinterpret_cast<u4*>(y));
-                } else if (whole) {
-                    __builtin_memcpy(y, &v, 16);                  // at any number's address
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (n + k < p.n) y[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+                        for (int k = 0; k < 8; ++k)
+                            if (n + k < p.n) y[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+                    }
                 }
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+    };
+    auto of_kind = [&](auto kind) {
+        if (TWO && p.act == lin::ACT_GELU) leave(kind, std::integral_constant<int, lin::ACT_GELU>());
+        else leave(kind, std::integral_constant<int, lin::ACT_SILU>());
+    };
+    if (OUT == OUT_PART || p.kind == SRC_F32) of_kind(std::integral_constant<int, SRC_F32>());
+    else if (p.kind == SRC_BF16) of_kind(std::integral_constant<int, SRC_BF16>());
+    else of_kind(std::integral_constant<int, SRC_F16>());
 }
 
 template <int TN, int TM, int WN, int WM, int OUT>

@@ -67,17 +67,14 @@ __device__ __forceinline__ Tile tile_at(const Product& p, int id, int height) {
     return Tile{0, 0, 0};
 }
 
-// the input row of a tile's row, and the output's; slots outside 0..m-1 read the first row and have no output (-1)
-__device__ __forceinline__ int64_t input_row(const Product& p, int at) {
-    if (!p.experts) return at;
-    const int slot = p.order[at];
-    return (uint32_t)slot < (uint32_t)p.m ? slot / p.each : 0;
-}
-__device__ __forceinline__ int64_t output_row(const Product& p, int at) {
+// What a tile's row `at` is: the output's row, -1 of a slot outside 0..m-1, which has none; and the input's (the first, of such
+// a slot)
+__device__ __forceinline__ int output_row(const Product& p, int at) {
     if (!p.experts) return at;
     const int slot = p.order[at];
     return (uint32_t)slot < (uint32_t)p.m ? slot : -1;
 }
+__device__ __forceinline__ int input_row(const Product& p, int output) { return p.experts ? tmax(output, 0) / p.each : output; }
 
 }  // namespace mx
 }  // namespace spa
