@@ -23,6 +23,7 @@ struct Product {
     int experts;                         // 0: one matrix for all rows
     const int32_t *order, *starts;
     int each;                            // slot p takes row p / each
+    uint32_t magic;                      // the upper half of p times it is p / each; 0: divide
     void* y;
     int64_t ldy;
     int kind, act;

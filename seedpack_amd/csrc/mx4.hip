@@ -364,6 +364,8 @@ int product(const char* who, Product p, int64_t x_rows, int64_t k, int64_t n, in
         // rows are read at 32-bit offsets from the matrix's first
         if (x_rows * p.pitch * 16 >= (1ll << 32)) return fail(SPA_ERR_ARG, "%s: %lld rows of %lld by expert are more than 4 GiB of codes", who, (long long)x_rows, (long long)k);
         p.each = (int)(slots / x_rows);
+        // 2^32 / each, rounded up by less than 1: exact where what slot times that adds stays below 1 / each
+        p.magic = p.each > 1 && slots * p.each < (1ll << 32) ? (uint32_t)((1ull << 32) / p.each + 1) : 0;
         p.experts = (int)experts;
         p.order = order;
         p.starts = starts;

@@ -49,7 +49,7 @@ __device__ __forceinline__ void few(const Product& p, int split) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int width = W / split * 16 * NT, nt = (p.n + width - 1) / width;
     const int part = wave % split, n0 = blockIdx.x % nt * width + wave / split * 16 * NT;
-    const Tile t = tile_at(p, blockIdx.x / nt, 16 * MT);
+    const Tile t = tile_at(p, p.experts > 64 ? Tiles{} : tiles_of(p, 16 * MT), blockIdx.x / nt, 16 * MT);
     if (t.rows == 0) return;
     const int64_t row16 = (int64_t)p.pitch * 16;
     const uint8_t *wc[NT][1 + TWO], *ws[NT][1 + TWO], *xc[MT], *xs[MT];

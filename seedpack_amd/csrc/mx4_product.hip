@@ -57,7 +57,8 @@ __device__ __forceinline__ void product(const Product& p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Tiles are dealt so that each of the 8 XCDs, which take workgroups in turn, has a run of neighbours: its L2 then
     // serves their shared rows. By expert a tile of inputs is followed through all of its expert's weights.
-    const int nt = (p.n + TNE - 1) / TNE, mt = p.experts ? tiles_of(p, TM) : (p.m + TM - 1) / TM;
+    const Tiles tiles = tiles_of(p, TM);
+    const int nt = (p.n + TNE - 1) / TNE, mt = tiles.total;
     const int total = nt * mt;
     int id, piece = 0;
     bool second = false;                                     // of the gated form's two matrices, each a product of its own
@@ -79,12 +80,12 @@ __device__ __forceinline__ void product(const Product& p) {
     int n0;
     Tile t;
     if (p.experts) {
-        t = tile_at(p, id / nt, TM);
+        t = tile_at(p, tiles, id / nt, TM);
         n0 = id % nt * TNE;
     } else {
         constexpr int GROUP = 8;
         const int band = id / (GROUP * nt), in = id - band * GROUP * nt, height = tmin(GROUP, mt - band * GROUP);
-        t = tile_at(p, band * GROUP + in % height, TM);
+        t = tile_at(p, tiles, band * GROUP + in % height, TM);
         n0 = in / height * TNE;
     }
 

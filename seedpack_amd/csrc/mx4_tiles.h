@@ -24,21 +24,40 @@ __device__ __forceinline__ Span span_of(const Product& p, int e) {
     return Span{begin, tmin(tmax(p.starts[e + 1], begin), p.m)};
 }
 
-// the tiles that there are
-__device__ __forceinline__ int tiles_of(const Product& p, int height) {
-    int sum = 0;
-    for (int e = threadIdx.x & 63; e < p.experts; e += 64) {
-        const Span s = span_of(p, e);
-        sum += (s.end - s.begin + height - 1) / height;
-    }
+// inclusive sums over the wave
+__device__ __forceinline__ int running(int v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
-    return __builtin_amdgcn_readfirstlane(sum);
+    for (int s = 1; s < 64; s <<= 1) {
+        const int t = __shfl_up(v, s);
+        if (lane >= s) v += t;
+    }
+    return v;
 }
 
-// Tile `id` of `height` rows; no rows behind the last. An expert's tiles follow those of the experts before it: each
-// lane counts the tiles of its own, 64 experts at a time.
-__device__ __forceinline__ Tile tile_at(const Product& p, int id, int height) {
+// The tiles of a product of up to 64 experts, an expert a lane; of more experts they are counted again for each question.
+struct Tiles {
+    Span span;
+    int own, sum, total;                 // an expert's tiles, with those before it, and all
+};
+__device__ __forceinline__ Tiles tiles_of(const Product& p, int height) {
+    const int lane = threadIdx.x & 63;
+    Tiles t{};
+    if (!p.experts) {
+        t.total = (p.m + height - 1) / height;
+        return t;
+    }
+    for (int e0 = 0; e0 < p.experts; e0 += 64) {
+        t.span = span_of(p, e0 + lane);
+        t.own = (t.span.end - t.span.begin + height - 1) / height;
+        t.sum = running(t.own);
+        t.total += __builtin_amdgcn_readlane(t.sum, 63);
+    }
+    return t;
+}
+
+// Tile `id` of `height` rows; no rows behind the last. An expert's tiles follow those of the experts before it.
+__device__ __forceinline__ Tile tile_at(const Product& p, const Tiles& all, int id, int height) {
     if (!p.experts) {
         const int first = id * height;
         return Tile{0, first, first < p.m ? tmin(height, p.m - first) : 0};
@@ -46,23 +65,21 @@ __device__ __forceinline__ Tile tile_at(const Product& p, int id, int height) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 64) {
-        const auto [begin, end] = span_of(p, e0 + lane);
-        const int own = (end - begin + height - 1) / height;
-        int sum = own;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int v = __shfl_up(sum, s);
-            if (lane >= s) sum += v;
+        Tiles t = all;
+        if (p.experts > 64) {
+            t.span = span_of(p, e0 + lane);
+            t.own = (t.span.end - t.span.begin + height - 1) / height;
+            t.sum = running(t.own);
         }
-        const uint64_t past = __ballot(before + sum > id);
+        const uint64_t past = __ballot(before + t.sum > id);
         if (past) {
             const int at = __builtin_ctzll(past);
-            const int b = __shfl(begin, at), n = __shfl(end, at), in = id - before - __shfl(sum - own, at);
-            const int first = b + in * height;
-            return Tile{__builtin_amdgcn_readfirstlane(e0 + at), __builtin_amdgcn_readfirstlane(first),
-                        __builtin_amdgcn_readfirstlane(tmin(height, n - first))};
+            const int begin = __builtin_amdgcn_readlane(t.span.begin, at), end = __builtin_amdgcn_readlane(t.span.end, at);
+            const int in = id - before - (__builtin_amdgcn_readlane(t.sum, at) - __builtin_amdgcn_readlane(t.own, at));
+            const int first = begin + in * height;
+            return Tile{e0 + at, first, tmin(height, end - first)};
         }
-        before += __shfl(sum, 63);
+        before += __builtin_amdgcn_readlane(t.sum, 63);
     }
     return Tile{0, 0, 0};
 }
@@ -74,7 +91,11 @@ __device__ __forceinline__ int output_row(const Product& p, int at) {
     const int slot = p.order[at];
     return (uint32_t)slot < (uint32_t)p.m ? slot : -1;
 }
-__device__ __forceinline__ int input_row(const Product& p, int output) { return p.experts ? tmax(output, 0) / p.each : output; }
+__device__ __forceinline__ int input_row(const Product& p, int output) {
+    if (!p.experts || p.each == 1) return tmax(output, 0);
+    const uint32_t slot = (uint32_t)tmax(output, 0);
+    return (int)(p.magic ? __umulhi(slot, p.magic) : slot / (uint32_t)p.each);
+}
 
 }  // namespace mx
 }  // namespace spa
