@@ -1,4 +1,4 @@
-// Reductions over 16 or 64 neighbouring lanes whose result every lane holds, by moves between lanes that need no LDS.
+// Reductions over 16, 32 or 64 neighbouring lanes whose result every lane holds, by moves between lanes that need no LDS.
 #pragma once
 
 #include "common.h"
@@ -50,19 +50,21 @@ template <int ROW, typename T> __device__ __forceinline__ void across_rows(T v, 
     __builtin_memcpy(&odd, c, sizeof(T));
 }
 
-// op over the L = 16 or 64 lanes of a row, in an order of its own that is the same for every lane: neighbours, pairs,
+// op over the L = 16, 32 or 64 lanes of a row, in an order of its own that is the same for every lane: neighbours, pairs,
 // and, the pairs being alike, mirrored fours and eights, then rows of 16.
 template <int L, typename T, typename F> __device__ __forceinline__ T over_row(T v, F op) {
     v = op(v, lane_move<0xb1>(v));                               // lanes 1 0 3 2
     v = op(v, lane_move<0x4e>(v));                               // lanes 2 3 0 1
     v = op(v, lane_move<0x141>(v));                              // eight lanes mirrored
     v = op(v, lane_move<0x140>(v));                              // sixteen lanes mirrored
-    if constexpr (L == 64) {
+    if constexpr (L >= 32) {
         T even, odd;
         across_rows<16>(v, even, odd);
         v = op(even, odd);
-        across_rows<32>(v, even, odd);
-        v = op(even, odd);
+        if constexpr (L == 64) {
+            across_rows<32>(v, even, odd);
+            v = op(even, odd);
+        }
     }
     return v;
 }

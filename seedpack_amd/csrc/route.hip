@@ -5,7 +5,7 @@
 // themselves (both scores rise with them), or, with a bias or groups, s + b in 64 bits, for keys are compared with each
 // other: in 32 bits one row in some thousands would have two of its experts' keys rounded across each other.
 //
-// A row's lanes, 16 or 64, hold its experts. A key carries its expert's number in its low bits (reversed: of equal
+// A row's lanes, 16, 32 or 64, hold its experts. A key carries its expert's number in its low bits (reversed: of equal
 // keys the lowest number wins), which makes all keys of a row different: each lane sorts its own few, and the
 // row's next expert is the largest of the lanes' heads, whose lane moves its list up.
 #include "../../include/seedpack_amd.h"
@@ -563,20 +563,21 @@ __global__ __launch_bounds__(1024) void k_route_few(const Route a, const Order o
 
 // How a routing is launched: 64 lanes a row where 16 would leave a long chain of work to few waves (4 rows of 256 experts in
 // groups: 13.8 us by 16 lanes), or hold more than 16 numbers each; four times the rows a workgroup of those where there are
-// enough, for fewer tiles to add up.
+// enough, for fewer tiles to add up. Else 16 lanes, or 32 for 129 to 256 experts without bias and groups (8191 rows of 256 in
+// float32: 8.8 us; by 64 lanes 14.8); with them 32 lose (21.5 us; by 16 lanes 17.9).
 struct Shape {
-    bool few, slim;          // one workgroup does all; 16 lanes a row
-    int threads, rows, reps; // rows of a workgroup at once, and how often
+    bool few;                       // one workgroup does all
+    int lanes, threads, rows, reps; // a row's lanes; rows of a workgroup at once, and how often
 };
 size_t group_lds(const Route& a, int rows) { return a.groups > 1 ? (size_t)rows * group_keys(a.experts, a.groups) * 8 : 0; }
 Shape shape_of(const Route& a, bool deep, bool sorted) {
     Shape s{};
     const int64_t slots = a.rows * a.each;
     s.few = sorted && a.rows <= 64 && slots <= FEW && order_lds(slots, a.experts) <= 50 * 1024 && group_lds(a, 16) <= 50 * 1024;
-    s.slim = a.experts <= (deep ? 256 : 128) && a.rows > 4096;
-    s.threads = s.slim && !deep ? 1024 : 512;
-    s.rows = s.threads / (s.slim ? 16 : 64);
-    s.reps = s.slim || a.rows <= 4096 ? 1 : 4;
+    s.lanes = a.rows <= 4096 || a.experts > 256 ? 64 : a.experts <= 128 || deep ? 16 : 32;
+    s.threads = s.lanes == 16 && !deep ? 1024 : 512;
+    s.rows = s.threads / s.lanes;
+    s.reps = s.lanes < 64 || a.rows <= 4096 ? 1 : 4;
     return s;
 }
 
@@ -606,11 +607,13 @@ template <int KIND, bool DEEP> int route_kind(const Route& a, Order& o, bool sor
         return SPA_OK;
     };
     int rc = SPA_OK;
-    if (s.slim) {
+    if (s.lanes == 16) {
         constexpr int T = DEEP ? 512 : 1024;
         if (a.experts <= 64) rc = go(k_route<KIND, 16, 4, DEEP, T>);
         else if (a.experts <= 128) rc = go(k_route<KIND, 16, 8, DEEP, T>);
         else if constexpr (DEEP) rc = go(k_route<KIND, 16, 16, DEEP, T>);
+    } else if (s.lanes == 32) {
+        if constexpr (!DEEP) rc = go(k_route<KIND, 32, 8, DEEP, 512>);
     } else {
         if (a.experts <= 64) rc = go(k_route<KIND, 64, 1, DEEP, 512>);
         else if (a.experts <= 128) rc = go(k_route<KIND, 64, 2, DEEP, 512>);

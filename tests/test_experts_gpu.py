@@ -87,6 +87,26 @@ def test_route_groups_and_bias(rows, e, each, groups, keep, best, biased, score,
     check_route(store(g.normal(0, 1, (rows, e)), kind), each, score, bias=bias, groups=groups, keep=keep, best=best)
 
 
+@pytest.mark.parametrize("rows", [64, 65, 4096, 4097, 4500])
+@pytest.mark.parametrize("e,each,groups", [(64, 32, 8), (65, 5, 5), (128, 8, 4), (129, 8, 3), (256, 32, 64), (257, 9, 1), (512, 3, 16), (1024, 8, 64)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_route_by_few_and_many_lanes(kind, e, each, groups, rows):
+    """each number of lanes a row, of a lane's experts and of a workgroup's rows, whole and partly masked, with ties"""
+    g = rng(10, rows, e)
+    l = store(g.normal(0, 1, (rows, e)), kind)
+    l[g.random(l.shape) < 0.2] = store(np.array([-np.inf]), kind)[0]
+    l[::9] = store(np.array([-np.inf]), kind)[0]
+    l[::7, ::3] = store(np.array([0.5]), kind)[0]
+    bias = g.normal(0, 0.2, e).astype(F32)
+    check_route(l, each, "softmax", renorm=False)
+    check_route(l, each, "sigmoid", scale=1.5)
+    check_route(l, each, "sigmoid", bias=bias)
+    if groups > 1:
+        least = -(-each * groups // e)
+        check_route(l, each, "softmax", bias=bias, groups=groups, keep=min(groups, least + 1), best=2)
+        check_route(l, each, "sigmoid", groups=groups, keep=least, best=1)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_bias_alone(score):
     g = rng(3)
