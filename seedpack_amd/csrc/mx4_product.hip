@@ -91,20 +91,33 @@ __device__ __forceinline__ void product(const Product& p) {
 
     const uint32_t row16 = (uint32_t)p.pitch * 16;
     const int64_t wfirst = (int64_t)t.expert * p.n + n0, xfirst = p.experts ? 0 : t.first;
-    // the byte offset, in rows, of tile row r from its operand's first; rows behind the last are the last
-    auto tile_row = [&](int r) -> uint32_t {
-        if (r < TN) return (uint32_t)tmin(r - (TWO && r >= TNE ? TNE : 0), p.n - 1 - n0);
-        const int m = tmin(r - TN, t.rows - 1);
-        return p.experts ? (uint32_t)input_row(p, output_row(p, t.first + m)) : (uint32_t)m;
-    };
+    // What the lane's input rows are, and its output's: each asked for at its own use, they would wait for memory one by one, so
+    // all are asked for here, and waited for behind the first fetches of weights.
+    constexpr int LW = TN / 8 / NW, LX = LOADS - LW;         // loads of weights, of inputs
+    const int wn = wave % WN, wm = wave / WN;
+    static_assert(TM / WM == 64, "tile shape");
+    int row[LX + 2];                                         // those of its loads, of its scales, and the output's
+    {
+        const int lr = lane >> 3;
+#pragma unroll
+        for (int j = 0; j < LX + 2; ++j) {
+            const int r = j < LX ? (j * NW + wave) * 8 + lr : j == LX ? wave * 32 + (lane >> 1) : wm * 64 + lane;
+            row[j] = tmin(r, t.rows - 1);                    // rows behind the last are the last
+        }
+        if (p.experts) {
+#pragma unroll
+            for (int j = 0; j < LX + 2; ++j) row[j] = p.order[t.first + row[j]];
+        }
+    }
+    // a weights' row of the tile, from the first
+    auto weight_row = [&](int r) { return (uint32_t)tmin(r - (TWO && r >= TNE ? TNE : 0), p.n - 1 - n0); };
     uint32_t off[LOADS], soff[2];
     const int lr = lane >> 3, chunk = (lane & 7) ^ ((lr >> 1) + 4 * (wave & 1));
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) off[j] = tile_row((j * NW + wave) * 8 + lr) * row16 + 16 * chunk;
+    for (int j = 0; j < LW; ++j) off[j] = weight_row((j * NW + wave) * 8 + lr) * row16 + 16 * chunk;
     // A wave's scales: 32 of the weights' rows by one load, 32 of the inputs' by another, two pieces of 16 bytes a row; the
     // pieces of every other run of 8 rows lie exchanged, for a fragment's reads.
-#pragma unroll
-    for (int h = 0; h < 2; ++h) soff[h] = tile_row(h * TN + wave * 32 + (lane >> 1)) * (uint32_t)p.pitch;
+    soff[0] = weight_row(wave * 32 + (lane >> 1)) * (uint32_t)p.pitch;
     const int spiece = 16 * ((lane & 1) ^ (lane >> 4 & 1));
     constexpr int RAW = 0x00027000;                               // a plain buffer of bytes
     auto buffer = [&](const uint8_t* b, int64_t first, int64_t row) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(b + first * row), 0, -1, RAW); };
@@ -140,10 +153,6 @@ __device__ __forceinline__ void product(const Product& p) {
     const std::integral_constant<int, 1> H1;
     auto odd_end = [&](int kt) { return 16 * (kt >> 1) > left - 16 && left > 8 ? 8 : 0; };
 
-    const int wn = wave % WN, wm = wave / WN;
-    // the output's rows of the wave, one a lane: looked up as the outputs leave, each run of them would wait for memory
-    static_assert(TM / WM == 64, "tile shape");
-    const int out_rows = OUT == OUT_PART || wm * 64 + lane >= t.rows ? -1 : output_row(p, t.first + wm * 64 + lane);
     const int fr = lane & 31, fk = lane >> 5;                // a fragment's row and its half of 64 k
     int arow[FN], brow[FM];
 #pragma unroll
@@ -247,14 +256,20 @@ __device__ __forceinline__ void product(const Product& p) {
         if (steps > 1) tile_step(steps - 2, std::true_type(), std::false_type(), act);
         tile_step(steps - 1, std::false_type(), std::false_type(), act);
     };
-    if (left > 8) {
-        fetch_scales(0, H0);
-        fetch_scales(0, H1);
-    } else {
-        fetch_words(H0);
-        fetch_words(H1);
+    fetch(0, 0, 0, LW);
+    if (left > 8) fetch_scales(0, H0);
+    else fetch_words(H0);
+    int out_rows = row[LX + 1] + t.first;                     // of the wave, one a lane
+    if (p.experts) {
+        out_rows = (uint32_t)row[LX + 1] < (uint32_t)p.m ? row[LX + 1] : -1;
+        input_rows<LX + 1>(p, row);
     }
-    fetch(0, 0, 0, LOADS);
+#pragma unroll
+    for (int j = 0; j < LX; ++j) off[LW + j] = (uint32_t)row[j] * row16 + 16 * chunk;
+    soff[1] = (uint32_t)row[LX] * (uint32_t)p.pitch;
+    if (left > 8) fetch_scales(0, H1);
+    else fetch_words(H1);
+    fetch(0, 0, LW, LOADS);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (steps > 1) {
         fetch(1, 1, 0, EARLY);

@@ -97,5 +97,19 @@ __device__ __forceinline__ int input_row(const Product& p, int output) {
     return (int)(p.magic ? __umulhi(slot, p.magic) : slot / (uint32_t)p.each);
 }
 
+// the input's rows of N slots; one outside 0..m-1 has the first
+template <int N> __device__ __forceinline__ void input_rows(const Product& p, int* slots) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) slots[i] = (uint32_t)slots[i] < (uint32_t)p.m ? slots[i] : 0;
+    if (p.each == 1) return;
+    if (p.magic) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) slots[i] = (int)__umulhi((uint32_t)slots[i], p.magic);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) slots[i] = (int)((uint32_t)slots[i] / (uint32_t)p.each);
+    }
+}
+
 }  // namespace mx
 }  // namespace spa
