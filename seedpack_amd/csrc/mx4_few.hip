@@ -53,7 +53,7 @@ __device__ __forceinline__ void few(const Product& p, int split) {
     if (t.rows == 0) return;
     const int64_t row16 = (int64_t)p.pitch * 16;
     const uint8_t *wc[NT][1 + TWO], *ws[NT][1 + TWO], *xc[MT], *xs[MT];
-    int out[MT];                                             // a lane's rows of the output
+    int in[MT], out[MT];                                     // a lane's rows of the input and the output
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const int64_t row = (int64_t)t.expert * p.n + tmin(n0 + 16 * i + r, p.n - 1);
@@ -65,11 +65,18 @@ __device__ __forceinline__ void few(const Product& p, int split) {
         }
     }
 #pragma unroll
+    for (int j = 0; j < MT; ++j) in[j] = out[j] = t.first + tmin(16 * j + r, t.rows - 1);
+    if (p.experts) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) in[j] = p.order[out[j]];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) out[j] = (uint32_t)in[j] < (uint32_t)p.m ? in[j] : -1;
+        input_rows<MT>(p, in);
+    }
+#pragma unroll
     for (int j = 0; j < MT; ++j) {
-        out[j] = output_row(p, t.first + tmin(16 * j + r, t.rows - 1));
-        const int64_t row = input_row(p, out[j]);
-        xc[j] = p.xc + row * row16;
-        xs[j] = p.xs + row * p.pitch;
+        xc[j] = p.xc + in[j] * row16;
+        xs[j] = p.xs + in[j] * (int64_t)p.pitch;
     }
     f4 acc[1 + TWO][NT][MT];
 #pragma unroll

@@ -84,20 +84,13 @@ __device__ __forceinline__ Tile tile_at(const Product& p, const Tiles& all, int 
     return Tile{0, 0, 0};
 }
 
-// What a tile's row `at` is: the output's row, -1 of a slot outside 0..m-1, which has none; and the input's (the first, of such
-// a slot)
+// The output's row of a tile's row `at`; -1 of a slot outside 0..m-1, which has none.
 __device__ __forceinline__ int output_row(const Product& p, int at) {
     if (!p.experts) return at;
     const int slot = p.order[at];
     return (uint32_t)slot < (uint32_t)p.m ? slot : -1;
 }
-__device__ __forceinline__ int input_row(const Product& p, int output) {
-    if (!p.experts || p.each == 1) return tmax(output, 0);
-    const uint32_t slot = (uint32_t)tmax(output, 0);
-    return (int)(p.magic ? __umulhi(slot, p.magic) : slot / (uint32_t)p.each);
-}
-
-// the input's rows of N slots; one outside 0..m-1 has the first
+// The input's rows of N slots; one outside 0..m-1 has the first.
 template <int N> __device__ __forceinline__ void input_rows(const Product& p, int* slots) {
 #pragma unroll
     for (int i = 0; i < N; ++i) slots[i] = (uint32_t)slots[i] < (uint32_t)p.m ? slots[i] : 0;
