@@ -58,7 +58,7 @@ __device__ __forceinline__ void product(const Product& p) {
     // Tiles are dealt so that each of the 8 XCDs, which take workgroups in turn, has a run of neighbours: its L2 then
     // serves their shared rows. By expert a tile of inputs is followed through all of its expert's weights.
     const Tiles tiles = tiles_of(p, TM);
-    const int nt = (p.n + TNE - 1) / TNE, mt = tiles.total;
+    const int nt = (p.n + TNE - 1) / TNE, mt = tmin(tiles.total, most_tiles(p, TM));   // more only where starts do not rise
     const int total = nt * mt;
     int id, piece = 0;
     bool second = false;                                     // of the gated form's two matrices, each a product of its own

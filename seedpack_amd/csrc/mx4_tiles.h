@@ -11,8 +11,8 @@ struct Tile {
 };
 
 // The tiles that there may be: every expert with rows has one that is not full.
-inline int64_t most_tiles(const Product& p, int height) {
-    if (!p.experts) return ((int64_t)p.m + height - 1) / height;
+__host__ __device__ inline int most_tiles(const Product& p, int height) {
+    if (!p.experts) return (p.m + height - 1) / height;
     return p.m / height + (p.m < p.experts ? p.m : p.experts);
 }
 

@@ -703,7 +703,8 @@ __global__ __launch_bounds__(256) void k_route_back(const Back a) {
         g[h] = (float)(a.score == SIGMOID && mine[h] >= 0 ? v[h] * logistic(-l[h]) : v[h]);
     }
     if (whole) {
-        const float f = (float)(row_sum<L>(sum) / total);
+        sum = row_sum<L>(sum);
+        const float f = total == 0.f ? 0.f : (float)(sum / total);   // a row of -inf has no shares
 #pragma unroll
         for (int j = 0; j < PER; ++j) p[j] = -p[j] * f;
     }
@@ -776,7 +777,7 @@ int check_shape(const char* who, int kind, int64_t rows, int64_t experts, int64_
     if (score != SOFTMAX && score != SIGMOID) return fail(SPA_ERR_ARG, "%s: unknown score %d", who, score);
     if (experts < 1 || experts > MOST_EXPERTS) return fail(SPA_ERR_ARG, "%s: %lld experts (1 to %d are taken)", who, (long long)experts, MOST_EXPERTS);
     if (each < 1 || each > MOST_EACH || each > experts) return fail(SPA_ERR_ARG, "%s: %lld of %lld experts a row (1 to %d are taken)", who, (long long)each, (long long)experts, MOST_EACH);
-    if (rows < 0 || rows * each > INT32_MAX - 1024 || rows > INT32_MAX || stride < experts) return fail(SPA_ERR_ARG, "%s: bad shape %lld x %lld, stride %lld", who, (long long)rows, (long long)experts, (long long)stride);
+    if (rows < 0 || rows > INT32_MAX || rows * each > INT32_MAX - 1024 || stride < experts) return fail(SPA_ERR_ARG, "%s: bad shape %lld x %lld, stride %lld", who, (long long)rows, (long long)experts, (long long)stride);
     return SPA_OK;
 }
 int check_work(const char* who, const void* work, uint64_t have, uint64_t need) {
