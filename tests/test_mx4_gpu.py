@@ -8,6 +8,7 @@ gated: with g and v off by dg and dv, act(g) v is off by 1.13 dg |v| + |act(g)| 
 below 1.13), and by the activation's own arithmetic: a logistic good to 4 steps of 2^-24 and the rounding of its logit, which
 costs |logit| 2^-23 of it at most: silu |g|, gelu 1.6 (|g| + 0.045 |g|^3), where the value is above 2^-24 of |g| (logits below
 18)."""
+import functools
 import sys
 
 import numpy as np
@@ -174,8 +175,12 @@ def check_product(x, w, got, kind):
 
 
 def check_gated(x, gate, upw, act, got, kind):
-    g, v = x @ gate.T, x @ upw.T
-    dg, dv = lost(x.shape[1], abs(x) @ abs(gate).T), lost(x.shape[1], abs(x) @ abs(upw).T)
+    k = x.shape[1]
+    close_gated(x @ gate.T, x @ upw.T, lost(k, abs(x) @ abs(gate).T), lost(k, abs(x) @ abs(upw).T), act, got, kind)
+
+
+def close_gated(g, v, dg, dv, act, got, kind):
+    """dg, dv: what the gate's and the up projection's sums may be off by"""
     a = oracle.act(g, act)
     logit = abs(g) if act == "silu" else 1.6 * (abs(g) + 0.045 * abs(g) ** 3)
     own = np.minimum(logit, 18) * 2.0 ** -23 + 6 * 2.0 ** -24
@@ -208,6 +213,42 @@ def test_gated(m, n, k, act, kind):
     check_gated(x, gate, upw, act, y.to_host(), kind)
 
 
+# Sizes at which the forms for more rows and weights are taken: 32 rows a wave; tiles of 128, whole and in pieces of k whose
+# steps do not divide; tiles of 256, at rows of one, of an odd number and of many steps.
+LARGER = [(190, 700, 3300), (100, 1000, 5000), (70, 900, 10000), (300, 2100, 600), (1300, 1290, 2310), (2100, 4099, 1030), (2300, 2500, 255),
+          (2300, 2500, 700), (4200, 4000, 250)]
+
+
+@functools.lru_cache(1)
+def larger(m, n, k):
+    """inputs and the definition's products of one size -> x, two matrices, and each one's products and magnitudes"""
+    g = rng(16, m, n, k)
+    x, a, b = random_rows(g, m, k, 1), random_rows(g, n, k, 1), random_rows(g, n, k, 1)
+    shift = int(np.log2(k) / 2) + 1                  # gates of about one
+    a = a[0], smaller(a[1], shift), a[2] * 2.0 ** -shift
+    return x, a, b, [(x[2] @ w.T, abs(x[2]) @ abs(w).T) for w in (a[2], b[2])]
+
+
+@pytest.mark.parametrize("m,n,k", LARGER)
+@pytest.mark.parametrize("kind", KINDS)
+def test_larger_products(kind, m, n, k):
+    x, a, b, ((ya, ta), (yb, tb)) = larger(m, n, k)
+    xm, am, bm = matrix(*x[:2], m, k), matrix(*a[:2], n, k), matrix(*b[:2], n, k)
+    close(mx4.project(xm, bm, dtype=kind).to_host(), yb, lost(k, tb), kind)
+    for act in ("silu", "gelu"):
+        close_gated(ya, yb, lost(k, ta), lost(k, tb), act, mx4.gated(xm, am, bm, act, dtype=kind).to_host(), kind)
+
+
+LARGER_ROUTED = [(200, 2, 1, 500, 5200), (100, 4, 1, 2600, 3300), (600, 7, 2, 2000, 256), (3000, 9, 2, 1300, 600), (1200, 5, 3, 2100, 1300),
+                 (1500, 70, 2, 520, 520), (2600, 6, 2, 1300, 250), (3000, 90, 2, 800, 800)]
+
+
+@pytest.mark.parametrize("rows,e,each,n,k", LARGER_ROUTED)
+@pytest.mark.parametrize("kind", [BF16, F32])
+def test_larger_products_by_expert(kind, rows, e, each, n, k):
+    check_by_expert(rows, e, each, n, k, False, kind)
+
+
 ROUTED = [(1, 4, 1, 64, 256), (1, 8, 4, 33, 300), (5, 16, 3, 100, 512), (32, 64, 4, 64, 1024), (64, 3, 2, 130, 640), (300, 5, 2, 300, 768), (700, 4, 3, 257, 256),
           (40, 200, 2, 40, 64), (1000, 2, 1, 512, 1024)]
 
@@ -217,6 +258,10 @@ ROUTED = [(1, 4, 1, 64, 256), (1, 8, 4, 33, 300), (5, 16, 3, 100, 512), (32, 64,
 @pytest.mark.parametrize("rows,e,each,n,k", ROUTED)
 def test_products_by_expert(rows, e, each, n, k, by_slot, kind):
     """experts without rows, with one and with most; slots without an expert keep what is in their rows"""
+    check_by_expert(rows, e, each, n, k, by_slot, kind)
+
+
+def check_by_expert(rows, e, each, n, k, by_slot, kind):
     g = rng(6, rows, e, each)
     which = g.integers(-1, e + 1, (rows, each)).astype(np.int32)
     which[g.random(which.shape) < 0.4] = e - 1
@@ -321,6 +366,23 @@ def test_an_order_that_is_not_one():
         mx4.project(matrix(xc, xs, rows, k), matrix(wc, ws, n, k, e), r, out=hold.view(4 * 12 * n, (12, n), F32))
         got = hold.to_host().reshape(3, 12, n)
         assert (got[[0, 2]] == 9).all()
+
+
+@pytest.mark.parametrize("n", [1, 128])
+def test_slots_whose_rows_take_a_division(n):
+    """slots times slots a row past 32 bits, in an order from the last to the first"""
+    each, k, e = 32, 256, 2
+    rows = (1 << 32) // each ** 2 + 5
+    slots = rows * each
+    g = rng(15, n)
+    (xc, xs, x), (wc, ws, w) = random_rows(g, 7, k), random_rows(g, e * n, k)
+    turns = lambda a: np.ascontiguousarray(np.tile(a, (rows // 7 + 1, 1))[:rows])
+    r = experts.Routing(dev.DeviceArray((rows, each), np.int32), up(np.arange(slots - 1, -1, -1, dtype=np.int32)), up(np.array([0, 0, slots], np.int32)))
+    y = dev.DeviceArray((slots, n), BF16)
+    mx4.project(matrix(turns(xc), turns(xs), rows, k), matrix(wc, ws, n, k, e), r, out=y)
+    for at in (0, slots // 2 - 499, slots - 1000):
+        got = dev.DeviceArray((1000, n), BF16, ptr=y.ptr + at * n * 2, owner=y).to_host()
+        check_product(x[np.arange(at, at + 1000) // each % 7], w[n:], got, BF16)
 
 
 @pytest.mark.parametrize("m", [2, 70, 600])
