@@ -104,13 +104,17 @@ __global__ __launch_bounds__(256) void k_quantize(const Rows a) {
 }
 
 // Blocks along columns: the matrix of x^T. A workgroup takes 64 columns of 256 rows, a lane a column of 32 of them; the
-// codes leave by way of LDS, 128 bytes of a column at a time.
+// codes leave by way of LDS, 128 bytes of a column at a time. Neighbouring columns are of one XCD, which takes every
+// eighth workgroup: where rows begin at any address, their runs of 64 numbers share lines (2053 x 7169 float32: 88 MB read
+// and 17.4 us with the columns dealt in turn, 59 and 14.0 so).
 template <int KIND>
 __global__ __launch_bounds__(512) void k_quantize_across(const Rows a) {
     __shared__ __align__(16) uint32_t codes[64][33];
     __shared__ uint8_t scales[64][8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c0 = (int64_t)blockIdx.y * 64, c = c0 + lane, r0 = (int64_t)blockIdx.x * 256 + wave * 32;
+    const uint32_t strips = (uint32_t)((a.cols + 63) / 64), xcd = blockIdx.x & 7;
+    const uint32_t tile = xcd * (gridDim.x / 8) + tmin(xcd, gridDim.x % 8) + (blockIdx.x >> 3), piece = tile / strips;
+    const int64_t c0 = (int64_t)(tile - piece * strips) * 64, c = c0 + lane, r0 = (int64_t)piece * 256 + wave * 32;
     const bool in = c < a.cols;
     float v[32], top = 0.f;
 #pragma unroll
@@ -134,11 +138,11 @@ __global__ __launch_bounds__(512) void k_quantize_across(const Rows a) {
     __syncthreads();
     for (int u = threadIdx.x; u < 64 * 32; u += 512) {
         const int64_t to = c0 + u / 32;
-        if (to < a.cols) reinterpret_cast<uint32_t*>(a.codes)[(to * a.pitch + blockIdx.x * 8) * 4 + u % 32] = codes[u / 32][u % 32];
+        if (to < a.cols) reinterpret_cast<uint32_t*>(a.codes)[(to * a.pitch + piece * 8) * 4 + u % 32] = codes[u / 32][u % 32];
     }
     for (int u = threadIdx.x; u < 64 * 8; u += 512) {
         const int64_t to = c0 + u / 8;
-        if (to < a.cols) a.scales[to * a.pitch + blockIdx.x * 8 + u % 8] = scales[u / 8][u % 8];
+        if (to < a.cols) a.scales[to * a.pitch + piece * 8 + u % 8] = scales[u / 8][u % 8];
     }
 }
 
@@ -240,20 +244,11 @@ int spa_mx4_quantize(const void* x, int kind, int64_t rows, int64_t cols, int64_
     Rows a{x, rows, cols, stride, (int)pitch_of(across ? rows : cols), on(x, 16) && stride % (kind == SPA_SRC_F32 ? 4 : 8) == 0, codes, scales};
     hipStream_t st = (hipStream_t)stream;
     if (across) {
-        const int64_t strips = (cols + 63) / 64;
-        for (int64_t y0 = 0; y0 < strips; y0 += 65535) {          // a launch's second dimension is limited
-            Rows b = a;
-            const int64_t skip = y0 * 64;
-            b.x = static_cast<const char*>(x) + skip * (kind == SPA_SRC_F32 ? 4 : 2);
-            b.cols = cols - skip;
-            b.codes = codes + skip * a.pitch * 16;
-            b.scales = scales + skip * a.pitch;
-            const dim3 grid((unsigned)(a.pitch / 8), (unsigned)(strips - y0 < 65535 ? strips - y0 : 65535));
-            if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_quantize_across<SRC_BF16>, grid, dim3(512), 0, st, b);
-            else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_quantize_across<SRC_F16>, grid, dim3(512), 0, st, b);
-            else hipLaunchKernelGGL(k_quantize_across<SRC_F32>, grid, dim3(512), 0, st, b);
-            SPA_HIP_TRY(hipGetLastError());
-        }
+        const dim3 grid((unsigned)((cols + 63) / 64 * (a.pitch / 8)));
+        if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_quantize_across<SRC_BF16>, grid, dim3(512), 0, st, a);
+        else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_quantize_across<SRC_F16>, grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL(k_quantize_across<SRC_F32>, grid, dim3(512), 0, st, a);
+        SPA_HIP_TRY(hipGetLastError());
         return SPA_OK;
     }
     const dim3 grid((unsigned)((rows * a.pitch * 4 + 255) / 256));
