@@ -605,7 +605,8 @@ uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts)
 /* ---- experts (no reference counterpart) ----
  * Routing sends each row to `each` of `experts` experts: slot p = row * each + j is row's place j. Logits, rows of results and
  * their gradients are BF16, F16 or F32 (SPA_SRC_*), numbers and weights of slots int32 and float32, dense. Nothing
- * is allocated, and calls may be captured. `work` as with the products. Up to 1024 experts, 32 a row. */
+ * is allocated, and calls may be captured. `work` as with the products. Up to 1024 experts, 32 a row. Outputs must not
+ * overlap inputs. */
 
 /* Each row's experts, the best first, and their weights. score 0: softmax over the row, 1: 1 / (1 + e^-l). The chosen
  * have the largest keys: the logits, or, with a bias ([experts], or NULL) or more than one group, score + bias in 64 bits (keys
@@ -646,7 +647,8 @@ int spa_join_backward(const void* y, int kind, int64_t rows, int64_t each, int64
  * aligned), pitch = spa_mx4_pitch(cols) blocks of 32: cols / 256 rounded up, times 8. Block b of a row holds its
  * numbers 32 b to 32 b + 31: j in the low half of byte j, j + 16 in the high half (as GGUF's MXFP4 does). A code is a sign
  * and 0 .5 1 1.5 2 3 4 6, a scale s stands for 2^(s - 127), 255 for a block of NaN. Blocks behind a row's last number are
- * zeros, codes and scales. Up to 4,000,000 columns. Nothing is allocated, and calls may be captured. */
+ * zeros, codes and scales: conversions write them, and products count on them. Up to 4,000,000 columns. Nothing is allocated,
+ * and calls may be captured. Outputs must not overlap inputs. */
 int64_t spa_mx4_pitch(int64_t cols);
 
 /* x (BF16, F16 or F32) to blocks along its rows, or, across, along its columns: the matrix of x^T, cols rows of `rows`.
@@ -664,7 +666,8 @@ int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t*
  * output is rounded once to BF16, F16 or F32. experts = 0: one w for all rows (order and starts are not read,
  * slots is x_rows). Else w is `experts` matrices one behind another, order and starts are spa_by_expert's for `slots` slots,
  * a multiple of x_rows: slot p is row p of y, from row p / (slots / x_rows) of x. Rows of slots without an expert are left as
- * they are. Numbers of order or starts out of range read or write nothing outside the arrays. */
+ * they are, and x has less than 4 GiB of codes. Numbers of order or starts out of range read or write nothing outside the
+ * arrays. */
 int spa_mx4_project(const uint8_t* x_codes, const uint8_t* x_scales, int64_t x_rows, int64_t k, const uint8_t* w_codes,
                     const uint8_t* w_scales, int64_t n, int64_t experts, const int32_t* order, const int32_t* starts, int64_t slots,
                     void* y, int y_kind, int64_t y_stride, void* work, uint64_t work_bytes, void* stream);

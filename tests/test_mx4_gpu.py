@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 
 from seedpack_amd import device as dev
-from seedpack_amd import experts, mx4
+from seedpack_amd import experts, linear, mx4
 from seedpack_amd._lib import SpaError, check, lib
 
 from . import experts_oracle as oracle
@@ -415,7 +415,7 @@ def bits(v):
 @pytest.mark.parametrize("rows", [1, 7, 300])
 def test_a_mixture_of_experts(rows):
     """logits to results: route, quantize, gated, quantize, project, join, each step against the definition on the step's own
-    inputs; then the gradients back to the logits"""
+    inputs; the experts' sums of squares; then the gradients back to the logits"""
     g = rng(12, rows)
     e, each, k, n = 24, 4, 320, 192
     x, l = bits(g.normal(0, 1, (rows, k))), g.normal(0, 1, (rows, e)).astype(F32)
@@ -441,6 +441,11 @@ def test_a_mixture_of_experts(rows):
     w = oracle.weights(wide(l), which, "sigmoid", True, 2.0)
     terms = wide(y.to_host()).reshape(rows, each, k) * w[:, :, None]
     close(out, terms.sum(1), (each + 1) * 2.0 ** -24 * abs(terms).sum(1), BF16)
+    sums, counts = up(np.zeros((e, k), F32)), up(np.zeros(e, np.int64))
+    linear.add_squares(up(x), sums, counts, r.which)
+    squares = np.array([(wide(x)[(which == i).any(1)] ** 2).sum(0) for i in range(e)])
+    np.testing.assert_array_equal(counts.to_host(), np.bincount(flat, minlength=e))
+    close(sums.to_host(), squares, (rows + 1) * 2.0 ** -24 * squares, F32)   # a square's rounding and one for each row added
     d = bits(g.normal(0, 1, (rows, k)))
     _, dw = experts.join_backward(y, r.weights, up(d), r.which, e)
     dl = experts.route_backward(up(l), r.which, dw, "sigmoid", scale=2.0).to_host()
