@@ -610,7 +610,7 @@ uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts)
 
 /* Each row's experts, the best first, and their weights. score 0: softmax over the row, 1: 1 / (1 + e^-l). The chosen
  * have the largest keys: the logits, or, with a bias ([experts], or NULL) or more than one group, score + bias in 64 bits (keys
- * whose first 42 bits agree count as equal). Of equal keys the lowest number wins, NaN is above all. With `groups`
+ * that agree to 42 bits of their mantissas count as equal). Of equal keys the lowest number wins, NaN is above all. With `groups`
  * equal runs of experts only the `keep` best take part; a group is worth the sum of its `best` (1 or 2) highest keys. A
  * logit of -infinity, or a key of it, is never chosen: where fewer than `each` are left, which is -1 and the weight 0.
  * Weights are scale * score, with renorm divided by the row's chosen scores' sum. order and starts (both or neither)

@@ -74,7 +74,7 @@ __device__ __forceinline__ void load_row(const void* logits, int64_t at, int exp
 }
 
 // Keys whose order is that of their numbers, zeros of both signs alike and every NaN above all, with the expert's number
-// below. 0: not to be chosen. Keys of 64 bits keep 42 of the mantissa.
+// below. 0: not to be chosen. Keys of 64 bits keep 42 of the mantissa's bits.
 __device__ __forceinline__ uint64_t key_of(float l, int i) {
     if (l == -INFINITY) return 0;
     uint32_t u = __float_as_uint(l + 0.f);
@@ -251,7 +251,7 @@ __device__ __forceinline__ void route_row(const Route& a, int64_t row, bool in, 
                     two = fmax(fmax(two, t), fmin(one, o));
                     one = fmax(one, o);
                 }
-                if (g < a.groups && lane % lanes == 0) score[g] = a.best == 2 && per > 1 ? one + two : one;
+                if (g < a.groups && lane % lanes == 0) score[g] = a.best == 2 && per > 1 && one < INFINITY ? one + two : one;   // no inf - inf
             }
             own_lds();
             kept = 0;

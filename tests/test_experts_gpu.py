@@ -167,6 +167,18 @@ def test_route_not_a_number(score):
     assert np.isfinite(w[keep]).all()
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_not_a_number_in_a_group(score):
+    """a group with a NaN and nothing beside it is above all, and no more than `keep` groups are kept"""
+    l = rng(20).normal(0, 1, (3, 24)).astype(F32)
+    l[1, 4:8] = np.nan, -np.inf, -np.inf, -np.inf
+    which = experts.route(up(l), 4, score, groups=6, keep=1).which.to_host()
+    if score == "sigmoid":                           # with softmax all of the row's scores are NaN
+        assert list(which[1]) == [4, -1, -1, -1]
+    assert (which[1] < 8).all()
+    np.testing.assert_array_equal(which[[0, 2]], oracle.choose(wide(l[[0, 2]]), 4, score, groups=6, keep=1))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("e,stride", [(64, 72), (64, 65), (130, 136), (5, 5)])
 def test_route_strides(e, stride, kind):
@@ -343,6 +355,57 @@ def test_join_strides(n, stride, offset, kind):
     close(dw.to_host(), (dd * v).sum(2), n * 2.0 ** -24 * abs(dd * v).sum(2), F32)
     nine = np.full(1, 9, kind)[0]
     assert (got[:, n:] == nine).all() and (gy[:, n:] == nine).all() and (bo.to_host()[:offset] == nine).all()
+
+
+def last(a, rows):
+    """the last rows of an array"""
+    n = a.shape[1]
+    return dev.DeviceArray((rows, n), a.dtype, ptr=a.ptr + (a.shape[0] - rows) * n * a.dtype.itemsize, owner=a)
+
+
+def fill_last(a, h):
+    check(lib().spa_memcpy_h2d(last(a, len(h)).ptr, h.ctypes.data, h.nbytes, None))
+
+
+def test_logits_past_4_gib():
+    rows, e, each = (1 << 32) // (256 * 2) + 70001, 256, 4
+    g = rng(21)
+    l = dev.DeviceArray((rows, e), BF16)
+    l.zero()
+    h = store(g.normal(0, 1, (50, e)), BF16)
+    fill_last(l, h)
+    r = experts.route(l, each, sort=False)
+    want = oracle.choose(wide(h), each, "softmax")
+    np.testing.assert_array_equal(last(r.which, 50).to_host(), want)
+    close(last(r.weights, 50).to_host(), oracle.weights(wide(h), want, "softmax", True, 1.0), 2.0 ** -36, F32)
+    dw = dev.DeviceArray((rows, each), F32)
+    dw.zero()
+    d = g.normal(0, 1, (50, each)).astype(F32)
+    fill_last(dw, d)
+    got = experts.route_backward(l, r.which, dw)
+    want, t = oracle.route_backward(wide(h), want, d, "softmax", True, 1.0)
+    close(last(got, 50).to_host(), want, 68 * 2.0 ** -24 * t, BF16)
+    assert not dev.DeviceArray((1000, e), BF16, ptr=got.ptr, owner=got).to_host().any()
+
+
+def test_joined_rows_past_4_gib():
+    rows, each, n = 33001, 2, 33000
+    g = rng(22)
+    y, w, d = dev.DeviceArray((rows * each, n), BF16), dev.DeviceArray((rows, each), F32), dev.DeviceArray((rows, n), BF16)
+    for a in (y, w, d):
+        a.zero()
+    hy, hw, hd = store(g.normal(0, 1, (6, n)), BF16), g.normal(0, 1, (3, each)).astype(F32), store(g.normal(0, 1, (3, n)), BF16)
+    for a, h in ((y, hy), (w, hw), (d, hd)):
+        fill_last(a, h)
+    out = experts.join(y, w)
+    terms = wide(hy).reshape(3, each, n) * wide(hw)[:, :, None]
+    close(last(out, 3).to_host(), terms.sum(1), (each + 1) * 2.0 ** -24 * abs(terms).sum(1), BF16)
+    dy, dw = experts.join_backward(y, w, d)
+    close(last(dy, 6).to_host(), (wide(hd)[:, None] * wide(hw)[:, :, None]).reshape(6, n), 2.0 ** -24 * abs(wide(hd)[:, None] * wide(hw)[:, :, None]).reshape(6, n), BF16)
+    dots = wide(hy).reshape(3, each, n) * wide(hd)[:, None]
+    close(last(dw, 3).to_host(), dots.sum(2), n * 2.0 ** -24 * abs(dots).sum(2), F32)
+    for a in (out, dy):
+        assert not dev.DeviceArray((1000, n), BF16, ptr=a.ptr, owner=a).to_host().any()
 
 
 def test_threads_at_once():

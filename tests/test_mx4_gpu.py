@@ -149,6 +149,33 @@ def test_quantize_across_many_columns():
     np.testing.assert_array_equal(np.array(rows), oracle.values(codes, scales, 2))
 
 
+@pytest.mark.parametrize("across", [False, True])
+def test_quantize_past_4_gib(across):
+    """the last rows of numbers and of values begin behind the first 4 GiB"""
+    m, k = 66001, 33000
+    g = rng(17)
+    x = dev.DeviceArray((m, k), BF16)
+    x.zero()
+    h = store(g.normal(0, 1, (17, k)), BF16)
+    check(lib().spa_memcpy_h2d(x.ptr + (m - 17) * k * 2, h.ctypes.data, h.nbytes, None))
+    q = mx4.quantize(x, across)
+    r, c = (k, m) if across else (m, k)
+    y = dev.DeviceArray((r, c), BF16)
+    mx4.values(q, out=y)
+    if across:                                       # the last block of each column holds these rows
+        p, b = mx4.pitch(m), m // 32
+        codes, scales = oracle.quantize(wide(h).T)
+        want = oracle.values(codes, scales, 17)
+        got = dev.DeviceArray((1000, c), BF16, ptr=y.ptr + (r - 1000) * c * 2, owner=y).to_host()
+        assert (wide(got[:, m - 17:]) == want[k - 1000:]).all() and not (wide(got[:, :m - 17]) != 0).any()
+        np.testing.assert_array_equal(q.scales.to_host().reshape(k, p)[:, b], scales[:, 0])
+    else:
+        codes, scales = oracle.quantize(wide(h))
+        got = dev.DeviceArray((17, k), BF16, ptr=y.ptr + (m - 17) * k * 2, owner=y).to_host()
+        assert (wide(got) == oracle.values(codes, scales, k)).all()
+        assert not (wide(dev.DeviceArray((1000, k), BF16, ptr=y.ptr, owner=y).to_host()) != 0).any()
+
+
 @pytest.mark.parametrize("rows,cols,count,offset", [(1, 32, 1, 0), (7, 96, 2, 1), (5, 2880, 3, 3), (33, 256, 1, 2)])
 def test_from_blocks(rows, cols, count, offset):
     g = rng(3, rows, cols)
@@ -404,6 +431,25 @@ def test_weights_past_4_gib(m):
     got = y.to_host()
     check_product(x, v, got[:, n - 50:], BF16)
     assert (got[:, :n - 50] == 0).all()
+
+
+@pytest.mark.parametrize("n", [8, 700])
+def test_rows_past_4_gib(n):
+    m, k = (1 << 32) // 8192 + 4001, 16384
+    p = mx4.pitch(k)
+    x = mx4.empty(m, k)
+    x.codes.zero()
+    x.scales.zero()
+    g = rng(18, n)
+    (xc, xs, v), (wc, ws, w) = random_rows(g, 50, k), random_rows(g, n, k)
+    check(lib().spa_memcpy_h2d(x.codes.ptr + (m - 50) * p * 16, xc.ctypes.data, xc.nbytes, None))
+    check(lib().spa_memcpy_h2d(x.scales.ptr + (m - 50) * p, xs.ctypes.data, xs.nbytes, None))
+    got = mx4.project(x, matrix(wc, ws, n, k)).to_host()
+    check_product(v, w, got[m - 50:], BF16)
+    assert not (wide(got[:m - 50]) != 0).any()
+    with pytest.raises(SpaError):                    # by expert rows lie at 32-bit offsets
+        mx4.project(x, matrix(wc, ws, n, k, 1), experts.Routing(dev.DeviceArray((m, 1), np.int32), dev.DeviceArray(m, np.int32), dev.DeviceArray(2, np.int32)),
+                    out=dev.DeviceArray((m, n), BF16))
 
 
 # ------------------------------------------------------------------------------------------ as they are used
