@@ -291,25 +291,28 @@ int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t*
 namespace {
 
 // What a product takes, by the forms' times on one MI355X, in us:
-//   FEW16, FEW32  16 x 16 and 32 x 32 outputs a wave: 3.3 and 6.0 for a launch, then 6.6 and 6.9 for 26.7 MB of weights, which
+//   FEW16, FEW32  16 x 16 and 32 x 32 outputs a wave: 3.3 and 4.5 for a launch, then 6.6 and 6.9 for 26.7 MB of weights, which
 //                 each tile of 16 or 32 rows reads again
-//   SMALL         128 x 128 tiles: 4.5 and 0.74 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
-//                 in pieces of k, where there are too few tiles: 2.5 for the joining launch and 5 TB/s for its sums
-//   LARGE         256 x 256 tiles, one to a compute unit: 7 and 1.95 a step (1.5 with most units idle)
-// k = 4096 of 12288 outputs, us:  rows  16: 9.8 11.4 14.7 20.3   32: 16.5 13.2 15.3 21.3   64: 29.3 18.3 16.4 23.1
-//   128: 55 32 17.9 24.5   256: 107 62 18.4 30.5   4096: - - 136 112;   k = 12288 of 4096, SMALL whole and in 4 pieces:
-//   64: 37.5 17.1   256: 41.9 23.3   512: 42.3 31.7.
-// By expert the rows' spread is not known on the host: half of the experts that have any are taken to end in a tile of their
-// own.
+//   SMALL         128 x 128 tiles: 3 to 5 and 0.74 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
+//                 in pieces of k, where there are too few tiles: 2 for the joining launch and 3.3 TB/s for its sums
+//   LARGE         256 x 256 tiles, one to a compute unit: 5 and 1.95 a step, 1.4 with most units idle
+// k = 4096 of 12288 outputs, us:  rows  16: 10.1 11.5 13.8 19.1   32: 16.6 13.3 14.2 19.8   64: 29.6 18.1 14.9 21.0
+//   128: 55 34 16.8 22.0   256: 107 59 17.1 28.5   4096: - - 130 107;   k = 12288 of 4096, SMALL whole and in 2, 4 and 8 pieces:
+//   64: 34.6 22.1 16.2 15.7   256: 40.6 27.2 22.9 25.9   512: 40.9 31.5 31.9 43.2; k = 4096 of 4096: 256: 13.7 15.6 20.6 23.8.
+// By expert the rows' spread is not known on the host: rows are taken to be dealt at random, and half of the experts that have any
+// to end in a tile of their own. Tiles of few rows cost less than full ones, so rounds of them are not rounded up. 2 x 1536 x
+// 2048 of 64 experts, four a row, FEW16, SMALL and LARGE: rows 1: 7.4 9.7 12.8   4: 14.3 12.7 14.2   32: 29.7 29.2 31.6
+//   512: 117 49 54   2048: 361 80 81   4096: - 121 109.
 enum Form { FEW16, FEW32, SMALL, LARGE };
 struct Plan {
     int form, pieces;
 };
 Plan plan(int64_t m, int64_t n, int64_t pitch, int64_t experts, bool gated) {
     const double steps = (double)pitch / 8, sides = gated ? 2 : 1, mb = (double)n * pitch * 17 * sides * 1e-6 / 26.7;
-    const int64_t used = experts && experts < m ? experts : experts ? m : 0;
-    auto rows = [&](int64_t t) { return experts ? (double)(m / t) + (used + 1) / 2 : (double)((m + t - 1) / t); };
-    auto small = [&](double tiles, double k) { return tiles <= 256 ? 4.5 + 0.74 * k : ceil(tiles / 512) * (5 + 1.19 * k); };
+    const double used = experts ? experts * (1 - exp(-(double)m / experts)) : 0;
+    auto rows = [&](double t) { return experts ? fmax(used, m / t + used / 2) : ceil(m / t); };
+    auto rounds = [&](double r) { return experts ? fmax(r, 1) : ceil(r); };
+    auto small = [&](double tiles, double k) { return tiles <= 256 ? 3 + tiles / 128 + 0.74 * k : rounds(tiles / 512) * (5 + 1.19 * k); };
     Plan best{FEW16, 1};
     double least = 3.3 + 6.6 * rows(16) * mb;
     auto take = [&](int form, int pieces, double us) {
@@ -318,13 +321,13 @@ Plan plan(int64_t m, int64_t n, int64_t pitch, int64_t experts, bool gated) {
             least = us;
         }
     };
-    take(FEW32, 1, 6.0 + 6.9 * rows(32) * mb);
+    take(FEW32, 1, 4.5 + 6.9 * rows(32) * mb);
     const double wide = ceil(n * sides / 128.0), tiles = wide * rows(128);
     take(SMALL, 1, small(tiles, steps));
     for (int p = 2; p <= 8 && 2 * p <= steps; ++p)
-        take(SMALL, p, small(tiles * p, ceil(steps / p)) + 2.5 + (double)m * n * 8 * p * sides / 5e6);
+        take(SMALL, p, small(tiles * p, ceil(steps / p)) + 2 + (double)m * n * 8 * p * sides / 3.3e6);
     const double large = ceil(n * sides / 256.0) * rows(256);
-    take(LARGE, 1, ceil(large / 256) * (7 + (large <= 64 ? 1.5 : 1.95) * steps));
+    take(LARGE, 1, rounds(large / 256) * (5 + (1.4 + 0.55 * fmin(large / 256, 1)) * steps));
     return best;
 }
 uint64_t part_bytes(const Plan& c, int64_t m, int64_t n, bool gated) {

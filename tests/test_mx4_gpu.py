@@ -243,7 +243,7 @@ def test_gated(m, n, k, act, kind):
 # Sizes at which the forms for more rows and weights are taken: 32 rows a wave; tiles of 128, whole and in pieces of k whose
 # steps do not divide; tiles of 256, at rows of one, of an odd number and of many steps.
 LARGER = [(190, 700, 3300), (100, 1000, 5000), (70, 900, 10000), (300, 2100, 600), (1300, 1290, 2310), (2100, 4099, 1030), (2300, 2500, 255),
-          (2300, 2500, 700), (4200, 4000, 250)]
+          (2300, 2500, 700), (4200, 4000, 250), (600, 700, 9000)]
 
 
 @functools.lru_cache(1)
@@ -267,7 +267,7 @@ def test_larger_products(kind, m, n, k):
 
 
 LARGER_ROUTED = [(200, 2, 1, 500, 5200), (100, 4, 1, 2600, 3300), (600, 7, 2, 2000, 256), (3000, 9, 2, 1300, 600), (1200, 5, 3, 2100, 1300),
-                 (1500, 70, 2, 520, 520), (2600, 6, 2, 1300, 250), (3000, 90, 2, 800, 800)]
+                 (1500, 70, 2, 520, 520), (2600, 6, 2, 1300, 250), (3000, 90, 2, 800, 800), (300, 3, 1, 1000, 9000), (4000, 12, 2, 2100, 600)]
 
 
 @pytest.mark.parametrize("rows,e,each,n,k", LARGER_ROUTED)
