@@ -22,16 +22,9 @@ template <int CTRL, typename T> __device__ __forceinline__ T lane_move(T v) {
     }
     return v;
 }
-template <typename T> __device__ __forceinline__ T lane_xor(T v, int mask) {
-    if constexpr (sizeof(T) == 8) {
-        uint64_t b;
-        __builtin_memcpy(&b, &v, 8);
-        b = (uint64_t)(uint32_t)__shfl_xor((int)(b >> 32), mask) << 32 | (uint32_t)__shfl_xor((int)b, mask);
-        __builtin_memcpy(&v, &b, 8);
-        return v;
-    } else {
-        return __shfl_xor(v, mask);
-    }
+__device__ __forceinline__ double lane_xor(double v, int mask) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)__shfl_xor((int)(b >> 32), mask) << 32 | (uint32_t)__shfl_xor((int)b, mask)));
 }
 
 // A number's two copies after rows of 16 (or 32) lanes changed places between them: the even rows' numbers everywhere, and the
