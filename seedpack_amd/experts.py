@@ -36,13 +36,13 @@ class Routing:
     __slots__ = ("which", "order", "starts", "weights")
 
     def __init__(self, which, order=None, starts=None, weights=None):
-        if which.dtype != np.int32 or len(which.shape) != 2:
+        if which.dtype != _I32 or len(which.shape) != 2:
             raise ValueError(f"which is {which.shape} {which.dtype}: (rows, each) int32 is taken")
         if (order is None) != (starts is None):
             raise ValueError("order and starts go together")
-        if order is not None and (order.dtype != np.int32 or starts.dtype != np.int32 or order.size != which.size or starts.size < 2):
+        if order is not None and (order.dtype != _I32 or starts.dtype != _I32 or order.size != which.size or starts.size < 2):
             raise ValueError(f"order {order.shape} {order.dtype} and starts {starts.shape} {starts.dtype} for {which.size} slots")
-        if weights is not None and (weights.dtype != np.float32 or weights.shape != which.shape):
+        if weights is not None and (weights.dtype != _F32 or weights.shape != which.shape):
             raise ValueError(f"weights {weights.shape} {weights.dtype} beside which {which.shape}")
         self.which, self.order, self.starts, self.weights = which, order, starts, weights
 
@@ -83,7 +83,7 @@ def route(logits, each, score="softmax", bias=None, groups=1, keep=1, best=2, re
     the slots' order too."""
     kind, m, e, ld = _rows("logits", logits, logits_stride)
     score = _score(score)
-    if bias is not None and (bias.dtype != np.float32 or bias.size != e):
+    if bias is not None and (bias.dtype != _F32 or bias.size != e):
         raise ValueError(f"bias {bias.shape} {bias.dtype} for {e} experts (float32)")
     which = _made("which", which, (m, each), _I32, stream)
     weights = _made("weights", weights, (m, each), _F32, stream)
@@ -107,7 +107,7 @@ def route_backward(logits, which, dweights, score="softmax", renorm=True, scale=
     kind, m, e, ld = _rows("logits", logits, logits_stride)
     score = _score(score)
     _ids(which, m)
-    if len(which.shape) != 2 or dweights.dtype != np.float32 or dweights.shape != which.shape:
+    if len(which.shape) != 2 or dweights.dtype != _F32 or dweights.shape != which.shape:
         raise ValueError(f"dweights {dweights.shape} {dweights.dtype} beside which {which.shape}")
     dlogits, ldd = _out("dlogits", dlogits, m, e, logits.dtype, dlogits_stride, stream)
     check(lib().spa_route_backward(logits.ptr, kind, m, e, ld, score, which.shape[1], bool(renorm), scale, which.ptr, dweights.ptr,
@@ -118,7 +118,7 @@ def route_backward(logits, which, dweights, score="softmax", renorm=True, scale=
 def by_expert(which, experts, order=None, starts=None, work=None, stream=None):
     """which (rows, each) int32 -> Routing with the slots in the order of their experts (those of one expert in their own, those
     without an expert last) and where each expert's begin"""
-    if which.dtype != np.int32 or len(which.shape) != 2:
+    if which.dtype != _I32 or len(which.shape) != 2:
         raise ValueError(f"which is {which.shape} {which.dtype}: (rows, each) int32 is taken")
     order = _made("order", order, (which.size,), _I32, stream)
     starts = _made("starts", starts, (experts + 1,), _I32, stream)
@@ -130,11 +130,11 @@ def by_expert(which, experts, order=None, starts=None, work=None, stream=None):
 
 def _slots(y, weights, which, experts, y_stride):
     kind, slots, n, ld = _rows("y", y, y_stride)
-    if weights.dtype != np.float32 or len(weights.shape) != 2 or weights.size != slots or not weights.shape[1]:
+    if weights.dtype != _F32 or len(weights.shape) != 2 or weights.size != slots or not weights.shape[1]:
         raise ValueError(f"weights {weights.shape} {weights.dtype} for {slots} rows of results: (rows, each) float32 is taken")
     if (which is None) != (experts is None):
         raise ValueError("which and the number of experts go together")
-    if which is not None and (which.dtype != np.int32 or which.shape != weights.shape):
+    if which is not None and (which.dtype != _I32 or which.shape != weights.shape):
         raise ValueError(f"which {which.shape} {which.dtype} beside weights {weights.shape}")
     return kind, weights.shape[0], weights.shape[1], n, ld
 

@@ -21,6 +21,8 @@ from . import device as dev
 from ._lib import check, lib
 from .linear import ACT, _KIND, _not_captured, _out, _rows, _scratch
 
+_U8 = np.dtype(np.uint8)
+
 
 def pitch(cols):
     """the blocks that a row of `cols` numbers takes: whole runs of eight"""
@@ -40,7 +42,7 @@ class Matrix:
         if rows < 0 or cols <= 0 or count < 1:
             raise ValueError(f"bad shape {count} x {rows} x {cols}")
         need = count * rows * pitch(cols)
-        if codes.dtype != np.uint8 or scales.dtype != np.uint8:
+        if codes.dtype != _U8 or scales.dtype != _U8:
             raise TypeError(f"codes and scales are uint8, not {codes.dtype} and {scales.dtype}")
         if codes.nbytes < 16 * need or scales.nbytes < need:
             raise ValueError(f"{codes.nbytes} and {scales.nbytes} bytes hold no {count} x {rows} x {cols} codes and scales ({16 * need} and {need} bytes)")
