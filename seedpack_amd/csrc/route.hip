@@ -473,7 +473,7 @@ int64_t most_placed(int64_t experts) {
     while (order_lds(n, experts) > 60 * 1024) n /= 2;
     return n;
 }
-// the tiles of an order, and its workspace
+// the tiles of an order, and its workspace; one tile has no counts, and no byte of `work` is its
 void lay_out(Order& o, int64_t slots, int64_t experts, int64_t tile, void* work) {
     o.slots = (int)slots;
     o.experts = (int)experts;
@@ -482,6 +482,7 @@ void lay_out(Order& o, int64_t slots, int64_t experts, int64_t tile, void* work)
     o.tiles = (int)((slots + tile - 1) / tile);
     o.group = (int)(most_placed(experts) / tile);
     if (!o.group) o.group = 1;
+    if (o.tiles <= 1) return;
     o.counts = static_cast<uint16_t*>(work);
     o.sums = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(work) + ((int64_t)o.tiles * (experts + 1) * 2 + 255) / 256 * 256);
 }

@@ -436,3 +436,21 @@ def test_a_workspace_that_is_too_small_is_refused():
     x = up(rng(18).normal(0, 1, (5000, 64)).astype(F32))
     with pytest.raises(SpaError):
         experts.route(x, 4, work=dev.DeviceArray(256, np.uint8))
+
+
+@pytest.mark.parametrize("e,groups", [(512, 8), (512, 64), (1024, 16), (290, 58), (64, 1)])
+@pytest.mark.parametrize("rows", [1, 8])
+def test_a_workspace_of_no_bytes_is_left_alone(rows, e, groups):
+    """up to 8 rows need no workspace, in whichever form: a block that comes along with a length of 0, at any address, stays"""
+    each = 3
+    assert lib().spa_route_work_bytes(rows, e, each, 1) == 0
+    l = rng(23, e, rows).normal(0, 1, (rows, e)).astype(F32)
+    x, block = up(l), up(np.full(1 << 14, 0xa5, np.uint8))
+    o = {"which": dev.DeviceArray((rows, each), np.int32), "weights": dev.DeviceArray((rows, each), F32), "order": dev.DeviceArray(rows * each, np.int32),
+         "starts": dev.DeviceArray(e + 1, np.int32)}
+    check(lib().spa_route(x.ptr, 2, rows, e, e, 0, None, groups, min(groups, 4), 2, each, 1, 1.0, *(a.ptr for a in o.values()), block.ptr + 1024, 0, None))
+    want = oracle.choose(wide(l), each, "softmax", groups=groups, keep=min(groups, 4))
+    order, starts = oracle.by_expert(want, e)
+    for name, h in (("which", want), ("order", order), ("starts", starts)):
+        np.testing.assert_array_equal(o[name].to_host(), h)
+    assert (block.to_host() == 0xa5).all()
