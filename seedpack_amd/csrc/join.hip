@@ -12,6 +12,7 @@ namespace {
 struct Join {
     const void *y, *dout;
     int64_t rows, n, ldy, ldo, ldd;
+    int64_t first;           // slot of a launch
     int each, experts;
     const float* weights;
     const int32_t* which;    // or NULL: every slot has an expert
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void k_join_back(const Join a) {
     constexpr int V = KIND == SRC_F32 ? 4 : 8;
     __shared__ float part[4];
     const uint32_t xcd = blockIdx.x & 7;
-    const int64_t slot = xcd * (gridDim.x / 8) + tmin(xcd, gridDim.x % 8) + (blockIdx.x >> 3), row = slot / a.each;
+    const int64_t slot = a.first + xcd * (gridDim.x / 8) + tmin(xcd, gridDim.x % 8) + (blockIdx.x >> 3), row = slot / a.each;
     const bool has = has_expert(a, slot);
     const float w = has ? a.weights[slot] : 0.f;
     float dot = 0.f;
@@ -141,7 +142,7 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check(const char* who, int kind, int64_t rows, int64_t each, int64_t n, const int32_t* which, int64_t experts) {
     if (kind != SPA_SRC_BF16 && kind != SPA_SRC_F16 && kind != SPA_SRC_F32) return fail(SPA_ERR_TYPE, "%s: rows of kind %d (BF16, F16 and F32 are taken)", who, kind);
-    if (rows < 0 || each < 1 || n < 1 || n > INT32_MAX || rows > INT32_MAX || each > INT32_MAX || rows * each > INT32_MAX - 1024 || rows * ((n + 3) / 4) / 256 >= INT32_MAX)
+    if (rows < 0 || each < 1 || n < 1 || n > INT32_MAX || rows > INT32_MAX || each > INT32_MAX || rows * each > INT32_MAX - 1024)
         return fail(SPA_ERR_ARG, "%s: bad shape %lld rows of %lld x %lld", who, (long long)rows, (long long)each, (long long)n);
     if (which && (experts < 1 || experts > INT32_MAX)) return fail(SPA_ERR_ARG, "%s: %lld experts", who, (long long)experts);
     return SPA_OK;
@@ -173,7 +174,9 @@ int spa_join(const void* y, int kind, int64_t rows, int64_t each, int64_t n, int
     a.which = which;
     a.out = out;
     a.wide = on16(y) && y_stride % v == 0;
-    const dim3 grid((unsigned)((rows * ((n + v - 1) / v) + 255) / 256));
+    const int64_t workgroups = (rows * ((n + v - 1) / v) + 255) / 256;
+    if (!one_launch(workgroups, 256)) return fail(SPA_ERR_ARG, "join: %lld rows of %lld are more than one launch takes", (long long)rows, (long long)n);
+    const dim3 grid((unsigned)workgroups);
     if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_join<SRC_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a);
     else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_join<SRC_F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(k_join<SRC_F32>, grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -204,11 +207,17 @@ int spa_join_backward(const void* y, int kind, int64_t rows, int64_t each, int64
     a.dy = dy;
     a.dweights = dweights;
     a.wide = on16(y) && on16(dout) && y_stride % v == 0 && dout_stride % v == 0;
-    const dim3 grid((unsigned)(rows * each));
-    if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_join_back<SRC_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-    else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_join_back<SRC_F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(k_join_back<SRC_F32>, grid, dim3(256), 0, (hipStream_t)stream, a);
-    SPA_HIP_TRY(hipGetLastError());
+    // a launch takes fewer slots than there may be
+    constexpr int64_t PART = 1 << 23;
+    static_assert(PART <= UINT32_MAX / 256, "one launch");
+    for (a.first = 0; a.first < rows * each; a.first += PART) {
+        const int64_t left = rows * each - a.first;
+        const dim3 grid((unsigned)(left < PART ? left : PART));
+        if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_join_back<SRC_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+        else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_join_back<SRC_F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL(k_join_back<SRC_F32>, grid, dim3(256), 0, (hipStream_t)stream, a);
+        SPA_HIP_TRY(hipGetLastError());
+    }
     return SPA_OK;
 }
 

@@ -37,6 +37,9 @@ int launch_iq1(const QuantArgs& a);      // IQ1_S IQ1_M
 // Sets the thread's last error message (printf-style) and returns `code`.
 int fail(int code, const char* fmt, ...);
 
+// A dispatch counts its work-items in 32 bits.
+inline bool one_launch(int64_t groups, int threads) { return groups <= (int64_t)(UINT32_MAX / (uint32_t)threads); }
+
 }  // namespace spa
 
 #define SPA_HIP_TRY(expr)                                                                  \

@@ -222,6 +222,12 @@ int check_matrix(const char* who, int64_t rows, int64_t cols, const void* codes,
     return SPA_OK;
 }
 
+// the workgroups of a conversion of rows x cols numbers, `threads` each
+int check_launch(const char* who, int64_t workgroups, int threads, int64_t rows, int64_t cols) {
+    if (!one_launch(workgroups, threads)) return fail(SPA_ERR_ARG, "%s: %lld x %lld numbers are more than one launch takes", who, (long long)rows, (long long)cols);
+    return SPA_OK;
+}
+
 }  // namespace
 }  // namespace mx
 }  // namespace spa
@@ -244,14 +250,18 @@ int spa_mx4_quantize(const void* x, int kind, int64_t rows, int64_t cols, int64_
     Rows a{x, rows, cols, stride, (int)pitch_of(across ? rows : cols), on(x, 16) && stride % (kind == SPA_SRC_F32 ? 4 : 8) == 0, codes, scales};
     hipStream_t st = (hipStream_t)stream;
     if (across) {
-        const dim3 grid((unsigned)((cols + 63) / 64 * (a.pitch / 8)));
+        const int64_t workgroups = (cols + 63) / 64 * (a.pitch / 8);
+        if (int rc = check_launch("mx4_quantize", workgroups, 512, rows, cols)) return rc;
+        const dim3 grid((unsigned)workgroups);
         if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_quantize_across<SRC_BF16>, grid, dim3(512), 0, st, a);
         else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_quantize_across<SRC_F16>, grid, dim3(512), 0, st, a);
         else hipLaunchKernelGGL(k_quantize_across<SRC_F32>, grid, dim3(512), 0, st, a);
         SPA_HIP_TRY(hipGetLastError());
         return SPA_OK;
     }
-    const dim3 grid((unsigned)((rows * a.pitch * 4 + 255) / 256));
+    const int64_t workgroups = (rows * a.pitch * 4 + 255) / 256;
+    if (int rc = check_launch("mx4_quantize", workgroups, 256, rows, cols)) return rc;
+    const dim3 grid((unsigned)workgroups);
     if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_quantize<SRC_BF16>, grid, dim3(256), 0, st, a);
     else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_quantize<SRC_F16>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(k_quantize<SRC_F32>, grid, dim3(256), 0, st, a);
@@ -268,7 +278,9 @@ int spa_mx4_values(const uint8_t* codes, const uint8_t* scales, int64_t rows, in
     if (!y) return fail(SPA_ERR_ARG, "mx4_values: a pointer is NULL");
     Values a{codes, scales, rows, cols, stride, (int)pitch_of(cols), y};
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)((rows * ((cols + 31) / 32) * 4 + 255) / 256));
+    const int64_t workgroups = (rows * ((cols + 31) / 32) * 4 + 255) / 256;
+    if (int rc = check_launch("mx4_values", workgroups, 256, rows, cols)) return rc;
+    const dim3 grid((unsigned)workgroups);
     if (kind == SPA_SRC_BF16) hipLaunchKernelGGL(k_values<SRC_BF16>, grid, dim3(256), 0, st, a);
     else if (kind == SPA_SRC_F16) hipLaunchKernelGGL(k_values<SRC_F16>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(k_values<SRC_F32>, grid, dim3(256), 0, st, a);
@@ -281,8 +293,9 @@ int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t*
     if (cols % 32) return fail(SPA_ERR_ARG, "mx4_from_blocks: rows of %lld are not whole blocks of 32", (long long)cols);
     if (!rows) return SPA_OK;
     if (!blocks) return fail(SPA_ERR_ARG, "mx4_from_blocks: a pointer is NULL");
-    const int64_t pitch = pitch_of(cols);
-    hipLaunchKernelGGL(k_from_blocks, dim3((unsigned)((rows * pitch * 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+    const int64_t pitch = pitch_of(cols), workgroups = (rows * pitch * 4 + 255) / 256;
+    if (int rc = check_launch("mx4_from_blocks", workgroups, 256, rows, cols)) return rc;
+    hipLaunchKernelGGL(k_from_blocks, dim3((unsigned)workgroups), dim3(256), 0, (hipStream_t)stream,
                        (const uint8_t*)blocks, rows, cols / 32, (int)pitch, codes, scales);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;

@@ -178,7 +178,7 @@ template <int MT, int NT> int launch(const Product& p, hipStream_t st) {
     while (split < W && 2 * split <= pieces) split *= 2;
     const int width = W / split * 16 * NT;
     const int64_t groups = (int64_t)((p.n + width - 1) / width) * most_tiles(p, 16 * MT);
-    if (groups > INT32_MAX) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
+    if (!one_launch(groups, W * 64)) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
     if (p.w1c) hipLaunchKernelGGL((k_few<MT, NT, true>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
     else hipLaunchKernelGGL((k_few<MT, NT, false>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
     SPA_HIP_TRY(hipGetLastError());

@@ -397,7 +397,7 @@ __global__ __launch_bounds__(256) void k_join_pieces(const Product p) {
 template <int TN, int TM, int WN, int WM, int OUT> int launch(const Product& p, hipStream_t st) {
     constexpr int TNE = OUT == OUT_GATED ? TN / 2 : TN;
     const int64_t groups = (int64_t)((p.n + TNE - 1) / TNE) * most_tiles(p, TM) * (OUT == OUT_PART ? p.pieces * (p.w1c ? 2 : 1) : 1);
-    if (groups > INT32_MAX - 8) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
+    if (!one_launch(groups, WN * WM * 64)) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
     hipLaunchKernelGGL((k_product<TN, TM, WN, WM, OUT>), dim3((unsigned)groups), dim3(WN * WM * 64), 0, st, p);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
@@ -407,9 +407,11 @@ template <int TN, int TM, int WN, int WM, int OUT> int launch(const Product& p, 
 
 int product_many(const Product& p, bool large, hipStream_t st) {
     if (p.pieces > 1) {
+        const int64_t workgroups = ((int64_t)p.m * ((p.n + 3) / 4) + 255) / 256;
+        if (!one_launch(workgroups, 256)) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
         const int rc = launch<128, 128, 2, 2, OUT_PART>(p, st);
         if (rc) return rc;
-        const dim3 grid((unsigned)(((int64_t)p.m * ((p.n + 3) / 4) + 255) / 256));
+        const dim3 grid((unsigned)workgroups);
         if (p.w1c) hipLaunchKernelGGL(k_join_pieces<true>, grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL(k_join_pieces<false>, grid, dim3(256), 0, st, p);
         SPA_HIP_TRY(hipGetLastError());

@@ -599,11 +599,12 @@ template <int KIND, bool DEEP> int route_kind(const Route& a, Order& o, bool sor
         if (a.experts <= 512) return go(k_route_few<KIND, 8, DEEP>);
         return go(k_route_few<KIND, 16, DEEP>);
     }
-    const int64_t rows = (int64_t)s.rows * s.reps;
+    const int64_t rows = (int64_t)s.rows * s.reps, workgroups = (a.rows + rows - 1) / rows;
+    if (!one_launch(workgroups, s.threads)) return fail(SPA_ERR_ARG, "route: %lld rows of %d experts are more than one launch takes", (long long)a.rows, a.experts);
     if (sorted) lay_out(o, a.rows * a.each, a.experts, rows * a.each, work);
     const size_t bytes = (sorted ? (size_t)(a.experts + 1 + 3) / 4 * 16 : 0) + (DEEP ? group_lds(a, s.rows) : 0);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3((unsigned)s.threads), bytes, st, a, o, s.reps);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)workgroups), dim3((unsigned)s.threads), bytes, st, a, o, s.reps);
         SPA_HIP_TRY(hipGetLastError());
         return SPA_OK;
     };
@@ -760,7 +761,9 @@ __global__ __launch_bounds__(256) void k_route_back(const Back a) {
 
 template <int KIND> int route_back(const Back& a, hipStream_t st) {
     auto go = [&](auto kernel, int rows) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(256), 0, st, a);
+        const int64_t workgroups = (a.rows + rows - 1) / rows;
+        if (!one_launch(workgroups, 256)) return fail(SPA_ERR_ARG, "route_backward: %lld rows of %d experts are more than one launch takes", (long long)a.rows, a.experts);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)workgroups), dim3(256), 0, st, a);
         SPA_HIP_TRY(hipGetLastError());
         return SPA_OK;
     };

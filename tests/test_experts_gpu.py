@@ -454,3 +454,17 @@ def test_a_workspace_of_no_bytes_is_left_alone(rows, e, groups):
     for name, h in (("which", want), ("order", order), ("starts", starts)):
         np.testing.assert_array_equal(o[name].to_host(), h)
     assert (block.to_host() == 0xa5).all()
+
+
+def test_join_backward_of_more_slots_than_one_launch_takes():
+    """2^24 workgroups of 256 are one too many: the launches' ends lie inside a row"""
+    each, n = 3, 2
+    rows = (1 << 24) // each + 1001
+    g = rng(24)
+    turns = lambda a, m: np.ascontiguousarray(np.tile(a, (m // len(a) + 1, 1))[:m])
+    y, w, d = turns(g.normal(0, 1, (997, n)).astype(F32), rows * each), turns(g.normal(0, 1, (991, each)).astype(F32), rows), turns(g.normal(0, 1, (983, n)).astype(F32), rows)
+    dy, dw = experts.join_backward(up(y), up(w), up(d))
+    dd = np.repeat(d, each, 0)
+    np.testing.assert_array_equal(dy.to_host(), dd * w.reshape(-1, 1))         # one float32 product
+    terms = dd.astype(np.float64) * y
+    close(dw.to_host().reshape(-1), terms.sum(1), n * 2.0 ** -24 * abs(terms).sum(1), F32)

@@ -140,3 +140,23 @@ def test_products_refuse(change, code):
 def test_python_refuses(call):
     with pytest.raises((ValueError, TypeError)):
         call()
+
+
+def test_calls_past_one_launch_are_refused():
+    """a dispatch counts its work-items in 32 bits; the sizes are the first that need 2^32"""
+    L, w = lib(), (P, 1 << 60, None)
+    for rows, e in ((1 << 28, 16), (1 << 27, 256), (1 << 28, 300)):
+        assert L.spa_route(P, 0, rows, e, e, 0, None, 1, 1, 2, 1, 1, 1.0, P, P, None, None, None, 0, None) == ARG
+        assert L.spa_route(P, 0, rows, e, e, 0, None, 1, 1, 2, 1, 1, 1.0, P, P, P, P, *w) == ARG
+    assert L.spa_route(P, 0, 1 << 28, 16, 16, 0, None, 2, 1, 2, 1, 1, 1.0, P, P, P, P, *w) == ARG
+    for rows, e in ((1 << 28, 16), (1 << 26, 300)):
+        assert L.spa_route_backward(P, 0, rows, e, e, 0, 1, 1, 1.0, P, P, P, e, None) == ARG
+    for kind, n in ((0, 64), (1, 57), (2, 32)):
+        assert L.spa_join(P, kind, 1 << 29, 1, n, n, P, None, 0, P, n, None) == ARG
+    assert L.spa_mx4_quantize(P, 0, 1 << 27, 256, 256, 0, P, P, None) == ARG
+    assert L.spa_mx4_quantize(P, 0, 256, 1 << 29, 1 << 29, 1, P, P, None) == ARG
+    assert L.spa_mx4_values(P, P, 1 << 30, 32, P, 0, 32, None) == ARG
+    assert L.spa_mx4_from_blocks(P, 1 << 27, 256, P, P, None) == ARG
+    for m, n in ((1 << 28, 1), (1 << 30, 3000)):       # 32 rows, and a tile of 256, by 512 work-items
+        assert L.spa_mx4_project(P, P, m, 256, P, P, n, 0, None, None, 0, P, 0, n, *w) == ARG
+        assert L.spa_mx4_gated(P, P, m, 256, P, P, P, P, n, 0, 0, None, None, 0, P, 0, n, *w) == ARG
