@@ -31,7 +31,15 @@ struct Product {
     float* part;                         // [pieces, of the gate's and of the up projection][m][n]
 };
 
-int product_few(const Product& p, bool wide, hipStream_t st);
+// A workgroup's waves of a product of few rows, and how many of them share their rows: as many as there are pieces of 512 of k
+constexpr int FEW_WAVES = 8;
+inline int few_split(int pitch) {
+    int split = 1;
+    while (split < FEW_WAVES && 2 * split <= (pitch + 15) / 16) split *= 2;
+    return split;
+}
+
+int product_few(const Product& p, bool wide, hipStream_t st);   // wide: 32 x 32 outputs a wave, of one matrix
 int product_many(const Product& p, bool large, hipStream_t st);
 
 }  // namespace mx

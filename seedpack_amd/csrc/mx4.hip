@@ -304,43 +304,58 @@ int spa_mx4_from_blocks(const void* blocks, int64_t rows, int64_t cols, uint8_t*
 namespace {
 
 // What a product takes, by the forms' times on one MI355X, in us:
-//   FEW16, FEW32  16 x 16 and 32 x 32 outputs a wave: 3.3 and 4.5 for a launch, then 6.6 and 6.9 for 26.7 MB of weights, which
-//                 each tile of 16 or 32 rows reads again
-//   SMALL         128 x 128 tiles: 3 to 5 and 0.74 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
+//   FEW16, FEW32  16 x 16 and 32 x 32 outputs a wave: 2.9 for a launch; then rounds of 256 workgroups, each of which takes, for a MB
+//                 of weights, 41 and 1.65 more for each input row of a tile (32 x 32: 62 and 0.5). Two matrices are 60 and 0.5 where the
+//                 rounds follow one another; 32 x 32 won at none of 148 sizes of them and is not there
+//   SMALL         128 x 128 tiles: 4.7 and 0.7 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
 //                 in pieces of k, where there are too few tiles: 2 for the joining launch and 3.3 TB/s for its sums
-//   LARGE         256 x 256 tiles, one to a compute unit: 5 and 1.95 a step, 1.4 with most units idle
-// k = 4096 of 12288 outputs, us:  rows  16: 10.1 11.5 13.8 19.1   32: 16.6 13.3 14.2 19.8   64: 29.6 18.1 14.9 21.0
-//   128: 55 34 16.8 22.0   256: 107 59 17.1 28.5   4096: - - 130 107;   k = 12288 of 4096, SMALL whole and in 2, 4 and 8 pieces:
-//   64: 34.6 22.1 16.2 15.7   256: 40.6 27.2 22.9 25.9   512: 40.9 31.5 31.9 43.2; k = 4096 of 4096: 256: 13.7 15.6 20.6 23.8.
+//   LARGE         256 x 256 tiles, one to a compute unit: 8 and 1.75 a step, 1.25 with most units idle
+// Tiles take no less than 3 and the weights' bytes at 5 TB/s, where few rows read 285 MB at 6 TB/s. Weights past the cache behind the
+// L2s, us by rows, FEW16 FEW32 SMALL LARGE and SMALL in 2 and 4 pieces of k:
+//   12288 x 4096    1: 7.1 9.7 12.6 17.9 11.8 11.7    16: 9.2 10.9 12.9 18.3 12.1 12.4    64: 28.6 17.7 14.1 20.2 14.7 14.8
+//                 256: 110 62.5 16.5 30.6 24.4 34.7
+//   12288 x 8192    1: 13.2 20.5 29.9 42.5 20.6 18.3  16: 18.6 25.0 30.2 43.1 20.9 18.7   32: 31.7 29.4 30.7 45.1 21.7 20.1
+//   131072 x 4096   1: 47.6 71.6 56.4 61.6 63.6 72.9  16: 80.2 92.7 58.2 63.2 69.1 81.7
+//   65536 x 8192    1: 55.3 89.3 68.0 69.9 58.6 63.2  16: 83.7 103 68.8 71.2 61.8 67.5
+//   2048 x 16384   32: 11.4 20.9 39.6 58.9 24.5 16.0  64: 20.3 20.8 40.5 60.5 25.1 16.8 (in 8 pieces 13.6 and 15.2)
+//   4096 x 4096    64: 11.6 7.7 13.2 19.7 11.5 11.5
+//   2 x 12288 x 4096    1: 15.4 23.2 18.0 24.9 18.8 22.8    32: 31.3 26.6 18.6 26.1 20.4 25.2
 // By expert the rows' spread is not known on the host: rows are taken to be dealt at random, and half of the experts that have any
-// to end in a tile of their own. Tiles of few rows cost less than full ones, so rounds of them are not rounded up. 2 x 1536 x
-// 2048 of 64 experts, four a row, FEW16, SMALL and LARGE: rows 1: 7.4 9.7 12.8   4: 14.3 12.7 14.2   32: 29.7 29.2 31.6
-//   512: 117 49 54   2048: 361 80 81   4096: - 121 109.
+// to end in a tile of their own. Tiles of few rows cost less than full ones, so rounds of them are not rounded up.
+//   32 of 4096 x 7168, by slots   4: 13.3 17.8 21.2 30.0 17.7 19.1   32: 57.9 79.6 77.6 93.0 71.6 72.4   512: 183 167 97.9 108 114 127
+//   64 of 2 x 1536 x 2048         4: 7.3 9.5 9.3 12.3 10.4 11.6      32: 23.5 40.5 26.7 30.4 29.5 34.3   512: 65 96 48.6 52.3 63 78
+// The choice is the best or within 15% of it at 384 of 400 sizes; the rest are calls of a few us and uneven spreads of rows.
 enum Form { FEW16, FEW32, SMALL, LARGE };
 struct Plan {
     int form, pieces;
 };
 Plan plan(int64_t m, int64_t n, int64_t pitch, int64_t experts, bool gated) {
-    const double steps = (double)pitch / 8, sides = gated ? 2 : 1, mb = (double)n * pitch * 17 * sides * 1e-6 / 26.7;
-    const double used = experts ? experts * (1 - exp(-(double)m / experts)) : 0;
+    const double steps = (double)pitch / 8, sides = gated ? 2 : 1;
+    const double used = experts ? experts * (1 - exp(-(double)m / experts)) : 1;
+    const double read = 3 + 17e-6 * n * pitch * sides * used / 5;
     auto rows = [&](double t) { return experts ? fmax(used, m / t + used / 2) : ceil(m / t); };
     auto rounds = [&](double r) { return experts ? fmax(r, 1) : ceil(r); };
-    auto small = [&](double tiles, double k) { return tiles <= 256 ? 3 + tiles / 128 + 0.74 * k : rounds(tiles / 512) * (5 + 1.19 * k); };
+    auto few = [&](int tiles, double us, double us_row) {
+        const double width = FEW_WAVES / few_split((int)pitch) * 16 * tiles, tall = rows(16 * tiles), in = fmin(16 * tiles, m / tall);
+        const double turns = ceil(n / width) * tall / 256, each = (us + us_row * in) * (experts || turns >= 4 ? fmax(turns, 1) : ceil(turns));
+        return 2.9 + 17e-6 * width * pitch * sides * (gated ? fmax(each, (60 + 0.5 * in) * turns) : each);
+    };
+    auto small = [&](double tiles, double k) { return fmax(tiles <= 256 ? 4.7 + tiles / 200 + 0.7 * k : rounds(tiles / 512) * (5 + 1.19 * k), read); };
     Plan best{FEW16, 1};
-    double least = 3.3 + 6.6 * rows(16) * mb;
+    double least = few(1, 41, 1.65);
     auto take = [&](int form, int pieces, double us) {
         if (us < least) {
             best = Plan{form, pieces};
             least = us;
         }
     };
-    take(FEW32, 1, 4.5 + 6.9 * rows(32) * mb);
-    const double wide = ceil(n * sides / 128.0), tiles = wide * rows(128);
+    if (!gated) take(FEW32, 1, few(2, 62, 0.5));
+    const double tiles = ceil(n * sides / 128.0) * rows(128);
     take(SMALL, 1, small(tiles, steps));
     for (int p = 2; p <= 8 && 2 * p <= steps; ++p)
         take(SMALL, p, small(tiles * p, ceil(steps / p)) + 2 + (double)m * n * 8 * p * sides / 3.3e6);
     const double large = ceil(n * sides / 256.0) * rows(256);
-    take(LARGE, 1, rounds(large / 256) * (5 + (1.4 + 0.55 * fmin(large / 256, 1)) * steps));
+    take(LARGE, 1, fmax(rounds(large / 256) * (8 + (1.25 + 0.5 * fmin(large / 256, 1)) * steps), read));
     return best;
 }
 uint64_t part_bytes(const Plan& c, int64_t m, int64_t n, bool gated) {

@@ -40,7 +40,7 @@ __device__ __forceinline__ f4 multiply(const Part& w, const Part& x, f4 acc) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.codes[3]), operand(x.codes[3]), acc, 4, 4, 3, (int)w.scales, 3, (int)x.scales);
 }
 
-constexpr int W = 8;                                             // waves
+constexpr int W = FEW_WAVES;
 
 template <int MT, int NT, bool TWO>
 __device__ __forceinline__ void few(const Product& p, int split) {
@@ -172,22 +172,22 @@ __global__ __launch_bounds__(W * 64) void k_few(const Product p, int split) {
     few<MT, NT, TWO>(p, split);
 }
 
-template <int MT, int NT> int launch(const Product& p, hipStream_t st) {
-    const int pieces = (p.pitch + 15) / 16;
-    int split = 1;
-    while (split < W && 2 * split <= pieces) split *= 2;
+template <int MT, int NT, bool TWO> int launch(const Product& p, hipStream_t st) {
+    const int split = few_split(p.pitch);
     const int width = W / split * 16 * NT;
     const int64_t groups = (int64_t)((p.n + width - 1) / width) * most_tiles(p, 16 * MT);
     if (!one_launch(groups, W * 64)) return fail(SPA_ERR_ARG, "product: %d x %d outputs are too many", p.m, p.n);
-    if (p.w1c) hipLaunchKernelGGL((k_few<MT, NT, true>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
-    else hipLaunchKernelGGL((k_few<MT, NT, false>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
+    hipLaunchKernelGGL((k_few<MT, NT, TWO>), dim3((unsigned)groups), dim3(W * 64), 0, st, p, split);
     SPA_HIP_TRY(hipGetLastError());
     return SPA_OK;
 }
 
 }  // namespace
 
-int product_few(const Product& p, bool wide, hipStream_t st) { return wide ? launch<2, 2>(p, st) : launch<1, 1>(p, st); }
+int product_few(const Product& p, bool wide, hipStream_t st) {
+    if (wide) return launch<2, 2, false>(p, st);
+    return p.w1c ? launch<1, 1, true>(p, st) : launch<1, 1, false>(p, st);
+}
 
 }  // namespace mx
 }  // namespace spa

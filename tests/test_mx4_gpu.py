@@ -452,6 +452,42 @@ def test_rows_past_4_gib(n):
                     out=dev.DeviceArray((m, n), BF16))
 
 
+def turns(a, m):
+    """a's rows over and over, m of them"""
+    return np.ascontiguousarray(np.tile(a, (m // len(a) + 1, 1))[:m])
+
+
+@pytest.mark.parametrize("n,k", [(131072, 4096), (65536, 8192), (12288, 8192), (2048, 16384)])
+@pytest.mark.parametrize("m", [1, 4, 16, 32])
+def test_few_rows_of_large_matrices(m, n, k):
+    """weights of hundreds of MB: 199 rows over and over"""
+    g = rng(19, m, n)
+    (xc, xs, x), (wc, ws, w) = random_rows(g, m, k), random_rows(g, 199, k)
+    y = mx4.project(matrix(xc, xs, m, k), matrix(turns(wc, n), turns(ws, n), n, k), dtype=F32).to_host()
+    at = np.arange(n) % 199
+    close(y, (x @ w.T)[:, at], lost(k, abs(x) @ abs(w).T)[:, at], F32)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m", [1, 4, 16, 32])
+def test_few_rows_of_large_gated_matrices(m, act):
+    n, k = 12288, 4096
+    g = rng(20, m)
+    (xc, xs, x), (gc, gs, gate), (uc, us, upw) = random_rows(g, m, k, 1), random_rows(g, 199, k, 1), random_rows(g, 199, k, 1)
+    gs, gate = smaller(gs, 7), gate * 2.0 ** -7
+    y = mx4.gated(matrix(xc, xs, m, k), matrix(turns(gc, n), turns(gs, n), n, k), matrix(turns(uc, n), turns(us, n), n, k), act, dtype=F32).to_host()
+    at = np.arange(n) % 199
+    close_gated((x @ gate.T)[:, at], (x @ upw.T)[:, at], lost(k, abs(x) @ abs(gate).T)[:, at], lost(k, abs(x) @ abs(upw).T)[:, at], act, y, F32)
+
+
+# tiles of 256 of one step, of an odd number and of many; 32 rows a wave where they fill the chip
+@pytest.mark.parametrize("m,n,k", [(4100, 8300, 200), (2300, 5000, 700), (2100, 4100, 4300), (48, 4096, 4096), (130, 1900, 2900)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_forms_of_whole_products(kind, m, n, k):
+    x, _, b, (_, (y, t)) = larger(m, n, k)
+    close(mx4.project(matrix(*x[:2], m, k), matrix(*b[:2], n, k), dtype=kind).to_host(), y, lost(k, t), kind)
+
+
 # ------------------------------------------------------------------------------------------ as they are used
 
 def bits(v):
