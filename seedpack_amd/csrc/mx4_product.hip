@@ -33,10 +33,11 @@ template <int U> __device__ __forceinline__ f16v mul(u4 w, u4 x, f16v c, uint32_
 
 enum Out { OUT_PLAIN, OUT_GATED, OUT_PART };                  // PART: float32 sums of a piece of k of one matrix
 
-// An activation's value by the hardware's 2^x and 1 / x, both good to an ulp: the logit's rounding in units of log2 costs
-// |logit| 2^-24 of the result. (With a logit of two parts, as the products of 16 bits have it, the outputs of 128 x 256 take
-// 5 us, not 3.)
-template <int ACT> __device__ __forceinline__ float act_short(float g) {
+// An activation's value by the hardware's 2^x and 1 / x, both good to an ulp. Outputs of 16 bits do without the logit's second
+// part: its rounding in units of log2 costs |logit| 2^-24 of the result, a 64th of their half step at most, and with two parts the
+// outputs of 128 x 256 take 5 us, not 3. Outputs in float32 would show it (a gate of -80 was off by 60 2^-24).
+template <int KIND, int ACT> __device__ __forceinline__ float act_of(float g) {
+    if constexpr (KIND == SRC_F32) return lin::act_value(g, ACT);
     return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * lin::act_logit(g, ACT)));
 }
 
@@ -300,7 +301,7 @@ __device__ __forceinline__ void product(const Product& p) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         v[c] = acc[i][j][4 * q + c];
-                        if (TWO) v[c] = act_short<ACT>(v[c]) * acc[i + (TWO ? FN / 2 : 0)][j][4 * q + c];
+                        if (TWO) v[c] = act_of<KIND, ACT>(v[c]) * acc[i + (TWO ? FN / 2 : 0)][j][4 * q + c];
                     }
                     *reinterpret_cast<f4*>(stage + fr * PITCH + 32 * i + 8 * q + 4 * fk) = v;
                 }

@@ -452,6 +452,36 @@ def test_rows_past_4_gib(n):
                     out=dev.DeviceArray((m, n), BF16))
 
 
+def exact_gates(g, n, k):
+    """gates between -85 and 85 whose products with ones at the head of each block are exact in float32, by their highest bits in four
+    blocks -> (codes, scales, their sums)"""
+    left, w = g.uniform(-85, 85, n), np.zeros((n, k))
+    for b in range(4):
+        part = np.zeros((n, 32))
+        part[:, 0] = np.where(abs(left) < 2.0 ** -10, 0, left)
+        w[:, 32 * b] = oracle.values(*oracle.quantize(part), 32)[:, 0]
+        left = left - w[:, 32 * b]
+    return *oracle.quantize(w), w.sum(1)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 1000, 256), (48, 1000, 256), (600, 1000, 256), (2300, 2500, 256), (600, 700, 9000)])
+def test_silu_of_exact_gates_in_float32(m, n, k):
+    """in every form alike: the exponential and the reciprocal are good to 2^-23 each, three roundings of 2^-24 and two of what is small
+    beside them; the gates take part to all of their bits, so that none of it grows with them"""
+    g = rng(21, n, k)
+    one = np.zeros((m, k))
+    one[:, :256:32] = 1
+    first = np.zeros((n, k))
+    first[:, 0] = 1
+    gc, gs, gate = exact_gates(g, n, k)
+    y = mx4.gated(matrix(*oracle.quantize(one), m, k), matrix(gc, gs, n, k), matrix(*oracle.quantize(first), n, k), "silu", dtype=F32).to_host()
+    want = oracle.act(gate, "silu")
+    off = (abs(y - want) / abs(want)).max(0)
+    assert gate.min() < -60 and gate.max() > 60
+    worst = off.argmax()
+    assert off[worst] <= 9 * 2.0 ** -24, (off[worst] * 2 ** 24, gate[worst])
+
+
 def turns(a, m):
     """a's rows over and over, m of them"""
     return np.ascontiguousarray(np.tile(a, (m // len(a) + 1, 1))[:m])
