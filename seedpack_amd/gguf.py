@@ -14,15 +14,17 @@ import numpy as np
 
 from ._lib import lib
 
-F32, F16, Q8_0, BF16 = 0, 1, 8, 30
+F32, F16, Q8_0, BF16, MXFP4 = 0, 1, 8, 30, 39
 TYPE_NAMES = {0: "F32", 1: "F16", 2: "Q4_0", 3: "Q4_1", 6: "Q5_0", 7: "Q5_1", 8: "Q8_0", 10: "Q2_K", 11: "Q3_K",
               12: "Q4_K", 13: "Q5_K", 14: "Q6_K", 16: "IQ2_XXS", 17: "IQ2_XS", 18: "IQ3_XXS", 19: "IQ1_S",
-              20: "IQ4_NL", 21: "IQ3_S", 22: "IQ2_S", 23: "IQ4_XS", 29: "IQ1_M", 30: "BF16", 42: "Q2_0"}
-# ggml type -> (elements per block, bytes per block)
+              20: "IQ4_NL", 21: "IQ3_S", 22: "IQ2_S", 23: "IQ4_XS", 29: "IQ1_M", 30: "BF16", 39: "MXFP4", 42: "Q2_0"}
+# ggml type -> (elements per block, bytes per block), of the types that an archive codes
 BLOCK = {0: (1, 4), 1: (1, 2), 30: (1, 2), 2: (32, 18), 3: (32, 20), 6: (32, 22), 7: (32, 24), 8: (32, 34),
          9: (32, 36), 10: (256, 84), 11: (256, 110), 12: (256, 144), 13: (256, 176), 14: (256, 210), 15: (256, 292),
          16: (256, 66), 17: (256, 74), 18: (256, 98), 19: (256, 50), 20: (32, 18), 21: (256, 110), 22: (256, 82),
          23: (256, 136), 24: (1, 1), 25: (1, 2), 26: (1, 4), 27: (1, 8), 28: (1, 8), 29: (256, 56), 42: (64, 18)}
+# of those that are only read, for mx4.from_blocks: an archive takes a file that holds them as it takes any other file
+READ = {MXFP4: (32, 17)}
 
 # GGUF value type -> struct code of the scalar types
 _SCALARS = {0: "B", 1: "b", 2: "H", 3: "h", 4: "I", 5: "i", 6: "f", 7: "?", 10: "Q", 11: "q", 12: "d"}
@@ -71,7 +73,7 @@ class GGUF:
         self.data_start = -(-self._pos // align) * align
         self.tensors = []
         for name, dims, t, off in table:
-            be, bb = BLOCK[t]
+            be, bb = BLOCK.get(t) or READ[t]
             n = int(np.prod(dims, dtype=np.int64))
             self.tensors.append(Tensor(name, dims, t, self.data_start + off, n // be * bb))
         del self._mv
@@ -119,34 +121,43 @@ class GGUF:
         return [self._value(it) for _ in range(n)]
 
 
+def coded(g):
+    """a GGUF's tensors, all of types that an archive codes (KeyError otherwise)"""
+    for t in g.tensors:
+        BLOCK[t.type]
+    return g.tensors
+
+
 def tensors_of(path):
-    """the tensor table of the GGUF file at `path` ([] if it is not one), from its header only"""
+    """the tensor table of the GGUF file at `path` ([] if it is not one that an archive codes), from its header only"""
     import mmap
     try:
         with open(path, "rb") as f, mmap.mmap(f.fileno(), 0, access=mmap.ACCESS_READ) as mm:
-            return GGUF(mm, light=True).tensors
+            return coded(GGUF(mm, light=True))
     except (ValueError, OSError, struct.error, KeyError):
         return []
 
 
 def header_of(path):
-    """(metadata, tensor table) of the GGUF file at `path` (({}, []) if it is not one), from its
+    """(metadata, tensor table) of the GGUF file at `path` (({}, []) if it is not one that an archive codes), from its
     header only, in one pass"""
     import mmap
     try:
         with open(path, "rb") as f, mmap.mmap(f.fileno(), 0, access=mmap.ACCESS_READ) as mm:
             g = GGUF(mm, light=True)
-            return g.meta, g.tensors
+            return g.meta, coded(g)
     except (ValueError, OSError, struct.error, KeyError):
         return {}, []
 
 
 def meta_of(path):
-    """the key/value metadata of a GGUF file ({} if it is not one), from its header only"""
+    """the key/value metadata of a GGUF file ({} if it is not one that an archive codes), from its header only"""
     import mmap
     try:
         with open(path, "rb") as f, mmap.mmap(f.fileno(), 0, access=mmap.ACCESS_READ) as mm:
-            return GGUF(mm, light=True).meta
+            g = GGUF(mm, light=True)
+            coded(g)
+            return g.meta
     except (ValueError, OSError, struct.error, KeyError):
         return {}
 
@@ -199,7 +210,7 @@ def header_bytes(kv, tensors, align=32):
         parts += [_enc_string(k), struct.pack("<I", vt), body]
     rel, o = [], 0
     for name, shape, t in tensors:
-        be, bb = BLOCK[t]
+        be, bb = BLOCK.get(t) or READ[t]
         nb = int(np.prod(shape, dtype=np.int64)) // be * bb
         rel.append((o, nb))
         parts += [_enc_string(name), struct.pack("<I", len(shape)), struct.pack(f"<{len(shape)}Q", *shape),

@@ -83,7 +83,8 @@ def values(q, out=None, dtype=np.float32, out_stride=None, stream=None):
 
 
 def from_blocks(blocks, rows, cols, count=1, out=None, stream=None):
-    """count matrices of GGUF MXFP4 blocks, 17 bytes for 32 numbers, as they lie in a file -> Matrix"""
+    """count matrices of GGUF MXFP4 blocks, 17 bytes for 32 numbers, as they lie in a file -> Matrix: the bytes of a gguf.Tensor
+    of type gguf.MXFP4, whose shape is (cols, rows) or (cols, rows, count)"""
     if cols % 32:
         raise ValueError(f"rows of {cols} are not whole blocks of 32")
     need = count * rows * (cols // 32) * 17

@@ -121,7 +121,7 @@ def scan_file(path):
     size = os.path.getsize(path)
     data = np.memmap(path, np.uint8, "r") if size else np.zeros(0, np.uint8)
     g = gguf.GGUF(data, light=True)
-    ts = sorted(g.tensors, key=lambda t: t.offset)
+    ts = sorted(gguf.coded(g), key=lambda t: t.offset)
     gaps, at = [], g.data_start
     for t in ts:
         if t.offset > at:

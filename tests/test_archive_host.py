@@ -77,6 +77,22 @@ def test_pairs_form_needs_the_merge_structure():
 
 # ------------------------------------------------------------------ GGUF
 
+def test_gguf_with_4_bit_blocks_is_read_and_archived_as_any_other_file(tmp_path):
+    from seedpack_amd import repo, siblings
+    tensors = [("gate", (2880, 8, 3), gguf.MXFP4), ("norm", (2880,), gguf.F32)]
+    head, where, size = gguf.header_bytes({"general.architecture": "a"}, tensors)
+    data = head + bytes(size - len(head))
+    g = gguf.GGUF(data)
+    assert [(t.name, t.shape, t.type, t.offset, t.nbytes) for t in g.tensors] == [(n, s, ty, o, nb) for (n, s, ty), (o, nb) in zip(tensors, where)]
+    assert [t.nbytes for t in g.tensors] == [3 * 8 * 90 * 17, 2880 * 4] and gguf.TYPE_NAMES[g.tensors[0].type] == "MXFP4"
+    path = tmp_path / "m.gguf"
+    path.write_bytes(data)
+    assert gguf.tensors_of(path) == [] and gguf.header_of(path) == ({}, []) and gguf.meta_of(path) == {}
+    assert repo.file_role(str(path)) is None
+    with pytest.raises(KeyError):
+        siblings.scan_file(path)
+
+
 def test_gguf_round_trip_and_light_mode():
     kv = {"general.architecture": "qwen35", "general.alignment": 64, "a.u32": 7, "a.i64": -5, "a.f32": 0.25,
           "a.bool": True, "a.ints": [1, -2, 3], "a.floats": [0.5, 1.5], "tokenizer.ggml.tokens": [f"t{i}" for i in range(100)],

@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 
 from seedpack_amd import device as dev
-from seedpack_amd import experts, linear, mx4
+from seedpack_amd import experts, gguf, linear, mx4
 from seedpack_amd._lib import SpaError, check, lib
 
 from . import experts_oracle as oracle
@@ -189,6 +189,23 @@ def test_from_blocks(rows, cols, count, offset):
     scales[:, :cols // 32] = b[:, 0].reshape(count * rows, -1)
     np.testing.assert_array_equal(q.codes.to_host().reshape(codes.shape), codes)
     np.testing.assert_array_equal(q.scales.to_host().reshape(scales.shape), scales)
+
+
+def test_from_a_file():
+    """a file's tensor of 4-bit blocks, by the reader's table"""
+    rows, cols, count = 7, 96, 3
+    g = rng(23)
+    b = g.integers(0, 250, (count * rows * cols // 32, 17), dtype=np.uint8)
+    head, where, size = gguf.header_bytes({"general.architecture": "a"}, [("norm", (96,), gguf.F32), ("gate", (cols, rows, count), gguf.MXFP4)])
+    data = np.zeros(size, np.uint8)
+    data[:len(head)] = np.frombuffer(head, np.uint8)
+    at, nbytes = where[1]
+    data[at:at + nbytes] = b.reshape(-1)
+    t = gguf.GGUF(data).tensors[1]
+    assert (t.type, t.shape) == (gguf.MXFP4, (cols, rows, count))
+    q = mx4.from_blocks(up(data[t.offset:t.offset + t.nbytes]), t.shape[1], t.shape[0], t.shape[2])
+    want = oracle.values(np.ascontiguousarray(b[:, 1:]).reshape(count * rows, -1), np.ascontiguousarray(b[:, 0]).reshape(count * rows, -1), cols)
+    np.testing.assert_array_equal(mx4.values(q).to_host(), store(want, F32))
 
 
 # ------------------------------------------------------------------------------------------ products
