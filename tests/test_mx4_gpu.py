@@ -334,6 +334,27 @@ def check_by_expert(rows, e, each, n, k, by_slot, kind):
     assert (y[free] == nine[free]).all() and (h[free] == nine[free]).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,e,each,n,k", [(5, 16, 3, 100, 512), (700, 4, 3, 257, 256), (3000, 9, 2, 1300, 600), (300, 3, 1, 1000, 9000), (3000, 90, 2, 800, 800)])
+def test_gelu_by_expert(rows, e, each, n, k, kind):
+    g = rng(22, rows, e)
+    which = g.integers(-1, e + 1, (rows, each)).astype(np.int32)
+    r = experts.by_expert(up(which), e)
+    (xc, xs, x), (wc, ws, w), (vc, vs, v) = random_rows(g, rows, k, 1), random_rows(g, e * n, k, 1), random_rows(g, e * n, k, 1)
+    shift = int(np.log2(k) / 2) + 1
+    ws, w = smaller(ws, shift), w * 2.0 ** -shift
+    nine = np.full((rows * each, n), 9, kind)
+    h = up(nine)
+    mx4.gated(matrix(xc, xs, rows, k), matrix(wc, ws, n, k, e), matrix(vc, vs, n, k, e), "gelu", r, out=h)
+    h, flat = h.to_host(), which.reshape(-1)
+    for i in range(e):
+        at = np.flatnonzero(flat == i)
+        if len(at):
+            check_gated(x[at // each], w[i * n:(i + 1) * n], v[i * n:(i + 1) * n], "gelu", h[at], kind)
+    free = (flat < 0) | (flat >= e)
+    assert (h[free] == nine[free]).all()
+
+
 @pytest.mark.parametrize("m", [3, 20, 300])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("n,stride,offset", [(64, 72, 0), (70, 75, 0), (64, 64, 1)])
