@@ -322,7 +322,7 @@ __device__ __forceinline__ void route_row(const Route& a, int64_t row, bool in, 
 // The routing kernel counts its own rows' experts, a launch adds the counts up, one workgroup an expert, and the last places
 // some of the counted tiles at a time; a few rows are routed and ordered by one workgroup, in one launch. (Placing
 // workgroups that add up all counts themselves, for one launch less, took 13.5 us for 256 tiles of 128 experts, not 3 and 5.8.)
-constexpr int TILE = 512;                // slots that a workgroup places at most
+constexpr int TILE = 512;                // slots that a workgroup places, unless the routing's tiles are larger
 constexpr int FEW = 2048;                // slots that one workgroup routes and orders
 
 struct Order {
@@ -360,7 +360,8 @@ __device__ __forceinline__ uint32_t running(uint32_t v, uint32_t* scratch) {
     return v;
 }
 
-size_t order_lds(int64_t slots, int64_t experts) { return (size_t)((slots + 63) / 64 * 2 + 8) * (experts + 1); }
+constexpr size_t order_lds(int64_t slots, int64_t experts) { return (size_t)((slots + 63) / 64 * 2 + 8) * (experts + 1); }
+static_assert(order_lds(TILE, MOST_EXPERTS) <= 64 * 1024, "a tile is placed in the LDS of any launch");
 
 // Places the slots first .. first + n - 1 of `which` (in LDS or memory, from `first` on) by a workgroup of T threads; tile: its
 // number. LDS: order_lds(n, experts) bytes, 16-byte aligned.
@@ -467,12 +468,6 @@ __global__ __launch_bounds__(256) void k_sums(const Order o) {
     if (threadIdx.x == 0) o.sums[(int64_t)o.tiles * keys + e] = carry;
 }
 
-// the slots that a workgroup places, its counts in LDS that needs no leave
-int64_t most_placed(int64_t experts) {
-    int64_t n = TILE;
-    while (order_lds(n, experts) > 60 * 1024) n /= 2;
-    return n;
-}
 // the tiles of an order, and its workspace; one tile has no counts, and no byte of `work` is its
 void lay_out(Order& o, int64_t slots, int64_t experts, int64_t tile, void* work) {
     o.slots = (int)slots;
@@ -480,7 +475,7 @@ void lay_out(Order& o, int64_t slots, int64_t experts, int64_t tile, void* work)
     while (experts >> o.bits) ++o.bits;
     o.tile = (int)tile;
     o.tiles = (int)((slots + tile - 1) / tile);
-    o.group = (int)(most_placed(experts) / tile);
+    o.group = (int)(TILE / tile);
     if (!o.group) o.group = 1;
     if (o.tiles <= 1) return;
     o.counts = static_cast<uint16_t*>(work);
@@ -507,7 +502,7 @@ int by_expert(const int32_t* which, int64_t slots, int64_t experts, int32_t* ord
     o.which = which;
     o.order = order;
     o.starts = starts;
-    lay_out(o, slots, experts, most_placed(experts), work);
+    lay_out(o, slots, experts, TILE, work);
     if (o.tiles > 1) {
         hipLaunchKernelGGL(k_count, dim3((unsigned)o.tiles), dim3(1024), (size_t)(experts + 1) * 4, st, o);
         SPA_HIP_TRY(hipGetLastError());
@@ -570,6 +565,7 @@ struct Shape {
     bool few;                       // one workgroup does all
     int lanes, threads, rows, reps; // a row's lanes; rows of a workgroup at once, and how often
 };
+// LDS of a workgroup's rows in groups: 70 KB for 32 rows of 256 experts in 8 groups, 99 KB in 64, of the 160 KB that there are
 size_t group_lds(const Route& a, int rows) { return a.groups > 1 ? (size_t)rows * group_keys(a.experts, a.groups) * 8 : 0; }
 Shape shape_of(const Route& a, bool deep, bool sorted) {
     Shape s{};
@@ -803,7 +799,7 @@ extern "C" {
 
 uint64_t spa_by_expert_work_bytes(int64_t slots, int64_t experts) {
     if (slots <= 0 || experts < 1 || experts > MOST_EXPERTS) return 0;
-    return order_bytes(slots, experts, most_placed(experts));
+    return order_bytes(slots, experts, TILE);
 }
 
 int spa_by_expert(const int32_t* which, int64_t slots, int64_t experts, int32_t* order, int32_t* starts, void* work,

@@ -78,7 +78,8 @@ def route(logits, each, score="softmax", bias=None, groups=1, keep=1, best=2, re
     """logits (rows, experts) -> Routing: each row's `each` experts of the largest keys, the best first (of equal ones the
     lowest number). score "softmax" (over the row) or "sigmoid"; keys are the logits, or, with a bias (experts,) float32 or
     groups, score + bias. groups: the experts are that many equal runs, of which the `keep` best take part; a run is worth
-    the sum of its `best` (1 or 2) highest keys. A logit of -inf is never chosen; a row with too few experts has -1
+    the sum of its `best` (1 or 2) highest keys. (score + bias is a sum in 64 bits; sums that agree to 42 bits of their mantissas are
+    equal, as the logistics of all logits above 30 are.) A logit of -inf is never chosen; a row with too few experts has -1
     and weight 0 in its last places. Weights are scale * score, with renorm divided by the sum of the row's chosen scores. sort:
     the slots' order too."""
     kind, m, e, ld = _rows("logits", logits, logits_stride)

@@ -468,3 +468,14 @@ def test_join_backward_of_more_slots_than_one_launch_takes():
     np.testing.assert_array_equal(dy.to_host(), dd * w.reshape(-1, 1))         # one float32 product
     terms = dd.astype(np.float64) * y
     close(dw.to_host().reshape(-1), terms.sum(1), n * 2.0 ** -24 * abs(terms).sum(1), F32)
+
+
+def test_keys_of_42_bits():
+    """with a bias or groups, keys that agree to 42 bits of their mantissas are equal: the logistic of 31 and of 32 lies within 2^-43 of
+    1, that of 29 does not"""
+    l = np.full((2, 16), -1, F32)
+    l[:, 9], l[0, 3], l[1, 3] = 32, 31, 29
+    for one in (dict(bias=up(np.zeros(16, F32))), dict(groups=2, keep=2)):
+        which = experts.route(up(l), 2, "sigmoid", **one).which.to_host()
+        assert list(which[0]) == [3, 9] and list(which[1]) == [9, 3]
+    assert (experts.route(up(l), 2, "sigmoid").which.to_host() == [9, 3]).all()       # the logits themselves are the keys
