@@ -606,7 +606,7 @@ uint64_t spa_add_squares_work_bytes(int64_t rows, int64_t cols, int64_t experts)
  * Routing sends each row to `each` of `experts` experts: slot p = row * each + j is row's place j. Logits, rows of results and
  * their gradients are BF16, F16 or F32 (SPA_SRC_*), numbers and weights of slots int32 and float32, dense. Nothing
  * is allocated, and calls may be captured. `work` as with the products. Up to 1024 experts, 32 a row, and 2^31 - 1025 slots;
- * what one launch's 2^32 work-items do not take is refused (2^28 rows of up to 128 experts routed, 2^32 runs of 16 bytes joined).
+ * what would need 2^32 work-items in one launch is refused (2^28 rows of up to 128 experts routed, 2^32 runs of 16 bytes joined).
  * Outputs must not overlap inputs. */
 
 /* Each row's experts, the best first, and their weights. score 0: softmax over the row, 1: 1 / (1 + e^-l). The chosen
@@ -648,8 +648,8 @@ int spa_join_backward(const void* y, int kind, int64_t rows, int64_t each, int64
  * aligned), pitch = spa_mx4_pitch(cols) blocks of 32: cols / 256 rounded up, times 8. Block b of a row holds its
  * numbers 32 b to 32 b + 31: j in the low half of byte j, j + 16 in the high half (as GGUF's MXFP4 does). A code is a sign
  * and 0 .5 1 1.5 2 3 4 6, a scale s stands for 2^(s - 127), 255 for a block of NaN. Blocks behind a row's last number are
- * zeros, codes and scales: conversions write them, and products count on them. Up to 4,000,000 columns, and what one launch's
- * 2^32 work-items take (2^30 blocks made or read; 2^23 tiles of 512 work-items a product). Nothing is allocated, and calls may
+ * zeros, codes and scales: conversions write them, and products count on them. Up to 4,000,000 columns; what would need 2^32
+ * work-items in one launch is refused (2^30 blocks made or read, 2^23 tiles of a product). Nothing is allocated, and calls may
  * be captured. Outputs must not overlap inputs. */
 int64_t spa_mx4_pitch(int64_t cols);
 
