@@ -307,7 +307,7 @@ namespace {
 //   FEW16, FEW32  16 x 16 and 32 x 32 outputs a wave: 2.9 for a launch; then rounds of 256 workgroups, each of which takes, for a MB
 //                 of weights, 41 and 1.65 more for each input row of a tile (32 x 32: 62 and 0.5). Two matrices are 60 and 0.5 where the
 //                 rounds follow one another; 32 x 32 won at none of 148 sizes of them and is not there
-//   SMALL         128 x 128 tiles: 4.7 and 0.7 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
+//   SMALL         128 x 128 tiles: 4.2 and 0.7 a step of 256 of k where a compute unit has one, 5 and 1.19 where it has two;
 //                 in pieces of k, where there are too few tiles: 2 for the joining launch and 3.3 TB/s for its sums
 //   LARGE         256 x 256 tiles, one to a compute unit: 8 and 1.75 a step, 1.25 with most units idle
 // Tiles take no less than 3 and the weights' bytes at 5 TB/s, where few rows read 285 MB at 6 TB/s. Weights past the cache behind the
@@ -321,10 +321,11 @@ namespace {
 //   4096 x 4096    64: 11.6 7.7 13.2 19.7 11.5 11.5
 //   2 x 12288 x 4096    1: 15.4 23.2 18.0 24.9 18.8 22.8    32: 31.3 26.6 18.6 26.1 20.4 25.2
 // By expert the rows' spread is not known on the host: rows are taken to be dealt at random, and half of the experts that have any
-// to end in a tile of their own. Tiles of few rows cost less than full ones, so rounds of them are not rounded up.
+// to end in a tile of their own. Tiles of few rows cost less than full ones, so rounds of them are not rounded up. Waves of few
+// rows count tiles anew in each workgroup: 0.6 more for the launch and 0.3 a round, 0.9 of more than 64 experts.
 //   32 of 4096 x 7168, by slots   4: 13.3 17.8 21.2 30.0 17.7 19.1   32: 57.9 79.6 77.6 93.0 71.6 72.4   512: 183 167 97.9 108 114 127
 //   64 of 2 x 1536 x 2048         4: 7.3 9.5 9.3 12.3 10.4 11.6      32: 23.5 40.5 26.7 30.4 29.5 34.3   512: 65 96 48.6 52.3 63 78
-// The choice is the best or within 15% of it at 384 of 400 sizes; the rest are calls of a few us and uneven spreads of rows.
+// The choice is the best or within 15% of it at 385 of 400 sizes; the rest are calls of a few us and uneven spreads of rows.
 enum Form { FEW16, FEW32, SMALL, LARGE };
 struct Plan {
     int form, pieces;
@@ -337,10 +338,11 @@ Plan plan(int64_t m, int64_t n, int64_t pitch, int64_t experts, bool gated) {
     auto rounds = [&](double r) { return experts ? fmax(r, 1) : ceil(r); };
     auto few = [&](int tiles, double us, double us_row) {
         const double width = FEW_WAVES / few_split((int)pitch) * 16 * tiles, tall = rows(16 * tiles), in = fmin(16 * tiles, m / tall);
-        const double turns = ceil(n / width) * tall / 256, each = (us + us_row * in) * (experts || turns >= 4 ? fmax(turns, 1) : ceil(turns));
-        return 2.9 + 17e-6 * width * pitch * sides * (gated ? fmax(each, (60 + 0.5 * in) * turns) : each);
+        const double turns = ceil(n / width) * tall / 256, whole = experts || turns >= 4 ? fmax(turns, 1) : ceil(turns), row = 17e-6 * pitch * sides;
+        const double each = (us + us_row * in) * fmin(width, n) * row + (experts ? experts > 64 ? 0.9 : 0.3 : 0);
+        return 2.9 + (experts ? 0.6 : 0) + fmax(each * whole, gated ? (60 + 0.5 * in) * width * row * turns : 0);
     };
-    auto small = [&](double tiles, double k) { return fmax(tiles <= 256 ? 4.7 + tiles / 200 + 0.7 * k : rounds(tiles / 512) * (5 + 1.19 * k), read); };
+    auto small = [&](double tiles, double k) { return fmax(tiles <= 256 ? 4.2 + tiles / 200 + 0.7 * k : rounds(tiles / 512) * (5 + 1.19 * k), read); };
     Plan best{FEW16, 1};
     double least = few(1, 41, 1.65);
     auto take = [&](int form, int pieces, double us) {
